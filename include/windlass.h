@@ -275,6 +275,52 @@ int32_t wl_argmax(const float* dev_logits, int32_t V, int32_t rows, int32_t* dev
 int32_t wl_sample(const float* dev_logits, int32_t V, double temperature, double top_p, double draw, int32_t* dev_id,
                   void* stream);
 
+/* ---- the 4-bit KV cache. No counterpart in the reference, whose cache is fp16: a quarter and a bit of the bytes
+ * (4.5 bits a value against 16) for longer contexts and more sequences. A key or value head is cut into blocks of 32
+ * values; a block holds an fp16 scale d = m / -8 (m: its value of largest magnitude) and 32 codes of 4 bits, and stands
+ * for (code - 8) d, Q4_0's values (a block that holds an infinity or NaN reads as NaN). One cache holds the keys and
+ * values of one layer of one sequence: 18 * head_dim bytes for 16 positions of a KV head, 16-byte aligned.
+ *
+ * Common arguments: T rows; dev_caches[t] = row t's cache (an array of T device pointers in device memory), dev_pos[t] =
+ * its position there, capacity = positions every cache of the call has room for. A row with a negative position is
+ * padding: nothing is read or written for it (its attention and read-back give zeros). A row whose position is not
+ * below capacity, or whose cache is null or not 16-byte aligned, is refused on the device: nothing is written to a
+ * cache, its attention and read-back give NaN. head_dim is 64, 96, 128 or 256, heads a multiple of kv_heads; other
+ * shapes return WL_EUNSUPPORTED. Float buffers are 16-byte aligned, contiguous, and on the current device (WL_EINVAL
+ * otherwise). The calls enqueue on `stream` and return; they allocate nothing and may be captured into a graph. ---- */
+
+/* Bytes of the cache of one layer of one sequence with room for `positions` positions. */
+int32_t wl_kv4_bytes(int32_t kv_heads, int32_t head_dim, int64_t positions, int64_t* bytes);
+/* Rotary positions of q and k, and the append of k and v at dev_pos[t] (Transformer.Rope and the cache's append,
+ * src/Transformer.cs:399-433, :208-218, with 4 bits for fp16): dev_q_out [T][heads * head_dim] = dev_q rotated (the two
+ * may be the same buffer), dev_k and dev_v [T][kv_heads * head_dim] quantised, k rotated first. rope_table: dev table
+ * [capacity][rope_dims] of (cos, sin) pairs, one for each position and pair, so that any scaling of the angles for long
+ * contexts is the table's; rope_dims (even, 0 .. head_dim) dims of each head are rotated, pairs (i, i + rope_dims / 2)
+ * with neox != 0, else (2i, 2i + 1), and the rest copied. The rows' (cache, position) must differ. The codes are decided
+ * in 64-bit arithmetic. */
+int32_t wl_kv4_append(const float* dev_q, float* dev_q_out, const float* dev_k, const float* dev_v, int32_t T, int32_t heads,
+                      int32_t kv_heads, int32_t head_dim, const float* dev_rope_table, int32_t rope_dims, int32_t neox,
+                      void* const* dev_caches, const int32_t* dev_pos, int64_t capacity, void* stream);
+/* What the caches hold: the values of position dev_pos[t] of row t's cache, rounded to fp16, into dev_k and dev_v
+ * [T][kv_heads * head_dim] (fp16). */
+int32_t wl_kv4_read(void* const* dev_caches, const int32_t* dev_pos, int32_t T, int32_t kv_heads, int32_t head_dim,
+                    int64_t capacity, void* dev_k, void* dev_v, void* stream);
+/* Attention (src/Transformer.cs:351-395) over the caches: row t attends to positions j <= dev_pos[t]; with window > 0 only
+ * to those with j > dev_pos[t] - window or j < sinks (the first tokens stay visible). dev_out [T][heads * head_dim]. The
+ * rows come in runs of rows_per_seq consecutive rows that read the same cache (T a multiple of it; 1 = every row may
+ * have its own): runs of more than 8 rows (prompts) share the cache's tiles, and only a run's first cache pointer is
+ * read. With runs of up to 8 rows a row's result does not depend on the other rows of a call of up to 64 rows.
+ * dev_workspace (256-byte aligned, wl_kv4_workspace_bytes of the same arguments) is initialised once with
+ * wl_kv4_workspace_init and then kept for any calls that are ordered after one another; calls that may overlap (two
+ * streams, two graphs in flight) need a workspace each. */
+int32_t wl_kv4_attention(const float* dev_q, int32_t T, int32_t rows_per_seq, int32_t heads, int32_t kv_heads,
+                         int32_t head_dim, float scale, void* const* dev_caches, const int32_t* dev_pos, int64_t capacity,
+                         int32_t window, int32_t sinks, float* dev_out, void* dev_workspace, int64_t workspace_bytes,
+                         void* stream);
+int32_t wl_kv4_workspace_bytes(int32_t T, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                               int64_t capacity, int32_t window, int32_t sinks, int64_t* bytes);
+int32_t wl_kv4_workspace_init(void* dev_workspace, int64_t workspace_bytes, void* stream);
+
 /* Synchronises `device` and reports whether a device-side wait of a kernel-level export (wl_matvec, wl_matvec_tiles,
  * wl_matvec_static, wl_gemm_tiles, wl_matmul) gave up since the last report: WL_ETIMEDOUT (and the code) if one did,
  * else WL_OK. The waits are bounded at 2 s of device time, so this is a stalled copy, not a slow one. The model's own

@@ -118,6 +118,12 @@ def lib():
         "wl_sample": (I32, [P, I32, C.c_double, C.c_double, C.c_double, P, P]),
         "wl_generate_greedy": (I32, [P, P, I32, I32, P, I32, I32, P, C.POINTER(I32), P]),
         "wl_argmax": (I32, [P, I32, I32, P, P]), "wl_route": (I32, [P, I32, I32, I32, I32, P, P, P]), "wl_kernel_status": (I32, [I32]),
+        "wl_kv4_bytes": (I32, [I32, I32, I64, C.POINTER(I64)]),
+        "wl_kv4_append": (I32, [P, P, P, P, I32, I32, I32, I32, P, I32, I32, P, P, I64, P]),
+        "wl_kv4_read": (I32, [P, P, I32, I32, I32, I64, P, P, P]),
+        "wl_kv4_attention": (I32, [P, I32, I32, I32, I32, I32, F, P, P, I64, I32, I32, P, P, I64, P]),
+        "wl_kv4_workspace_bytes": (I32, [I32, I32, I32, I32, I32, I64, I32, I32, C.POINTER(I64)]),
+        "wl_kv4_workspace_init": (I32, [P, I64, P]),
         "wl_dequant": (I32, [I32, P, I64, P, P]),
         "wl_matvec": (I32, [I32, P, I32, I32, P, I32, P, P]),
         "wl_matvec_static": (I32, [I32, P, I32, I32, P, I32, P, P]),

@@ -4,6 +4,8 @@
 #include <cstring>
 #include <mutex>
 #include <new>
+#include <string>
+#include <utility>
 #include <vector>
 #include "../../include/windlass.h"
 #include "wl_common.h"
@@ -682,6 +684,135 @@ int32_t wl_sample(const float* dev_logits, int32_t V, double temperature, double
             throw;
         }
         WL_CUDA(cudaFree(ws));
+        return WL_OK;
+    });
+}
+
+namespace {
+// Empty when `p` is 16-byte aligned memory of the current device (or managed memory); else what is wrong with it.
+std::string device_buffer_fault(const void* p, const char* what, size_t align = 16)
+{
+    if (!p) return std::string(what) + " is null";
+    if ((uintptr_t)p % align) return std::string(what) + " must be " + std::to_string(align) + "-byte aligned";
+    cudaPointerAttributes a{};
+    int dev = 0;
+    WL_CUDA(cudaGetDevice(&dev));
+    WL_CUDA(cudaPointerGetAttributes(&a, p));
+    if (a.type == cudaMemoryTypeManaged) return "";
+    if (a.type != cudaMemoryTypeDevice) return std::string(what) + " is not device memory";
+    if (a.device != dev)
+        return std::string(what) + " is on device " + std::to_string(a.device) + ", the current device is " + std::to_string(dev);
+    return "";
+}
+
+int32_t kv4_shape(const char* name, int32_t heads, int32_t kv_heads, int32_t head_dim, int64_t capacity)
+{
+    if (heads <= 0 || kv_heads <= 0 || head_dim <= 0) return wl::fail(WL_EINVAL, std::string(name) + ": heads, kv_heads and head_dim must be positive");
+    if (!wl::k::kv4_supported(heads, kv_heads, head_dim) || heads > 65535)
+        return wl::fail(WL_EUNSUPPORTED, std::string(name) + ": head_dim 64, 96, 128 or 256 and heads a multiple of kv_heads");
+    if (capacity <= 0 || capacity > INT32_MAX) return wl::fail(WL_EINVAL, std::string(name) + ": capacity must be 1 to 2^31 - 1 positions");
+    return WL_OK;
+}
+
+#define WL_CHECK_BUFFERS(name, ...)                                                                     \
+    do {                                                                                                \
+        const std::pair<const void*, const char*> list_[] = {__VA_ARGS__};                              \
+        for (const auto& b_ : list_) {                                                                  \
+            const std::string f_ = device_buffer_fault(b_.first, b_.second);                            \
+            if (!f_.empty()) return wl::fail(WL_EINVAL, std::string(name) + ": " + f_);                 \
+        }                                                                                               \
+    } while (0)
+}  // namespace
+
+int32_t wl_kv4_bytes(int32_t kv_heads, int32_t head_dim, int64_t positions, int64_t* bytes)
+{
+    return guarded([&]() -> int32_t {
+        if (!bytes) return wl::fail(WL_EINVAL, "wl_kv4_bytes: null pointer");
+        if (const int32_t st = kv4_shape("wl_kv4_bytes", kv_heads, kv_heads, head_dim, positions)) return st;
+        *bytes = wl::k::kv4_bytes(kv_heads, head_dim, positions);
+        return WL_OK;
+    });
+}
+
+int32_t wl_kv4_append(const float* dev_q, float* dev_q_out, const float* dev_k, const float* dev_v, int32_t T, int32_t heads,
+                      int32_t kv_heads, int32_t head_dim, const float* dev_rope_table, int32_t rope_dims, int32_t neox,
+                      void* const* dev_caches, const int32_t* dev_pos, int64_t capacity, void* stream)
+{
+    return guarded([&]() -> int32_t {
+        if (T < 0) return wl::fail(WL_EINVAL, "wl_kv4_append: T must not be negative");
+        if (const int32_t st = kv4_shape("wl_kv4_append", heads, kv_heads, head_dim, capacity)) return st;
+        if (rope_dims < 0 || rope_dims > head_dim || rope_dims % 2) return wl::fail(WL_EINVAL, "wl_kv4_append: rope_dims must be even, 0 to head_dim");
+        if (!dev_q || !dev_q_out || !dev_k || !dev_v || !dev_caches || !dev_pos || (rope_dims > 0 && !dev_rope_table))
+            return wl::fail(WL_EINVAL, "wl_kv4_append: null pointer");
+        if (T == 0) return WL_OK;
+        WL_CHECK_BUFFERS("wl_kv4_append", {dev_q, "dev_q"}, {dev_q_out, "dev_q_out"}, {dev_k, "dev_k"}, {dev_v, "dev_v"});
+        wl::k::kv4_append(dev_q, dev_q_out, dev_k, dev_v, T, heads, kv_heads, head_dim, dev_rope_table, rope_dims, neox ? 1 : 0,
+                          wl::k::Kv4Cache{dev_caches, 8, 0}, dev_pos, capacity, (cudaStream_t)stream);
+        return WL_OK;
+    });
+}
+
+int32_t wl_kv4_read(void* const* dev_caches, const int32_t* dev_pos, int32_t T, int32_t kv_heads, int32_t head_dim,
+                    int64_t capacity, void* dev_k, void* dev_v, void* stream)
+{
+    return guarded([&]() -> int32_t {
+        if (T < 0) return wl::fail(WL_EINVAL, "wl_kv4_read: T must not be negative");
+        if (const int32_t st = kv4_shape("wl_kv4_read", kv_heads, kv_heads, head_dim, capacity)) return st;
+        if (!dev_caches || !dev_pos || !dev_k || !dev_v) return wl::fail(WL_EINVAL, "wl_kv4_read: null pointer");
+        if (T == 0) return WL_OK;
+        WL_CHECK_BUFFERS("wl_kv4_read", {dev_k, "dev_k"}, {dev_v, "dev_v"});
+        wl::k::kv4_read(wl::k::Kv4Cache{dev_caches, 8, 0}, dev_pos, T, kv_heads, head_dim, capacity, dev_k, dev_v, (cudaStream_t)stream);
+        return WL_OK;
+    });
+}
+
+namespace {
+int32_t kv4_attention_args(const char* name, int32_t T, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                           int64_t capacity, int32_t window, int32_t sinks)
+{
+    if (T < 0) return wl::fail(WL_EINVAL, std::string(name) + ": T must not be negative");
+    if (const int32_t st = kv4_shape(name, heads, kv_heads, head_dim, capacity)) return st;
+    if (rows_per_seq <= 0 || T % rows_per_seq) return wl::fail(WL_EINVAL, std::string(name) + ": T must be a multiple of rows_per_seq");
+    if (window < 0 || sinks < 0) return wl::fail(WL_EINVAL, std::string(name) + ": window and sinks must not be negative");
+    return WL_OK;
+}
+}  // namespace
+
+int32_t wl_kv4_workspace_bytes(int32_t T, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                               int64_t capacity, int32_t window, int32_t sinks, int64_t* bytes)
+{
+    return guarded([&]() -> int32_t {
+        if (!bytes) return wl::fail(WL_EINVAL, "wl_kv4_workspace_bytes: null pointer");
+        if (const int32_t st = kv4_attention_args("wl_kv4_workspace_bytes", T, rows_per_seq, heads, kv_heads, head_dim, capacity, window, sinks)) return st;
+        *bytes = wl::k::kv4_workspace_bytes(T, rows_per_seq, heads, kv_heads, head_dim, capacity, window, sinks);
+        return WL_OK;
+    });
+}
+
+int32_t wl_kv4_workspace_init(void* dev_workspace, int64_t workspace_bytes, void* stream)
+{
+    return guarded([&]() -> int32_t {
+        if (!dev_workspace) return wl::fail(WL_EINVAL, "wl_kv4_workspace_init: null pointer");
+        if (workspace_bytes < (int64_t)wl::k::kv4_ticket_bytes()) return wl::fail(WL_EINVAL, "wl_kv4_workspace_init: the workspace is too small");
+        WL_CUDA(cudaMemsetAsync(dev_workspace, 0, wl::k::kv4_ticket_bytes(), (cudaStream_t)stream));
+        return WL_OK;
+    });
+}
+
+int32_t wl_kv4_attention(const float* dev_q, int32_t T, int32_t rows_per_seq, int32_t heads, int32_t kv_heads,
+                         int32_t head_dim, float scale, void* const* dev_caches, const int32_t* dev_pos, int64_t capacity,
+                         int32_t window, int32_t sinks, float* dev_out, void* dev_workspace, int64_t workspace_bytes,
+                         void* stream)
+{
+    return guarded([&]() -> int32_t {
+        if (const int32_t st = kv4_attention_args("wl_kv4_attention", T, rows_per_seq, heads, kv_heads, head_dim, capacity, window, sinks)) return st;
+        if (!dev_q || !dev_caches || !dev_pos || !dev_out || !dev_workspace) return wl::fail(WL_EINVAL, "wl_kv4_attention: null pointer");
+        if (workspace_bytes < wl::k::kv4_workspace_bytes(T, rows_per_seq, heads, kv_heads, head_dim, capacity, window, sinks))
+            return wl::fail(WL_EINVAL, "wl_kv4_attention: the workspace is too small (wl_kv4_workspace_bytes)");
+        if (T == 0) return WL_OK;
+        WL_CHECK_BUFFERS("wl_kv4_attention", {dev_q, "dev_q"}, {dev_out, "dev_out"}, {dev_workspace, "dev_workspace"});
+        wl::k::kv4_attention(dev_q, T, rows_per_seq, heads, kv_heads, head_dim, scale, wl::k::Kv4Cache{dev_caches, 8, 0}, dev_pos,
+                             capacity, window, sinks, dev_out, dev_workspace, (int*)wl::k::static_scratch(), (cudaStream_t)stream);
         return WL_OK;
     });
 }

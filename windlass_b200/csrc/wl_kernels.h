@@ -293,5 +293,27 @@ void shared_expert_add(float* outp, const float* sh, const float* gl, int T, int
 void synth(int type, uint64_t seed, uint32_t tid, int64_t rows, int64_t cols, float sigma, float offset, uint8_t* out,
            cudaStream_t s);
 
+// ---- the 4-bit KV cache (wl_kv4.cu) ----
+// Where the rows' caches are: with pitch = sizeof(RowKV), RowKV entries (keys and values share one cache at k, layer l at
+// k + l * layer_stride); with pitch = 8, an array of cache pointers.
+struct Kv4Cache {
+    const void* rows;
+    int pitch, layer;
+};
+bool kv4_supported(int heads, int kv_heads, int head_dim);
+// Bytes of one layer's cache of one sequence of `positions` positions.
+int64_t kv4_bytes(int kv_heads, int head_dim, int64_t positions);
+void kv4_append(const float* q, float* q_out, const float* k, const float* v, int T, int heads, int kv_heads, int head_dim,
+                const float* table, int rope_dims, int neox, const Kv4Cache& cache, const int32_t* pos, int64_t capacity,
+                cudaStream_t s);
+void kv4_read(const Kv4Cache& cache, const int32_t* pos, int T, int kv_heads, int head_dim, int64_t capacity, void* k, void* v,
+              cudaStream_t s);
+// Attention of T rows, R consecutive rows reading one cache (1: each its own). ws: kv4_workspace_bytes, its first
+// kv4_ticket_bytes() zero before the first call.
+int64_t kv4_workspace_bytes(int T, int R, int heads, int kv_heads, int head_dim, int64_t capacity, int window, int sinks);
+size_t kv4_ticket_bytes();
+void kv4_attention(const float* q, int T, int R, int heads, int kv_heads, int head_dim, float scale, const Kv4Cache& cache,
+                   const int32_t* pos, int64_t capacity, int window, int sinks, float* out, void* ws, int* err, cudaStream_t s);
+
 }  // namespace k
 }  // namespace wl

@@ -1,0 +1,1003 @@
+// The 4-bit KV cache: rotary append, read-back and attention (whole context, or a sliding window with sinks).
+//
+// Values. A key or value head is cut into blocks of 32. A block keeps an fp16 scale d = m / -8, m its value of largest
+// magnitude (the positive one of a pair), and 32 codes c = clamp(floor(x / d + 8.5), 0, 15); it stands for (c - 8) d
+// (the values of a Q4_0 block). A block that holds an infinity or a NaN gets d = NaN and reads as NaN.
+//
+// Layout. A cache is an array of tiles [position / 16][kv head], each 18 * HD bytes: the keys' codes (8 HD bytes), the
+// values' codes (8 HD), the keys' scales [16][HD / 32] and the values' scales [16][HD / 32]. One 1-D bulk copy brings a
+// tile, and the codes lie in the order in which the MMA fragments read them, so that a lane's 16-byte shared-memory
+// loads are its fragments and nothing is shuffled. With NB = HD / 32 blocks and W = min(4, NB), a code area is planes
+// of 4 blocks, each [half][lane = 4 g + c][W] 32-bit words:
+//   keys:   word (half, g, c, b) = position 8 half + g, dims 32 b + 8 c + 0..7 in nibbles 0..7;
+//   values: word (half, g, c, b) = positions 8 half + 2 c (low 16 bits) and + 1 (high), dims 32 b + 4 g + 0..3.
+//
+// Attention. The query heads of one KV head share its codes: a tile of 8 queries (heads of a row, or rows of a prompt)
+// is the 16-row side of m16n8k16 MMAs, each query twice: rows 0-7 its values' fp16 roundings, rows 8-15 what the
+// roundings left (together 22 bits of the row's largest value). Codes become fp16 integers -8..7 exactly (a mask and
+// an OR put a nibble below 1024's exponent, a subtraction takes the 1024 off: 9 instructions for 8 codes), products are
+// exact, sums fp32; the block scales are applied outside: to each block's fp32 sums for the scores, and to the weights
+// before they are split for the values (p * d, per block). So the codes' rounding is the only one below fp32.
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+#include <cuda_fp16.h>
+#include "wl_common.h"
+#include "wl_kernels.h"
+#include "wl_launch.cuh"
+#include "wl_mma.cuh"
+
+namespace wl {
+namespace k {
+
+namespace {
+
+constexpr int KV4_P = 16;                   // positions per tile
+constexpr int kv4_tile_bytes(int HD) { return 18 * HD; }
+
+// Cache of row t: its base pointer (a RowKV with a layer offset, or a bare array of pointers).
+struct Kv4Rows {
+    const uint8_t* p;
+    int pitch, layer;
+    __device__ __forceinline__ uint8_t* base(int t) const
+    {
+        const uint8_t* e = p + (int64_t)t * pitch;
+        uint8_t* b = *reinterpret_cast<uint8_t* const*>(e);
+        if (pitch == (int)sizeof(RowKV)) b += (int64_t)layer * reinterpret_cast<const RowKV*>(e)->layer_stride * 2;
+        return b;
+    }
+};
+
+// A row's state: 0 live, 1 padding (position < 0: nothing is read or written for it), 2 refused (a position past the
+// cache, a null or misaligned cache).
+__device__ __forceinline__ int kv4_row_state(const uint8_t* base, int64_t p, int64_t capacity)
+{
+    if (p < 0) return 1;
+    return p >= capacity || !base || ((uintptr_t)base & 15) ? 2 : 0;
+}
+
+// Word index of (half, lane, block) in a code area.
+template <int HD> __device__ __forceinline__ int kv4_word(int half, int lane, int b)
+{
+    constexpr int NB = HD / 32, W = NB < 4 ? NB : 4;
+    return (b >> 2) * 256 + (half * 32 + lane) * W + (b & 3);
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// append and read
+// ------------------------------------------------------------------------------------------------------------------
+// A thread owns 8 consecutive dims of one head; four threads a block of 32. The rotation of k and the codes are
+// computed in 64 bits: a code's border is a step of the value, so a difference in the last bit of 32 would decide
+// codes, and 64-bit arithmetic costs nothing here (about 30 operations a value against the bytes a row moves).
+template <int HD>
+__global__ void __launch_bounds__(128) k_kv4_append(const float* q, float* q_out, const float* k, const float* v, int T,
+                                                    int heads, int kv_heads, const float* table, int rope_dims, int neox,
+                                                    Kv4Rows rows, const int32_t* pos, int64_t capacity, int q_blocks)
+{
+    constexpr int CH = HD / 8;              // 8-dim chunks of a head
+    pdl_trigger();
+    pdl_wait();
+    const int half = rope_dims / 2;
+    for (int t = blockIdx.y; t < T; t += gridDim.y) {
+        const int p = pos[t];
+        uint8_t* base = rows.base(t);
+        if (kv4_row_state(base, p, capacity)) continue;
+        const float* cs = table + (int64_t)p * rope_dims;
+        if ((int)blockIdx.x < q_blocks) {
+            const int u = blockIdx.x * 128 + threadIdx.x;
+            if (u >= heads * CH) continue;
+            const int d0 = u % CH * 8;
+            const float* x = q + ((int64_t)t * heads + u / CH) * HD;
+            float* y = q_out + ((int64_t)t * heads + u / CH) * HD;
+            if (d0 >= rope_dims) {
+                if (q_out != q) {
+                    *reinterpret_cast<float4*>(y + d0) = *reinterpret_cast<const float4*>(x + d0);
+                    *reinterpret_cast<float4*>(y + d0 + 4) = *reinterpret_cast<const float4*>(x + d0 + 4);
+                }
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int d = d0 + e;
+                if (d >= rope_dims) {
+                    if (q_out != q) y[d] = x[d];
+                    continue;
+                }
+                // the thread of a pair's first dim writes both, so that rotating in place never reads a rotated value
+                const bool first = neox ? d < half : (d & 1) == 0;
+                if (!first) continue;
+                const int i = neox ? d : d >> 1, d1 = neox ? d + half : d + 1;
+                const float c = cs[2 * i], sn = cs[2 * i + 1], x0 = x[d], x1 = x[d1];
+                y[d] = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, sn));
+                y[d1] = __fadd_rn(__fmul_rn(x0, sn), __fmul_rn(x1, c));
+            }
+            continue;
+        }
+        const int u = ((int)blockIdx.x - q_blocks) * 128 + threadIdx.x;
+        const int units = kv_heads * CH;
+        const bool live = u < 2 * units, is_v = u >= units;
+        const int uu = live ? (is_v ? u - units : u) : 0;
+        const int h = uu / CH, d0 = uu % CH * 8;
+        const float* x = (is_v ? v : k) + ((int64_t)t * kv_heads + h) * HD;
+        float xf[8];
+        *reinterpret_cast<float4*>(xf) = *reinterpret_cast<const float4*>(x + d0);
+        *reinterpret_cast<float4*>(xf + 4) = *reinterpret_cast<const float4*>(x + d0 + 4);
+        double xd[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            xd[e] = xf[e];
+            const int d = d0 + e;
+            if (!is_v && d < rope_dims) {
+                const bool first = neox ? d < half : (d & 1) == 0;
+                const int i = neox ? (first ? d : d - half) : d >> 1;
+                const double c = cs[2 * i], sn = cs[2 * i + 1];
+                const double o = neox ? (double)x[first ? d + half : d - half] : (double)xf[e ^ 1];
+                // products of 24-bit factors are exact in 53 bits, so one rounding follows either way
+                xd[e] = first ? xd[e] * c - o * sn : o * sn + xd[e] * c;
+            }
+        }
+        double hi = xd[0], lo = xd[0];
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            hi = xd[e] > hi ? xd[e] : hi;
+            lo = xd[e] < lo ? xd[e] : lo;
+            bad |= !(fabs(xd[e]) <= 1.7e308);
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            const double a = __shfl_xor_sync(0xffffffffu, hi, o), b = __shfl_xor_sync(0xffffffffu, lo, o);
+            hi = a > hi ? a : hi;
+            lo = b < lo ? b : lo;
+        }
+        bad = (__ballot_sync(0xffffffffu, bad) >> (threadIdx.x & 28)) & 15u;
+        const double m = hi >= -lo ? hi : lo;
+        float df = (float)(m / -8.0);
+        df = fminf(fmaxf(df, -65504.f), 65504.f);       // a scale past fp16's largest saturates
+        const __half dh = bad ? __ushort_as_half((unsigned short)0x7e00) : __float2half_rn(df);
+        const double dd = (double)__half2float(dh), inv = dd != 0.0 ? 1.0 / dd : 0.0;
+        uint32_t w = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const double c = floor(__dadd_rn(__dmul_rn(xd[e], inv), 8.5));
+            w |= (uint32_t)(c >= 15.0 ? 15 : c > 0.0 ? (int)c : 0) << (4 * e);      // (a NaN gives 0)
+        }
+        if (!live) continue;
+        uint8_t* tile = base + ((int64_t)(p >> 4) * kv_heads + h) * kv4_tile_bytes(HD);
+        const int b = d0 >> 5, c4 = d0 >> 3 & 3, r = p & 15;
+        if (!is_v) {
+            reinterpret_cast<uint32_t*>(tile)[kv4_word<HD>(r >> 3, (r & 7) * 4 + c4, b)] = w;
+        } else {
+            // dims 8 c4 .. +3 and + 4 .. +7 are g = 2 c4 and 2 c4 + 1
+            uint16_t* vw = reinterpret_cast<uint16_t*>(tile + 8 * HD);
+            const int lane = (r & 7) >> 1;
+            vw[2 * kv4_word<HD>(r >> 3, 8 * c4 + lane, b) + (r & 1)] = (uint16_t)w;
+            vw[2 * kv4_word<HD>(r >> 3, 8 * c4 + 4 + lane, b) + (r & 1)] = (uint16_t)(w >> 16);
+        }
+        if (c4 == 0)
+            reinterpret_cast<__half*>(tile + (is_v ? 17 : 16) * HD)[r * (HD / 32) + b] = dh;
+    }
+}
+
+// The fp16 values that position pos[t] of row t's cache stands for; zeros for a padding row, NaN for a refused one.
+template <int HD>
+__global__ void __launch_bounds__(128) k_kv4_read(Kv4Rows rows, const int32_t* pos, int T, int kv_heads, int64_t capacity,
+                                                  __half* k_out, __half* v_out)
+{
+    constexpr int CH = HD / 8;
+    pdl_trigger();
+    pdl_wait();
+    const int units = kv_heads * CH;
+    const int u = blockIdx.x * 128 + threadIdx.x;
+    if (u >= 2 * units) return;
+    const bool is_v = u >= units;
+    const int uu = is_v ? u - units : u, h = uu / CH, d0 = uu % CH * 8, b = d0 >> 5, c4 = d0 >> 3 & 3;
+    for (int t = blockIdx.y; t < T; t += gridDim.y) {
+        const int p = pos[t];
+        const uint8_t* base = rows.base(t);
+        const int st = kv4_row_state(base, p, capacity);
+        __half out[8];
+        if (st) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out[e] = st == 1 ? __half(__ushort_as_half((unsigned short)0)) : __half(__ushort_as_half((unsigned short)0x7e00));
+        } else {
+            const uint8_t* tile = base + ((int64_t)(p >> 4) * kv_heads + h) * kv4_tile_bytes(HD);
+            const int r = p & 15;
+            uint32_t w;
+            if (!is_v) {
+                w = reinterpret_cast<const uint32_t*>(tile)[kv4_word<HD>(r >> 3, (r & 7) * 4 + c4, b)];
+            } else {
+                const uint16_t* vw = reinterpret_cast<const uint16_t*>(tile + 8 * HD);
+                const int lane = (r & 7) >> 1;
+                w = (uint32_t)vw[2 * kv4_word<HD>(r >> 3, 8 * c4 + lane, b) + (r & 1)] |
+                    (uint32_t)vw[2 * kv4_word<HD>(r >> 3, 8 * c4 + 4 + lane, b) + (r & 1)] << 16;
+            }
+            const float d = __half2float(reinterpret_cast<const __half*>(tile + (is_v ? 17 : 16) * HD)[r * (HD / 32) + b]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out[e] = __float2half_rn((float)((int)(w >> (4 * e) & 15u) - 8) * d);
+        }
+        *reinterpret_cast<uint4*>((is_v ? v_out : k_out) + ((int64_t)t * kv_heads + h) * HD + d0) = *reinterpret_cast<uint4*>(out);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// attention
+// ------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void mma_zero(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%10,%10,%10,%10};\n"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Eight 4-bit codes to four fp16 pairs of c - 8: nibbles (0, 4), (1, 5), (2, 6), (3, 7).
+__device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&r)[4])
+{
+    const __half2 m1032 = __floats2half2_rn(1032.f, 1032.f), s16 = __floats2half2_rn(0.0625f, 0.0625f),
+                  m72 = __floats2half2_rn(-72.f, -72.f);
+    const uint32_t w8 = w >> 8;
+    r[0] = h2_bits(__hsub2(bits_h2((w & 0x000F000Fu) | 0x64006400u), m1032));
+    r[1] = h2_bits(__hfma2(bits_h2((w & 0x00F000F0u) | 0x64006400u), s16, m72));
+    r[2] = h2_bits(__hsub2(bits_h2((w8 & 0x000F000Fu) | 0x64006400u), m1032));
+    r[3] = h2_bits(__hfma2(bits_h2((w8 & 0x00F000F0u) | 0x64006400u), s16, m72));
+}
+
+// fp16 roundings of a pair and of what they leave.
+__device__ __forceinline__ void split_h2(float a, float b, uint32_t& hi, uint32_t& lo)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    hi = h2_bits(h);
+    lo = h2_bits(__floats2half2_rn(a - f.x, b - f.y));
+}
+
+// The words of one lane's fragments: NB consecutive (planes of 4) 32-bit words.
+template <int HD> __device__ __forceinline__ void lane_words(const uint8_t* area, int half, int lane, uint32_t (&w)[HD / 32])
+{
+    constexpr int NB = HD / 32;
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(area);
+    if constexpr (NB == 2) {
+        const uint2 x = lds64(p + (half * 32 + lane) * 2);
+        w[0] = x.x; w[1] = x.y;
+    } else if constexpr (NB == 3) {
+#pragma unroll
+        for (int b = 0; b < 3; ++b) w[b] = p[(half * 32 + lane) * 3 + b];
+    } else {
+#pragma unroll
+        for (int pl = 0; pl < NB / 4; ++pl) {
+            const uint4 x = lds128(p + pl * 256 + (half * 32 + lane) * 4);
+            w[4 * pl] = x.x; w[4 * pl + 1] = x.y; w[4 * pl + 2] = x.z; w[4 * pl + 3] = x.w;
+        }
+    }
+}
+
+// The scales of positions r, r + 1 (r even): NB fp16 pairs' words, position-major.
+template <int HD> __device__ __forceinline__ void lane_scales(const uint8_t* area, int r, uint32_t (&w)[HD / 32])
+{
+    constexpr int NB = HD / 32;
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(area) + r * NB / 2;
+    if constexpr (NB == 2) {
+        const uint2 x = lds64(p);
+        w[0] = x.x; w[1] = x.y;
+    } else if constexpr (NB == 3) {
+#pragma unroll
+        for (int b = 0; b < 3; ++b) w[b] = p[b];
+    } else {
+#pragma unroll
+        for (int i = 0; i < NB / 4; ++i) {
+            const uint4 x = lds128(p + 4 * i);
+            w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+        }
+    }
+}
+// Scale b of position e (0, 1) of those words.
+template <int NB> __device__ __forceinline__ float scale_of(const uint32_t (&w)[NB], int e, int b)
+{
+    const int i = e * NB + b;
+    const float2 f = __half22float2(bits_h2(w[i >> 1]));
+    return i & 1 ? f.y : f.x;
+}
+
+// One query's visible positions: j < n and (j >= first or j < sink).
+struct Vis {
+    int n, first, sink;
+    __device__ __forceinline__ bool operator()(int j) const { return j < n && (j >= first || j < sink); }
+};
+__device__ __forceinline__ Vis visible(int p, int window, int sinks)
+{
+    const int n = p + 1, first = window > 0 && n > window ? n - window : 0;
+    return Vis{n, first, min(sinks, first)};
+}
+
+// The tiles that hold positions of [0, sink) or [first, n): item i of the list is tile i below head, else i + skip.
+struct TileList {
+    int head, skip, count;
+    __device__ __forceinline__ int at(int i) const { return i < head ? i : i + skip; }
+};
+__device__ __forceinline__ TileList tile_list(int n, int first, int sink)
+{
+    const int t1 = first >> 4, head = min((sink + 15) >> 4, t1), last = (n - 1) >> 4;
+    return TileList{head, t1 - head, n > 0 ? head + last - t1 + 1 : 0};
+}
+
+// Running softmax of MT tiles of 8 queries: lane (g, c) keeps query g's maximum (in log2 units), its own share of the
+// sum, and the output's fragments (o[.][0,1] the rows of the weights' roundings, [2,3] of what they left).
+template <int HD, int MT> struct AttState {
+    float m[MT], l[MT], o[MT][HD / 8][4];
+    float vs, vlim;             // the values' scales are multiplied by vs = 2^k while all are at most vlim = 2^(15-k)
+    __device__ __forceinline__ void init()
+    {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+#pragma unroll
+            for (int j = 0; j < HD / 8; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
+        }
+        vs = 32768.f;
+        vlim = 1.f;
+    }
+};
+
+// One tile of 16 positions for MT query tiles. qf(i, b, s) gives the A fragment of query tile i, block b, step s (dims
+// 32 b + 8 c + {2s, 2s + 4, 2s + 1, 2s + 5} of lane c); ks[i] undoes the queries' power of two.
+template <int HD, int MT, class QF>
+__device__ __forceinline__ void kv4_tile(const uint8_t* sm, int lane, int tile0, const Vis (&vis)[MT], bool full, const QF& qf,
+                                         const float (&ks)[MT], AttState<HD, MT>& st)
+{
+    constexpr int NB = HD / 32;
+    const int c = lane & 3;
+    float s[MT][4];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        uint32_t kw[NB], dw[NB];
+        lane_words<HD>(sm, half, lane, kw);
+        lane_scales<HD>(sm + 16 * HD, 8 * half + 2 * c, dw);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) s[i][2 * half] = s[i][2 * half + 1] = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            uint32_t r[4];
+            unpack8(kw[b], r);
+            const float d0 = scale_of<NB>(dw, 0, b), d1 = scale_of<NB>(dw, 1, b);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                float d[4];
+                mma_zero(d, qf(i, b, 0), r[0], r[1]);
+                const uint4 a = qf(i, b, 1);
+                mma16816(d, a.x, a.y, a.z, a.w, r[2], r[3]);
+                s[i][2 * half] += d0 * (d[0] + d[2]);
+                s[i][2 * half + 1] += d1 * (d[1] + d[3]);
+            }
+        }
+    }
+    // positions of s[.][0..3]: 2c, 2c + 1, 2c + 8, 2c + 9
+    uint32_t seen[MT], any_seen = 0u;       // bits of the positions that this lane's queries see
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][e] *= ks[i];
+        if (!full) {
+            seen[i] = 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (vis[i](tile0 + 2 * c + (e & 1) + 8 * (e >> 1))) seen[i] |= 1u << e;
+                else s[i][e] = -INFINITY;
+            }
+            any_seen |= seen[i];
+        }
+        float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(st.m[i], mx), mu = mn == -INFINITY ? 0.f : mn;
+        if (__any_sync(0xffffffffu, mn > st.m[i])) {
+            const float a = ex2(st.m[i] - mu);
+            st.l[i] *= a;
+#pragma unroll
+            for (int j = 0; j < HD / 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) st.o[i][j][e] *= a;
+            st.m[i] = mn;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            s[i][e] = ex2(s[i][e] - mu);
+            sum += s[i][e];
+        }
+        st.l[i] += sum;
+    }
+    uint32_t vd[2][NB], vw[2][NB];
+    lane_scales<HD>(sm + 17 * HD, 2 * c, vd[0]);
+    lane_scales<HD>(sm + 17 * HD, 2 * c + 8, vd[1]);
+    if (!full) {
+        // a position that no query of this lane sees may hold anything: its scales (perhaps NaN) count as zero
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int i = 0; i < 2 * NB; ++i)
+                if (!(any_seen >> (2 * hf + i / NB) & 1u)) vd[hf][i >> 1] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+    }
+    {
+        __half2 mx = __habs2(bits_h2(vd[0][0]));
+#pragma unroll
+        for (int i = 1; i < 2 * NB; ++i) mx = __hmax2(mx, __habs2(bits_h2(vd[i / NB][i % NB])));
+        float a = fmaxf(__low2float(mx), __high2float(mx));
+        if (__any_sync(0xffffffffu, a > st.vlim)) {
+            // larger scales than any so far: a smaller power of two, and the sums follow
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+            int e = 14 - ilogbf(a);
+            e = e < -1 ? -1 : e;
+            const float nv = ldexpf(1.f, e), f = nv / st.vs;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < HD / 8; ++j)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) st.o[i][j][x] *= f;
+            st.vs = nv;
+            st.vlim = ldexpf(1.f, 15 - e);
+        }
+        const __half2 v2 = __float2half2_rn(st.vs);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int i = 0; i < NB; ++i) vd[hf][i] = h2_bits(__hmul2(bits_h2(vd[hf][i]), v2));
+    }
+    lane_words<HD>(sm + 8 * HD, 0, lane, vw[0]);
+    lane_words<HD>(sm + 8 * HD, 1, lane, vw[1]);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        uint32_t r0[4], r1[4];
+        unpack8(vw[0][b], r0);
+        unpack8(vw[1][b], r1);
+        const float d0 = scale_of<NB>(vd[0], 0, b), d1 = scale_of<NB>(vd[0], 1, b), d2 = scale_of<NB>(vd[1], 0, b),
+                    d3 = scale_of<NB>(vd[1], 1, b);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            uint32_t a0, a1, a2, a3;
+            float p0 = s[i][0] * d0, p1 = s[i][1] * d1, p2 = s[i][2] * d2, p3 = s[i][3] * d3;
+            if (MT > 1 && !full) {          // (a scale that only the lane's other queries see may be NaN)
+                p0 = seen[i] & 1u ? p0 : 0.f;
+                p1 = seen[i] & 2u ? p1 : 0.f;
+                p2 = seen[i] & 4u ? p2 : 0.f;
+                p3 = seen[i] & 8u ? p3 : 0.f;
+            }
+            split_h2(p0, p1, a0, a1);
+            split_h2(p2, p3, a2, a3);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma16816(st.o[i][4 * b + j], a0, a1, a2, a3, r0[j], r1[j]);
+        }
+    }
+}
+
+// The A fragments of lane (g, c)'s query row (nullptr: zeros): qa[b][s]. Returns the factor that undoes the power of
+// two which brings the row's largest value to 2^13..2^14, where fp16 and its remainder keep 22 bits.
+template <int HD> __device__ __forceinline__ float load_query(const float* x, int lane, float f, uint4 (&qa)[HD / 32][2])
+{
+    constexpr int NB = HD / 32;
+    const int c = lane & 3;
+    float v[NB][8];
+    float mx = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+        if (x) {
+            lo = *reinterpret_cast<const float4*>(x + 32 * b + 8 * c);
+            hi = *reinterpret_cast<const float4*>(x + 32 * b + 8 * c + 4);
+        }
+        const float y[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[b][e] = y[e] * f;
+            mx = fmaxf(mx, fabsf(v[b][e]));
+        }
+    }
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    int e = mx > 0.f && mx <= 3e38f ? 13 - ilogbf(mx) : 0;
+    e = e > 100 ? 100 : e < -100 ? -100 : e;
+    const float up = ldexpf(1.f, e);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            split_h2(v[b][2 * s] * up, v[b][2 * s + 4] * up, qa[b][s].x, qa[b][s].y);
+            split_h2(v[b][2 * s + 1] * up, v[b][2 * s + 5] * up, qa[b][s].z, qa[b][s].w);
+        }
+    return ldexpf(1.f, -e);
+}
+
+struct Kv4Att {
+    const float* q;
+    float* out;
+    Kv4Rows rows;
+    const int32_t* pos;
+    int64_t capacity;
+    int T, R, heads, kv_heads, S, s_max;    // S: ranges a row may be cut into (the stride of the partials)
+    float scale;
+    int window, sinks;
+    float* part;                            // [T][heads][S][HD]
+    float* ml;                              // [T][heads][S][2]: maximum (log2 units), sum
+    int* tickets;
+    int* err;
+};
+
+constexpr int ATT_WARPS = 4;                // warps of an attention CTA
+constexpr int ATT_TPS = 16;                 // tiles a range holds at least (when a row has more than one)
+constexpr int att_stages(int HD) { return HD <= 128 ? 4 : 3; }
+
+// Joins the `n` ranges of (row t, head) for 4 output values at dim d, in range order.
+template <int HD>
+__device__ __forceinline__ float4 join_ranges(const Kv4Att& a, int64_t th, int n, int d)
+{
+    const float2* ml = reinterpret_cast<const float2*>(a.ml) + th * a.S;
+    const float* pp = a.part + th * a.S * HD + d;
+    float M = -INFINITY;
+    for (int s = 0; s < n; ++s) M = fmaxf(M, __ldcg(ml + s).x);
+    const float mu = M == -INFINITY ? 0.f : M;
+    float L = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+        const float2 x = __ldcg(ml + s);
+        const float4 p = __ldcg(reinterpret_cast<const float4*>(pp + (int64_t)s * HD));
+        const float w = ex2(x.x - mu);
+        L += w * x.y;
+        o0 += w * p.x;
+        o1 += w * p.y;
+        o2 += w * p.z;
+        o3 += w * p.w;
+    }
+    const float inv = L != 0.f ? 1.f / L : 0.f;     // (a NaN sum stays NaN; no visible position: zeros)
+    return make_float4(o0 * inv, o1 * inv, o2 * inv, o3 * inv);
+}
+
+// Takes a ticket after the CTA's partials; true in the CTA that took the last of n.
+__device__ __forceinline__ bool last_ticket(int* ctr, int n)
+{
+    __shared__ int last;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int ticket;
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(ticket) : "l"(ctr) : "memory");
+        last = ticket == n - 1;
+        if (last) *ctr = 0;
+    }
+    __syncthreads();
+    return last;
+}
+
+// Rows on their own (decode): CTA (range, KV head and tile of 8 query heads, row); each warp streams its own tiles, every
+// fourth of the range, through its ring of bulk copies, and the warps' sums are joined in warp order. The ranges follow
+// from the row's own length, so a row's bits do not depend on the other rows.
+template <int HD>
+__global__ void __launch_bounds__(32 * ATT_WARPS, HD <= 128 ? 3 : 2) k_kv4_attn(const Kv4Att a)
+{
+    constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD), ST = att_stages(HD), NT = 32 * ATT_WARPS;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ __align__(8) uint64_t bars[ATT_WARPS][ST];
+    __shared__ float sm_m[ATT_WARPS][8], sm_l[ATT_WARPS][8];
+    pdl_trigger();
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int G = a.heads / a.kv_heads, MG = (G + 7) / 8;
+    const int kvh = blockIdx.y / MG, mg = blockIdx.y % MG, t = blockIdx.z, sp = blockIdx.x;
+    const int nh = min(8, G - 8 * mg), head0 = kvh * G + 8 * mg;
+    const int p = a.pos[t];
+    const uint8_t* base = a.rows.base(t);
+    const int state = kv4_row_state(base, p, a.capacity);
+    if (state) {
+        if (sp == 0)
+            for (int i = threadIdx.x; i < nh * HD; i += NT)
+                a.out[((int64_t)t * a.heads + head0) * HD + i] = state == 1 ? 0.f : NAN;
+        return;
+    }
+    const Vis vis[1] = {visible(p, a.window, a.sinks)};
+    const TileList tl = tile_list(vis[0].n, vis[0].first, vis[0].sink);
+    const int S = min(a.s_max, (tl.count + ATT_TPS - 1) / ATT_TPS);
+    if (sp >= S) return;
+    const int i0 = (int)((int64_t)tl.count * sp / S), i1 = (int)((int64_t)tl.count * (sp + 1) / S);
+    const int mine = (i1 - i0 - warp + ATT_WARPS - 1) / ATT_WARPS;      // tiles i0 + warp, + 4, ...
+    uint8_t* ring = smem + warp * ST * TB;
+    const uint8_t* src = base + (int64_t)kvh * TB;
+    auto issue = [&](int i) {
+        uint64_t* bar = &bars[warp][i % ST];
+        mbar_expect_tx(bar, TB);
+        bulk_load(ring + i % ST * TB, src + (int64_t)tl.at(i0 + warp + ATT_WARPS * i) * a.kv_heads * TB, TB, bar);
+    };
+    if (lane == 0) {
+        for (int s = 0; s < ST; ++s) mbar_init(&bars[warp][s], 1);
+        fence_mbar_init();
+        for (int s = 0; s < ST && s < mine; ++s) issue(s);
+    }
+    uint4 qa[NB][2];
+    const float ks[1] = {load_query<HD>(g < nh ? a.q + ((int64_t)t * a.heads + head0 + g) * HD : nullptr, lane,
+                                        a.scale * 1.4426950408889634f, qa)};
+    __syncwarp();
+    AttState<HD, 1> st;
+    st.init();
+    auto qf = [&](int, int b, int s) { return qa[b][s]; };
+    for (int i = 0; i < mine; ++i) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bars[warp][i % ST], (uint32_t)(i / ST & 1), a.err, 21))) break;
+        const int tile0 = tl.at(i0 + warp + ATT_WARPS * i) * KV4_P;
+        const bool full = tile0 + KV4_P <= vis[0].n && tile0 >= vis[0].first;
+        kv4_tile<HD, 1>(ring + i % ST * TB, lane, tile0, vis, full, qf, ks, st);
+        __syncwarp();
+        if (lane == 0 && i + ST < mine) issue(i + ST);
+    }
+    // the warps' sums, joined through the ring's memory (every copy has landed and been read)
+    st.l[0] += __shfl_xor_sync(0xffffffffu, st.l[0], 1);
+    st.l[0] += __shfl_xor_sync(0xffffffffu, st.l[0], 2);
+    __syncthreads();
+    float* so = reinterpret_cast<float*>(smem);
+    const float undo = 1.f / st.vs;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float4 v;
+            v.x = (st.o[0][4 * b][e] + st.o[0][4 * b][e + 2]) * undo;
+            v.y = (st.o[0][4 * b + 1][e] + st.o[0][4 * b + 1][e + 2]) * undo;
+            v.z = (st.o[0][4 * b + 2][e] + st.o[0][4 * b + 2][e + 2]) * undo;
+            v.w = (st.o[0][4 * b + 3][e] + st.o[0][4 * b + 3][e + 2]) * undo;
+            *reinterpret_cast<float4*>(so + (warp * 8 + g) * HD + 32 * b + 8 * c + 4 * e) = v;
+        }
+    if (c == 0) {
+        sm_m[warp][g] = st.m[0];
+        sm_l[warp][g] = st.l[0];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < nh * HD / 4; i += NT) {
+        const int h = i / (HD / 4), d = i % (HD / 4) * 4;
+        float M = sm_m[0][h];
+#pragma unroll
+        for (int w = 1; w < ATT_WARPS; ++w) M = fmaxf(M, sm_m[w][h]);
+        const float mu = M == -INFINITY ? 0.f : M;
+        float L = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < ATT_WARPS; ++w) {
+            const float f = ex2(sm_m[w][h] - mu);
+            const float4 x = *reinterpret_cast<const float4*>(so + (w * 8 + h) * HD + d);
+            L += f * sm_l[w][h];
+            o.x += f * x.x;
+            o.y += f * x.y;
+            o.z += f * x.z;
+            o.w += f * x.w;
+        }
+        const int64_t th = (int64_t)t * a.heads + head0 + h;
+        if (S == 1) {
+            const float inv = 1.f / L;
+            *reinterpret_cast<float4*>(a.out + th * HD + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        } else {
+            *reinterpret_cast<float4*>(a.part + (th * a.S + sp) * HD + d) = o;
+            if (d == 0) reinterpret_cast<float2*>(a.ml)[th * a.S + sp] = make_float2(M, L);
+        }
+    }
+    if (S == 1) return;
+    if (!last_ticket(a.tickets + t * gridDim.y + blockIdx.y, S)) return;
+    for (int i = threadIdx.x; i < nh * HD / 4; i += NT) {
+        const int h = i / (HD / 4), d = i % (HD / 4) * 4;
+        const int64_t th = (int64_t)t * a.heads + head0 + h;
+        *reinterpret_cast<float4*>(a.out + th * HD + d) = join_ranges<HD>(a, th, S, d);
+    }
+}
+
+// Runs of R rows that read one cache (prompts): the (row, head) pairs of a run and KV head are queries 0 .. R G - 1; a CTA
+// takes QB of them, each warp MT tiles of 8, and all warps share each tile of the cache (one ring of bulk copies), so
+// a tile's codes are unpacked once for 8 MT queries.
+template <int HD, int MT>
+__global__ void __launch_bounds__(32 * ATT_WARPS, 2) k_kv4_attn_run(const Kv4Att a, int q_blocks)
+{
+    constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD), ST = 4, QW = 8 * MT, QB = ATT_WARPS * QW;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ __align__(8) uint64_t fullb[ST], emptyb[ST];
+    __shared__ int rng[4];
+    uint4* sq = reinterpret_cast<uint4*>(smem + ST * TB);       // [warp][MT][NB][2][32]
+    pdl_trigger();
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int G = a.heads / a.kv_heads, kvh = blockIdx.y;
+    // the last queries (of a prompt: those that see most) first
+    const int qb = q_blocks - 1 - (int)blockIdx.x / a.S, sp = blockIdx.x % a.S, run = blockIdx.z;
+    const int nq = a.R * G, q0 = qb * QB;
+    const uint8_t* base = a.rows.base(run * a.R);
+    // the positions that the CTA's rows see together
+    if (threadIdx.x == 0) {
+        rng[0] = 0;
+        rng[1] = INT_MAX;
+        rng[2] = 0;
+    }
+    __syncthreads();
+    {
+        const int r0 = q0 / G, r1 = min(a.R - 1, (min(q0 + QB, nq) - 1) / G);
+        for (int r = r0 + threadIdx.x; r <= r1; r += 32 * ATT_WARPS) {
+            const int p = a.pos[run * a.R + r];
+            if (kv4_row_state(base, p, a.capacity)) continue;
+            const Vis v = visible(p, a.window, a.sinks);
+            atomicMax(&rng[0], v.n);
+            atomicMin(&rng[1], v.first);
+            atomicMax(&rng[2], v.sink);
+        }
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(&fullb[s], 1);
+            mbar_init(&emptyb[s], ATT_WARPS);
+        }
+        fence_mbar_init();
+    }
+    __syncthreads();
+    const TileList tl = rng[0] > 0 ? tile_list(rng[0], rng[1], rng[2]) : TileList{0, 0, 0};
+    const int S = a.S;
+    const int i0 = (int)((int64_t)tl.count * sp / S), i1 = (int)((int64_t)tl.count * (sp + 1) / S), nt = i1 - i0;
+    const uint8_t* src = base + (int64_t)kvh * TB;
+    auto issue = [&](int i) {
+        uint64_t* bar = &fullb[i % ST];
+        mbar_expect_tx(bar, TB);
+        bulk_load(smem + i % ST * TB, src + (int64_t)tl.at(i0 + i) * a.kv_heads * TB, TB, bar);
+    };
+    if (threadIdx.x == 0)
+        for (int s = 0; s < ST && s < nt; ++s) issue(s);
+    Vis vis[MT];
+    float ks[MT];
+    int state[MT];
+    int64_t th[MT];             // (row, head) of the lane's query, or -1
+    int w_n = 0, w_min_n = INT_MAX, w_first = INT_MAX, w_max_first = 0, w_sink = 0;
+    uint4* wq = sq + warp * MT * NB * 64;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int qi = q0 + warp * QW + 8 * i + g;
+        th[i] = -1;
+        state[i] = 1;
+        vis[i] = Vis{0, 0, 0};
+        if (qi < nq) {
+            const int t = run * a.R + qi / G;
+            th[i] = (int64_t)t * a.heads + kvh * G + qi % G;
+            const int p = a.pos[t];
+            state[i] = kv4_row_state(base, p, a.capacity);
+            if (!state[i]) vis[i] = visible(p, a.window, a.sinks);
+        }
+        uint4 qa[NB][2];
+        ks[i] = load_query<HD>(th[i] >= 0 ? a.q + th[i] * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) wq[((i * NB + b) * 2 + s) * 32 + lane] = qa[b][s];
+        if (vis[i].n > 0) {
+            w_n = max(w_n, vis[i].n);
+            w_min_n = min(w_min_n, vis[i].n);
+            w_first = min(w_first, vis[i].first);
+            w_max_first = max(w_max_first, vis[i].first);
+            w_sink = max(w_sink, vis[i].sink);
+        }
+        else w_min_n = 0;
+    }
+    w_n = __reduce_max_sync(0xffffffffu, w_n);
+    w_min_n = __reduce_min_sync(0xffffffffu, w_min_n);
+    w_first = __reduce_min_sync(0xffffffffu, w_first);
+    w_max_first = __reduce_max_sync(0xffffffffu, w_max_first);
+    w_sink = __reduce_max_sync(0xffffffffu, w_sink);
+    __syncwarp();
+    AttState<HD, MT> st;
+    st.init();
+    auto qf = [&](int i, int b, int s) { return wq[((i * NB + b) * 2 + s) * 32 + lane]; };
+    for (int i = 0; i < nt; ++i) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&fullb[i % ST], (uint32_t)(i / ST & 1), a.err, 22))) break;
+        const int tile0 = tl.at(i0 + i) * KV4_P;
+        if (tile0 < w_n && (tile0 + KV4_P > w_first || tile0 < w_sink)) {
+            const bool full = tile0 + KV4_P <= w_min_n && tile0 >= w_max_first;
+            kv4_tile<HD, MT>(smem + i % ST * TB, lane, tile0, vis, full, qf, ks, st);
+        }
+        __syncwarp();
+        bool ok = true;
+        if (lane == 0) {
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&emptyb[i % ST])) : "memory");
+            if (warp == 0 && i + ST < nt) {
+                ok = mbar_wait_bounded(&emptyb[i % ST], (uint32_t)(i / ST & 1), a.err, 23);
+                if (ok) issue(i + ST);
+            }
+        }
+        if (!__all_sync(0xffffffffu, ok)) break;
+    }
+    const float undo = 1.f / st.vs;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 1);
+        st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 2);
+        if (th[i] < 0) continue;
+        const bool whole = S == 1;
+        const float f = !whole ? undo : state[i] == 2 ? NAN : st.l[i] != 0.f ? undo / st.l[i] : 0.f;
+        float* dst = whole ? a.out + th[i] * HD : a.part + (th[i] * S + sp) * HD;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float4 v;
+                v.x = (st.o[i][4 * b][e] + st.o[i][4 * b][e + 2]) * f;
+                v.y = (st.o[i][4 * b + 1][e] + st.o[i][4 * b + 1][e + 2]) * f;
+                v.z = (st.o[i][4 * b + 2][e] + st.o[i][4 * b + 2][e + 2]) * f;
+                v.w = (st.o[i][4 * b + 3][e] + st.o[i][4 * b + 3][e + 2]) * f;
+                *reinterpret_cast<float4*>(dst + 32 * b + 8 * c + 4 * e) = v;
+            }
+        if (!whole && c == 0) reinterpret_cast<float2*>(a.ml)[th[i] * S + sp] = make_float2(st.m[i], state[i] == 2 ? NAN : st.l[i]);
+    }
+    if (S == 1) return;
+    if (!last_ticket(a.tickets + ((int64_t)run * a.kv_heads + kvh) * q_blocks + qb, S)) return;
+    for (int i = threadIdx.x; i < QB * HD / 4; i += 32 * ATT_WARPS) {
+        const int qi = q0 + i / (HD / 4), d = i % (HD / 4) * 4;
+        if (qi >= nq) break;
+        const int64_t x = ((int64_t)run * a.R + qi / G) * a.heads + kvh * G + qi % G;
+        *reinterpret_cast<float4*>(a.out + x * HD + d) = join_ranges<HD>(a, x, S, d);
+    }
+}
+
+constexpr int64_t KV4_TICKETS = 1 << 18;    // tickets at the head of a workspace (zero between calls)
+
+// How a call is cut.
+struct Kv4Plan {
+    bool runs;              // the rows' runs share their cache's tiles (k_kv4_attn_run)
+    int S, s_max, q_blocks, MT, MG;
+    int64_t part_floats;
+};
+
+Kv4Plan kv4_plan(int T, int R, int heads, int kv_heads, int head_dim, int64_t capacity, int window, int sinks)
+{
+    Kv4Plan p{};
+    const int G = heads / kv_heads;
+    p.MG = (G + 7) / 8;
+    int64_t tiles = (capacity + KV4_P - 1) / KV4_P;
+    if (window > 0) tiles = std::min<int64_t>(tiles, ((int64_t)window + 15) / 16 + 1 + ((int64_t)sinks + 15) / 16);
+    p.runs = R > 8;
+    p.MT = head_dim <= 128 ? 2 : 1;
+    const int QB = ATT_WARPS * 8 * p.MT;
+    p.q_blocks = (int)(((int64_t)R * G + QB - 1) / QB);
+    int64_t ctas;
+    if (p.runs) {
+        // as many ranges as fill the SMs twice, each of 16 tiles at least
+        ctas = (int64_t)(T / R) * p.q_blocks * kv_heads;
+        p.s_max = (int)std::max<int64_t>(1, std::min<int64_t>({32, tiles / ATT_TPS, (2 * 148 + ctas - 1) / ctas}));
+        p.S = p.s_max;
+    } else {
+        // the most ranges of one row, from the shape alone (a row's bits must not depend on the others): one row's
+        // CTAs fill the SMs three deep. Beyond 64 rows the rows alone do.
+        ctas = (int64_t)T * kv_heads * p.MG;
+        p.s_max = T > 64 ? 1 : std::max(1, std::min(64, 3 * 148 / (kv_heads * p.MG)));
+        p.S = (int)std::max<int64_t>(1, std::min<int64_t>(p.s_max, (tiles + ATT_TPS - 1) / ATT_TPS));
+    }
+    if (ctas > KV4_TICKETS) p.S = p.s_max = 1;
+    p.part_floats = p.S > 1 ? (int64_t)T * heads * p.S * (head_dim + 2) : 0;
+    return p;
+}
+
+template <typename K> void set_smem(K kern, size_t bytes)
+{
+    // (an attribute of the function on the current device; setting it again costs under a microsecond and is allowed
+    // during a capture)
+    if (bytes > 48 * 1024) WL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
+
+template <int HD> void attn_rows(const Kv4Att& a, const Kv4Plan& p, cudaStream_t s)
+{
+    const size_t smem = (size_t)ATT_WARPS * att_stages(HD) * kv4_tile_bytes(HD);
+    static_assert(ATT_WARPS * att_stages(HD) * kv4_tile_bytes(HD) >= ATT_WARPS * 8 * HD * 4, "the warps' sums fit the ring");
+    set_smem(k_kv4_attn<HD>, smem);
+    launch(k_kv4_attn<HD>, dim3(p.S, a.kv_heads * p.MG, a.T), dim3(32 * ATT_WARPS), smem, s, a);
+    note_launch();
+}
+
+template <int HD> void attn_runs(const Kv4Att& a, const Kv4Plan& p, cudaStream_t s)
+{
+    constexpr int MT = HD <= 128 ? 2 : 1;
+    const size_t smem = 4 * kv4_tile_bytes(HD) + (size_t)ATT_WARPS * MT * (HD / 32) * 2 * 512;
+    set_smem(k_kv4_attn_run<HD, MT>, smem);
+    launch(k_kv4_attn_run<HD, MT>, dim3(p.q_blocks * p.S, a.kv_heads, a.T / a.R), dim3(32 * ATT_WARPS), smem, s, a, p.q_blocks);
+    note_launch();
+}
+
+template <int HD>
+void append_hd(const float* q, float* q_out, const float* k, const float* v, int T, int heads, int kv_heads, const float* table,
+               int rope_dims, int neox, const Kv4Rows& rows, const int32_t* pos, int64_t capacity, cudaStream_t s)
+{
+    const int q_blocks = rope_dims > 0 || q_out != q ? (heads * (HD / 8) + 127) / 128 : 0;
+    const int kv_blocks = (2 * kv_heads * (HD / 8) + 127) / 128;
+    launch(k_kv4_append<HD>, dim3(q_blocks + kv_blocks, std::min(T, 65535)), dim3(128), 0, s, q, q_out, k, v, T, heads, kv_heads,
+           table, rope_dims, neox, rows, pos, capacity, q_blocks);
+    note_launch();
+}
+
+template <int HD>
+void read_hd(const Kv4Rows& rows, const int32_t* pos, int T, int kv_heads, int64_t capacity, void* k, void* v, cudaStream_t s)
+{
+    launch(k_kv4_read<HD>, dim3((2 * kv_heads * (HD / 8) + 127) / 128, std::min(T, 65535)), dim3(128), 0, s, rows, pos, T,
+           kv_heads, capacity, (__half*)k, (__half*)v);
+    note_launch();
+}
+
+}  // namespace
+
+bool kv4_supported(int heads, int kv_heads, int head_dim)
+{
+    return heads > 0 && kv_heads > 0 && heads % kv_heads == 0 &&
+           (head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 256);
+}
+
+int64_t kv4_bytes(int kv_heads, int head_dim, int64_t positions)
+{
+    return (positions + KV4_P - 1) / KV4_P * kv_heads * kv4_tile_bytes(head_dim);
+}
+
+int64_t kv4_workspace_bytes(int T, int R, int heads, int kv_heads, int head_dim, int64_t capacity, int window, int sinks)
+{
+    return KV4_TICKETS * 4 + 4 * kv4_plan(T, R, heads, kv_heads, head_dim, capacity, window, sinks).part_floats;
+}
+
+size_t kv4_ticket_bytes() { return (size_t)KV4_TICKETS * 4; }
+
+void kv4_append(const float* q, float* q_out, const float* k, const float* v, int T, int heads, int kv_heads, int head_dim,
+                const float* table, int rope_dims, int neox, const Kv4Cache& cache, const int32_t* pos, int64_t capacity,
+                cudaStream_t s)
+{
+    if (T <= 0) return;
+    const Kv4Rows r{(const uint8_t*)cache.rows, cache.pitch, cache.layer};
+    switch (head_dim) {
+    case 64: append_hd<64>(q, q_out, k, v, T, heads, kv_heads, table, rope_dims, neox, r, pos, capacity, s); break;
+    case 96: append_hd<96>(q, q_out, k, v, T, heads, kv_heads, table, rope_dims, neox, r, pos, capacity, s); break;
+    case 128: append_hd<128>(q, q_out, k, v, T, heads, kv_heads, table, rope_dims, neox, r, pos, capacity, s); break;
+    default: append_hd<256>(q, q_out, k, v, T, heads, kv_heads, table, rope_dims, neox, r, pos, capacity, s); break;
+    }
+}
+
+void kv4_read(const Kv4Cache& cache, const int32_t* pos, int T, int kv_heads, int head_dim, int64_t capacity, void* k, void* v,
+              cudaStream_t s)
+{
+    if (T <= 0) return;
+    const Kv4Rows r{(const uint8_t*)cache.rows, cache.pitch, cache.layer};
+    switch (head_dim) {
+    case 64: read_hd<64>(r, pos, T, kv_heads, capacity, k, v, s); break;
+    case 96: read_hd<96>(r, pos, T, kv_heads, capacity, k, v, s); break;
+    case 128: read_hd<128>(r, pos, T, kv_heads, capacity, k, v, s); break;
+    default: read_hd<256>(r, pos, T, kv_heads, capacity, k, v, s); break;
+    }
+}
+
+void kv4_attention(const float* q, int T, int R, int heads, int kv_heads, int head_dim, float scale, const Kv4Cache& cache,
+                   const int32_t* pos, int64_t capacity, int window, int sinks, float* out, void* ws, int* err, cudaStream_t s)
+{
+    if (T <= 0) return;
+    const Kv4Plan p = kv4_plan(T, R, heads, kv_heads, head_dim, capacity, window, sinks);
+    // (a launch takes 65535 rows or runs; calls of more have one range a row and no partials)
+    const int unit = p.runs ? R : 1;
+    for (int64_t t0 = 0; t0 < T; t0 += (int64_t)65535 * unit) {
+        Kv4Att a{};
+        a.q = q + t0 * heads * head_dim;
+        a.out = out + t0 * heads * head_dim;
+        a.rows = Kv4Rows{(const uint8_t*)cache.rows + t0 * cache.pitch, cache.pitch, cache.layer};
+        a.pos = pos + t0;
+        a.T = (int)std::min<int64_t>(T - t0, (int64_t)65535 * unit);
+        a.capacity = capacity; a.R = R; a.heads = heads; a.kv_heads = kv_heads; a.S = p.S; a.s_max = p.s_max;
+        a.scale = scale; a.window = window; a.sinks = sinks;
+        a.tickets = (int*)ws;
+        a.part = (float*)((uint8_t*)ws + KV4_TICKETS * 4);
+        a.ml = a.part + (int64_t)T * heads * p.S * head_dim;
+        a.err = err;
+        switch (head_dim) {
+        case 64: p.runs ? attn_runs<64>(a, p, s) : attn_rows<64>(a, p, s); break;
+        case 96: p.runs ? attn_runs<96>(a, p, s) : attn_rows<96>(a, p, s); break;
+        case 128: p.runs ? attn_runs<128>(a, p, s) : attn_rows<128>(a, p, s); break;
+        default: p.runs ? attn_runs<256>(a, p, s) : attn_rows<256>(a, p, s); break;
+        }
+    }
+}
+
+}  // namespace k
+}  // namespace wl
