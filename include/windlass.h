@@ -230,6 +230,27 @@ int32_t wl_forward_batch_sample(wl_model* model, wl_seq* const* seqs, const int3
                                 const double* temperature, const double* top_p, const double* draws, int32_t* ids_out,
                                 volatile const int32_t* cancel, wl_progress_fn progress, void* user);
 
+/* A row's sampling options beyond Sampler.Sample's. The ids in order: logit descending, equal logits by ascending id;
+ * p[i] = exp((logit[i] - max) / temperature) in double (none for a NaN or -inf logit). Kept: of the first top_k ids
+ * (top_k <= 0: all) the shortest prefix whose sum of p reaches top_p times theirs (top_p >= 1: all), of it the ids with
+ * p >= min_p (min_p <= 0: all), at least the first. The choice is the first kept id at which the running sum reaches draw *
+ * (the kept ids' sum), in that order, or in id order when nothing is filtered (top_k <= 0 or >= V, top_p >= 1, min_p <= 0).
+ * temperature <= 0: the greedy id, the rest is not read. A row without a logit above -inf gives 0. The sums are exact
+ * sums of p rounded to multiples of 2^-(62 - ceil(log2 V)), so the choice is the same in every run. */
+typedef struct wl_sample_opts {
+    double temperature, top_p, min_p;
+    double draw;             /* the caller's uniform double in [0, 1) */
+    int64_t top_k;
+} wl_sample_opts;
+/* wl_forward_sample with those options (host memory). */
+int32_t wl_forward_sample_opts(wl_model* model, wl_seq* seq, const int32_t* tokens, int32_t T, int32_t pos0,
+                               const wl_sample_opts* opts, int32_t* id_out, volatile const int32_t* cancel,
+                               wl_progress_fn progress, void* user);
+/* wl_forward_batch_sample with opts[i] (host memory) for row i; all rows are sampled in one launch. */
+int32_t wl_forward_batch_sample_opts(wl_model* model, wl_seq* const* seqs, const int32_t* tokens, int32_t N,
+                                     const wl_sample_opts* opts, int32_t* ids_out, volatile const int32_t* cancel,
+                                     wl_progress_fn progress, void* user);
+
 /* Greedy decode of seq (NULL = the model's own) chained on the device, the decode loop of Engine.cs:187-203 at
  * temperature 0: step s forwards `token` (s = 0) or ids_out[s-1] at the sequence's next position and writes the
  * argmax of its logits to ids_out[s]. The id never visits the host between steps: `chunk` steps (0 = 16, at most 64)
@@ -320,6 +341,13 @@ int32_t wl_kv4_attention(const float* dev_q, int32_t T, int32_t rows_per_seq, in
 int32_t wl_kv4_workspace_bytes(int32_t T, int32_t rows_per_seq, int32_t heads, int32_t kv_heads, int32_t head_dim,
                                int64_t capacity, int32_t window, int32_t sinks, int64_t* bytes);
 int32_t wl_kv4_workspace_init(void* dev_workspace, int64_t workspace_bytes, void* stream);
+
+/* The choice of wl_forward_batch_sample_opts on `rows` rows of V device floats, row r at dev_logits + r * ld (ld >= V), with
+ * the options dev_opts[r] (device memory, 8-byte aligned): dev_ids[r] = the chosen id, or -1 where temperature > 0 and
+ * the draw is not in [0, 1). Enqueues one launch on `stream`; needs no workspace and may be captured into a graph, whose
+ * replays read the options anew. */
+int32_t wl_sample_rows(const float* dev_logits, int64_t ld, int32_t V, int32_t rows, const wl_sample_opts* dev_opts,
+                       int32_t* dev_ids, void* stream);
 
 /* Synchronises `device` and reports whether a device-side wait of a kernel-level export (wl_matvec, wl_matvec_tiles,
  * wl_matvec_static, wl_gemm_tiles, wl_matmul) gave up since the last report: WL_ETIMEDOUT (and the code) if one did,

@@ -86,3 +86,17 @@ def test_the_reference_reads_what_it_writes():
                 code, shift, sc = R._places(hd, p, is_v)
                 used[code] = used[sc] = used[sc + 1] = True
         assert used[:R.tile_bytes(hd)].all()
+
+
+def test_sampler_refusals(wl):
+    L = wl.lib()
+    for a in ((None, 10, 10, 1, ONE, ONE), (ONE, 10, 10, 1, None, ONE), (ONE, 10, 10, 1, ONE, None), (ONE, 9, 10, 1, ONE, ONE),
+              (ONE, 10, 0, 1, ONE, ONE), (ONE, 10, 10, -1, ONE, ONE)):
+        assert L.wl_sample_rows(*a, None) == wl.WL_EINVAL, a
+    assert L.wl_sample_rows(ONE, 10, 10, 0, ONE, ONE, None) == wl.WL_OK
+    assert L.wl_forward_sample_opts(None, None, None, 1, 0, None, None, None, wl.PROGRESS(), None) == wl.WL_EINVAL
+    assert L.wl_forward_batch_sample_opts(None, None, None, 1, None, None, None, wl.PROGRESS(), None) == wl.WL_EINVAL
+    o = wl.SampleOpts(1.0, 1.0, 0.0, 1.0, 0)
+    out = (C.c_int32 * 1)()
+    assert L.wl_forward_sample_opts(None, None, None, 1, 0, C.byref(o), out, None, wl.PROGRESS(), None) == wl.WL_EINVAL
+    assert b"draw" in L.wl_last_error()

@@ -79,6 +79,11 @@ class SynthSpec(C.Structure):
                [("seed", C.c_uint64)]
 
 
+class SampleOpts(C.Structure):
+    _fields_ = [("temperature", C.c_double), ("top_p", C.c_double), ("min_p", C.c_double), ("draw", C.c_double),
+                ("top_k", C.c_int64)]
+
+
 PROGRESS = C.CFUNCTYPE(None, C.c_int32, C.c_int32, C.c_void_p)
 
 _lib = None
@@ -115,6 +120,9 @@ def lib():
         "wl_forward_mixed": (I32, [P, P, P, I32, P, P, P, P, PROGRESS, P]),
         "wl_forward_sample": (I32, [P, P, P, I32, I32, C.c_double, C.c_double, C.c_double, P, P, PROGRESS, P]),
         "wl_forward_batch_sample": (I32, [P, P, P, I32, P, P, P, P, P, PROGRESS, P]),
+        "wl_forward_sample_opts": (I32, [P, P, P, I32, I32, P, P, P, PROGRESS, P]),
+        "wl_forward_batch_sample_opts": (I32, [P, P, P, I32, P, P, P, PROGRESS, P]),
+        "wl_sample_rows": (I32, [P, I64, I32, I32, P, P, P]),
         "wl_sample": (I32, [P, I32, C.c_double, C.c_double, C.c_double, P, P]),
         "wl_generate_greedy": (I32, [P, P, I32, I32, P, I32, I32, P, C.POINTER(I32), P]),
         "wl_argmax": (I32, [P, I32, I32, P, P]), "wl_route": (I32, [P, I32, I32, I32, I32, P, P, P]), "wl_kernel_status": (I32, [I32]),

@@ -519,6 +519,32 @@ int32_t wl_forward_batch_sample(wl_model* model, wl_seq* const* seqs, const int3
     });
 }
 
+int32_t wl_forward_sample_opts(wl_model* model, wl_seq* seq, const int32_t* tokens, int32_t T, int32_t pos0,
+                               const wl_sample_opts* opts, int32_t* id_out, volatile const int32_t* cancel,
+                               wl_progress_fn progress, void* user)
+{
+    return guarded([&]() -> int32_t {
+        if (!opts || (!id_out && model && T != 0)) return wl::fail(WL_EINVAL, "wl_forward_sample_opts: model, tokens, opts and id_out are required");
+        if (opts->temperature > 0.0 && !(opts->draw >= 0.0 && opts->draw < 1.0)) return wl::fail(WL_EINVAL, "wl_forward_sample_opts: the draw must be in [0, 1)");
+        const wl::Model::SampleRows sr{nullptr, nullptr, nullptr, opts};
+        return forward_rows("wl_forward_sample_opts", model, seq, tokens, T, pos0, 0, nullptr, id_out, cancel, progress, user, &sr);
+    });
+}
+
+int32_t wl_forward_batch_sample_opts(wl_model* model, wl_seq* const* seqs, const int32_t* tokens, int32_t N,
+                                     const wl_sample_opts* opts, int32_t* ids_out, volatile const int32_t* cancel,
+                                     wl_progress_fn progress, void* user)
+{
+    return guarded([&]() -> int32_t {
+        if (!ids_out || !opts) return wl::fail(WL_EINVAL, "wl_forward_batch_sample_opts: model, seqs, tokens, opts and ids_out are required");
+        for (int i = 0; i < N; ++i)
+            if (opts[i].temperature > 0.0 && !(opts[i].draw >= 0.0 && opts[i].draw < 1.0))
+                return wl::fail(WL_EINVAL, "wl_forward_batch_sample_opts: every draw must be in [0, 1)");
+        const wl::Model::SampleRows sr{nullptr, nullptr, nullptr, opts};
+        return forward_batch_rows("wl_forward_batch_sample_opts", model, seqs, tokens, N, nullptr, ids_out, cancel, progress, user, &sr);
+    });
+}
+
 int32_t wl_forward_mixed(wl_model* model, wl_seq* const* seqs, const int32_t* counts, int32_t N, const int32_t* tokens,
                          float* logits_out, int32_t* ids_out, volatile const int32_t* cancel, wl_progress_fn progress,
                          void* user)
@@ -813,6 +839,22 @@ int32_t wl_kv4_attention(const float* dev_q, int32_t T, int32_t rows_per_seq, in
         WL_CHECK_BUFFERS("wl_kv4_attention", {dev_q, "dev_q"}, {dev_out, "dev_out"}, {dev_workspace, "dev_workspace"});
         wl::k::kv4_attention(dev_q, T, rows_per_seq, heads, kv_heads, head_dim, scale, wl::k::Kv4Cache{dev_caches, 8, 0}, dev_pos,
                              capacity, window, sinks, dev_out, dev_workspace, (int*)wl::k::static_scratch(), (cudaStream_t)stream);
+        return WL_OK;
+    });
+}
+
+int32_t wl_sample_rows(const float* dev_logits, int64_t ld, int32_t V, int32_t rows, const wl_sample_opts* dev_opts,
+                       int32_t* dev_ids, void* stream)
+{
+    return guarded([&]() -> int32_t {
+        if (V <= 0 || rows < 0 || ld < V) return wl::fail(WL_EINVAL, "wl_sample_rows: V must be positive, rows not negative and ld at least V");
+        if (!dev_logits || !dev_opts || !dev_ids) return wl::fail(WL_EINVAL, "wl_sample_rows: null pointer");
+        if (rows == 0) return WL_OK;
+        const std::string f = device_buffer_fault(dev_logits, "dev_logits", 4);
+        if (!f.empty()) return wl::fail(WL_EINVAL, "wl_sample_rows: " + f);
+        const std::string g = device_buffer_fault(dev_opts, "dev_opts", 8);
+        if (!g.empty()) return wl::fail(WL_EINVAL, "wl_sample_rows: " + g);
+        wl::k::sample_rows(dev_logits, ld, V, rows, dev_opts, dev_ids, (cudaStream_t)stream);
         return WL_OK;
     });
 }

@@ -5,6 +5,8 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
+struct wl_sample_opts;      // (windlass.h)
+
 namespace wl {
 
 // Where row t of a step keeps its fp16 KV cache: layer l's keys start at k + l*layer_stride (values likewise at
@@ -292,6 +294,9 @@ void shared_expert_add(float* outp, const float* sh, const float* gl, int T, int
 // F32 tensors get offset + sigma*z (offset 1 for norm weights); quantized types get sigma*z, quantized.
 void synth(int type, uint64_t seed, uint32_t tid, int64_t rows, int64_t cols, float sigma, float offset, uint8_t* out,
            cudaStream_t s);
+
+// Sampling of rows x[r * ld .. + V) with the device options opts[r] (wl_sample_rows.cu): ids[r] = row r's choice.
+void sample_rows(const float* logits, int64_t ld, int V, int rows, const wl_sample_opts* opts, int32_t* ids, cudaStream_t s);
 
 // ---- the 4-bit KV cache (wl_kv4.cu) ----
 // Where the rows' caches are: with pitch = sizeof(RowKV), RowKV entries (keys and values share one cache at k, layer l at

@@ -821,7 +821,7 @@ Model::~Model()
     dfree(logits_part_); dfree(logits_all_); dfree(flag_d_); hfree(flag_h_);
     dfree(pg_); dfree(pu_); dfree(py_); dfree(expert_count_d_);
     dfree(ids_d_); dfree(amax_key_); dfree(amax_count_); dfree(gen_d_); hfree(h_ids_); hfree(h_gen_);
-    dfree(sample_ws_);
+    dfree(sample_ws_); dfree(sample_opts_d_); hfree(h_sample_opts_);
     if (pprep_) cudaFree(pprep_);
     comm_.reset();           // after the graphs that hold its collectives
     for (const ProfileMark& m : marks_) { cudaEventDestroy(m.start); cudaEventDestroy(m.stop); }
@@ -1474,7 +1474,23 @@ int32_t Model::run(int T, const std::vector<RowKV>& rows, const std::vector<int3
         head(T, first);
         stage_release(c_.layers);
     }
-    if (ids && sampling_) {
+    if (ids && sampling_ && sampling_->opts) {
+        const int n = T - first;
+        if (n > sample_opts_cap_) {
+            dfree(sample_opts_d_);
+            hfree(h_sample_opts_);
+            sample_opts_cap_ = 0;
+            sample_opts_d_ = dalloc<wl_sample_opts>(n);
+            h_sample_opts_ = halloc<wl_sample_opts>(n);
+            sample_opts_cap_ = n;
+        }
+        std::copy(sampling_->opts, sampling_->opts + n, h_sample_opts_);
+        WL_CUDA(cudaMemcpyAsync(sample_opts_d_, h_sample_opts_, sizeof(wl_sample_opts) * (size_t)n, cudaMemcpyHostToDevice, stream_));
+        k::sample_rows(logits_, c_.vocab, c_.vocab, n, sample_opts_d_, ids_d_, stream_);
+        WL_CUDA(cudaMemcpyAsync(h_ids_, ids_d_, sizeof(int32_t) * (size_t)n, cudaMemcpyDeviceToHost, stream_));
+        WL_CUDA(cudaStreamSynchronize(stream_));
+        for (int r = 0; r < n; ++r) ids[r] = h_ids_[r];
+    } else if (ids && sampling_) {
         if (!sample_ws_) {
             sample_ws_ = dalloc<uint8_t>((int64_t)k::sample_workspace_bytes(c_.vocab));
             k::sample_workspace_init(sample_ws_, stream_);
@@ -1759,6 +1775,12 @@ struct SamplingScope {
 
 void check_sample_rows(const Model::SampleRows& sr, int n)
 {
+    if (sr.opts) {
+        for (int r = 0; r < n; ++r)
+            if (sr.opts[r].temperature > 0.0 && !(sr.opts[r].draw >= 0.0 && sr.opts[r].draw < 1.0))
+                WL_THROW(WL_EINVAL, "A sampling draw must be in [0, 1).");
+        return;
+    }
     if (!sr.temperature || !sr.top_p || !sr.draw) WL_THROW(WL_EINVAL, "Sampling needs a temperature, top_p and draw for each row.");
     for (int r = 0; r < n; ++r)
         if (sr.temperature[r] > 0.0 && !(sr.draw[r] >= 0.0 && sr.draw[r] < 1.0))

@@ -97,6 +97,7 @@ public:
         const double* temperature;
         const double* top_p;
         const double* draw;
+        const wl_sample_opts* opts = nullptr;   // with top-k and min-p too (the three above are then not read)
     };
     int32_t forward_sample(Seq* seq, const int32_t* tokens, int T, int pos0, const SampleRows& sr, int32_t* id,
                            volatile const int32_t* cancel, wl_progress_fn progress, void* user);
@@ -311,6 +312,9 @@ private:
     // workspace (one row's, made at the first sampled call; its first 256 bytes stay zero between rows)
     const SampleRows* sampling_ = nullptr;
     void* sample_ws_ = nullptr;
+    wl_sample_opts* sample_opts_d_ = nullptr;   // a call's options on the device, their pinned copy, and room for rows
+    wl_sample_opts* h_sample_opts_ = nullptr;
+    int sample_opts_cap_ = 0;
     int32_t* gen_d_ = nullptr;
     int32_t* h_gen_ = nullptr;
     float* ew_d_ = nullptr;

@@ -198,6 +198,35 @@ class CudaTransformer:
                                             cancel.ptr if cancel else None, cb, None))
         return out[:N]
 
+    def forward_sample_opts(self, tokens, draw, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, pos0=0, cancel=None,
+                            on_stage=None, seq=None):
+        """forward_sample() with top-k and min-p too (wl_sample_opts): the last row's sampled id."""
+        tokens = np.ascontiguousarray(tokens, dtype=np.int32)
+        out = np.empty(1, dtype=np.int32)
+        o = _lib.SampleOpts(temperature, top_p, min_p, draw, top_k)
+        cb = _lib.PROGRESS(lambda d, t, u: on_stage(d, t)) if on_stage else _lib.PROGRESS()
+        check(lib().wl_forward_sample_opts(self._h, seq._h if seq is not None else None, tokens.ctypes.data_as(C.c_void_p),
+                                           int(tokens.size), pos0, C.byref(o), out.ctypes.data_as(C.c_void_p),
+                                           cancel.ptr if cancel else None, cb, None))
+        return int(out[0])
+
+    def forward_batch_sample_opts(self, seqs, tokens, draws, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, cancel=None,
+                                  on_stage=None):
+        """forward_batch_sample() with top-k and min-p too (arrays of N, or scalars for every row): an int32 array of N
+        ids, all rows sampled in one launch."""
+        tokens = np.ascontiguousarray(tokens, dtype=np.int32)
+        N = int(tokens.size)
+        arr = (C.c_void_p * max(N, 1))(*[s._h for s in seqs])
+        o = (_lib.SampleOpts * max(N, 1))()
+        for name, v in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p), ("draw", draws), ("top_k", top_k)):
+            for i, x in enumerate(np.broadcast_to(np.asarray(v), (max(N, 1),)).tolist()):
+                setattr(o[i], name, x)
+        out = np.empty(max(N, 1), dtype=np.int32)
+        cb = _lib.PROGRESS(lambda d_, t_, u: on_stage(d_, t_)) if on_stage else _lib.PROGRESS()
+        check(lib().wl_forward_batch_sample_opts(self._h, arr, tokens.ctypes.data_as(C.c_void_p), N, o,
+                                                 out.ctypes.data_as(C.c_void_p), cancel.ptr if cancel else None, cb, None))
+        return out[:N]
+
     def forward_mixed(self, seqs, token_lists, cancel=None, on_stage=None, argmax=False):
         """One pass over several sequences' new tokens (a decode step that prompts join): sequence i takes
         token_lists[i]; returns each sequence's last-row logits ([N][vocab]), or its greedy id (argmax=True)."""
