@@ -92,7 +92,13 @@ typedef struct wl_options {
                                 8 MB chunks through a ring of four pinned buffers, O_DIRECT where the file system
                                 allows it, on a reader thread that overlaps the reads with the copies, so the host
                                 holds no copy of the model; 0 lays every stage out once in pinned host memory */
-    int32_t reserved[5];
+    int32_t kv_type;         /* the sequences' KV cache: 0 or WL_TYPE_F16 = fp16 (the reference's), WL_TYPE_Q4_0 = 4-bit
+                                blocks (wl_kv4_append): 0.28 of the memory, and of what a decode step's attention reads;
+                                head_dim 64, 96, 128 or 256 */
+    int32_t attn_window;     /* with kv_type WL_TYPE_Q4_0: > 0 lets position p see the positions j > p - attn_window and the
+                                first attn_sinks ones only; 0 = every position (the reference's) */
+    int32_t attn_sinks;
+    int32_t reserved[2];
     uint8_t tp_id[128];      /* the group's id: wl_tp_unique_id on one rank, the same bytes passed to every rank */
 } wl_options;
 
@@ -158,7 +164,7 @@ int32_t wl_info_get(const wl_model* model, wl_info* info);
 int32_t wl_stats_get(const wl_model* model, wl_stats* stats);
 
 /* Transformer.NewSequence / Sequence.Truncate / Sequence.Length (src/Transformer.cs:60, src/Batch.cs:28).
- * A sequence owns its fp16 KV cache in device memory; free every sequence before its model. */
+ * A sequence owns its KV cache (wl_options.kv_type) in device memory; free every sequence before its model. */
 int32_t wl_seq_new(wl_model* model, wl_seq** out);
 int32_t wl_seq_free(wl_seq* seq);
 int32_t wl_seq_truncate(wl_seq* seq, int32_t n);

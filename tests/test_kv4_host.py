@@ -100,3 +100,19 @@ def test_sampler_refusals(wl):
     out = (C.c_int32 * 1)()
     assert L.wl_forward_sample_opts(None, None, None, 1, 0, C.byref(o), out, None, wl.PROGRESS(), None) == wl.WL_EINVAL
     assert b"draw" in L.wl_last_error()
+
+
+def test_model_options_are_refused_before_any_device_work(wl):
+    from windlass_b200.transformer import config0_spec, synth_spec
+    L = wl.lib()
+
+    def open_(spec=None, **kw):
+        h = C.c_void_p()
+        return L.wl_open_synthetic(C.byref(spec or config0_spec()), C.byref(wl.options(**kw)), C.byref(h))
+    assert open_(kv_type=3) == wl.WL_EUNSUPPORTED and b"kv_type" in L.wl_last_error()
+    assert open_(attn_window=64) == wl.WL_EUNSUPPORTED and b"attn_window" in L.wl_last_error()
+    assert open_(kv_type=2, attn_window=-1) == wl.WL_EINVAL
+    assert open_(kv_type=2, attn_window=64, attn_sinks=-1) == wl.WL_EINVAL
+    assert open_(kv_type=2, attn_sinks=4) == wl.WL_EINVAL
+    spec = synth_spec("llama", 1, 320, 4, 4, 80, 256, 512, 512)
+    assert open_(spec, kv_type=2) == wl.WL_EUNSUPPORTED and b"head_dim" in L.wl_last_error()

@@ -64,6 +64,9 @@ void Model::init_device(const wl_options& opt)
     max_batch_ = opt.max_batch > 0 ? opt.max_batch : 64;
     use_graphs_ = opt.use_graphs != 0;
     prefill_path_ = opt.prefill_path;
+    kv4_ = opt.size >= (int32_t)sizeof(wl_options) && opt.kv_type == WL_TYPE_Q4_0;
+    window_ = kv4_ ? opt.attn_window : 0;
+    sinks_ = kv4_ ? opt.attn_sinks : 0;
 }
 
 // Tensor parallelism (tp_size > 1): checks the shape can be split, makes c_ this rank's share of the heads and joins
@@ -94,6 +97,22 @@ static void check_tp(const Config& c, const wl_options& opt)
         WL_THROW(WL_EUNSUPPORTED, "Tensor parallelism over " + g + " GPUs leaves an unsupported attention shape per GPU.");
     const int vp = (c.vocab + G - 1) / G;
     if ((int64_t)vp * (G - 1) >= c.vocab) WL_THROW(WL_EUNSUPPORTED, "The vocabulary is too small to split over " + g + " GPUs.");
+}
+
+// The KV cache's options, checked before any device work.
+static void check_kv(const Config& c, const wl_options& opt)
+{
+    if (opt.size < (int32_t)sizeof(wl_options)) return;
+    if (opt.kv_type != 0 && opt.kv_type != WL_TYPE_F16 && opt.kv_type != WL_TYPE_Q4_0)
+        WL_THROW(WL_EUNSUPPORTED, "kv_type must be 0 or WL_TYPE_F16 (fp16) or WL_TYPE_Q4_0 (4-bit blocks).");
+    if (opt.attn_window < 0 || opt.attn_sinks < 0) WL_THROW(WL_EINVAL, "attn_window and attn_sinks must not be negative.");
+    if (opt.attn_sinks > 0 && opt.attn_window == 0) WL_THROW(WL_EINVAL, "attn_sinks needs an attn_window.");
+    if (opt.kv_type != WL_TYPE_Q4_0) {
+        if (opt.attn_window > 0) WL_THROW(WL_EUNSUPPORTED, "attn_window needs kv_type WL_TYPE_Q4_0.");
+        return;
+    }
+    if (!k::kv4_supported(c.heads, c.kv_heads, c.head_dim))
+        WL_THROW(WL_EUNSUPPORTED, "kv_type WL_TYPE_Q4_0 needs a head_dim of 64, 96, 128 or 256, not " + std::to_string(c.head_dim) + ".");
 }
 
 // Tensor parallelism (tp_size > 1): makes c_ this rank's share of the heads and joins the NCCL group (blocking until
@@ -613,6 +632,7 @@ Model* Model::open_file(const std::string& path, const wl_options& opt)
     Gguf g(path);
     const Config c = read_config(g);
     check_tp(c, opt);
+    check_kv(c, opt);
     std::unique_ptr<Model> m(new Model());
     m->c_ = c;
     m->file_path_ = path;
@@ -650,6 +670,7 @@ Model* Model::open_synthetic(const wl_synth_spec& sp, const wl_options& opt)
     if (c.layers <= 0 || c.embd <= 0 || c.heads <= 0 || c.kv_heads <= 0 || c.heads % c.kv_heads || c.vocab <= 0)
         WL_THROW(WL_EINVAL, "bad synthetic shape");
     check_tp(c, opt);
+    check_kv(c, opt);
     m->init_device(opt);
     m->max_context_ = opt.max_context > 0 ? opt.max_context : std::min(c.context_length, 8192);
     const float sigma = sp.sigma > 0 ? sp.sigma : 0.02f;
@@ -821,6 +842,7 @@ Model::~Model()
     dfree(logits_part_); dfree(logits_all_); dfree(flag_d_); hfree(flag_h_);
     dfree(pg_); dfree(pu_); dfree(py_); dfree(expert_count_d_);
     dfree(ids_d_); dfree(amax_key_); dfree(amax_count_); dfree(gen_d_); hfree(h_ids_); hfree(h_gen_);
+    if (kv4_ws_) cudaFree(kv4_ws_);
     dfree(sample_ws_); dfree(sample_opts_d_); hfree(h_sample_opts_);
     if (pprep_) cudaFree(pprep_);
     comm_.reset();           // after the graphs that hold its collectives
@@ -857,10 +879,34 @@ void Model::free_seq(Seq* s)
 }
 
 // Transformer.Reserve (src/Transformer.cs:62-73): grow to max(positions, min(context, max(256, 2*capacity))).
+int64_t Model::kv_layer_words(int capacity) const
+{
+    return kv4_ ? k::kv4_bytes(c_.kv_heads, c_.head_dim, capacity) / 2 : (int64_t)capacity * c_.kvdim();
+}
+
+RowKV Model::row_kv(const Seq* s) const
+{
+    const int64_t stride = kv_layer_words(s->capacity);
+    return RowKV{s->kv, kv4_ ? s->kv : s->kv + (int64_t)c_.layers * stride, stride};
+}
+
 void Model::reserve(Seq* s, int positions)
 {
     if (positions <= s->capacity) return;
     const int cap = std::max(positions, std::min(max_context_, std::max(256, s->capacity * 2)));
+    if (kv4_) {
+        // a layer's tiles in position order, so what is held is each layer's first bytes
+        const int64_t words = kv_layer_words(cap);
+        uint16_t* nk = dalloc<uint16_t>(c_.layers * words);
+        if (s->kv && s->length > 0)
+            WL_CUDA(cudaMemcpy2DAsync(nk, words * 2, s->kv, kv_layer_words(s->capacity) * 2, (size_t)kv_layer_words(s->length) * 2,
+                                      c_.layers, cudaMemcpyDeviceToDevice, stream_));
+        WL_CUDA(cudaStreamSynchronize(stream_));
+        if (s->kv) cudaFree(s->kv);
+        s->kv = nk;
+        s->capacity = cap;
+        return;
+    }
     const int64_t KD = c_.kvdim(), per_layer = (int64_t)cap * KD;
     uint16_t* nk = dalloc<uint16_t>(2 * (int64_t)c_.layers * per_layer);
     if (s->kv && s->length > 0) {
@@ -914,6 +960,20 @@ void Model::ensure_workspace(int T, int logit_rows)
         ws_T_ = n;
         ws_gen_++;
         drop_graphs();
+    }
+    if (kv4_) {
+        const int64_t need = k::kv4_workspace_max(T, c_.heads, c_.kv_heads, c_.head_dim, max_context_, window_, sinks_);
+        if (need > kv4_ws_bytes_) {
+            WL_CUDA(cudaStreamSynchronize(stream_));
+            if (kv4_ws_) cudaFree(kv4_ws_);
+            kv4_ws_ = nullptr;
+            kv4_ws_bytes_ = 0;
+            kv4_ws_ = dalloc<uint8_t>(need);
+            kv4_ws_bytes_ = need;
+            WL_CUDA(cudaMemsetAsync(kv4_ws_, 0, k::kv4_ticket_bytes(), stream_));
+            ws_gen_++;
+            drop_graphs();
+        }
     }
     if (!xprep_buf_) {
         int max_cols = c_.embd;
@@ -1290,6 +1350,11 @@ void Model::layer(int l, int T, int max_n)
     if (L.qb.present()) k::add_bias(q_, L.qb.d, T, QD, stream_);
     if (L.kb.present()) k::add_bias(k_, L.kb.d, T, KD, stream_);
     if (L.vb.present()) k::add_bias(v_, L.vb.d, T, KD, stream_);
+    const float scale = c_.attention_scale != 0.f ? c_.attention_scale : 1.f / (float)std::sqrt((double)HD);
+    bool prepped = false;
+    k::XPrep ap{};
+    if (kv4_) kv4_layer(l, T, scale);
+    else {
     const int rm = profile_begin();
     bool roped = false;
     if (c_.qk_norm_full) {
@@ -1313,15 +1378,14 @@ void Model::layer(int l, int T, int max_n)
                        rope_table_, rows_d_, l, stream_);
     profile_end(rm, WL_PROFILE_ROPE, 0.0);
     const k::AttnRope ar_rope{k_, v_, rope_table_, c_.rope_dims, c_.rope_neox ? 1 : 0};
-    const float scale = c_.attention_scale != 0.f ? c_.attention_scale : 1.f / (float)std::sqrt((double)HD);
     // the o matvec's activations come out of the attention combine when it can prepare them
     const bool want_prep = L.o.tiles && T <= 8 && xprep_buf_;
-    k::XPrep ap{};
     if (want_prep) ap = k::xprep_view(xprep_buf_, QD, T);
     const int mark = profile_begin();
-    const bool prepped = k::attention(q_, T, c_.heads, c_.kv_heads, HD, scale, rows_d_, l, pos_d_, att_part_, att_,
+    prepped = k::attention(q_, T, c_.heads, c_.kv_heads, HD, scale, rows_d_, l, pos_d_, att_part_, att_,
                                       want_prep ? &ap : nullptr, stream_, rope_in_attention ? &ar_rope : nullptr);
     profile_end(mark, WL_PROFILE_ATTENTION, 0.0);
+    }
     prep_x_ = nullptr;
     if (prepped) { prep_x_ = att_; prep_cols_ = QD; prep_nc_ = T; }
     matmul_reduce(L.o, att_, T);
@@ -1346,6 +1410,35 @@ void Model::layer(int l, int T, int max_n)
     } else {
         pending_residual_ = true;           // x += o happens inside the next norm (next layer or the head)
     }
+}
+
+// The 4-bit cache's part of a layer: the heads' norms, RoPE and the append, then attention run by run.
+void Model::kv4_layer(int l, int T, float scale)
+{
+    const LayerW& L = L_[l];
+    const int QD = c_.qdim(), KD = c_.kvdim(), HD = c_.head_dim;
+    const k::Kv4Cache cache{rows_d_, (int)sizeof(RowKV), l};
+    const int rm = profile_begin();
+    if (c_.qk_norm_full) {
+        k::rmsnorm(q_, T, QD, L.q_norm.d, c_.rms_eps, q_, stream_);
+        k::rmsnorm(k_, T, KD, L.k_norm.d, c_.rms_eps, k_, stream_);
+    } else if (c_.qk_norm) {
+        k::rmsnorm(q_, T * c_.heads, HD, L.q_norm.d, c_.rms_eps, q_, stream_);
+        k::rmsnorm(k_, T * c_.kv_heads, HD, L.k_norm.d, c_.rms_eps, k_, stream_);
+    }
+    k::kv4_append(q_, q_, k_, v_, T, c_.heads, c_.kv_heads, HD, rope_table_, c_.rope_dims, c_.rope_neox ? 1 : 0, cache, pos_d_,
+                  max_context_, stream_);
+    profile_end(rm, WL_PROFILE_ROPE, 0.0);
+    const int mark = profile_begin();
+    const AttnSeg all{0, T, 1};
+    const AttnSeg* segs = segs_.empty() ? &all : segs_.data();
+    for (size_t i = 0; i < std::max<size_t>(1, segs_.size()); ++i) {
+        const AttnSeg& g = segs[i];
+        const k::Kv4Cache c{rows_d_ + g.start, (int)sizeof(RowKV), l};
+        k::kv4_attention(q_ + (int64_t)g.start * QD, g.count, g.run, c_.heads, c_.kv_heads, HD, scale, c, pos_d_ + g.start, max_context_,
+                         window_, sinks_, att_ + (int64_t)g.start * QD, kv4_ws_, err_d_, stream_);
+    }
+    profile_end(mark, WL_PROFILE_ATTENTION, 0.0);
 }
 
 // The pre-norm of a sublayer: x += o (the previous sublayer's output, when pending), xn = RmsNormRows(x) * w, and,
@@ -1604,8 +1697,7 @@ double Model::bench_decode(Seq* const* seqs, int N, int steps)
     std::vector<int32_t> pos_all((size_t)steps * N), toks(N);
     std::vector<RowKV> rows(N);
     for (int i = 0; i < N; ++i) {
-        const int64_t stride = (int64_t)seqs[i]->capacity * c_.kvdim();
-        rows[i] = RowKV{seqs[i]->kv, seqs[i]->kv + (int64_t)c_.layers * stride, stride};
+        rows[i] = row_kv(seqs[i]);
         toks[i] = (int32_t)((1103515245u * (uint32_t)(i + 1) + 12345u) % (uint32_t)c_.vocab);
         for (int s = 0; s < steps; ++s) pos_all[(size_t)s * N + i] = len[i] + s;
     }
@@ -1804,6 +1896,15 @@ int32_t Model::forward_batch_sample(Seq* const* seqs, const int32_t* tokens, int
     return forward_batch_impl(seqs, tokens, N, nullptr, ids, cancel, progress, user);
 }
 
+namespace {
+// A pass's rows in runs, cleared however the pass ends.
+template <typename V> struct SegScope {
+    V& v;
+    explicit SegScope(V& x) : v(x) { v.clear(); }
+    ~SegScope() { v.clear(); }
+};
+}  // namespace
+
 int32_t Model::forward_impl(Seq* sq, const int32_t* tokens, int T, int pos0, bool all_logits, float* out, int32_t* ids,
                             volatile const int32_t* cancel, wl_progress_fn progress, void* user)
 {
@@ -1815,8 +1916,9 @@ int32_t Model::forward_impl(Seq* sq, const int32_t* tokens, int T, int pos0, boo
     WL_CUDA(cudaSetDevice(device_));
     sq->length = pos0;
     reserve(sq, pos0 + T);
-    const int64_t stride = (int64_t)sq->capacity * c_.kvdim();
-    std::vector<RowKV> rows(T, RowKV{sq->kv, sq->kv + (int64_t)c_.layers * stride, stride});
+    std::vector<RowKV> rows(T, row_kv(sq));
+    const SegScope segs(segs_);
+    if (kv4_ && T > 8) segs_.push_back({0, T, T});
     std::vector<int32_t> pos(T);
     for (int t = 0; t < T; ++t) pos[t] = pos0 + t;
     stats_.forward_calls++;
@@ -1856,8 +1958,7 @@ int32_t Model::forward_batch_impl(Seq* const* seqs, const int32_t* tokens, int N
     std::vector<RowKV> rows(N);
     for (int i = 0; i < N; ++i) {
         reserve(seqs[i], pos[i] + 1);
-        const int64_t stride = (int64_t)seqs[i]->capacity * c_.kvdim();
-        rows[i] = RowKV{seqs[i]->kv, seqs[i]->kv + (int64_t)c_.layers * stride, stride};
+        rows[i] = row_kv(seqs[i]);
     }
     stats_.batch_calls++;
     // MatMulEach (src/Transformer.cs:544-561): each row bit-identical to running alone, so no GEMM for this step
@@ -1899,14 +2000,22 @@ int32_t Model::forward_mixed(Seq* const* seqs, const int32_t* counts, int N, con
     std::vector<RowKV> row(N);
     for (int i = 0; i < N; ++i) {
         reserve(seqs[i], seqs[i]->length + counts[i]);
-        const int64_t stride = (int64_t)seqs[i]->capacity * c_.kvdim();
-        row[i] = RowKV{seqs[i]->kv, seqs[i]->kv + (int64_t)c_.layers * stride, stride};
+        row[i] = row_kv(seqs[i]);
     }
     std::vector<RowKV> rows((size_t)T);
     std::vector<int32_t> pos((size_t)T), toks((size_t)T);
+    const SegScope segs(segs_);
     int k = 0;
     int64_t off = 0;
     for (int i = 0; i < N; ++i) {
+        // the rows before a sequence's last one read its cache together; what is left of short ones, and the last rows of
+        // all, each alone
+        if (kv4_ && T > 8) {
+            const int n = counts[i] - 1;
+            if (n > 8) segs_.push_back({k, n, n});
+            else if (n > 0 && !segs_.empty() && segs_.back().run == 1) segs_.back().count += n;
+            else if (n > 0) segs_.push_back({k, n, 1});
+        }
         for (int j = 0; j + 1 < counts[i]; ++j, ++k) {
             rows[k] = row[i];
             pos[k] = seqs[i]->length + j;
@@ -1914,6 +2023,7 @@ int32_t Model::forward_mixed(Seq* const* seqs, const int32_t* counts, int N, con
         }
         off += counts[i];
     }
+    if (kv4_ && T > 8) segs_.push_back({k, N, 1});
     off = 0;
     for (int i = 0; i < N; ++i, ++k) {
         off += counts[i];
@@ -1958,8 +2068,7 @@ int32_t Model::generate_greedy(Seq* sq, int32_t token, int max_new, const int32_
         gen_d_ = dalloc<int32_t>(MAX_CHUNK);
         h_gen_ = halloc<int32_t>(MAX_CHUNK);
     }
-    const int64_t stride = (int64_t)sq->capacity * c_.kvdim();
-    const RowKV row{sq->kv, sq->kv + (int64_t)c_.layers * stride, stride};
+    const RowKV row = row_kv(sq);
     upload_step(1, &row, &len, &token);
     stats_.forward_calls++;
     int done = 0;

@@ -56,7 +56,8 @@ struct Config {
 
 class Model;
 
-// Sequence (src/Batch.cs:13-36): one request's fp16 KV cache in device memory, [2][layers][capacity][kv_dim].
+// Sequence (src/Batch.cs:13-36): one request's KV cache in device memory: fp16, [2][layers][capacity][kv_dim], or 4-bit
+// tiles (wl_kv4.cu), [layers][capacity / 16][kv_heads] of keys and values together.
 struct Seq {
     Model* model = nullptr;
     uint16_t* kv = nullptr;
@@ -194,6 +195,9 @@ private:
     void load_from_gguf(const Gguf& g);
     void build_rope_table(const float* rope_freqs, int n_rope_freqs);
     void reserve(Seq* s, int positions);
+    int64_t kv_layer_words(int capacity) const;     // 16-bit words between two layers of a sequence's cache
+    RowKV row_kv(const Seq* s) const;
+    void kv4_layer(int l, int T, float scale);
     void ensure_workspace(int T, int logit_rows);
     void layer(int l, int T, int max_n);
     void pre_norm(int T, const Vec& w, bool prep_for_mma);
@@ -246,6 +250,16 @@ private:
     Vec out_norm_;
     float* rope_table_ = nullptr;         // [max_context][rope_dims] cos/sin pairs
     Seq* own_ = nullptr;
+    // the 4-bit KV cache (wl_options.kv_type), its window and its attention's workspace
+    bool kv4_ = false;
+    int window_ = 0, sinks_ = 0;
+    void* kv4_ws_ = nullptr;
+    int64_t kv4_ws_bytes_ = 0;
+    // a pass's rows in runs that share a cache: rows [start, start + count) in runs of `run` (empty: every row alone)
+    struct AttnSeg {
+        int start, count, run;
+    };
+    std::vector<AttnSeg> segs_;
     Stats stats_;
     int64_t weight_bytes_ = 0;
 
