@@ -14,10 +14,11 @@
 //
 // Attention. The query heads of one KV head share its codes: a tile of 8 queries (heads of a row, or rows of a prompt)
 // is the 16-row side of m16n8k16 MMAs, each query twice: rows 0-7 its values' fp16 roundings, rows 8-15 what the
-// roundings left (together 22 bits of the row's largest value). Codes become fp16 integers -8..7 exactly (a mask and
-// an OR put a nibble below 1024's exponent, a subtraction takes the 1024 off: 9 instructions for 8 codes), products are
-// exact, sums fp32; the block scales are applied outside: to each block's fp32 sums for the scores, and to the weights
-// before they are split for the values (p * d, per block). So the codes' rounding is the only one below fp32.
+// roundings left (together 22 bits of the row's largest value). Keys enter the MMA as their codes 0..15, which are fp16
+// subnormals once a mask has cut them out (c 2^-24, or 16 c 2^-24 with the query's share divided by 16), and 8 times the
+// sum of the query's block is taken off; values enter as fp16 integers -8..7. All products are exact, sums are fp32; the
+// block scales are applied outside: to each block's fp32 sums for the scores, and to the weights before they are split
+// for the values (p * d, per block). So the codes' rounding is the only one below fp32.
 #include <algorithm>
 #include <climits>
 #include <cstdint>
@@ -238,25 +239,78 @@ __device__ __forceinline__ void mma_zero(float (&d)[4], const uint4& a, uint32_t
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// Eight 4-bit codes to four fp16 pairs of c - 8: nibbles (0, 4), (1, 5), (2, 6), (3, 7).
-__device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&r)[4])
+// (w & mask) | bits in one instruction.
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits)
+{
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+    return r;
+}
+
+// Eight codes to four fp16 pairs of c - 8: nibbles (0, 4), (1, 5), (2, 6), (3, 7). A nibble below 1024's exponent is
+// 1024 + c, or 1024 + 16 c four bits up.
+__device__ __forceinline__ void unpack_signed(uint32_t w, uint32_t (&r)[4])
 {
     const __half2 m1032 = __floats2half2_rn(1032.f, 1032.f), s16 = __floats2half2_rn(0.0625f, 0.0625f),
                   m72 = __floats2half2_rn(-72.f, -72.f);
     const uint32_t w8 = w >> 8;
-    r[0] = h2_bits(__hsub2(bits_h2((w & 0x000F000Fu) | 0x64006400u), m1032));
-    r[1] = h2_bits(__hfma2(bits_h2((w & 0x00F000F0u) | 0x64006400u), s16, m72));
-    r[2] = h2_bits(__hsub2(bits_h2((w8 & 0x000F000Fu) | 0x64006400u), m1032));
-    r[3] = h2_bits(__hfma2(bits_h2((w8 & 0x00F000F0u) | 0x64006400u), s16, m72));
+    r[0] = h2_bits(__hsub2(bits_h2(and_or(w, 0x000F000Fu, 0x64006400u)), m1032));
+    r[1] = h2_bits(__hfma2(bits_h2(and_or(w, 0x00F000F0u, 0x64006400u)), s16, m72));
+    r[2] = h2_bits(__hsub2(bits_h2(and_or(w8, 0x000F000Fu, 0x64006400u)), m1032));
+    r[3] = h2_bits(__hfma2(bits_h2(and_or(w8, 0x00F000F0u, 0x64006400u)), s16, m72));
+}
+
+// The same as fp16 subnormals c 2^-24 (pairs 0 and 2) and 16 c 2^-24 (pairs 1 and 3): masks only.
+__device__ __forceinline__ void unpack_raw(uint32_t w, uint32_t (&r)[4])
+{
+    const uint32_t w8 = w >> 8;
+    r[0] = w & 0x000F000Fu;
+    r[1] = w & 0x00F000F0u;
+    r[2] = w8 & 0x000F000Fu;
+    r[3] = w8 & 0x00F000F0u;
+}
+
+// Pairs of floats in one instruction.
+__device__ __forceinline__ uint64_t f2(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 unf2(uint64_t v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
 
 // fp16 roundings of a pair and of what they leave.
-__device__ __forceinline__ void split_h2(float a, float b, uint32_t& hi, uint32_t& lo)
+__device__ __forceinline__ void split_h2(uint64_t ab, uint32_t& hi, uint32_t& lo)
 {
-    const __half2 h = __floats2half2_rn(a, b);
+    const float2 v = unf2(ab);
+    const __half2 h = __floats2half2_rn(v.x, v.y);
     const float2 f = __half22float2(h);
+    const float2 d = unf2(fma2(f2(f.x, f.y), f2(-1.f, -1.f), ab));
     hi = h2_bits(h);
-    lo = h2_bits(__floats2half2_rn(a - f.x, b - f.y));
+    lo = h2_bits(__floats2half2_rn(d.x, d.y));
 }
 
 // The words of one lane's fragments: NB consecutive (planes of 4) 32-bit words.
@@ -328,11 +382,15 @@ __device__ __forceinline__ TileList tile_list(int n, int first, int sink)
     return TileList{head, t1 - head, n > 0 ? head + last - t1 + 1 : 0};
 }
 
-// Running softmax of MT tiles of 8 queries: lane (g, c) keeps query g's maximum (in log2 units), its own share of the
-// sum, and the output's fragments (o[.][0,1] the rows of the weights' roundings, [2,3] of what they left).
+// A running maximum is followed only when it is passed by a factor 2^6: weights up to 2^6 cost nothing, and the output's
+// sums are rescaled a few times a row and not at most tiles.
+constexpr float ATT_SLACK = 6.f;
+
+// Running softmax of MT tiles of 8 queries: lane (g, c) keeps query g's reference maximum (in log2 units), its own share of
+// the sum, and the output's fragments (o[.][0,1] the rows of the weights' roundings, [2,3] of what they left).
 template <int HD, int MT> struct AttState {
     float m[MT], l[MT], o[MT][HD / 8][4];
-    float vs, vlim;             // the values' scales are multiplied by vs = 2^k while all are at most vlim = 2^(15-k)
+    float vs;                   // the values' scales are multiplied by vs = 2^k, so that a weight's product stays below 2^15
     __device__ __forceinline__ void init()
     {
 #pragma unroll
@@ -342,49 +400,56 @@ template <int HD, int MT> struct AttState {
 #pragma unroll
             for (int j = 0; j < HD / 8; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
         }
-        vs = 32768.f;
-        vlim = 1.f;
+        vs = 256.f;
     }
 };
 
+// What a lane keeps of its queries besides their fragments: ks undoes the query's power of two (and the codes' 2^-24);
+// off[b] = 8 * 2^-24 * (the sum of block b's dims), what codes of 0..15 give too much.
+template <int NB> struct QueryTerms {
+    float ks, off[NB];
+};
+
 // One tile of 16 positions for MT query tiles. qf(i, b, s) gives the A fragment of query tile i, block b, step s (dims
-// 32 b + 8 c + {2s, 2s + 4, 2s + 1, 2s + 5} of lane c); ks[i] undoes the queries' power of two.
+// 32 b + 8 c + {2s, 2s + 4} of lane c, and, divided by 16, {2s + 1, 2s + 5}).
 template <int HD, int MT, class QF>
 __device__ __forceinline__ void kv4_tile(const uint8_t* sm, int lane, int tile0, const Vis (&vis)[MT], bool full, const QF& qf,
-                                         const float (&ks)[MT], AttState<HD, MT>& st)
+                                         const QueryTerms<HD / 32> (&qt)[MT], AttState<HD, MT>& st)
 {
     constexpr int NB = HD / 32;
     const int c = lane & 3;
-    float s[MT][4];
+    uint64_t s2[MT][2];                     // scores of positions (2c, 2c + 1) and (2c + 8, 2c + 9), in the query's units
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         uint32_t kw[NB], dw[NB];
         lane_words<HD>(sm, half, lane, kw);
         lane_scales<HD>(sm + 16 * HD, 8 * half + 2 * c, dw);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) s[i][2 * half] = s[i][2 * half + 1] = 0.f;
+        for (int i = 0; i < MT; ++i) s2[i][half] = f2(0.f, 0.f);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             uint32_t r[4];
-            unpack8(kw[b], r);
-            const float d0 = scale_of<NB>(dw, 0, b), d1 = scale_of<NB>(dw, 1, b);
+            unpack_raw(kw[b], r);
+            const uint64_t d01 = f2(scale_of<NB>(dw, 0, b), scale_of<NB>(dw, 1, b));
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 float d[4];
                 mma_zero(d, qf(i, b, 0), r[0], r[1]);
                 const uint4 a = qf(i, b, 1);
                 mma16816(d, a.x, a.y, a.z, a.w, r[2], r[3]);
-                s[i][2 * half] += d0 * (d[0] + d[2]);
-                s[i][2 * half + 1] += d1 * (d[1] + d[3]);
+                const uint64_t u = add2(add2(f2(d[0], d[1]), f2(d[2], d[3])), f2(-qt[i].off[b], -qt[i].off[b]));
+                s2[i][half] = fma2(d01, u, s2[i][half]);
             }
         }
     }
-    // positions of s[.][0..3]: 2c, 2c + 1, 2c + 8, 2c + 9
+    float s[MT][4];                         // then the weights
     uint32_t seen[MT], any_seen = 0u;       // bits of the positions that this lane's queries see
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[i][e] *= ks[i];
+        {
+            const float2 a = unf2(s2[i][0]), b = unf2(s2[i][1]);
+            s[i][0] = a.x; s[i][1] = a.y; s[i][2] = b.x; s[i][3] = b.y;
+        }
         if (!full) {
             seen[i] = 0u;
 #pragma unroll
@@ -396,10 +461,9 @@ __device__ __forceinline__ void kv4_tile(const uint8_t* sm, int lane, int tile0,
         }
         float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(st.m[i], mx), mu = mn == -INFINITY ? 0.f : mn;
-        if (__any_sync(0xffffffffu, mn > st.m[i])) {
-            const float a = ex2(st.m[i] - mu);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * qt[i].ks;
+        if (__any_sync(0xffffffffu, mx > st.m[i] + ATT_SLACK)) {
+            const float mn = mx > st.m[i] ? mx : st.m[i], a = st.m[i] == -INFINITY ? 0.f : ex2(st.m[i] - mn);
             st.l[i] *= a;
 #pragma unroll
             for (int j = 0; j < HD / 8; ++j)
@@ -407,13 +471,11 @@ __device__ __forceinline__ void kv4_tile(const uint8_t* sm, int lane, int tile0,
                 for (int e = 0; e < 4; ++e) st.o[i][j][e] *= a;
             st.m[i] = mn;
         }
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            s[i][e] = ex2(s[i][e] - mu);
-            sum += s[i][e];
-        }
-        st.l[i] += sum;
+        const float mu = st.m[i] == -INFINITY ? 0.f : st.m[i];
+        const uint64_t k2 = f2(qt[i].ks, qt[i].ks), m2 = f2(-mu, -mu);
+        const float2 a = unf2(fma2(f2(s[i][0], s[i][1]), k2, m2)), b = unf2(fma2(f2(s[i][2], s[i][3]), k2, m2));
+        s[i][0] = ex2(a.x); s[i][1] = ex2(a.y); s[i][2] = ex2(b.x); s[i][3] = ex2(b.y);
+        st.l[i] += (s[i][0] + s[i][1]) + (s[i][2] + s[i][3]);
     }
     uint32_t vd[2][NB], vw[2][NB];
     lane_scales<HD>(sm + 17 * HD, 2 * c, vd[0]);
@@ -427,25 +489,28 @@ __device__ __forceinline__ void kv4_tile(const uint8_t* sm, int lane, int tile0,
                 if (!(any_seen >> (2 * hf + i / NB) & 1u)) vd[hf][i >> 1] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
     }
     {
-        __half2 mx = __habs2(bits_h2(vd[0][0]));
+        // scales below 2 need no care: 2 * 2^8 * (a weight up to 2^6) is 2^15. The exponent's top bit tells the others.
+        uint32_t any = vd[0][0] | vd[1][0];
 #pragma unroll
-        for (int i = 1; i < 2 * NB; ++i) mx = __hmax2(mx, __habs2(bits_h2(vd[i / NB][i % NB])));
-        float a = fmaxf(__low2float(mx), __high2float(mx));
-        if (__any_sync(0xffffffffu, a > st.vlim)) {
-            // larger scales than any so far: a smaller power of two, and the sums follow
+        for (int i = 1; i < NB; ++i) any |= vd[0][i] | vd[1][i];
+        if (__any_sync(0xffffffffu, any & 0x40004000u)) {
+            __half2 mx = __habs2(bits_h2(vd[0][0]));
+#pragma unroll
+            for (int i = 1; i < 2 * NB; ++i) mx = __hmax2(mx, __habs2(bits_h2(vd[i / NB][i % NB])));
+            float a = fmaxf(__low2float(mx), __high2float(mx));
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-            int e = 14 - ilogbf(a);
-            e = e < -1 ? -1 : e;
-            const float nv = ldexpf(1.f, e), f = nv / st.vs;
+            if (a * st.vs > 512.f) {
+                // larger scales than any so far: a smaller power of two, and the sums follow
+                const float nv = ldexpf(1.f, max(8 - ilogbf(a), -7)), f = nv / st.vs;
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+                for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int j = 0; j < HD / 8; ++j)
+                    for (int j = 0; j < HD / 8; ++j)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) st.o[i][j][x] *= f;
-            st.vs = nv;
-            st.vlim = ldexpf(1.f, 15 - e);
+                        for (int x = 0; x < 4; ++x) st.o[i][j][x] *= f;
+                st.vs = nv;
+            }
         }
         const __half2 v2 = __float2half2_rn(st.vs);
 #pragma unroll
@@ -458,31 +523,31 @@ __device__ __forceinline__ void kv4_tile(const uint8_t* sm, int lane, int tile0,
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         uint32_t r0[4], r1[4];
-        unpack8(vw[0][b], r0);
-        unpack8(vw[1][b], r1);
-        const float d0 = scale_of<NB>(vd[0], 0, b), d1 = scale_of<NB>(vd[0], 1, b), d2 = scale_of<NB>(vd[1], 0, b),
-                    d3 = scale_of<NB>(vd[1], 1, b);
+        unpack_signed(vw[0][b], r0);
+        unpack_signed(vw[1][b], r1);
+        const uint64_t d01 = f2(scale_of<NB>(vd[0], 0, b), scale_of<NB>(vd[0], 1, b)),
+                       d23 = f2(scale_of<NB>(vd[1], 0, b), scale_of<NB>(vd[1], 1, b));
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             uint32_t a0, a1, a2, a3;
-            float p0 = s[i][0] * d0, p1 = s[i][1] * d1, p2 = s[i][2] * d2, p3 = s[i][3] * d3;
+            uint64_t p01 = mul2(f2(s[i][0], s[i][1]), d01), p23 = mul2(f2(s[i][2], s[i][3]), d23);
             if (MT > 1 && !full) {          // (a scale that only the lane's other queries see may be NaN)
-                p0 = seen[i] & 1u ? p0 : 0.f;
-                p1 = seen[i] & 2u ? p1 : 0.f;
-                p2 = seen[i] & 4u ? p2 : 0.f;
-                p3 = seen[i] & 8u ? p3 : 0.f;
+                const float2 x = unf2(p01), y = unf2(p23);
+                p01 = f2(seen[i] & 1u ? x.x : 0.f, seen[i] & 2u ? x.y : 0.f);
+                p23 = f2(seen[i] & 4u ? y.x : 0.f, seen[i] & 8u ? y.y : 0.f);
             }
-            split_h2(p0, p1, a0, a1);
-            split_h2(p2, p3, a2, a3);
+            split_h2(p01, a0, a1);
+            split_h2(p23, a2, a3);
 #pragma unroll
             for (int j = 0; j < 4; ++j) mma16816(st.o[i][4 * b + j], a0, a1, a2, a3, r0[j], r1[j]);
         }
     }
 }
 
-// The A fragments of lane (g, c)'s query row (nullptr: zeros): qa[b][s]. Returns the factor that undoes the power of
-// two which brings the row's largest value to 2^13..2^14, where fp16 and its remainder keep 22 bits.
-template <int HD> __device__ __forceinline__ float load_query(const float* x, int lane, float f, uint4 (&qa)[HD / 32][2])
+// The A fragments qa[b][s] of lane (g, c)'s query row (nullptr: zeros) and its terms. A power of two brings the row's largest
+// value to 2^13..2^14, where fp16 and its remainder keep 22 bits.
+template <int HD>
+__device__ __forceinline__ void load_query(const float* x, int lane, float f, uint4 (&qa)[HD / 32][2], QueryTerms<HD / 32>& qt)
 {
     constexpr int NB = HD / 32;
     const int c = lane & 3;
@@ -506,15 +571,23 @@ template <int HD> __device__ __forceinline__ float load_query(const float* x, in
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     int e = mx > 0.f && mx <= 3e38f ? 13 - ilogbf(mx) : 0;
     e = e > 100 ? 100 : e < -100 ? -100 : e;
-    const float up = ldexpf(1.f, e);
+    const float up = ldexpf(1.f, e), up16 = up * 0.0625f;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b) {
+        float sum = 0.f;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            split_h2(v[b][2 * s] * up, v[b][2 * s + 4] * up, qa[b][s].x, qa[b][s].y);
-            split_h2(v[b][2 * s + 1] * up, v[b][2 * s + 5] * up, qa[b][s].z, qa[b][s].w);
+            split_h2(f2(v[b][2 * s] * up, v[b][2 * s + 4] * up), qa[b][s].x, qa[b][s].y);
+            split_h2(f2(v[b][2 * s + 1] * up16, v[b][2 * s + 5] * up16), qa[b][s].z, qa[b][s].w);
+            const float2 h0 = __half22float2(bits_h2(qa[b][s].x)), l0 = __half22float2(bits_h2(qa[b][s].y));
+            const float2 h1 = __half22float2(bits_h2(qa[b][s].z)), l1 = __half22float2(bits_h2(qa[b][s].w));
+            sum += ((h0.x + h0.y) + (l0.x + l0.y)) + 16.f * ((h1.x + h1.y) + (l1.x + l1.y));
         }
-    return ldexpf(1.f, -e);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        qt.off[b] = sum * (8.f / 16777216.f);
+    }
+    qt.ks = ldexpf(1.f, 24 - e);
 }
 
 struct Kv4Att {
@@ -620,8 +693,8 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, HD <= 128 ? 3 : 2) k_kv4_attn(
         for (int s = 0; s < ST && s < mine; ++s) issue(s);
     }
     uint4 qa[NB][2];
-    const float ks[1] = {load_query<HD>(g < nh ? a.q + ((int64_t)t * a.heads + head0 + g) * HD : nullptr, lane,
-                                        a.scale * 1.4426950408889634f, qa)};
+    QueryTerms<NB> qt[1];
+    load_query<HD>(g < nh ? a.q + ((int64_t)t * a.heads + head0 + g) * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa, qt[0]);
     __syncwarp();
     AttState<HD, 1> st;
     st.init();
@@ -630,7 +703,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, HD <= 128 ? 3 : 2) k_kv4_attn(
         if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bars[warp][i % ST], (uint32_t)(i / ST & 1), a.err, 21))) break;
         const int tile0 = tl.at(i0 + warp + ATT_WARPS * i) * KV4_P;
         const bool full = tile0 + KV4_P <= vis[0].n && tile0 >= vis[0].first;
-        kv4_tile<HD, 1>(ring + i % ST * TB, lane, tile0, vis, full, qf, ks, st);
+        kv4_tile<HD, 1>(ring + i % ST * TB, lane, tile0, vis, full, qf, qt, st);
         __syncwarp();
         if (lane == 0 && i + ST < mine) issue(i + ST);
     }
@@ -749,7 +822,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, 2) k_kv4_attn_run(const Kv4Att
     if (threadIdx.x == 0)
         for (int s = 0; s < ST && s < nt; ++s) issue(s);
     Vis vis[MT];
-    float ks[MT];
+    QueryTerms<NB> qt[MT];
     int state[MT];
     int64_t th[MT];             // (row, head) of the lane's query, or -1
     int w_n = 0, w_min_n = INT_MAX, w_first = INT_MAX, w_max_first = 0, w_sink = 0;
@@ -768,7 +841,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, 2) k_kv4_attn_run(const Kv4Att
             if (!state[i]) vis[i] = visible(p, a.window, a.sinks);
         }
         uint4 qa[NB][2];
-        ks[i] = load_query<HD>(th[i] >= 0 ? a.q + th[i] * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa);
+        load_query<HD>(th[i] >= 0 ? a.q + th[i] * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa, qt[i]);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -796,7 +869,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, 2) k_kv4_attn_run(const Kv4Att
         const int tile0 = tl.at(i0 + i) * KV4_P;
         if (tile0 < w_n && (tile0 + KV4_P > w_first || tile0 < w_sink)) {
             const bool full = tile0 + KV4_P <= w_min_n && tile0 >= w_max_first;
-            kv4_tile<HD, MT>(smem + i % ST * TB, lane, tile0, vis, full, qf, ks, st);
+            kv4_tile<HD, MT>(smem + i % ST * TB, lane, tile0, vis, full, qf, qt, st);
         }
         __syncwarp();
         bool ok = true;
