@@ -144,7 +144,9 @@ def test_mixed_steps_and_a_sampled_serving_run(wl):
         mixed = m.forward_mixed(seqs, lists)
         for i, (r, pr) in enumerate(zip(ref, lists)):
             one = solo.forward(pr, seq=r)
-            assert np.abs(mixed[i] - one).max() < 0.03 * one.std(), i
+            # two paths (the tensor-core GEMM here, the matvec there), each with its own flips of 1% of the size: together
+            # sqrt(2) * 1% of the spread, and the largest of 4096 logits lies sqrt(2 ln 4096) = 4.1 of that out: 5.8%
+            assert np.abs(mixed[i] - one).max() < 0.058 * one.std(), i
         assert [s.length for s in seqs] == [len(x) for x in lists]
         # (the prompts took different paths, so that codes at a border may differ: continue from the same caches)
         n = len(lists)

@@ -67,13 +67,66 @@ template <int HD> __device__ __forceinline__ int kv4_word(int half, int lane, in
 // ------------------------------------------------------------------------------------------------------------------
 // append and read
 // ------------------------------------------------------------------------------------------------------------------
-// A thread owns 8 consecutive dims of one head; four threads a block of 32. The rotation of k and the codes are
-// computed in 64 bits: a code's border is a step of the value, so a difference in the last bit of 32 would decide
-// codes, and 64-bit arithmetic costs nothing here (about 30 operations a value against the bytes a row moves).
-template <int HD>
-__global__ void __launch_bounds__(128) k_kv4_append(const float* q, float* q_out, const float* k, const float* v, int T,
-                                                    int heads, int kv_heads, const float* table, int rope_dims, int neox,
-                                                    Kv4Rows rows, const int32_t* pos, int64_t capacity, int q_blocks)
+// q's part: a thread turns 4 consecutive dims (or, with NEOX pairs, 4 and their 4 partners), APP_Q such units, its loads in
+// flight together. k's and v's part: a thread owns 8 consecutive dims of one head; four threads a block of 32. The rotation
+// of k and the codes are computed in 64 bits: a code's border is a step of the value, so a difference in the last bit of
+// 32 would decide codes, and 64-bit arithmetic costs nothing here (about 30 operations a value against the bytes a row
+// moves). VEC: rope_dims is a multiple of 16 and the table 16-byte aligned, so that pairs, partners and angles come in
+// 16-byte loads; otherwise one by one.
+constexpr int APP_Q = 4;
+
+// 4 dims from d of a head's row x into y: rotated (the pairs' first dims of NEOX: both), or copied.
+template <bool VEC>
+__device__ __forceinline__ void rotate4(const float* x, float* y, const float* cs, int d, int rope_dims, bool neox, bool copy)
+{
+    const int half = rope_dims / 2;
+    if (d >= rope_dims) {
+        if (copy) *reinterpret_cast<float4*>(y + d) = *reinterpret_cast<const float4*>(x + d);
+    } else if (VEC && !neox) {
+        const float4 v = *reinterpret_cast<const float4*>(x + d), t = *reinterpret_cast<const float4*>(cs + d);
+        float4 o;
+        o.x = __fsub_rn(__fmul_rn(v.x, t.x), __fmul_rn(v.y, t.y));
+        o.y = __fadd_rn(__fmul_rn(v.x, t.y), __fmul_rn(v.y, t.x));
+        o.z = __fsub_rn(__fmul_rn(v.z, t.z), __fmul_rn(v.w, t.w));
+        o.w = __fadd_rn(__fmul_rn(v.z, t.w), __fmul_rn(v.w, t.z));
+        *reinterpret_cast<float4*>(y + d) = o;
+    } else if (VEC) {
+        if (d >= half) return;              // (the first dims' thread writes both)
+        const float4 v = *reinterpret_cast<const float4*>(x + d), u = *reinterpret_cast<const float4*>(x + d + half);
+        const float4 t0 = *reinterpret_cast<const float4*>(cs + 2 * d), t1 = *reinterpret_cast<const float4*>(cs + 2 * d + 4);
+        float4 o, w;
+        o.x = __fsub_rn(__fmul_rn(v.x, t0.x), __fmul_rn(u.x, t0.y));
+        w.x = __fadd_rn(__fmul_rn(v.x, t0.y), __fmul_rn(u.x, t0.x));
+        o.y = __fsub_rn(__fmul_rn(v.y, t0.z), __fmul_rn(u.y, t0.w));
+        w.y = __fadd_rn(__fmul_rn(v.y, t0.w), __fmul_rn(u.y, t0.z));
+        o.z = __fsub_rn(__fmul_rn(v.z, t1.x), __fmul_rn(u.z, t1.y));
+        w.z = __fadd_rn(__fmul_rn(v.z, t1.y), __fmul_rn(u.z, t1.x));
+        o.w = __fsub_rn(__fmul_rn(v.w, t1.z), __fmul_rn(u.w, t1.w));
+        w.w = __fadd_rn(__fmul_rn(v.w, t1.w), __fmul_rn(u.w, t1.z));
+        *reinterpret_cast<float4*>(y + d) = o;
+        *reinterpret_cast<float4*>(y + d + half) = w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int d0 = d + e;
+            if (d0 >= rope_dims) {
+                if (copy) y[d0] = x[d0];
+                continue;
+            }
+            // the thread of a pair's first dim writes both, so that rotating in place never reads a rotated value
+            if (neox ? d0 >= half : d0 & 1) continue;
+            const int i = neox ? d0 : d0 >> 1, d1 = neox ? d0 + half : d0 + 1;
+            const float c = cs[2 * i], sn = cs[2 * i + 1], x0 = x[d0], x1 = x[d1];
+            y[d0] = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, sn));
+            y[d1] = __fadd_rn(__fmul_rn(x0, sn), __fmul_rn(x1, c));
+        }
+    }
+}
+
+template <int HD, bool VEC>
+__global__ void __launch_bounds__(128, 8) k_kv4_append(const float* q, float* q_out, const float* k, const float* v, int T,
+                                                       int heads, int kv_heads, const float* table, int rope_dims, int neox,
+                                                       Kv4Rows rows, const int32_t* pos, int64_t capacity, int kv_blocks)
 {
     constexpr int CH = HD / 8;              // 8-dim chunks of a head
     pdl_trigger();
@@ -84,37 +137,18 @@ __global__ void __launch_bounds__(128) k_kv4_append(const float* q, float* q_out
         uint8_t* base = rows.base(t);
         if (kv4_row_state(base, p, capacity)) continue;
         const float* cs = table + (int64_t)p * rope_dims;
-        if ((int)blockIdx.x < q_blocks) {
-            const int u = blockIdx.x * 128 + threadIdx.x;
-            if (u >= heads * CH) continue;
-            const int d0 = u % CH * 8;
-            const float* x = q + ((int64_t)t * heads + u / CH) * HD;
-            float* y = q_out + ((int64_t)t * heads + u / CH) * HD;
-            if (d0 >= rope_dims) {
-                if (q_out != q) {
-                    *reinterpret_cast<float4*>(y + d0) = *reinterpret_cast<const float4*>(x + d0);
-                    *reinterpret_cast<float4*>(y + d0 + 4) = *reinterpret_cast<const float4*>(x + d0 + 4);
-                }
-                continue;
-            }
+        if ((int)blockIdx.x >= kv_blocks) {
+            const int u0 = ((int)blockIdx.x - kv_blocks) * 128 * APP_Q + threadIdx.x;
+            const float* x = q + (int64_t)t * heads * HD;
+            float* y = q_out + (int64_t)t * heads * HD;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int d = d0 + e;
-                if (d >= rope_dims) {
-                    if (q_out != q) y[d] = x[d];
-                    continue;
-                }
-                // the thread of a pair's first dim writes both, so that rotating in place never reads a rotated value
-                const bool first = neox ? d < half : (d & 1) == 0;
-                if (!first) continue;
-                const int i = neox ? d : d >> 1, d1 = neox ? d + half : d + 1;
-                const float c = cs[2 * i], sn = cs[2 * i + 1], x0 = x[d], x1 = x[d1];
-                y[d] = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, sn));
-                y[d1] = __fadd_rn(__fmul_rn(x0, sn), __fmul_rn(x1, c));
+            for (int i = 0; i < APP_Q; ++i) {
+                const int u = u0 + 128 * i, h = u / (HD / 4);
+                if (h < heads) rotate4<VEC>(x + h * HD, y + h * HD, cs, u % (HD / 4) * 4, rope_dims, neox != 0, q_out != q);
             }
             continue;
         }
-        const int u = ((int)blockIdx.x - q_blocks) * 128 + threadIdx.x;
+        const int u = blockIdx.x * 128 + threadIdx.x;
         const int units = kv_heads * CH;
         const bool live = u < 2 * units, is_v = u >= units;
         const int uu = live ? (is_v ? u - units : u) : 0;
@@ -125,16 +159,41 @@ __global__ void __launch_bounds__(128) k_kv4_append(const float* q, float* q_out
         *reinterpret_cast<float4*>(xf + 4) = *reinterpret_cast<const float4*>(x + d0 + 4);
         double xd[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            xd[e] = xf[e];
-            const int d = d0 + e;
-            if (!is_v && d < rope_dims) {
-                const bool first = neox ? d < half : (d & 1) == 0;
-                const int i = neox ? (first ? d : d - half) : d >> 1;
-                const double c = cs[2 * i], sn = cs[2 * i + 1];
-                const double o = neox ? (double)x[first ? d + half : d - half] : (double)xf[e ^ 1];
-                // products of 24-bit factors are exact in 53 bits, so one rounding follows either way
-                xd[e] = first ? xd[e] * c - o * sn : o * sn + xd[e] * c;
+        for (int e = 0; e < 8; ++e) xd[e] = xf[e];
+        if (!is_v && d0 < rope_dims) {
+            // products of 24-bit factors are exact in 53 bits, so one rounding follows, with or without fma
+            if (VEC && neox) {
+                const bool first = d0 < half;
+                const int i0 = first ? d0 : d0 - half;
+                const float* o = x + (first ? d0 + half : d0 - half);
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float4 t2 = *reinterpret_cast<const float4*>(cs + 2 * (i0 + e));
+                    const float2 o2 = *reinterpret_cast<const float2*>(o + e);
+                    xd[e] = first ? xd[e] * t2.x - (double)o2.x * t2.y : (double)o2.x * t2.y + xd[e] * t2.x;
+                    xd[e + 1] = first ? xd[e + 1] * t2.z - (double)o2.y * t2.w : (double)o2.y * t2.w + xd[e + 1] * t2.z;
+                }
+            } else if (VEC) {
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    const float4 t2 = *reinterpret_cast<const float4*>(cs + d0 + e);
+                    const double a = xd[e], b = xd[e + 1], g = xd[e + 2], r = xd[e + 3];
+                    xd[e] = a * t2.x - b * t2.y;
+                    xd[e + 1] = a * t2.y + b * t2.x;
+                    xd[e + 2] = g * t2.z - r * t2.w;
+                    xd[e + 3] = g * t2.w + r * t2.z;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int d = d0 + e;
+                    if (d >= rope_dims) continue;
+                    const bool first = neox ? d < half : (d & 1) == 0;
+                    const int i = neox ? (first ? d : d - half) : d >> 1;
+                    const double c = cs[2 * i], sn = cs[2 * i + 1];
+                    const double o = neox ? (double)x[first ? d + half : d - half] : (double)xf[e ^ 1];
+                    xd[e] = first ? xd[e] * c - o * sn : o * sn + xd[e] * c;
+                }
             }
         }
         double hi = xd[0], lo = xd[0];
@@ -231,12 +290,18 @@ __device__ __forceinline__ float ex2(float x)
     return y;
 }
 
+// D = A B and D += A B for m16n8k16 in fp16 with fp32 sums.
 __device__ __forceinline__ void mma_zero(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                 "{%10,%10,%10,%10};\n"
-                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_add(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 
 // (w & mask) | bits in one instruction.
@@ -410,22 +475,23 @@ template <int NB> struct QueryTerms {
     float ks, off[NB];
 };
 
-// One tile of 16 positions for MT query tiles. qf(i, b, s) gives the A fragment of query tile i, block b, step s (dims
-// 32 b + 8 c + {2s, 2s + 4} of lane c, and, divided by 16, {2s + 1, 2s + 5}).
-template <int HD, int MT, class QF>
-__device__ __forceinline__ void kv4_tile(const uint8_t* sm, int lane, int tile0, const Vis (&vis)[MT], bool full, const QF& qf,
-                                         const QueryTerms<HD / 32> (&qt)[MT], AttState<HD, MT>& st)
+// NT tiles of 16 positions (from positions tile0[.], one behind the other at sm) for MT query tiles. qf(i, b, s) gives the A
+// fragment of query tile i, block b, step s (dims 32 b + 8 c + {2s, 2s + 4} of lane c, and, divided by 16, {2s + 1, 2s + 5}).
+template <int HD, int MT, int NT, class QF>
+__device__ __forceinline__ void kv4_tiles(const uint8_t* sm, int lane, const int (&tile0)[NT], const Vis (&vis)[MT], bool full,
+                                          const QF& qf, const QueryTerms<HD / 32> (&qt)[MT], AttState<HD, MT>& st)
 {
-    constexpr int NB = HD / 32;
+    constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD);
     const int c = lane & 3;
-    uint64_t s2[MT][2];                     // scores of positions (2c, 2c + 1) and (2c + 8, 2c + 9), in the query's units
+    uint64_t s2[MT][2 * NT];                // scores of positions (2c, 2c + 1) and (2c + 8, 2c + 9), in the query's units
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int h = 0; h < 2 * NT; ++h) {
+        const uint8_t* t = sm + h / 2 * TB;
         uint32_t kw[NB], dw[NB];
-        lane_words<HD>(sm, half, lane, kw);
-        lane_scales<HD>(sm + 16 * HD, 8 * half + 2 * c, dw);
+        lane_words<HD>(t, h & 1, lane, kw);
+        lane_scales<HD>(t + 16 * HD, 8 * (h & 1) + 2 * c, dw);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) s2[i][half] = f2(0.f, 0.f);
+        for (int i = 0; i < MT; ++i) s2[i][h] = f2(0.f, 0.f);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             uint32_t r[4];
@@ -435,31 +501,35 @@ __device__ __forceinline__ void kv4_tile(const uint8_t* sm, int lane, int tile0,
             for (int i = 0; i < MT; ++i) {
                 float d[4];
                 mma_zero(d, qf(i, b, 0), r[0], r[1]);
-                const uint4 a = qf(i, b, 1);
-                mma16816(d, a.x, a.y, a.z, a.w, r[2], r[3]);
+                mma_add(d, qf(i, b, 1), r[2], r[3]);
                 const uint64_t u = add2(add2(f2(d[0], d[1]), f2(d[2], d[3])), f2(-qt[i].off[b], -qt[i].off[b]));
-                s2[i][half] = fma2(d01, u, s2[i][half]);
+                s2[i][h] = fma2(d01, u, s2[i][h]);
             }
         }
     }
-    float s[MT][4];                         // then the weights
-    uint32_t seen[MT], any_seen = 0u;       // bits of the positions that this lane's queries see
+    uint32_t seen[MT], any_seen = 0u;       // bits (4 a tile) of the positions that this lane's queries see
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        {
-            const float2 a = unf2(s2[i][0]), b = unf2(s2[i][1]);
-            s[i][0] = a.x; s[i][1] = a.y; s[i][2] = b.x; s[i][3] = b.y;
-        }
         if (!full) {
             seen[i] = 0u;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (vis[i](tile0 + 2 * c + (e & 1) + 8 * (e >> 1))) seen[i] |= 1u << e;
-                else s[i][e] = -INFINITY;
+            for (int h = 0; h < 2 * NT; ++h) {
+                float2 x = unf2(s2[i][h]);
+                const int j = tile0[h / 2] + 2 * c + 8 * (h & 1);
+                if (vis[i](j)) seen[i] |= 1u << (2 * h);
+                else x.x = -INFINITY;
+                if (vis[i](j + 1)) seen[i] |= 2u << (2 * h);
+                else x.y = -INFINITY;
+                s2[i][h] = f2(x.x, x.y);
             }
             any_seen |= seen[i];
         }
-        float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+        float mx = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2 * NT; ++h) {
+            const float2 x = unf2(s2[i][h]);
+            mx = fmaxf(mx, fmaxf(x.x, x.y));
+        }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * qt[i].ks;
         if (__any_sync(0xffffffffu, mx > st.m[i] + ATT_SLACK)) {
@@ -473,22 +543,28 @@ __device__ __forceinline__ void kv4_tile(const uint8_t* sm, int lane, int tile0,
         }
         const float mu = st.m[i] == -INFINITY ? 0.f : st.m[i];
         const uint64_t k2 = f2(qt[i].ks, qt[i].ks), m2 = f2(-mu, -mu);
-        const float2 a = unf2(fma2(f2(s[i][0], s[i][1]), k2, m2)), b = unf2(fma2(f2(s[i][2], s[i][3]), k2, m2));
-        s[i][0] = ex2(a.x); s[i][1] = ex2(a.y); s[i][2] = ex2(b.x); s[i][3] = ex2(b.y);
-        st.l[i] += (s[i][0] + s[i][1]) + (s[i][2] + s[i][3]);
-    }
-    uint32_t vd[2][NB], vw[2][NB];
-    lane_scales<HD>(sm + 17 * HD, 2 * c, vd[0]);
-    lane_scales<HD>(sm + 17 * HD, 2 * c + 8, vd[1]);
-    if (!full) {
-        // a position that no query of this lane sees may hold anything: its scales (perhaps NaN) count as zero
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-            for (int i = 0; i < 2 * NB; ++i)
-                if (!(any_seen >> (2 * hf + i / NB) & 1u)) vd[hf][i >> 1] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+        for (int h = 0; h < 2 * NT; ++h) {
+            const float2 x = unf2(fma2(s2[i][h], k2, m2));
+            const float p0 = ex2(x.x), p1 = ex2(x.y);
+            st.l[i] += p0 + p1;
+            s2[i][h] = f2(p0, p1);          // now the weights
+        }
     }
-    {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const uint8_t* t = sm + n * TB;
+        uint32_t vd[2][NB], vw[2][NB];
+        lane_scales<HD>(t + 17 * HD, 2 * c, vd[0]);
+        lane_scales<HD>(t + 17 * HD, 2 * c + 8, vd[1]);
+        if (!full) {
+            // a position that no query of this lane sees may hold anything: its scales (perhaps NaN) count as zero
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                for (int i = 0; i < 2 * NB; ++i)
+                    if (!(any_seen >> (4 * n + 2 * hf + i / NB) & 1u)) vd[hf][i >> 1] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+        }
         // scales below 2 need no care: 2 * 2^8 * (a weight up to 2^6) is 2^15. The exponent's top bit tells the others.
         uint32_t any = vd[0][0] | vd[1][0];
 #pragma unroll
@@ -517,29 +593,30 @@ __device__ __forceinline__ void kv4_tile(const uint8_t* sm, int lane, int tile0,
         for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
             for (int i = 0; i < NB; ++i) vd[hf][i] = h2_bits(__hmul2(bits_h2(vd[hf][i]), v2));
-    }
-    lane_words<HD>(sm + 8 * HD, 0, lane, vw[0]);
-    lane_words<HD>(sm + 8 * HD, 1, lane, vw[1]);
+        lane_words<HD>(t + 8 * HD, 0, lane, vw[0]);
+        lane_words<HD>(t + 8 * HD, 1, lane, vw[1]);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        uint32_t r0[4], r1[4];
-        unpack_signed(vw[0][b], r0);
-        unpack_signed(vw[1][b], r1);
-        const uint64_t d01 = f2(scale_of<NB>(vd[0], 0, b), scale_of<NB>(vd[0], 1, b)),
-                       d23 = f2(scale_of<NB>(vd[1], 0, b), scale_of<NB>(vd[1], 1, b));
+        for (int b = 0; b < NB; ++b) {
+            uint32_t r0[4], r1[4];
+            unpack_signed(vw[0][b], r0);
+            unpack_signed(vw[1][b], r1);
+            const uint64_t d01 = f2(scale_of<NB>(vd[0], 0, b), scale_of<NB>(vd[0], 1, b)),
+                           d23 = f2(scale_of<NB>(vd[1], 0, b), scale_of<NB>(vd[1], 1, b));
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            uint32_t a0, a1, a2, a3;
-            uint64_t p01 = mul2(f2(s[i][0], s[i][1]), d01), p23 = mul2(f2(s[i][2], s[i][3]), d23);
-            if (MT > 1 && !full) {          // (a scale that only the lane's other queries see may be NaN)
-                const float2 x = unf2(p01), y = unf2(p23);
-                p01 = f2(seen[i] & 1u ? x.x : 0.f, seen[i] & 2u ? x.y : 0.f);
-                p23 = f2(seen[i] & 4u ? y.x : 0.f, seen[i] & 8u ? y.y : 0.f);
+            for (int i = 0; i < MT; ++i) {
+                uint4 a;
+                uint64_t p01 = mul2(s2[i][2 * n], d01), p23 = mul2(s2[i][2 * n + 1], d23);
+                if (MT > 1 && !full) {      // (a scale that only the lane's other queries see may be NaN)
+                    const uint32_t see = seen[i] >> (4 * n);
+                    const float2 x = unf2(p01), y = unf2(p23);
+                    p01 = f2(see & 1u ? x.x : 0.f, see & 2u ? x.y : 0.f);
+                    p23 = f2(see & 4u ? y.x : 0.f, see & 8u ? y.y : 0.f);
+                }
+                split_h2(p01, a.x, a.y);
+                split_h2(p23, a.z, a.w);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma_add(st.o[i][4 * b + j], a, r0[j], r1[j]);
             }
-            split_h2(p01, a0, a1);
-            split_h2(p23, a2, a3);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mma16816(st.o[i][4 * b + j], a0, a1, a2, a3, r0[j], r1[j]);
         }
     }
 }
@@ -605,33 +682,69 @@ struct Kv4Att {
     int* err;
 };
 
-constexpr int ATT_WARPS = 4;                // warps of an attention CTA
-constexpr int ATT_TPS = 16;                 // tiles a range holds at least (when a row has more than one)
-constexpr int att_stages(int HD) { return HD <= 128 ? 4 : 3; }
+// A CTA of 8 warps, two an SM (128 registers, the queries' fragments in shared memory): against three CTAs of 4 warps with the
+// fragments in registers, one row over 131000 positions 52.8 against 55.6 us (fewer ranges to join), 8 rows of up to 4100
+// 15.5 against 19.1. A range holds 48 tiles at least: 6 to a warp.
+constexpr int ATT_WARPS = 8;
+constexpr int RUN_WARPS = 4;                // warps of a CTA of the runs' kernel
+constexpr int ATT_TPS = 48;
+constexpr int ATT_STAGES = 2;               // ring stages a warp, of two tiles each
+constexpr int att_ctas(int HD) { return HD <= 128 ? 2 : 1; }
+constexpr int ATT_MAX_RANGES = 96;
 
-// Joins the `n` ranges of (row t, head) for 4 output values at dim d, in range order.
-template <int HD>
-__device__ __forceinline__ float4 join_ranges(const Kv4Att& a, int64_t th, int n, int d)
+// Joins the n ranges of nh rows of heads (the i-th at (row, head) index row(i)) in range order, by a CTA of NT threads:
+// a warp takes a head's weights at a time, then every thread takes 4 output values at a time, its loads of 8 ranges in
+// flight together. w: nh * n floats of shared memory.
+template <int HD, int NT, class F> __device__ __forceinline__ void join_ranges(const Kv4Att& a, int nh, int n, float* w, const F& row)
 {
-    const float2* ml = reinterpret_cast<const float2*>(a.ml) + th * a.S;
-    const float* pp = a.part + th * a.S * HD + d;
-    float M = -INFINITY;
-    for (int s = 0; s < n; ++s) M = fmaxf(M, __ldcg(ml + s).x);
-    const float mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < n; ++s) {
-        const float2 x = __ldcg(ml + s);
-        const float4 p = __ldcg(reinterpret_cast<const float4*>(pp + (int64_t)s * HD));
-        const float w = ex2(x.x - mu);
-        L += w * x.y;
-        o0 += w * p.x;
-        o1 += w * p.y;
-        o2 += w * p.z;
-        o3 += w * p.w;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int h = warp; h < nh; h += NT / 32) {
+        const float2* ml = reinterpret_cast<const float2*>(a.ml) + row(h) * a.S;
+        float2 x[ATT_MAX_RANGES / 32];
+        float M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < ATT_MAX_RANGES / 32; ++i) {
+            const int s = lane + 32 * i;
+            x[i] = s < n ? __ldcg(ml + s) : make_float2(-INFINITY, 0.f);
+            M = fmaxf(M, x[i].x);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float mu = M == -INFINITY ? 0.f : M;
+        float L = 0.f;
+#pragma unroll
+        for (int i = 0; i < ATT_MAX_RANGES / 32; ++i) {
+            x[i].x = ex2(x[i].x - mu);
+            L += x[i].x * x[i].y;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        const float inv = L != 0.f ? 1.f / L : 0.f;     // (a NaN sum stays NaN; no visible position: zeros)
+#pragma unroll
+        for (int i = 0; i < ATT_MAX_RANGES / 32; ++i)
+            if (lane + 32 * i < n) w[h * n + lane + 32 * i] = x[i].x * inv;
     }
-    const float inv = L != 0.f ? 1.f / L : 0.f;     // (a NaN sum stays NaN; no visible position: zeros)
-    return make_float4(o0 * inv, o1 * inv, o2 * inv, o3 * inv);
+    __syncthreads();
+    for (int i = threadIdx.x; i < nh * (HD / 4); i += NT) {
+        const int h = i / (HD / 4), d = i % (HD / 4) * 4;
+        const float4* pp = reinterpret_cast<const float4*>(a.part + row(h) * a.S * HD + d);
+        const float* wh = w + h * n;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s0 = 0; s0 < n; s0 += 8) {
+            float4 p[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) p[k] = s0 + k < n ? __ldcg(pp + (int64_t)(s0 + k) * (HD / 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float f = s0 + k < n ? wh[s0 + k] : 0.f;
+                o.x += f * p[k].x;
+                o.y += f * p[k].y;
+                o.z += f * p[k].z;
+                o.w += f * p[k].w;
+            }
+        }
+        *reinterpret_cast<float4*>(a.out + row(h) * HD + d) = o;
+    }
 }
 
 // Takes a ticket after the CTA's partials; true in the CTA that took the last of n.
@@ -650,12 +763,12 @@ __device__ __forceinline__ bool last_ticket(int* ctr, int n)
 }
 
 // Rows on their own (decode): CTA (range, KV head and tile of 8 query heads, row); each warp streams its own tiles, every
-// fourth of the range, through its ring of bulk copies, and the warps' sums are joined in warp order. The ranges follow
+// fourth pair of the range, through its ring of bulk copies, and the warps' sums are joined in warp order. The ranges follow
 // from the row's own length, so a row's bits do not depend on the other rows.
 template <int HD>
-__global__ void __launch_bounds__(32 * ATT_WARPS, HD <= 128 ? 3 : 2) k_kv4_attn(const Kv4Att a)
+__global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const Kv4Att a)
 {
-    constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD), ST = att_stages(HD), NT = 32 * ATT_WARPS;
+    constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD), ST = ATT_STAGES, NT = 32 * ATT_WARPS;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[ATT_WARPS][ST];
     __shared__ float sm_m[ATT_WARPS][8], sm_l[ATT_WARPS][8];
@@ -679,33 +792,53 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, HD <= 128 ? 3 : 2) k_kv4_attn(
     const int S = min(a.s_max, (tl.count + ATT_TPS - 1) / ATT_TPS);
     if (sp >= S) return;
     const int i0 = (int)((int64_t)tl.count * sp / S), i1 = (int)((int64_t)tl.count * (sp + 1) / S);
-    const int mine = (i1 - i0 - warp + ATT_WARPS - 1) / ATT_WARPS;      // tiles i0 + warp, + 4, ...
-    uint8_t* ring = smem + warp * ST * TB;
+    // the warp's steps of two tiles: items i0 + 2 (warp + 4 i) and the next of the list
+    const int steps = ((i1 - i0 + 1) / 2 - warp + ATT_WARPS - 1) / ATT_WARPS;
+    uint8_t* ring = smem + warp * ST * 2 * TB;
     const uint8_t* src = base + (int64_t)kvh * TB;
     auto issue = [&](int i) {
         uint64_t* bar = &bars[warp][i % ST];
-        mbar_expect_tx(bar, TB);
-        bulk_load(ring + i % ST * TB, src + (int64_t)tl.at(i0 + warp + ATT_WARPS * i) * a.kv_heads * TB, TB, bar);
+        const int at = i0 + 2 * (warp + ATT_WARPS * i), two = at + 1 < i1;
+        mbar_expect_tx(bar, two ? 2 * TB : TB);
+        bulk_load(ring + i % ST * 2 * TB, src + (int64_t)tl.at(at) * a.kv_heads * TB, TB, bar);
+        if (two) bulk_load(ring + i % ST * 2 * TB + TB, src + (int64_t)tl.at(at + 1) * a.kv_heads * TB, TB, bar);
     };
     if (lane == 0) {
         for (int s = 0; s < ST; ++s) mbar_init(&bars[warp][s], 1);
         fence_mbar_init();
-        for (int s = 0; s < ST && s < mine; ++s) issue(s);
+        for (int s = 0; s < ST && s < steps; ++s) issue(s);
     }
-    uint4 qa[NB][2];
     QueryTerms<NB> qt[1];
-    load_query<HD>(g < nh ? a.q + ((int64_t)t * a.heads + head0 + g) * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa, qt[0]);
-    __syncwarp();
+    // the queries' fragments and terms, made by one warp
+    __shared__ __align__(16) uint4 sq[NB * 2 * 32];
+    __shared__ float sqt[(NB + 1) * 32];
+    if (warp == 0) {
+        uint4 qa[NB][2];
+        load_query<HD>(g < nh ? a.q + ((int64_t)t * a.heads + head0 + g) * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa, qt[0]);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            sq[b * 64 + lane] = qa[b][0];
+            sq[b * 64 + 32 + lane] = qa[b][1];
+            sqt[b * 32 + lane] = qt[0].off[b];
+        }
+        sqt[NB * 32 + lane] = qt[0].ks;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NB; ++b) qt[0].off[b] = sqt[b * 32 + lane];
+    qt[0].ks = sqt[NB * 32 + lane];
+    auto qf = [&](int, int b, int s) { return sq[b * 64 + s * 32 + lane]; };
     AttState<HD, 1> st;
     st.init();
-    auto qf = [&](int, int b, int s) { return qa[b][s]; };
-    for (int i = 0; i < mine; ++i) {
+    for (int i = 0; i < steps; ++i) {
         if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bars[warp][i % ST], (uint32_t)(i / ST & 1), a.err, 21))) break;
-        const int tile0 = tl.at(i0 + warp + ATT_WARPS * i) * KV4_P;
-        const bool full = tile0 + KV4_P <= vis[0].n && tile0 >= vis[0].first;
-        kv4_tile<HD, 1>(ring + i % ST * TB, lane, tile0, vis, full, qf, qt, st);
+        const int at = i0 + 2 * (warp + ATT_WARPS * i);
+        // (of an odd range's last step the second tile is not there: a position that no row sees)
+        const int tile0[2] = {tl.at(at) * KV4_P, at + 1 < i1 ? tl.at(at + 1) * KV4_P : INT_MAX - KV4_P};
+        const bool full = tile0[0] >= vis[0].first && tile0[1] < vis[0].n - KV4_P + 1;
+        kv4_tiles<HD, 1, 2>(ring + i % ST * 2 * TB, lane, tile0, vis, full, qf, qt, st);
         __syncwarp();
-        if (lane == 0 && i + ST < mine) issue(i + ST);
+        if (lane == 0 && i + ST < steps) issue(i + ST);
     }
     // the warps' sums, joined through the ring's memory (every copy has landed and been read)
     st.l[0] += __shfl_xor_sync(0xffffffffu, st.l[0], 1);
@@ -758,20 +891,17 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, HD <= 128 ? 3 : 2) k_kv4_attn(
     }
     if (S == 1) return;
     if (!last_ticket(a.tickets + t * gridDim.y + blockIdx.y, S)) return;
-    for (int i = threadIdx.x; i < nh * HD / 4; i += NT) {
-        const int h = i / (HD / 4), d = i % (HD / 4) * 4;
-        const int64_t th = (int64_t)t * a.heads + head0 + h;
-        *reinterpret_cast<float4*>(a.out + th * HD + d) = join_ranges<HD>(a, th, S, d);
-    }
+    const int64_t th0 = (int64_t)t * a.heads + head0;
+    join_ranges<HD, NT>(a, nh, S, so, [&](int h) { return th0 + h; });
 }
 
 // Runs of R rows that read one cache (prompts): the (row, head) pairs of a run and KV head are queries 0 .. R G - 1; a CTA
 // takes QB of them, each warp MT tiles of 8, and all warps share each tile of the cache (one ring of bulk copies), so
 // a tile's codes are unpacked once for 8 MT queries.
 template <int HD, int MT>
-__global__ void __launch_bounds__(32 * ATT_WARPS, 2) k_kv4_attn_run(const Kv4Att a, int q_blocks)
+__global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att a, int q_blocks)
 {
-    constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD), ST = 4, QW = 8 * MT, QB = ATT_WARPS * QW;
+    constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD), ST = 4, QW = 8 * MT, QB = RUN_WARPS * QW;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t fullb[ST], emptyb[ST];
     __shared__ int rng[4];
@@ -793,7 +923,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, 2) k_kv4_attn_run(const Kv4Att
     __syncthreads();
     {
         const int r0 = q0 / G, r1 = min(a.R - 1, (min(q0 + QB, nq) - 1) / G);
-        for (int r = r0 + threadIdx.x; r <= r1; r += 32 * ATT_WARPS) {
+        for (int r = r0 + threadIdx.x; r <= r1; r += 32 * RUN_WARPS) {
             const int p = a.pos[run * a.R + r];
             if (kv4_row_state(base, p, a.capacity)) continue;
             const Vis v = visible(p, a.window, a.sinks);
@@ -805,7 +935,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, 2) k_kv4_attn_run(const Kv4Att
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; ++s) {
             mbar_init(&fullb[s], 1);
-            mbar_init(&emptyb[s], ATT_WARPS);
+            mbar_init(&emptyb[s], RUN_WARPS);
         }
         fence_mbar_init();
     }
@@ -869,7 +999,8 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, 2) k_kv4_attn_run(const Kv4Att
         const int tile0 = tl.at(i0 + i) * KV4_P;
         if (tile0 < w_n && (tile0 + KV4_P > w_first || tile0 < w_sink)) {
             const bool full = tile0 + KV4_P <= w_min_n && tile0 >= w_max_first;
-            kv4_tile<HD, MT>(smem + i % ST * TB, lane, tile0, vis, full, qf, qt, st);
+            const int t0[1] = {tile0};
+            kv4_tiles<HD, MT, 1>(smem + i % ST * TB, lane, t0, vis, full, qf, qt, st);
         }
         __syncwarp();
         bool ok = true;
@@ -906,12 +1037,9 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, 2) k_kv4_attn_run(const Kv4Att
     }
     if (S == 1) return;
     if (!last_ticket(a.tickets + ((int64_t)run * a.kv_heads + kvh) * q_blocks + qb, S)) return;
-    for (int i = threadIdx.x; i < QB * HD / 4; i += 32 * ATT_WARPS) {
-        const int qi = q0 + i / (HD / 4), d = i % (HD / 4) * 4;
-        if (qi >= nq) break;
-        const int64_t x = ((int64_t)run * a.R + qi / G) * a.heads + kvh * G + qi % G;
-        *reinterpret_cast<float4*>(a.out + x * HD + d) = join_ranges<HD>(a, x, S, d);
-    }
+    join_ranges<HD, 32 * RUN_WARPS>(a, min(QB, nq - q0), S, reinterpret_cast<float*>(smem), [&](int i) {
+        return ((int64_t)run * a.R + (q0 + i) / G) * a.heads + kvh * G + (q0 + i) % G;
+    });
 }
 
 constexpr int64_t KV4_TICKETS = 1 << 18;    // tickets at the head of a workspace (zero between calls)
@@ -932,7 +1060,7 @@ Kv4Plan kv4_plan(int T, int R, int heads, int kv_heads, int head_dim, int64_t ca
     if (window > 0) tiles = std::min<int64_t>(tiles, ((int64_t)window + 15) / 16 + 1 + ((int64_t)sinks + 15) / 16);
     p.runs = R > 8;
     p.MT = head_dim <= 128 ? 2 : 1;
-    const int QB = ATT_WARPS * 8 * p.MT;
+    const int QB = RUN_WARPS * 8 * p.MT;
     p.q_blocks = (int)(((int64_t)R * G + QB - 1) / QB);
     int64_t ctas;
     if (p.runs) {
@@ -942,9 +1070,9 @@ Kv4Plan kv4_plan(int T, int R, int heads, int kv_heads, int head_dim, int64_t ca
         p.S = p.s_max;
     } else {
         // the most ranges of one row, from the shape alone (a row's bits must not depend on the others): one row's
-        // CTAs fill the SMs three deep. Beyond 64 rows the rows alone do.
+        // CTAs fill the SMs two deep. Beyond 64 rows the rows alone do.
         ctas = (int64_t)T * kv_heads * p.MG;
-        p.s_max = T > 64 ? 1 : std::max(1, std::min(64, 3 * 148 / (kv_heads * p.MG)));
+        p.s_max = T > 64 ? 1 : std::max(1, std::min(ATT_MAX_RANGES, 2 * 148 / (kv_heads * p.MG)));
         p.S = (int)std::max<int64_t>(1, std::min<int64_t>(p.s_max, (tiles + ATT_TPS - 1) / ATT_TPS));
     }
     if (ctas > KV4_TICKETS) p.S = p.s_max = 1;
@@ -961,8 +1089,8 @@ template <typename K> void set_smem(K kern, size_t bytes)
 
 template <int HD> void attn_rows(const Kv4Att& a, const Kv4Plan& p, cudaStream_t s)
 {
-    const size_t smem = (size_t)ATT_WARPS * att_stages(HD) * kv4_tile_bytes(HD);
-    static_assert(ATT_WARPS * att_stages(HD) * kv4_tile_bytes(HD) >= ATT_WARPS * 8 * HD * 4, "the warps' sums fit the ring");
+    const size_t smem = (size_t)ATT_WARPS * ATT_STAGES * 2 * kv4_tile_bytes(HD);
+    static_assert(ATT_WARPS * ATT_STAGES * 2 * kv4_tile_bytes(HD) >= ATT_WARPS * 8 * HD * 4, "the warps' sums fit the ring");
     set_smem(k_kv4_attn<HD>, smem);
     launch(k_kv4_attn<HD>, dim3(p.S, a.kv_heads * p.MG, a.T), dim3(32 * ATT_WARPS), smem, s, a);
     note_launch();
@@ -971,9 +1099,9 @@ template <int HD> void attn_rows(const Kv4Att& a, const Kv4Plan& p, cudaStream_t
 template <int HD> void attn_runs(const Kv4Att& a, const Kv4Plan& p, cudaStream_t s)
 {
     constexpr int MT = HD <= 128 ? 2 : 1;
-    const size_t smem = 4 * kv4_tile_bytes(HD) + (size_t)ATT_WARPS * MT * (HD / 32) * 2 * 512;
+    const size_t smem = 4 * kv4_tile_bytes(HD) + (size_t)RUN_WARPS * MT * (HD / 32) * 2 * 512;
     set_smem(k_kv4_attn_run<HD, MT>, smem);
-    launch(k_kv4_attn_run<HD, MT>, dim3(p.q_blocks * p.S, a.kv_heads, a.T / a.R), dim3(32 * ATT_WARPS), smem, s, a, p.q_blocks);
+    launch(k_kv4_attn_run<HD, MT>, dim3(p.q_blocks * p.S, a.kv_heads, a.T / a.R), dim3(32 * RUN_WARPS), smem, s, a, p.q_blocks);
     note_launch();
 }
 
@@ -981,10 +1109,11 @@ template <int HD>
 void append_hd(const float* q, float* q_out, const float* k, const float* v, int T, int heads, int kv_heads, const float* table,
                int rope_dims, int neox, const Kv4Rows& rows, const int32_t* pos, int64_t capacity, cudaStream_t s)
 {
-    const int q_blocks = rope_dims > 0 || q_out != q ? (heads * (HD / 8) + 127) / 128 : 0;
     const int kv_blocks = (2 * kv_heads * (HD / 8) + 127) / 128;
-    launch(k_kv4_append<HD>, dim3(q_blocks + kv_blocks, std::min(T, 65535)), dim3(128), 0, s, q, q_out, k, v, T, heads, kv_heads,
-           table, rope_dims, neox, rows, pos, capacity, q_blocks);
+    const int q_blocks = rope_dims > 0 || q_out != q ? (heads * (HD / 4) + 128 * APP_Q - 1) / (128 * APP_Q) : 0;
+    const bool vec = rope_dims % 16 == 0 && (uintptr_t)table % 16 == 0;
+    launch(vec ? k_kv4_append<HD, true> : k_kv4_append<HD, false>, dim3(kv_blocks + q_blocks, std::min(T, 65535)), dim3(128), 0, s, q, q_out,
+           k, v, T, heads, kv_heads, table, rope_dims, neox, rows, pos, capacity, kv_blocks);
     note_launch();
 }
 
