@@ -179,6 +179,25 @@ def test_attention_of_runs(wl, heads, kv_heads, hd, window, sinks):
     assert wl.lib().wl_kernel_status(0) == 0
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd", [(16, 2, 128), (8, 2, 64), (20, 4, 128), (7, 7, 64)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 17)])
+def test_attention_of_long_runs(wl, heads, kv_heads, hd, window, sinks):
+    """Several CTAs of queries a run, several steps of positions, ranges of a long cache joined, positions in any order."""
+    rng = np.random.default_rng(heads + window)
+    for rows, start, shuffle in ((130, 0, False), (130, 1000, True), (97, 2611, False)):
+        c, raw = filled(rng, 1, kv_heads, hd, start + rows + 5, [start + rows])
+        pos = [start + r for r in range(rows)]
+        if shuffle:
+            rng.shuffle(pos)
+            pos[17] = -1
+        q = rng.standard_normal((rows, heads, hd)).astype(np.float32) * 2
+        out = attend(wl, c, [0] * rows, pos, q, window, sinks, runs=rows)
+        check(out, q, raw, kv_heads, hd, [0] * rows, pos, window, sinks)
+        again = attend(wl, c, [0] * rows, pos, q, window, sinks, runs=rows)
+        assert np.array_equal(out.view(np.uint32), again.view(np.uint32))
+    assert wl.lib().wl_kernel_status(0) == 0
+
+
 def test_refused_rows_give_nan_and_leave_the_others(wl):
     rng = np.random.default_rng(8)
     heads, kv_heads, hd = 8, 2, 128
@@ -196,10 +215,10 @@ def test_refused_rows_give_nan_and_leave_the_others(wl):
     assert np.isnan(out[4]).all() and (out[7] == 0).all()
 
 
-@pytest.mark.parametrize("runs", [1, 20])
-def test_a_nan_reaches_only_the_rows_that_see_it(wl, runs):
+@pytest.mark.parametrize("runs,heads,hd", [(1, 8, 64), (20, 8, 64), (20, 32, 64), (20, 16, 128)])
+def test_a_nan_reaches_only_the_rows_that_see_it(wl, runs, heads, hd):
     rng = np.random.default_rng(runs)
-    heads, kv_heads, hd = 8, 2, 64
+    kv_heads = 2
     c, raw = filled(rng, 1, kv_heads, hd, 64, [60])
     bad = 47
     R.write(raw[0], kv_heads, hd, bad, np.zeros((kv_heads, hd), int), np.full((kv_heads, hd // 32), np.nan, np.float16), True)

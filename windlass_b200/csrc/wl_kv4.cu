@@ -20,49 +20,12 @@
 // block scales are applied outside: to each block's fp32 sums for the scores, and to the weights before they are split
 // for the values (p * d, per block). So the codes' rounding is the only one below fp32.
 #include <algorithm>
-#include <climits>
-#include <cstdint>
-#include <cuda_fp16.h>
-#include "wl_common.h"
-#include "wl_kernels.h"
-#include "wl_launch.cuh"
-#include "wl_mma.cuh"
+#include "wl_kv4.cuh"
 
 namespace wl {
 namespace k {
 
 namespace {
-
-constexpr int KV4_P = 16;                   // positions per tile
-constexpr int kv4_tile_bytes(int HD) { return 18 * HD; }
-
-// Cache of row t: its base pointer (a RowKV with a layer offset, or a bare array of pointers).
-struct Kv4Rows {
-    const uint8_t* p;
-    int pitch, layer;
-    __device__ __forceinline__ uint8_t* base(int t) const
-    {
-        const uint8_t* e = p + (int64_t)t * pitch;
-        uint8_t* b = *reinterpret_cast<uint8_t* const*>(e);
-        if (pitch == (int)sizeof(RowKV)) b += (int64_t)layer * reinterpret_cast<const RowKV*>(e)->layer_stride * 2;
-        return b;
-    }
-};
-
-// A row's state: 0 live, 1 padding (position < 0: nothing is read or written for it), 2 refused (a position past the
-// cache, a null or misaligned cache).
-__device__ __forceinline__ int kv4_row_state(const uint8_t* base, int64_t p, int64_t capacity)
-{
-    if (p < 0) return 1;
-    return p >= capacity || !base || ((uintptr_t)base & 15) ? 2 : 0;
-}
-
-// Word index of (half, lane, block) in a code area.
-template <int HD> __device__ __forceinline__ int kv4_word(int half, int lane, int b)
-{
-    constexpr int NB = HD / 32, W = NB < 4 ? NB : 4;
-    return (b >> 2) * 256 + (half * 32 + lane) * W + (b & 3);
-}
 
 // ------------------------------------------------------------------------------------------------------------------
 // append and read
@@ -283,173 +246,6 @@ __global__ void __launch_bounds__(128) k_kv4_read(Kv4Rows rows, const int32_t* p
 // ------------------------------------------------------------------------------------------------------------------
 // attention
 // ------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// D = A B and D += A B for m16n8k16 in fp16 with fp32 sums.
-__device__ __forceinline__ void mma_zero(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1)
-{
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
-}
-__device__ __forceinline__ void mma_add(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1)
-{
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
-
-// (w & mask) | bits in one instruction.
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits)
-{
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
-    return r;
-}
-
-// Eight codes to four fp16 pairs of c - 8: nibbles (0, 4), (1, 5), (2, 6), (3, 7). A nibble below 1024's exponent is
-// 1024 + c, or 1024 + 16 c four bits up.
-__device__ __forceinline__ void unpack_signed(uint32_t w, uint32_t (&r)[4])
-{
-    const __half2 m1032 = __floats2half2_rn(1032.f, 1032.f), s16 = __floats2half2_rn(0.0625f, 0.0625f),
-                  m72 = __floats2half2_rn(-72.f, -72.f);
-    const uint32_t w8 = w >> 8;
-    r[0] = h2_bits(__hsub2(bits_h2(and_or(w, 0x000F000Fu, 0x64006400u)), m1032));
-    r[1] = h2_bits(__hfma2(bits_h2(and_or(w, 0x00F000F0u, 0x64006400u)), s16, m72));
-    r[2] = h2_bits(__hsub2(bits_h2(and_or(w8, 0x000F000Fu, 0x64006400u)), m1032));
-    r[3] = h2_bits(__hfma2(bits_h2(and_or(w8, 0x00F000F0u, 0x64006400u)), s16, m72));
-}
-
-// The same as fp16 subnormals c 2^-24 (pairs 0 and 2) and 16 c 2^-24 (pairs 1 and 3): masks only.
-__device__ __forceinline__ void unpack_raw(uint32_t w, uint32_t (&r)[4])
-{
-    const uint32_t w8 = w >> 8;
-    r[0] = w & 0x000F000Fu;
-    r[1] = w & 0x00F000F0u;
-    r[2] = w8 & 0x000F000Fu;
-    r[3] = w8 & 0x00F000F0u;
-}
-
-// Pairs of floats in one instruction.
-__device__ __forceinline__ uint64_t f2(float lo, float hi)
-{
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 unf2(uint64_t v)
-{
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
-{
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
-{
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
-{
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
-// fp16 roundings of a pair and of what they leave.
-__device__ __forceinline__ void split_h2(uint64_t ab, uint32_t& hi, uint32_t& lo)
-{
-    const float2 v = unf2(ab);
-    const __half2 h = __floats2half2_rn(v.x, v.y);
-    const float2 f = __half22float2(h);
-    const float2 d = unf2(fma2(f2(f.x, f.y), f2(-1.f, -1.f), ab));
-    hi = h2_bits(h);
-    lo = h2_bits(__floats2half2_rn(d.x, d.y));
-}
-
-// The words of one lane's fragments: NB consecutive (planes of 4) 32-bit words.
-template <int HD> __device__ __forceinline__ void lane_words(const uint8_t* area, int half, int lane, uint32_t (&w)[HD / 32])
-{
-    constexpr int NB = HD / 32;
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(area);
-    if constexpr (NB == 2) {
-        const uint2 x = lds64(p + (half * 32 + lane) * 2);
-        w[0] = x.x; w[1] = x.y;
-    } else if constexpr (NB == 3) {
-#pragma unroll
-        for (int b = 0; b < 3; ++b) w[b] = p[(half * 32 + lane) * 3 + b];
-    } else {
-#pragma unroll
-        for (int pl = 0; pl < NB / 4; ++pl) {
-            const uint4 x = lds128(p + pl * 256 + (half * 32 + lane) * 4);
-            w[4 * pl] = x.x; w[4 * pl + 1] = x.y; w[4 * pl + 2] = x.z; w[4 * pl + 3] = x.w;
-        }
-    }
-}
-
-// The scales of positions r, r + 1 (r even): NB fp16 pairs' words, position-major.
-template <int HD> __device__ __forceinline__ void lane_scales(const uint8_t* area, int r, uint32_t (&w)[HD / 32])
-{
-    constexpr int NB = HD / 32;
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(area) + r * NB / 2;
-    if constexpr (NB == 2) {
-        const uint2 x = lds64(p);
-        w[0] = x.x; w[1] = x.y;
-    } else if constexpr (NB == 3) {
-#pragma unroll
-        for (int b = 0; b < 3; ++b) w[b] = p[b];
-    } else {
-#pragma unroll
-        for (int i = 0; i < NB / 4; ++i) {
-            const uint4 x = lds128(p + 4 * i);
-            w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
-        }
-    }
-}
-// Scale b of position e (0, 1) of those words.
-template <int NB> __device__ __forceinline__ float scale_of(const uint32_t (&w)[NB], int e, int b)
-{
-    const int i = e * NB + b;
-    const float2 f = __half22float2(bits_h2(w[i >> 1]));
-    return i & 1 ? f.y : f.x;
-}
-
-// One query's visible positions: j < n and (j >= first or j < sink).
-struct Vis {
-    int n, first, sink;
-    __device__ __forceinline__ bool operator()(int j) const { return j < n && (j >= first || j < sink); }
-};
-__device__ __forceinline__ Vis visible(int p, int window, int sinks)
-{
-    const int n = p + 1, first = window > 0 && n > window ? n - window : 0;
-    return Vis{n, first, min(sinks, first)};
-}
-
-// The tiles that hold positions of [0, sink) or [first, n): item i of the list is tile i below head, else i + skip.
-struct TileList {
-    int head, skip, count;
-    __device__ __forceinline__ int at(int i) const { return i < head ? i : i + skip; }
-};
-__device__ __forceinline__ TileList tile_list(int n, int first, int sink)
-{
-    const int t1 = first >> 4, head = min((sink + 15) >> 4, t1), last = (n - 1) >> 4;
-    return TileList{head, t1 - head, n > 0 ? head + last - t1 + 1 : 0};
-}
-
-// A running maximum is followed only when it is passed by a factor 2^6: weights up to 2^6 cost nothing, and the output's
-// sums are rescaled a few times a row and not at most tiles.
-constexpr float ATT_SLACK = 6.f;
 
 // Running softmax of MT tiles of 8 queries: lane (g, c) keeps query g's reference maximum (in log2 units), its own share of
 // the sum, and the output's fragments (o[.][0,1] the rows of the weights' roundings, [2,3] of what they left).
@@ -667,21 +463,6 @@ __device__ __forceinline__ void load_query(const float* x, int lane, float f, ui
     qt.ks = ldexpf(1.f, 24 - e);
 }
 
-struct Kv4Att {
-    const float* q;
-    float* out;
-    Kv4Rows rows;
-    const int32_t* pos;
-    int64_t capacity;
-    int T, R, heads, kv_heads, S, s_max;    // S: ranges a row may be cut into (the stride of the partials)
-    float scale;
-    int window, sinks;
-    float* part;                            // [T][heads][S][HD]
-    float* ml;                              // [T][heads][S][2]: maximum (log2 units), sum
-    int* tickets;
-    int* err;
-};
-
 // A CTA of 8 warps, two an SM (128 registers, the queries' fragments in shared memory): against three CTAs of 4 warps with the
 // fragments in registers, one row over 131000 positions 52.8 against 55.6 us (fewer ranges to join), 8 rows of up to 4100
 // 15.5 against 19.1. A range holds 48 tiles at least: 6 to a warp.
@@ -690,77 +471,6 @@ constexpr int RUN_WARPS = 4;                // warps of a CTA of the runs' kerne
 constexpr int ATT_TPS = 48;
 constexpr int ATT_STAGES = 2;               // ring stages a warp, of two tiles each
 constexpr int att_ctas(int HD) { return HD <= 128 ? 2 : 1; }
-constexpr int ATT_MAX_RANGES = 96;
-
-// Joins the n ranges of nh rows of heads (the i-th at (row, head) index row(i)) in range order, by a CTA of NT threads:
-// a warp takes a head's weights at a time, then every thread takes 4 output values at a time, its loads of 8 ranges in
-// flight together. w: nh * n floats of shared memory.
-template <int HD, int NT, class F> __device__ __forceinline__ void join_ranges(const Kv4Att& a, int nh, int n, float* w, const F& row)
-{
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int h = warp; h < nh; h += NT / 32) {
-        const float2* ml = reinterpret_cast<const float2*>(a.ml) + row(h) * a.S;
-        float2 x[ATT_MAX_RANGES / 32];
-        float M = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < ATT_MAX_RANGES / 32; ++i) {
-            const int s = lane + 32 * i;
-            x[i] = s < n ? __ldcg(ml + s) : make_float2(-INFINITY, 0.f);
-            M = fmaxf(M, x[i].x);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        const float mu = M == -INFINITY ? 0.f : M;
-        float L = 0.f;
-#pragma unroll
-        for (int i = 0; i < ATT_MAX_RANGES / 32; ++i) {
-            x[i].x = ex2(x[i].x - mu);
-            L += x[i].x * x[i].y;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        const float inv = L != 0.f ? 1.f / L : 0.f;     // (a NaN sum stays NaN; no visible position: zeros)
-#pragma unroll
-        for (int i = 0; i < ATT_MAX_RANGES / 32; ++i)
-            if (lane + 32 * i < n) w[h * n + lane + 32 * i] = x[i].x * inv;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < nh * (HD / 4); i += NT) {
-        const int h = i / (HD / 4), d = i % (HD / 4) * 4;
-        const float4* pp = reinterpret_cast<const float4*>(a.part + row(h) * a.S * HD + d);
-        const float* wh = w + h * n;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s0 = 0; s0 < n; s0 += 8) {
-            float4 p[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) p[k] = s0 + k < n ? __ldcg(pp + (int64_t)(s0 + k) * (HD / 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float f = s0 + k < n ? wh[s0 + k] : 0.f;
-                o.x += f * p[k].x;
-                o.y += f * p[k].y;
-                o.z += f * p[k].z;
-                o.w += f * p[k].w;
-            }
-        }
-        *reinterpret_cast<float4*>(a.out + row(h) * HD + d) = o;
-    }
-}
-
-// Takes a ticket after the CTA's partials; true in the CTA that took the last of n.
-__device__ __forceinline__ bool last_ticket(int* ctr, int n)
-{
-    __shared__ int last;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int ticket;
-        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(ticket) : "l"(ctr) : "memory");
-        last = ticket == n - 1;
-        if (last) *ctr = 0;
-    }
-    __syncthreads();
-    return last;
-}
 
 // Rows on their own (decode): CTA (range, KV head and tile of 8 query heads, row); each warp streams its own tiles, every
 // fourth pair of the range, through its ring of bulk copies, and the warps' sums are joined in warp order. The ranges follow
@@ -1044,9 +754,12 @@ __global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att
 
 constexpr int64_t KV4_TICKETS = 1 << 18;    // tickets at the head of a workspace (zero between calls)
 
+// Queries of a run and KV head from which the tensor-core kernel is taken (its CTAs hold 128).
+constexpr int MMA_MIN_QUERIES = 96;
+
 // How a call is cut.
 struct Kv4Plan {
-    bool runs;              // the rows' runs share their cache's tiles (k_kv4_attn_run)
+    bool runs, mma;         // the rows' runs share their cache's tiles: on the tensor cores (k_kv4_attn_mma) or k_kv4_attn_run
     int S, s_max, q_blocks, MT, MG;
     int64_t part_floats;
 };
@@ -1059,14 +772,16 @@ Kv4Plan kv4_plan(int T, int R, int heads, int kv_heads, int head_dim, int64_t ca
     int64_t tiles = (capacity + KV4_P - 1) / KV4_P;
     if (window > 0) tiles = std::min<int64_t>(tiles, ((int64_t)window + 15) / 16 + 1 + ((int64_t)sinks + 15) / 16);
     p.runs = R > 8;
+    p.mma = p.runs && (head_dim == 64 || head_dim == 128) && (int64_t)R * G >= MMA_MIN_QUERIES;
     p.MT = head_dim <= 128 ? 2 : 1;
-    const int QB = RUN_WARPS * 8 * p.MT;
+    const int QB = p.mma ? 128 : RUN_WARPS * 8 * p.MT;
     p.q_blocks = (int)(((int64_t)R * G + QB - 1) / QB);
     int64_t ctas;
     if (p.runs) {
-        // as many ranges as fill the SMs twice, each of 16 tiles at least
+        // as many ranges as fill the SMs (twice, with CTAs of four warps), each of 16 tiles at least
         ctas = (int64_t)(T / R) * p.q_blocks * kv_heads;
-        p.s_max = (int)std::max<int64_t>(1, std::min<int64_t>({32, tiles / ATT_TPS, (2 * 148 + ctas - 1) / ctas}));
+        const int64_t want = ((p.mma ? 1 : 2) * 148 + ctas - 1) / ctas;
+        p.s_max = (int)std::max<int64_t>(1, std::min<int64_t>({32, tiles / 16, want}));
         p.S = p.s_max;
     } else {
         // the most ranges of one row, from the shape alone (a row's bits must not depend on the others): one row's
@@ -1203,7 +918,8 @@ void kv4_attention(const float* q, int T, int R, int heads, int kv_heads, int he
         a.part = (float*)((uint8_t*)ws + KV4_TICKETS * 4);
         a.ml = a.part + (int64_t)T * heads * p.S * head_dim;
         a.err = err;
-        switch (head_dim) {
+        if (p.mma) kv4_attention_mma(a, head_dim, p.q_blocks, s);
+        else switch (head_dim) {
         case 64: p.runs ? attn_runs<64>(a, p, s) : attn_rows<64>(a, p, s); break;
         case 96: p.runs ? attn_runs<96>(a, p, s) : attn_rows<96>(a, p, s); break;
         case 128: p.runs ? attn_runs<128>(a, p, s) : attn_rows<128>(a, p, s); break;

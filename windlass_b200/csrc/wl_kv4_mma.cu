@@ -1,0 +1,598 @@
+// Attention of prompts over the 4-bit KV cache on the 5th-generation tensor cores (tcgen05, sm_100a).
+//
+// A CTA takes 128 queries ((row, head) pairs of a run of rows that share a cache) of one KV head and walks the visible
+// positions in steps of 128 (8 cache tiles). Scores and output are tcgen05 products with fp32 sums in tensor memory:
+//   S[128 queries][128 positions] = Q K',    O[128 queries][HD] += P V'.
+// Everything enters as two fp16 planes, a value's rounding and what it left: Q (scaled by a power of two a row) and the
+// weights P 22 bits, K' = (c - 8) d 2^-3 and V' = (c - 8) d vs exactly (a 4-bit code times an 11-bit scale has at most 15
+// bits; vs a power of two). Each product is three MMAs, hi hi + lo hi + hi lo; the dropped lo lo is below 2^-22 of it, so
+// the result is as exact as fp32 arithmetic. Q and P are the MMA's A operand in tensor memory (P in the place of the
+// scores it came from), K' and V' its B operand in shared memory.
+//   - warp 13 copies a step's cache tiles (contiguous 18 HD bytes each) into a ring of raw steps with bulk copies;
+//   - warps 4-11 turn codes into the planes of K' and V' in the 128-byte-swizzled K-major layout. The order of a step's
+//     positions is chosen so that a thread's codes are whole 16-byte chunks of it: within 32 positions, slot 8 c + 2 (2 t + h)
+//     + e is position 16 t + 8 h + 2 c + e; within 8 dims, 0 4 1 5 2 6 3 7. Both products use the same order;
+//   - warp 12 issues the MMAs;
+//   - warps 0-3 own a query a thread (its tensor-memory lane): maximum, weights and sum without a shuffle, P's planes
+//     back to tensor memory, and O rescaled when a maximum is passed by a factor 2^6.
+// The scores of step j + 1 are computed while the weights of step j are: two score buffers. Tensor memory: scores 2 x 128
+// columns, O, Q: 512 columns at HD = 128.
+#include <algorithm>
+#include "wl_kv4.cuh"
+
+namespace wl {
+namespace k {
+
+namespace {
+
+constexpr int PM_Q = 128, PM_P = 128;       // queries of a CTA, positions of a step
+constexpr int PM_TILES = PM_P / KV4_P;
+constexpr int PM_RAW = 4;                   // raw steps in flight
+constexpr int PM_DQ_WARP = 4, PM_DQ = 8, PM_MMA_WARP = 12, PM_RAW_WARP = 13, PM_THREADS = 448;
+// tensor memory columns
+constexpr int TM_S = 0, TM_O = 256, TM_QH = 384, TM_QL = 448;
+
+constexpr int pm_plane(int HD) { return HD * 256; }             // one fp16 plane of a step: 128 x HD
+constexpr int pm_smem(int HD) { return 4 * pm_plane(HD) + PM_RAW * PM_TILES * kv4_tile_bytes(HD) + 1024; }
+
+// A wait bounded by time (2 s); after one gives up, all of the CTA's waits return at once.
+__device__ __forceinline__ bool pm_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort)
+{
+    if (*abort) return false;
+    if (mbar_try_wait(bar, parity)) return true;
+    const unsigned long long t0 = globaltimer_ns();
+    while (!mbar_try_wait(bar, parity)) {
+        if (*abort) return false;
+        if (globaltimer_ns() - t0 > MBAR_WAIT_NS) {
+            atomicExch(err, 24);
+            *abort = 1;
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ void pm_arrive(uint64_t* bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+                 "%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+                   "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+                   "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,"
+                 "%31,%32};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+                   "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+                   "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+                   "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+                 : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Shared-memory matrix descriptor: K-major, 128-byte swizzle, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t pm_desc(const void* p)
+{
+    const uint64_t addr = smem_u32(p);
+    return ((addr & 0x3FFFFull) >> 4) | (1ull << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::f16 with fp16 operands, fp32 sums, M = 128.
+constexpr uint32_t pm_idesc(int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
+
+__device__ __forceinline__ void pm_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void pm_commit(uint64_t* bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// What the values' scales of a step call for (slot j % 3): the largest scale of 2 or more, and where scales are NaN (a value
+// row that held an infinity or NaN): bit n of word n / 32 of block b is slot n.
+template <int NB> struct StepCare {
+    uint32_t vmax;              // its float's bits; 0: all below 2
+    int any_nan;
+    uint32_t nan[NB][PM_P / 32];
+    __device__ __forceinline__ float vs() const
+    {
+        // V' = (c - 8) d vs stays below 2^13
+        return vmax ? ldexpf(1.f, max(8 - ilogbf(__uint_as_float(vmax)), -7)) : 256.f;
+    }
+    __device__ __forceinline__ void clear()
+    {
+        vmax = 0u;
+        any_nan = 0;
+        for (int b = 0; b < NB; ++b)
+            for (int i = 0; i < PM_P / 32; ++i) nan[b][i] = 0u;
+    }
+};
+
+template <int HD>
+__global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, int q_blocks)
+{
+    constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD), PL = pm_plane(HD);
+    static_assert(HD == 64 || HD == 128, "planes of whole 64-value swizzle atoms");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t *kh = smem, *kl = smem + PL, *vh = smem + 2 * PL, *vl = smem + 3 * PL, *raw = smem + 4 * PL;
+    __shared__ __align__(8) uint64_t raw_full[PM_RAW], raw_empty[PM_RAW], k_full, qk_done, v_full, pv_done, s_full[2], p_full[2];
+    __shared__ StepCare<NB> care[3];
+    __shared__ uint32_t tmem_base;
+    __shared__ int abort_flag, rng[3];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int G = a.heads / a.kv_heads, kvh = blockIdx.y;
+    // the last queries (of a prompt: those that see most) first
+    const int qb = q_blocks - 1 - (int)blockIdx.x / a.S, sp = blockIdx.x % a.S, run = blockIdx.z;
+    const int nq = a.R * G, q0 = qb * PM_Q;
+    const uint8_t* base = a.rows.base(run * a.R);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < PM_RAW; ++s) {
+            mbar_init(&raw_full[s], 1);
+            mbar_init(&raw_empty[s], PM_DQ);
+        }
+        mbar_init(&k_full, PM_DQ);
+        mbar_init(&v_full, PM_DQ);
+        mbar_init(&qk_done, 1);
+        mbar_init(&pv_done, 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&s_full[s], 1);
+            mbar_init(&p_full[s], 128);
+        }
+        abort_flag = 0;
+        rng[0] = 0;
+        rng[1] = INT_MAX;
+        rng[2] = 0;
+        for (int i = 0; i < 3; ++i) care[i].clear();
+        fence_mbar_init();
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    __syncthreads();
+    {
+        // the positions that the CTA's rows see together
+        const int r0 = q0 / G, r1 = min(a.R - 1, (min(q0 + PM_Q, nq) - 1) / G);
+        for (int r = r0 + threadIdx.x; r <= r1; r += PM_THREADS) {
+            const int p = a.pos[run * a.R + r];
+            if (kv4_row_state(base, p, a.capacity)) continue;
+            const Vis v = visible(p, a.window, a.sinks);
+            atomicMax(&rng[0], v.n);
+            atomicMin(&rng[1], v.first);
+            atomicMax(&rng[2], v.sink);
+        }
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = tmem_base;
+    const Vis seen{rng[0], rng[1], rng[2]};
+    const TileList tl = seen.n > 0 ? tile_list(seen.n, seen.first, seen.sink) : TileList{0, 0, 0};
+    const int i0 = (int)((int64_t)tl.count * sp / a.S), i1 = (int)((int64_t)tl.count * (sp + 1) / a.S);
+    const int steps = (i1 - i0 + PM_TILES - 1) / PM_TILES;
+    volatile int* abort = &abort_flag;
+
+    if (warp < 4) {
+        // ---- a query a thread
+        const uint32_t row = tmem + ((uint32_t)(32 * warp) << 16);
+        const int qi = q0 + threadIdx.x;
+        int64_t th = -1;
+        int state = 1;
+        Vis vis{0, 0, 0};
+        if (qi < nq) {
+            const int t = run * a.R + qi / G;
+            th = (int64_t)t * a.heads + kvh * G + qi % G;
+            const int p = a.pos[t];
+            state = kv4_row_state(base, p, a.capacity);
+            if (!state) vis = visible(p, a.window, a.sinks);
+        }
+        float ks;
+        {
+            // Q's planes: 2^13..2^14 at the row's largest value, dims in the order 0 4 1 5 2 6 3 7
+            const float f = a.scale * 1.4426950408889634f;
+            const float4* x = reinterpret_cast<const float4*>(a.q + th * HD);
+            float mx = 0.f;
+            if (th >= 0)
+                for (int i = 0; i < HD / 4; ++i) {
+                    const float4 v = x[i];
+                    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x * f), fabsf(v.y * f)), fmaxf(fabsf(v.z * f), fabsf(v.w * f))));
+                }
+            int e = mx > 0.f && mx <= 3e38f ? 13 - ilogbf(mx) : 0;
+            e = e > 100 ? 100 : e < -100 ? -100 : e;
+            const float up = ldexpf(1.f, e);
+            ks = ldexpf(1.f, 3 - e);
+#pragma unroll 1
+            for (int i = 0; i < HD / 64; ++i) {
+                uint32_t hi[32], lo[32];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f), w = v;
+                    if (th >= 0) {
+                        v = x[16 * i + 2 * c];
+                        w = x[16 * i + 2 * c + 1];
+                    }
+                    split_h2(f2(v.x * f * up, w.x * f * up), hi[4 * c], lo[4 * c]);
+                    split_h2(f2(v.y * f * up, w.y * f * up), hi[4 * c + 1], lo[4 * c + 1]);
+                    split_h2(f2(v.z * f * up, w.z * f * up), hi[4 * c + 2], lo[4 * c + 2]);
+                    split_h2(f2(v.w * f * up, w.w * f * up), hi[4 * c + 3], lo[4 * c + 3]);
+                }
+                tmem_st32(row + TM_QH + 32 * i, hi);
+                tmem_st32(row + TM_QL + 32 * i, lo);
+            }
+            tc_before();
+            // (the first p_full phase of buffer 1 says that Q is there: see the MMA warp)
+            pm_arrive(&p_full[1]);
+        }
+        const int w_min_n = __reduce_min_sync(0xffffffffu, vis.n), w_max_first = __reduce_max_sync(0xffffffffu, vis.first);
+        float m = -INFINITY, l = 0.f, vs = 256.f;
+        uint32_t poison = 0u;               // blocks of the output that a seen NaN reached
+        for (int j = 0; j < steps; ++j) {
+            const uint32_t sbuf = row + TM_S + (j & 1) * 128;
+            pm_wait(&s_full[j & 1], (uint32_t)(j / 2 & 1), a.err, abort);
+            tc_after();
+            // seen columns: all, or bit n of word n / 32
+            const int at = i0 + PM_TILES * j;
+            const bool full = at + PM_TILES <= i1 && tl.at(at) * KV4_P >= w_max_first && tl.at(at + PM_TILES - 1) * KV4_P + KV4_P <= w_min_n;
+            uint32_t bits[4];
+            if (!full) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    bits[g] = 0u;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const int it = at + 2 * g + t;
+                        if (it < i1) {
+                            const int p0 = tl.at(it) * KV4_P;
+#pragma unroll
+                            for (int i = 0; i < KV4_P; ++i)
+                                if (vis(p0 + i)) bits[g] |= 1u << (8 * (i % 8 / 2) + 2 * (2 * t + i / 8) + i % 2);
+                        }
+                    }
+                }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                uint32_t r[32];
+                tmem_ld32(sbuf + 32 * g, r);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float s = __uint_as_float(r[i]);
+                    mx = fmaxf(mx, full || (bits[g] >> i & 1u) ? s : -INFINITY);
+                }
+            }
+            mx *= ks;
+            StepCare<NB>& cr = care[j % 3];
+            const float vj = cr.vs();
+            const bool grow = mx > m + ATT_SLACK;
+            if (__any_sync(0xffffffffu, grow || vj < vs)) {
+                const float mn = grow ? mx : m;
+                float f = grow && m != -INFINITY ? ex2(m - mn) : 1.f;
+                l *= f;
+                m = mn;
+                if (vj < vs) {
+                    f *= vj / vs;
+                    vs = vj;
+                }
+                if (j > 0) {
+                    pm_wait(&pv_done, (uint32_t)(j - 1 & 1), a.err, abort);
+                    tc_after();
+#pragma unroll 1
+                    for (int i = 0; i < HD / 32; ++i) {
+                        uint32_t r[32];
+                        tmem_ld32(row + TM_O + 32 * i, r);
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) r[x] = __float_as_uint(__uint_as_float(r[x]) * f);
+                        tmem_st32(row + TM_O + 32 * i, r);
+                    }
+                }
+            }
+            if (cr.any_nan) {
+                // a value row with a NaN enters as zeros: it reaches the rows that see it here, and no other
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        if (cr.nan[b][g] & (full ? 0xffffffffu : bits[g])) poison |= 1u << b;
+            }
+            const float mu = m == -INFINITY ? 0.f : m, down = vs / vj;      // (a step of smaller scales than O's: its weights follow)
+            const uint64_t k2 = f2(ks, ks), m2 = f2(-mu, -mu), d2 = f2(down, down);
+            uint64_t sum = f2(0.f, 0.f);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                uint32_t r[32], o[32];
+                tmem_ld32(sbuf + 32 * g, r);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float2 x = unf2(fma2(f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), k2, m2));
+                    x.x = ex2(x.x);
+                    x.y = ex2(x.y);
+                    if (!full) {
+                        x.x = bits[g] >> (2 * i) & 1u ? x.x : 0.f;
+                        x.y = bits[g] >> (2 * i + 1) & 1u ? x.y : 0.f;
+                    }
+                    const uint64_t p = f2(x.x, x.y);
+                    sum = add2(sum, p);
+                    split_h2(mul2(p, d2), o[i], o[16 + i]);
+                }
+                tmem_st32(sbuf + 32 * g, o);        // in place: 16 columns of P's roundings, 16 of what they left
+            }
+            const float2 x = unf2(sum);
+            l += x.x + x.y;
+            tc_before();
+            pm_arrive(&p_full[j & 1]);
+        }
+        // ---- the output
+        if (steps > 1) pm_wait(&pv_done, (uint32_t)(steps & 1), a.err, abort);      // (each phase in turn: a wait tells two apart)
+        if (steps > 0) {
+            pm_wait(&pv_done, (uint32_t)(steps - 1 & 1), a.err, abort);
+            tc_after();
+        }
+        const bool whole = a.S == 1;
+        float f = whole ? (l != 0.f ? 1.f / (l * vs) : 0.f) : 1.f / vs;
+        if (state == 2) f = NAN;
+        float* dst = whole ? a.out + th * HD : a.part + (th * a.S + sp) * HD;
+#pragma unroll 1
+        for (int i = 0; i < HD / 32; ++i) {
+            uint32_t r[32];
+            if (steps > 0) tmem_ld32(row + TM_O + 32 * i, r);
+            if (th >= 0) {
+                const float g = poison >> i & 1u ? NAN : f;
+#pragma unroll
+                for (int x = 0; x < 32; x += 4) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (steps > 0) v = make_float4(__uint_as_float(r[x]), __uint_as_float(r[x + 1]), __uint_as_float(r[x + 2]), __uint_as_float(r[x + 3]));
+                    *reinterpret_cast<float4*>(dst + 32 * i + x) = make_float4(v.x * g, v.y * g, v.z * g, v.w * g);
+                }
+            }
+        }
+        if (!whole && th >= 0) reinterpret_cast<float2*>(a.ml)[th * a.S + sp] = make_float2(m, state == 2 ? NAN : l);
+    } else if (warp < PM_MMA_WARP) {
+        // ---- codes to planes
+        const int w = warp - PM_DQ_WARP, g = lane >> 2, c = lane & 3;
+        auto live = [&](int it, int r) {    // position r of list item it is seen by some row of the CTA
+            return it < i1 && seen(tl.at(it) * KV4_P + r);
+        };
+        for (int j = 0; j < steps; ++j) {
+            const int at = i0 + PM_TILES * j;
+            const uint8_t* rs = raw + j % PM_RAW * PM_TILES * TB;
+            StepCare<NB>& cr = care[j % 3];
+            pm_wait(&raw_full[j % PM_RAW], (uint32_t)(j / PM_RAW & 1), a.err, abort);
+            // the values' scales of tile w: two fp16 a lane
+            {
+                uint32_t big = 0u, nan = 0u;
+                const int i = 2 * lane;
+                if (i < KV4_P * NB) {
+                    const uint32_t x = reinterpret_cast<const uint32_t*>(rs + w * TB + 17 * HD)[lane];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t d = (x >> (16 * e)) & 0x7FFFu;
+                        if (d < 0x4000u || !live(at + w, (i + e) / NB)) continue;
+                        if (d > 0x7C00u) nan |= 1u << e;
+                        else big = max(big, __float_as_uint(__half2float(__ushort_as_half((unsigned short)d))));
+                    }
+                }
+                if (__any_sync(0xffffffffu, big | nan)) {
+                    if (big) atomicMax(&cr.vmax, big);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (nan >> e & 1u) {
+                            const int r = (i + e) / NB;
+                            cr.any_nan = 1;
+                            atomicOr(&cr.nan[(i + e) % NB][w / 2], 1u << (8 * (r % 8 / 2) + 2 * (2 * (w & 1) + r / 8) + r % 2));
+                        }
+                }
+                // (the slot of step j - 2, whose weights are written: every warp has waited for that step's PV)
+                if (threadIdx.x == 32 * PM_DQ_WARP && j > 0) care[(j + 1) % 3].clear();
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+            }
+            const __half2 vs2 = __float2half2_rn(cr.vs()), k2 = __float2half2_rn(0.125f);
+            // K': two (tile, half) units a warp, a position's 8 dims x NB a lane
+            if (j > 0) pm_wait(&qk_done, (uint32_t)(j - 1 & 1), a.err, abort);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int t = w, h = u;
+                uint32_t kw[NB], sw[NB / 2];
+                lane_words<HD>(rs + t * TB, h, lane, kw);
+                const uint8_t* sc = rs + t * TB + 16 * HD + (8 * h + g) * NB * 2;
+                if constexpr (NB == 4) {
+                    const uint2 x = lds64(sc);
+                    sw[0] = x.x;
+                    sw[1] = x.y;
+                } else {
+                    sw[0] = *reinterpret_cast<const uint32_t*>(sc);
+                }
+                if (!live(at + t, 8 * h + g)) {
+#pragma unroll
+                    for (int i = 0; i < NB / 2; ++i) sw[i] = 0u;
+                }
+                const int n = t / 2 * 32 + g / 2 * 8 + (2 * (t & 1) + h) * 2 + (g & 1);
+                const int off = n / 8 * 1024 + n % 8 * 128;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    // odd g takes the blocks of a pair the other way round: a phase's 8 lanes then write 8 different chunks
+                    const bool odd = g & 1;
+                    const int b = odd ? i ^ 1 : i;
+                    const uint32_t word = odd ? kw[i ^ 1] : kw[i];
+                    const uint32_t d16 = __byte_perm(sw[i / 2], 0, (i & 1) != odd ? 0x3232 : 0x1010);
+                    const __half2 d = __hmul2(bits_h2(d16), k2);
+                    uint32_t r[4], hi[4], lo[4];
+                    unpack_signed(word, r);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const __half2 y = __hmul2(bits_h2(r[x]), d);
+                        hi[x] = h2_bits(y);
+                        lo[x] = h2_bits(__hfma2(bits_h2(r[x]), d, __hneg2(y)));
+                    }
+                    const int ch = 4 * b + c;
+                    uint8_t* dst = kh + ch / 8 * (PM_P * 128) + off + ((ch % 8) ^ (n % 8)) * 16;
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(dst + PL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) pm_arrive(&k_full);
+            // V': 32 positions (two tiles) and half the blocks a warp; a lane 8 positions of 4 dims a block
+            if (j > 0) pm_wait(&pv_done, (uint32_t)(j - 1 & 1), a.err, abort);
+            {
+                const int grp = w / 2, b0 = (w & 1) * (NB / 2);
+                uint32_t vw[4][NB / 2], dv[4][NB / 2];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int t = 2 * grp + k / 2, h = k % 2;
+                    const uint8_t* tp = rs + t * TB;
+                    const uint8_t* vp = tp + 8 * HD + ((h * 32 + lane) * NB + b0) * 4;
+                    uint32_t s[NB];
+                    lane_scales<HD>(tp + 17 * HD, 8 * h + 2 * c, s);
+                    const uint32_t keep = (live(at + t, 8 * h + 2 * c) ? 0xFFFFu : 0u) | (live(at + t, 8 * h + 2 * c + 1) ? 0xFFFF0000u : 0u);
+                    if constexpr (NB == 4) {
+                        const uint2 x = lds64(vp);
+                        vw[k][0] = x.x;
+                        vw[k][1] = x.y;
+                        const uint32_t s0 = w & 1 ? s[1] : s[0], s1 = w & 1 ? s[3] : s[2];
+                        dv[k][0] = __byte_perm(s0, s1, 0x5410) & keep;
+                        dv[k][1] = __byte_perm(s0, s1, 0x7632) & keep;
+                    } else {
+                        vw[k][0] = *reinterpret_cast<const uint32_t*>(vp);
+                        dv[k][0] = __byte_perm(s[0], s[1], w & 1 ? 0x7632 : 0x5410) & keep;
+                    }
+#pragma unroll
+                    for (int i = 0; i < NB / 2; ++i) {
+                        // (a NaN scale, above infinity's bits, enters as zero)
+                        if (cr.any_nan) {
+                            if ((dv[k][i] & 0x7FFFu) > 0x7C00u) dv[k][i] &= 0xFFFF0000u;
+                            if ((dv[k][i] & 0x7FFF0000u) > 0x7C000000u) dv[k][i] &= 0xFFFFu;
+                        }
+                        dv[k][i] = h2_bits(__hmul2(bits_h2(dv[k][i]), vs2));
+                    }
+                }
+                const int ch = (grp & 1) * 4 + c;
+#pragma unroll
+                for (int i = 0; i < NB / 2; ++i) {
+                    uint32_t r[4][4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) unpack_signed(vw[k][i], r[k]);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const __half2 d = bits_h2(dv[k][i]), y = __hmul2(bits_h2(r[k][x]), d);
+                            hi[k] = h2_bits(y);
+                            lo[k] = h2_bits(__hfma2(bits_h2(r[k][x]), d, __hneg2(y)));
+                        }
+                        const int dim = 32 * (b0 + i) + 4 * g + x;
+                        uint8_t* dst = vh + grp / 2 * (HD * 128) + dim / 8 * 1024 + dim % 8 * 128 + (ch ^ (dim % 8)) * 16;
+                        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(dst + PL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                pm_arrive(&v_full);
+                pm_arrive(&raw_empty[j % PM_RAW]);
+            }
+        }
+    } else if (warp == PM_MMA_WARP) {
+        // ---- one thread issues the MMAs: scores of step j, then the output of step j - 1
+        if (lane == 0 && steps > 0) {
+            auto pv = [&](int j) {
+                // (buffer 1 has an extra first phase, Q's arrival, so its step j is phase j / 2 + 1)
+                pm_wait(&p_full[j & 1], (uint32_t)((j / 2 + (j & 1)) & 1), a.err, abort);
+                pm_wait(&v_full, (uint32_t)(j & 1), a.err, abort);
+                tc_after();
+                const uint32_t p = tmem + TM_S + (j & 1) * 128;
+#pragma unroll 1
+                for (int s = 0; s < PM_P / 16; ++s) {
+                    const int off = s / 4 * (HD * 128) + s % 4 * 32;
+                    const uint32_t ph = p + s / 2 * 32 + s % 2 * 8;
+                    pm_mma(tmem + TM_O, ph, pm_desc(vl + off), pm_idesc(HD), j > 0 || s > 0);
+                    pm_mma(tmem + TM_O, ph + 16, pm_desc(vh + off), pm_idesc(HD), 1u);
+                    pm_mma(tmem + TM_O, ph, pm_desc(vh + off), pm_idesc(HD), 1u);
+                }
+                pm_commit(&pv_done);
+            };
+            pm_wait(&p_full[1], 0u, a.err, abort);          // Q is in tensor memory
+            tc_after();
+            for (int j = 0; j < steps; ++j) {
+                pm_wait(&k_full, (uint32_t)(j & 1), a.err, abort);
+                if (j > 1) pm_wait(&pv_done, (uint32_t)(j & 1), a.err, abort);      // the weights that this score buffer held are used
+                tc_after();
+                const uint32_t d = tmem + TM_S + (j & 1) * 128;
+#pragma unroll 1
+                for (int s = 0; s < HD / 16; ++s) {
+                    const int off = s / 4 * (PM_P * 128) + s % 4 * 32;
+                    pm_mma(d, tmem + TM_QH + 8 * s, pm_desc(kl + off), pm_idesc(PM_P), s > 0);
+                    pm_mma(d, tmem + TM_QL + 8 * s, pm_desc(kh + off), pm_idesc(PM_P), 1u);
+                    pm_mma(d, tmem + TM_QH + 8 * s, pm_desc(kh + off), pm_idesc(PM_P), 1u);
+                }
+                pm_commit(&s_full[j & 1]);
+                pm_commit(&qk_done);
+                if (j > 0) pv(j - 1);
+            }
+            pv(steps - 1);
+        }
+    } else if (lane == 0) {
+        // ---- raw tiles
+        const uint8_t* src = base + (int64_t)kvh * TB;
+        for (int j = 0; j < steps; ++j) {
+            const int s = j % PM_RAW, at = i0 + PM_TILES * j, n = min(PM_TILES, i1 - at);
+            if (j >= PM_RAW) {
+                pm_wait(&raw_empty[s], (uint32_t)((j / PM_RAW + 1) & 1), a.err, abort);
+                fence_proxy_async();
+            }
+            mbar_expect_tx(&raw_full[s], n * TB);
+            for (int i = 0; i < n; ++i)
+                bulk_load(raw + (s * PM_TILES + i) * TB, src + (int64_t)tl.at(at + i) * a.kv_heads * TB, TB, &raw_full[s]);
+        }
+    }
+    tc_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+    if (a.S == 1) return;
+    if (!last_ticket(a.tickets + ((int64_t)run * a.kv_heads + kvh) * q_blocks + qb, a.S)) return;
+    join_ranges<HD, PM_THREADS>(a, min(PM_Q, nq - q0), a.S, reinterpret_cast<float*>(smem), [&](int i) {
+        return ((int64_t)run * a.R + (q0 + i) / G) * a.heads + kvh * G + (q0 + i) % G;
+    });
+}
+
+template <int HD> void launch_mma(const Kv4Att& a, int q_blocks, cudaStream_t s)
+{
+    WL_CUDA(cudaFuncSetAttribute(k_kv4_attn_mma<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, pm_smem(HD)));
+    // (launched plainly: it takes all of an SM's tensor memory, so it does not start beside another kernel's end)
+    k_kv4_attn_mma<HD><<<dim3(q_blocks * a.S, a.kv_heads, a.T / a.R), PM_THREADS, pm_smem(HD), s>>>(a, q_blocks);
+    note_launch();
+}
+
+}  // namespace
+
+void kv4_attention_mma(const Kv4Att& a, int head_dim, int q_blocks, cudaStream_t s)
+{
+    if (head_dim == 64) launch_mma<64>(a, q_blocks, s);
+    else launch_mma<128>(a, q_blocks, s);
+}
+
+}  // namespace k
+}  // namespace wl
