@@ -13,10 +13,14 @@
 //     positions is chosen so that a thread's codes are whole 16-byte chunks of it: within 32 positions, slot 8 c + 2 (2 t + h)
 //     + e is position 16 t + 8 h + 2 c + e; within 8 dims, 0 4 1 5 2 6 3 7. Both products use the same order;
 //   - warp 12 issues the MMAs;
-//   - warps 0-3 own a query a thread (its tensor-memory lane): maximum, weights and sum without a shuffle, P's planes
-//     back to tensor memory, and O rescaled when a maximum is passed by a factor 2^6.
-// The scores of step j + 1 are computed while the weights of step j are: two score buffers. Tensor memory: scores 2 x 128
-// columns, O, Q: 512 columns at HD = 128.
+//   - warps 0-3 own a query a thread (its tensor-memory lane): maximum, weights and sum without a shuffle, and P's planes
+//     back to tensor memory;
+//   - warps 4-11 also keep the output in registers (32 queries by HD / 2 dims a warp): a step's product starts from zero in
+//     tensor memory and is added here in fp32 (the tensor core's sums are cut off, not rounded: over 768 of them in one
+//     place the output was 8e-6 off, added step by step 1e-6), scaled by what the step changed in the query's maximum.
+// Order of the products: scores of step j + 1, output of step j - 1, scores of j + 2, ... While the output of j - 1 runs, K' of
+// j + 1 is made; while the scores of j + 1 run, V' of j, and the weights of j from the scores before: two score buffers,
+// one of K' and of V'. Tensor memory: scores 2 x 128 columns, the step's output 128, Q 128 (at HD = 128): all 512.
 #include <algorithm>
 #include "wl_kv4.cuh"
 
@@ -28,7 +32,8 @@ namespace {
 constexpr int PM_Q = 128, PM_P = 128;       // queries of a CTA, positions of a step
 constexpr int PM_TILES = PM_P / KV4_P;
 constexpr int PM_RAW = 4;                   // raw steps in flight
-constexpr int PM_DQ_WARP = 4, PM_DQ = 8, PM_MMA_WARP = 12, PM_RAW_WARP = 13, PM_THREADS = 448;
+constexpr int PM_DQ_WARP = 4, PM_DQ = 8, PM_MMA_WARP = 12, PM_RAW_WARP = 13, PM_THREADS = 512;
+constexpr int PM_SLOTS = 8;                 // steps whose care and factors are kept
 // tensor memory columns
 constexpr int TM_S = 0, TM_O = 256, TM_QH = 384, TM_QL = 448;
 
@@ -83,6 +88,9 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // Shared-memory matrix descriptor: K-major, 128-byte swizzle, 8-row groups 1024 bytes apart.
 __device__ __forceinline__ uint64_t pm_desc(const void* p)
 {
@@ -103,7 +111,7 @@ __device__ __forceinline__ void pm_commit(uint64_t* bar)
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// What the values' scales of a step call for (slot j % 3): the largest scale of 2 or more, and where scales are NaN (a value
+// What the values' scales of a step call for (slot j % PM_SLOTS): the largest scale of 2 or more, and where scales are NaN (a value
 // row that held an infinity or NaN): bit n of word n / 32 of block b is slot n.
 template <int NB> struct StepCare {
     uint32_t vmax;              // its float's bits; 0: all below 2
@@ -130,9 +138,13 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
     static_assert(HD == 64 || HD == 128, "planes of whole 64-value swizzle atoms");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint8_t *kh = smem, *kl = smem + PL, *vh = smem + 2 * PL, *vl = smem + 3 * PL, *raw = smem + 4 * PL;
-    __shared__ __align__(8) uint64_t raw_full[PM_RAW], raw_empty[PM_RAW], k_full, qk_done, v_full, pv_done, s_full[2], p_full[2];
-    __shared__ StepCare<NB> care[3];
+    uint8_t *kh = smem, *vh = smem + 2 * PL, *raw = smem + 4 * PL;      // (each plane's remainder PL behind it)
+    __shared__ __align__(8) uint64_t raw_full[PM_RAW], raw_empty[PM_RAW], q_full, k_full, qk_done, v_full, pv_done, o_free, s_full[2],
+        p_full[2];
+    __shared__ StepCare<NB> care[PM_SLOTS];
+    __shared__ float factor[PM_SLOTS][PM_Q];        // e^(old - new reference maximum) of a step and query
+    __shared__ float fin_l[PM_Q];
+    __shared__ uint32_t fin_poison[PM_Q];
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag, rng[3];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -146,8 +158,10 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             mbar_init(&raw_full[s], 1);
             mbar_init(&raw_empty[s], PM_DQ);
         }
+        mbar_init(&q_full, 128);
         mbar_init(&k_full, PM_DQ);
         mbar_init(&v_full, PM_DQ);
+        mbar_init(&o_free, PM_DQ);
         mbar_init(&qk_done, 1);
         mbar_init(&pv_done, 1);
         for (int s = 0; s < 2; ++s) {
@@ -158,7 +172,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         rng[0] = 0;
         rng[1] = INT_MAX;
         rng[2] = 0;
-        for (int i = 0; i < 3; ++i) care[i].clear();
+        for (int i = 0; i < PM_SLOTS; ++i) care[i].clear();
         fence_mbar_init();
     }
     if (warp == 0) {
@@ -187,18 +201,19 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
     const int i0 = (int)((int64_t)tl.count * sp / a.S), i1 = (int)((int64_t)tl.count * (sp + 1) / a.S);
     const int steps = (i1 - i0 + PM_TILES - 1) / PM_TILES;
     volatile int* abort = &abort_flag;
+    // a query's (row, head), or -1 past the run
+    auto query = [&](int qi) -> int64_t { return qi < nq ? (int64_t)(run * a.R + qi / G) * a.heads + kvh * G + qi % G : -1; };
 
+    // Registers: 512 threads of 128 at launch; 176 + 2 * 152 + 24 a thread of the four warpgroups = 504 of these 512.
     if (warp < 4) {
         // ---- a query a thread
+        regs_inc<176>();
         const uint32_t row = tmem + ((uint32_t)(32 * warp) << 16);
-        const int qi = q0 + threadIdx.x;
-        int64_t th = -1;
-        int state = 1;
+        const int64_t th = query(q0 + threadIdx.x);
         Vis vis{0, 0, 0};
-        if (qi < nq) {
-            const int t = run * a.R + qi / G;
-            th = (int64_t)t * a.heads + kvh * G + qi % G;
-            const int p = a.pos[t];
+        int state = 1;
+        if (th >= 0) {
+            const int p = a.pos[th / a.heads];
             state = kv4_row_state(base, p, a.capacity);
             if (!state) vis = visible(p, a.window, a.sinks);
         }
@@ -236,11 +251,10 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 tmem_st32(row + TM_QL + 32 * i, lo);
             }
             tc_before();
-            // (the first p_full phase of buffer 1 says that Q is there: see the MMA warp)
-            pm_arrive(&p_full[1]);
+            pm_arrive(&q_full);
         }
         const int w_min_n = __reduce_min_sync(0xffffffffu, vis.n), w_max_first = __reduce_max_sync(0xffffffffu, vis.first);
-        float m = -INFINITY, l = 0.f, vs = 256.f;
+        float m = -INFINITY, l = 0.f;
         uint32_t poison = 0u;               // blocks of the output that a seen NaN reached
         for (int j = 0; j < steps; ++j) {
             const uint32_t sbuf = row + TM_S + (j & 1) * 128;
@@ -271,38 +285,23 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             for (int g = 0; g < 4; ++g) {
                 uint32_t r[32];
                 tmem_ld32(sbuf + 32 * g, r);
+                if (full) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float s = __uint_as_float(r[i]);
-                    mx = fmaxf(mx, full || (bits[g] >> i & 1u) ? s : -INFINITY);
+                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, bits[g] >> i & 1u ? __uint_as_float(r[i]) : -INFINITY);
                 }
             }
             mx *= ks;
-            StepCare<NB>& cr = care[j % 3];
-            const float vj = cr.vs();
-            const bool grow = mx > m + ATT_SLACK;
-            if (__any_sync(0xffffffffu, grow || vj < vs)) {
-                const float mn = grow ? mx : m;
-                float f = grow && m != -INFINITY ? ex2(m - mn) : 1.f;
+            float f = 1.f;
+            if (mx > m + ATT_SLACK) {
+                f = m == -INFINITY ? 0.f : ex2(m - mx);
                 l *= f;
-                m = mn;
-                if (vj < vs) {
-                    f *= vj / vs;
-                    vs = vj;
-                }
-                if (j > 0) {
-                    pm_wait(&pv_done, (uint32_t)(j - 1 & 1), a.err, abort);
-                    tc_after();
-#pragma unroll 1
-                    for (int i = 0; i < HD / 32; ++i) {
-                        uint32_t r[32];
-                        tmem_ld32(row + TM_O + 32 * i, r);
-#pragma unroll
-                        for (int x = 0; x < 32; ++x) r[x] = __float_as_uint(__uint_as_float(r[x]) * f);
-                        tmem_st32(row + TM_O + 32 * i, r);
-                    }
-                }
+                m = mx;
             }
+            factor[j % PM_SLOTS][threadIdx.x] = f;
+            const StepCare<NB>& cr = care[j % PM_SLOTS];
             if (cr.any_nan) {
                 // a value row with a NaN enters as zeros: it reaches the rows that see it here, and no other
 #pragma unroll
@@ -311,8 +310,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                     for (int g = 0; g < 4; ++g)
                         if (cr.nan[b][g] & (full ? 0xffffffffu : bits[g])) poison |= 1u << b;
             }
-            const float mu = m == -INFINITY ? 0.f : m, down = vs / vj;      // (a step of smaller scales than O's: its weights follow)
-            const uint64_t k2 = f2(ks, ks), m2 = f2(-mu, -mu), d2 = f2(down, down);
+            const float mu = m == -INFINITY ? 0.f : m;
+            const uint64_t k2 = f2(ks, ks), m2 = f2(-mu, -mu);
             uint64_t sum = f2(0.f, 0.f);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -329,7 +328,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                     }
                     const uint64_t p = f2(x.x, x.y);
                     sum = add2(sum, p);
-                    split_h2(mul2(p, d2), o[i], o[16 + i]);
+                    split_h2(p, o[i], o[16 + i]);
                 }
                 tmem_st32(sbuf + 32 * g, o);        // in place: 16 columns of P's roundings, 16 of what they left
             }
@@ -338,79 +337,58 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             tc_before();
             pm_arrive(&p_full[j & 1]);
         }
-        // ---- the output
-        if (steps > 1) pm_wait(&pv_done, (uint32_t)(steps & 1), a.err, abort);      // (each phase in turn: a wait tells two apart)
-        if (steps > 0) {
-            pm_wait(&pv_done, (uint32_t)(steps - 1 & 1), a.err, abort);
-            tc_after();
-        }
-        const bool whole = a.S == 1;
-        float f = whole ? (l != 0.f ? 1.f / (l * vs) : 0.f) : 1.f / vs;
-        if (state == 2) f = NAN;
-        float* dst = whole ? a.out + th * HD : a.part + (th * a.S + sp) * HD;
-#pragma unroll 1
-        for (int i = 0; i < HD / 32; ++i) {
-            uint32_t r[32];
-            if (steps > 0) tmem_ld32(row + TM_O + 32 * i, r);
-            if (th >= 0) {
-                const float g = poison >> i & 1u ? NAN : f;
-#pragma unroll
-                for (int x = 0; x < 32; x += 4) {
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (steps > 0) v = make_float4(__uint_as_float(r[x]), __uint_as_float(r[x + 1]), __uint_as_float(r[x + 2]), __uint_as_float(r[x + 3]));
-                    *reinterpret_cast<float4*>(dst + 32 * i + x) = make_float4(v.x * g, v.y * g, v.z * g, v.w * g);
-                }
-            }
-        }
-        if (!whole && th >= 0) reinterpret_cast<float2*>(a.ml)[th * a.S + sp] = make_float2(m, state == 2 ? NAN : l);
+        fin_l[threadIdx.x] = state == 2 ? NAN : l;
+        fin_poison[threadIdx.x] = poison;
+        if (a.S > 1 && th >= 0) reinterpret_cast<float2*>(a.ml)[th * a.S + sp] = make_float2(m, state == 2 ? NAN : l);
+        asm volatile("bar.sync 2, 384;" ::: "memory");
     } else if (warp < PM_MMA_WARP) {
-        // ---- codes to planes
+        // ---- codes to planes, and the output
+        regs_inc<152>();
         const int w = warp - PM_DQ_WARP, g = lane >> 2, c = lane & 3;
         auto live = [&](int it, int r) {    // position r of list item it is seen by some row of the CTA
             return it < i1 && seen(tl.at(it) * KV4_P + r);
         };
-        for (int j = 0; j < steps; ++j) {
+        auto raw_step = [&](int j) -> const uint8_t* { return raw + j % PM_RAW * PM_TILES * TB; };
+        // step j's raw tiles are there; what its values' scales call for is known to all warps
+        auto survey = [&](int j) {
             const int at = i0 + PM_TILES * j;
-            const uint8_t* rs = raw + j % PM_RAW * PM_TILES * TB;
-            StepCare<NB>& cr = care[j % 3];
             pm_wait(&raw_full[j % PM_RAW], (uint32_t)(j / PM_RAW & 1), a.err, abort);
-            // the values' scales of tile w: two fp16 a lane
-            {
-                uint32_t big = 0u, nan = 0u;
-                const int i = 2 * lane;
-                if (i < KV4_P * NB) {
-                    const uint32_t x = reinterpret_cast<const uint32_t*>(rs + w * TB + 17 * HD)[lane];
+            StepCare<NB>& cr = care[j % PM_SLOTS];
+            uint32_t big = 0u, nan = 0u;
+            const int i = 2 * lane;         // two fp16 scales of tile w a lane
+            if (i < KV4_P * NB) {
+                const uint32_t x = reinterpret_cast<const uint32_t*>(raw_step(j) + w * TB + 17 * HD)[lane];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t d = (x >> (16 * e)) & 0x7FFFu;
-                        if (d < 0x4000u || !live(at + w, (i + e) / NB)) continue;
-                        if (d > 0x7C00u) nan |= 1u << e;
-                        else big = max(big, __float_as_uint(__half2float(__ushort_as_half((unsigned short)d))));
-                    }
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t d = (x >> (16 * e)) & 0x7FFFu;
+                    if (d < 0x4000u || !live(at + w, (i + e) / NB)) continue;
+                    if (d > 0x7C00u) nan |= 1u << e;
+                    else big = max(big, __float_as_uint(__half2float(__ushort_as_half((unsigned short)d))));
                 }
-                if (__any_sync(0xffffffffu, big | nan)) {
-                    if (big) atomicMax(&cr.vmax, big);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        if (nan >> e & 1u) {
-                            const int r = (i + e) / NB;
-                            cr.any_nan = 1;
-                            atomicOr(&cr.nan[(i + e) % NB][w / 2], 1u << (8 * (r % 8 / 2) + 2 * (2 * (w & 1) + r / 8) + r % 2));
-                        }
-                }
-                // (the slot of step j - 2, whose weights are written: every warp has waited for that step's PV)
-                if (threadIdx.x == 32 * PM_DQ_WARP && j > 0) care[(j + 1) % 3].clear();
-                asm volatile("bar.sync 1, 256;" ::: "memory");
             }
-            const __half2 vs2 = __float2half2_rn(cr.vs()), k2 = __float2half2_rn(0.125f);
-            // K': two (tile, half) units a warp, a position's 8 dims x NB a lane
-            if (j > 0) pm_wait(&qk_done, (uint32_t)(j - 1 & 1), a.err, abort);
+            if (__any_sync(0xffffffffu, big | nan)) {
+                if (big) atomicMax(&cr.vmax, big);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int t = w, h = u;
+                for (int e = 0; e < 2; ++e)
+                    if (nan >> e & 1u) {
+                        const int r = (i + e) / NB;
+                        cr.any_nan = 1;
+                        atomicOr(&cr.nan[(i + e) % NB][w / 2], 1u << (8 * (r % 8 / 2) + 2 * (2 * (w & 1) + r / 8) + r % 2));
+                    }
+            }
+            // (the next step's slot held step j - 3's, which every warp here has seen used: it has waited for that step's PV)
+            if (threadIdx.x == 32 * PM_DQ_WARP) care[(j + 1) % PM_SLOTS].clear();
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+        };
+        // K' of step j: two (tile, half) units a warp, a position's 8 dims x NB a lane
+        auto keys = [&](int j) {
+            const uint8_t* tp = raw_step(j) + w * TB;
+            const __half2 k2 = __float2half2_rn(0.125f);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
                 uint32_t kw[NB], sw[NB / 2];
-                lane_words<HD>(rs + t * TB, h, lane, kw);
-                const uint8_t* sc = rs + t * TB + 16 * HD + (8 * h + g) * NB * 2;
+                lane_words<HD>(tp, h, lane, kw);
+                const uint8_t* sc = tp + 16 * HD + (8 * h + g) * NB * 2;
                 if constexpr (NB == 4) {
                     const uint2 x = lds64(sc);
                     sw[0] = x.x;
@@ -418,11 +396,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 } else {
                     sw[0] = *reinterpret_cast<const uint32_t*>(sc);
                 }
-                if (!live(at + t, 8 * h + g)) {
+                if (!live(i0 + PM_TILES * j + w, 8 * h + g)) {
 #pragma unroll
                     for (int i = 0; i < NB / 2; ++i) sw[i] = 0u;
                 }
-                const int n = t / 2 * 32 + g / 2 * 8 + (2 * (t & 1) + h) * 2 + (g & 1);
+                const int n = w / 2 * 32 + g / 2 * 8 + (2 * (w & 1) + h) * 2 + (g & 1);
                 const int off = n / 8 * 1024 + n % 8 * 128;
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
@@ -449,60 +427,62 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) pm_arrive(&k_full);
-            // V': 32 positions (two tiles) and half the blocks a warp; a lane 8 positions of 4 dims a block
-            if (j > 0) pm_wait(&pv_done, (uint32_t)(j - 1 & 1), a.err, abort);
-            {
-                const int grp = w / 2, b0 = (w & 1) * (NB / 2);
-                uint32_t vw[4][NB / 2], dv[4][NB / 2];
+        };
+        // V' of step j: 32 positions (two tiles) and half the blocks a warp; a lane 8 positions of 4 dims a block
+        auto values = [&](int j) {
+            const uint8_t* rs = raw_step(j);
+            const StepCare<NB>& cr = care[j % PM_SLOTS];
+            const __half2 vs2 = __float2half2_rn(cr.vs());
+            const int any_nan = cr.any_nan, at = i0 + PM_TILES * j;
+            const int grp = w / 2, b0 = (w & 1) * (NB / 2);
+            uint32_t vw[4][NB / 2], dv[4][NB / 2];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int t = 2 * grp + k / 2, h = k % 2;
-                    const uint8_t* tp = rs + t * TB;
-                    const uint8_t* vp = tp + 8 * HD + ((h * 32 + lane) * NB + b0) * 4;
-                    uint32_t s[NB];
-                    lane_scales<HD>(tp + 17 * HD, 8 * h + 2 * c, s);
-                    const uint32_t keep = (live(at + t, 8 * h + 2 * c) ? 0xFFFFu : 0u) | (live(at + t, 8 * h + 2 * c + 1) ? 0xFFFF0000u : 0u);
-                    if constexpr (NB == 4) {
-                        const uint2 x = lds64(vp);
-                        vw[k][0] = x.x;
-                        vw[k][1] = x.y;
-                        const uint32_t s0 = w & 1 ? s[1] : s[0], s1 = w & 1 ? s[3] : s[2];
-                        dv[k][0] = __byte_perm(s0, s1, 0x5410) & keep;
-                        dv[k][1] = __byte_perm(s0, s1, 0x7632) & keep;
-                    } else {
-                        vw[k][0] = *reinterpret_cast<const uint32_t*>(vp);
-                        dv[k][0] = __byte_perm(s[0], s[1], w & 1 ? 0x7632 : 0x5410) & keep;
-                    }
-#pragma unroll
-                    for (int i = 0; i < NB / 2; ++i) {
-                        // (a NaN scale, above infinity's bits, enters as zero)
-                        if (cr.any_nan) {
-                            if ((dv[k][i] & 0x7FFFu) > 0x7C00u) dv[k][i] &= 0xFFFF0000u;
-                            if ((dv[k][i] & 0x7FFF0000u) > 0x7C000000u) dv[k][i] &= 0xFFFFu;
-                        }
-                        dv[k][i] = h2_bits(__hmul2(bits_h2(dv[k][i]), vs2));
-                    }
+            for (int k = 0; k < 4; ++k) {
+                const int t = 2 * grp + k / 2, h = k % 2;
+                const uint8_t* tp = rs + t * TB;
+                const uint8_t* vp = tp + 8 * HD + ((h * 32 + lane) * NB + b0) * 4;
+                uint32_t s[NB];
+                lane_scales<HD>(tp + 17 * HD, 8 * h + 2 * c, s);
+                const uint32_t keep = (live(at + t, 8 * h + 2 * c) ? 0xFFFFu : 0u) | (live(at + t, 8 * h + 2 * c + 1) ? 0xFFFF0000u : 0u);
+                if constexpr (NB == 4) {
+                    const uint2 x = lds64(vp);
+                    vw[k][0] = x.x;
+                    vw[k][1] = x.y;
+                    const uint32_t s0 = w & 1 ? s[1] : s[0], s1 = w & 1 ? s[3] : s[2];
+                    dv[k][0] = __byte_perm(s0, s1, 0x5410) & keep;
+                    dv[k][1] = __byte_perm(s0, s1, 0x7632) & keep;
+                } else {
+                    vw[k][0] = *reinterpret_cast<const uint32_t*>(vp);
+                    dv[k][0] = __byte_perm(s[0], s[1], w & 1 ? 0x7632 : 0x5410) & keep;
                 }
-                const int ch = (grp & 1) * 4 + c;
 #pragma unroll
                 for (int i = 0; i < NB / 2; ++i) {
-                    uint32_t r[4][4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) unpack_signed(vw[k][i], r[k]);
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        uint32_t hi[4], lo[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const __half2 d = bits_h2(dv[k][i]), y = __hmul2(bits_h2(r[k][x]), d);
-                            hi[k] = h2_bits(y);
-                            lo[k] = h2_bits(__hfma2(bits_h2(r[k][x]), d, __hneg2(y)));
-                        }
-                        const int dim = 32 * (b0 + i) + 4 * g + x;
-                        uint8_t* dst = vh + grp / 2 * (HD * 128) + dim / 8 * 1024 + dim % 8 * 128 + (ch ^ (dim % 8)) * 16;
-                        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4*>(dst + PL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    if (any_nan) {          // (a NaN scale, above infinity's bits, enters as zero)
+                        if ((dv[k][i] & 0x7FFFu) > 0x7C00u) dv[k][i] &= 0xFFFF0000u;
+                        if ((dv[k][i] & 0x7FFF0000u) > 0x7C000000u) dv[k][i] &= 0xFFFFu;
                     }
+                    dv[k][i] = h2_bits(__hmul2(bits_h2(dv[k][i]), vs2));
+                }
+            }
+            const int ch = (grp & 1) * 4 + c;
+#pragma unroll
+            for (int i = 0; i < NB / 2; ++i) {
+                uint32_t r[4][4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) unpack_signed(vw[k][i], r[k]);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const __half2 d = bits_h2(dv[k][i]), y = __hmul2(bits_h2(r[k][x]), d);
+                        hi[k] = h2_bits(y);
+                        lo[k] = h2_bits(__hfma2(bits_h2(r[k][x]), d, __hneg2(y)));
+                    }
+                    const int dim = 32 * (b0 + i) + 4 * g + x;
+                    uint8_t* dst = vh + grp / 2 * (HD * 128) + dim / 8 * 1024 + dim % 8 * 128 + (ch ^ (dim % 8)) * 16;
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(dst + PL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             }
             fence_proxy_async();
@@ -511,28 +491,86 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 pm_arrive(&v_full);
                 pm_arrive(&raw_empty[j % PM_RAW]);
             }
+        };
+        // the warp's part of the output: queries 32 (w % 4) + lane, dims HD / 2 * (w / 4) ..
+        const int qr = 32 * (w & 3) + lane, d0 = HD / 2 * (w / 4);
+        const uint32_t otm = tmem + ((uint32_t)(32 * (w & 3)) << 16) + TM_O + d0;
+        uint64_t o[HD / 4];
+#pragma unroll
+        for (int i = 0; i < HD / 4; ++i) o[i] = f2(0.f, 0.f);
+        auto collect = [&](int j) {         // step j's product into the output
+            pm_wait(&pv_done, (uint32_t)(j & 1), a.err, abort);
+            tc_after();
+            const float f = factor[j % PM_SLOTS][qr], u = 1.f / care[j % PM_SLOTS].vs();
+            const uint64_t f1 = f2(f, f), u1 = f2(u, u);
+            if (__any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll
+                for (int i = 0; i < HD / 4; ++i) o[i] = mul2(o[i], f1);
+            }
+#pragma unroll
+            for (int x = 0; x < HD / 64; ++x) {
+                uint32_t r[32];
+                tmem_ld32(otm + 32 * x, r);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    o[16 * x + i] = fma2(f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), u1, o[16 * x + i]);
+            }
+            tc_before();
+            __syncwarp();
+            if (lane == 0) pm_arrive(&o_free);
+        };
+        if (steps > 0) {
+            survey(0);
+            keys(0);
         }
-    } else if (warp == PM_MMA_WARP) {
-        // ---- one thread issues the MMAs: scores of step j, then the output of step j - 1
-        if (lane == 0 && steps > 0) {
+        for (int j = 0; j < steps; ++j) {
+            if (j + 1 < steps) {
+                survey(j + 1);
+                pm_wait(&qk_done, (uint32_t)(j & 1), a.err, abort);
+                keys(j + 1);
+            }
+            if (j > 0) collect(j - 1);
+            values(j);
+        }
+        if (steps > 0) collect(steps - 1);
+        asm volatile("bar.sync 2, 384;" ::: "memory");
+        const int64_t th = query(q0 + qr);
+        if (th >= 0) {
+            const bool whole = a.S == 1;
+            const float l = fin_l[qr];
+            const float f = !whole ? 1.f : l != 0.f ? 1.f / l : 0.f;    // (a refused row's NaN stays; nothing visible: zeros)
+            const uint32_t poison = fin_poison[qr];
+            float* dst = (whole ? a.out + th * HD : a.part + (th * a.S + sp) * HD) + d0;
+#pragma unroll
+            for (int i = 0; i < HD / 4; i += 2) {
+                const float g1 = poison >> ((d0 + 2 * i) / 32) & 1u ? NAN : f;
+                const float2 x = unf2(o[i]), y = unf2(o[i + 1]);
+                *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(x.x * g1, x.y * g1, y.x * g1, y.y * g1);
+            }
+        }
+    } else {
+        regs_dec<24>();
+        if (warp == PM_MMA_WARP && lane == 0 && steps > 0) {
+            // ---- one thread issues the MMAs. The products with remainders come first: sums are cut off at their size.
             auto pv = [&](int j) {
-                // (buffer 1 has an extra first phase, Q's arrival, so its step j is phase j / 2 + 1)
-                pm_wait(&p_full[j & 1], (uint32_t)((j / 2 + (j & 1)) & 1), a.err, abort);
+                pm_wait(&p_full[j & 1], (uint32_t)(j / 2 & 1), a.err, abort);
                 pm_wait(&v_full, (uint32_t)(j & 1), a.err, abort);
+                if (j > 0) pm_wait(&o_free, (uint32_t)(j - 1 & 1), a.err, abort);
                 tc_after();
                 const uint32_t p = tmem + TM_S + (j & 1) * 128;
 #pragma unroll 1
                 for (int s = 0; s < PM_P / 16; ++s) {
-                    const int off = s / 4 * (HD * 128) + s % 4 * 32;
+                    const uint64_t v = pm_desc(vh + s / 4 * (HD * 128) + s % 4 * 32);
                     const uint32_t ph = p + s / 2 * 32 + s % 2 * 8;
-                    pm_mma(tmem + TM_O, ph, pm_desc(vl + off), pm_idesc(HD), j > 0 || s > 0);
-                    pm_mma(tmem + TM_O, ph + 16, pm_desc(vh + off), pm_idesc(HD), 1u);
-                    pm_mma(tmem + TM_O, ph, pm_desc(vh + off), pm_idesc(HD), 1u);
+                    pm_mma(tmem + TM_O, ph, v + (PL >> 4), pm_idesc(HD), s > 0);
+                    pm_mma(tmem + TM_O, ph + 16, v, pm_idesc(HD), 1u);
                 }
+#pragma unroll 1
+                for (int s = 0; s < PM_P / 16; ++s)
+                    pm_mma(tmem + TM_O, p + s / 2 * 32 + s % 2 * 8, pm_desc(vh + s / 4 * (HD * 128) + s % 4 * 32), pm_idesc(HD), 1u);
                 pm_commit(&pv_done);
             };
-            pm_wait(&p_full[1], 0u, a.err, abort);          // Q is in tensor memory
-            tc_after();
+            pm_wait(&q_full, 0u, a.err, abort);
             for (int j = 0; j < steps; ++j) {
                 pm_wait(&k_full, (uint32_t)(j & 1), a.err, abort);
                 if (j > 1) pm_wait(&pv_done, (uint32_t)(j & 1), a.err, abort);      // the weights that this score buffer held are used
@@ -540,29 +578,31 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 const uint32_t d = tmem + TM_S + (j & 1) * 128;
 #pragma unroll 1
                 for (int s = 0; s < HD / 16; ++s) {
-                    const int off = s / 4 * (PM_P * 128) + s % 4 * 32;
-                    pm_mma(d, tmem + TM_QH + 8 * s, pm_desc(kl + off), pm_idesc(PM_P), s > 0);
-                    pm_mma(d, tmem + TM_QL + 8 * s, pm_desc(kh + off), pm_idesc(PM_P), 1u);
-                    pm_mma(d, tmem + TM_QH + 8 * s, pm_desc(kh + off), pm_idesc(PM_P), 1u);
+                    const uint64_t k = pm_desc(kh + s / 4 * (PM_P * 128) + s % 4 * 32);
+                    pm_mma(d, tmem + TM_QH + 8 * s, k + (PL >> 4), pm_idesc(PM_P), s > 0);
+                    pm_mma(d, tmem + TM_QL + 8 * s, k, pm_idesc(PM_P), 1u);
                 }
+#pragma unroll 1
+                for (int s = 0; s < HD / 16; ++s)
+                    pm_mma(d, tmem + TM_QH + 8 * s, pm_desc(kh + s / 4 * (PM_P * 128) + s % 4 * 32), pm_idesc(PM_P), 1u);
                 pm_commit(&s_full[j & 1]);
                 pm_commit(&qk_done);
                 if (j > 0) pv(j - 1);
             }
             pv(steps - 1);
-        }
-    } else if (lane == 0) {
-        // ---- raw tiles
-        const uint8_t* src = base + (int64_t)kvh * TB;
-        for (int j = 0; j < steps; ++j) {
-            const int s = j % PM_RAW, at = i0 + PM_TILES * j, n = min(PM_TILES, i1 - at);
-            if (j >= PM_RAW) {
-                pm_wait(&raw_empty[s], (uint32_t)((j / PM_RAW + 1) & 1), a.err, abort);
-                fence_proxy_async();
+        } else if (warp == PM_RAW_WARP && lane == 0) {
+            // ---- raw tiles
+            const uint8_t* src = base + (int64_t)kvh * TB;
+            for (int j = 0; j < steps; ++j) {
+                const int s = j % PM_RAW, at = i0 + PM_TILES * j, n = min(PM_TILES, i1 - at);
+                if (j >= PM_RAW) {
+                    pm_wait(&raw_empty[s], (uint32_t)((j / PM_RAW + 1) & 1), a.err, abort);
+                    fence_proxy_async();
+                }
+                mbar_expect_tx(&raw_full[s], n * TB);
+                for (int i = 0; i < n; ++i)
+                    bulk_load(raw + (s * PM_TILES + i) * TB, src + (int64_t)tl.at(at + i) * a.kv_heads * TB, TB, &raw_full[s]);
             }
-            mbar_expect_tx(&raw_full[s], n * TB);
-            for (int i = 0; i < n; ++i)
-                bulk_load(raw + (s * PM_TILES + i) * TB, src + (int64_t)tl.at(at + i) * a.kv_heads * TB, TB, &raw_full[s]);
         }
     }
     tc_before();
@@ -573,9 +613,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
     }
     if (a.S == 1) return;
     if (!last_ticket(a.tickets + ((int64_t)run * a.kv_heads + kvh) * q_blocks + qb, a.S)) return;
-    join_ranges<HD, PM_THREADS>(a, min(PM_Q, nq - q0), a.S, reinterpret_cast<float*>(smem), [&](int i) {
-        return ((int64_t)run * a.R + (q0 + i) / G) * a.heads + kvh * G + (q0 + i) % G;
-    });
+    join_ranges<HD, PM_THREADS>(a, min(PM_Q, nq - q0), a.S, reinterpret_cast<float*>(smem), [&](int i) { return query(q0 + i); });
 }
 
 template <int HD> void launch_mma(const Kv4Att& a, int q_blocks, cudaStream_t s)
