@@ -111,6 +111,19 @@ __device__ __forceinline__ void pm_commit(uint64_t* bar)
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// Bits [0, 16) of the positions p0 .. p0 + 15 that v sees.
+__device__ __forceinline__ uint32_t seen16(const Vis& v, int p0)
+{
+    auto below = [&](int n) { return n <= p0 ? 0u : n >= p0 + 16 ? 0xFFFFu : (1u << (n - p0)) - 1u; };
+    return below(v.n) & (~below(v.first) | below(v.sink));
+}
+// Those of a tile's 16 positions in the order of the step's slots: position 8 h + 2 c + e at bit 8 c + 2 h + e.
+__device__ __forceinline__ uint32_t slots16(uint32_t x)
+{
+    auto spread = [](uint32_t y) { return (y & 3u) | (y & 0xCu) << 6 | (y & 0x30u) << 12 | (y & 0xC0u) << 18; };
+    return spread(x) | spread(x >> 8) << 2;
+}
+
 // What the values' scales of a step call for (slot j % PM_SLOTS): the largest scale of 2 or more, and where scales are NaN (a value
 // row that held an infinity or NaN): bit n of word n / 32 of block b is slot n.
 template <int NB> struct StepCare {
@@ -260,38 +273,35 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             const uint32_t sbuf = row + TM_S + (j & 1) * 128;
             pm_wait(&s_full[j & 1], (uint32_t)(j / 2 & 1), a.err, abort);
             tc_after();
-            // seen columns: all, or bit n of word n / 32
             const int at = i0 + PM_TILES * j;
             const bool full = at + PM_TILES <= i1 && tl.at(at) * KV4_P >= w_max_first && tl.at(at + PM_TILES - 1) * KV4_P + KV4_P <= w_min_n;
-            uint32_t bits[4];
-            if (!full) {
+            // bit n: this query sees column 32 g + n
+            auto seen32 = [&](int g) {
+                uint32_t b = 0u;
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    bits[g] = 0u;
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const int it = at + 2 * g + t;
-                        if (it < i1) {
-                            const int p0 = tl.at(it) * KV4_P;
-#pragma unroll
-                            for (int i = 0; i < KV4_P; ++i)
-                                if (vis(p0 + i)) bits[g] |= 1u << (8 * (i % 8 / 2) + 2 * (2 * t + i / 8) + i % 2);
-                        }
-                    }
+                for (int t = 0; t < 2; ++t) {
+                    const int it = at + 2 * g + t;
+                    if (it < i1) b |= slots16(seen16(vis, tl.at(it) * KV4_P)) << (4 * t);
                 }
-            }
-            float mx = -INFINITY;
+                return b;
+            };
+            // a group's scores, those not seen at -inf (the loops are kept rolled: unrolled, the three roles' code outgrew
+            // the instruction caches and a step took twice as long)
+            auto scores = [&](int g, uint32_t (&r)[32]) {
+                tmem_ld32(sbuf + 32 * g, r);
+                if (!full) {
+                    const uint32_t b = seen32(g);
 #pragma unroll
+                    for (int i = 0; i < 32; ++i) r[i] = b >> i & 1u ? r[i] : 0xFF800000u;
+                }
+            };
+            float mx = -INFINITY;
+#pragma unroll 1
             for (int g = 0; g < 4; ++g) {
                 uint32_t r[32];
-                tmem_ld32(sbuf + 32 * g, r);
-                if (full) {
+                scores(g, r);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, bits[g] >> i & 1u ? __uint_as_float(r[i]) : -INFINITY);
-                }
+                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
             }
             mx *= ks;
             float f = 1.f;
@@ -304,29 +314,23 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             const StepCare<NB>& cr = care[j % PM_SLOTS];
             if (cr.any_nan) {
                 // a value row with a NaN enters as zeros: it reaches the rows that see it here, and no other
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int g = 0; g < 4; ++g)
-                        if (cr.nan[b][g] & (full ? 0xffffffffu : bits[g])) poison |= 1u << b;
+                for (int g = 0; g < 4; ++g) {
+                    const uint32_t see = full ? 0xffffffffu : seen32(g);
+                    for (int b = 0; b < NB; ++b)
+                        if (cr.nan[b][g] & see) poison |= 1u << b;
+                }
             }
             const float mu = m == -INFINITY ? 0.f : m;
             const uint64_t k2 = f2(ks, ks), m2 = f2(-mu, -mu);
             uint64_t sum = f2(0.f, 0.f);
-#pragma unroll
+#pragma unroll 1
             for (int g = 0; g < 4; ++g) {
                 uint32_t r[32], o[32];
-                tmem_ld32(sbuf + 32 * g, r);
+                scores(g, r);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float2 x = unf2(fma2(f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), k2, m2));
-                    x.x = ex2(x.x);
-                    x.y = ex2(x.y);
-                    if (!full) {
-                        x.x = bits[g] >> (2 * i) & 1u ? x.x : 0.f;
-                        x.y = bits[g] >> (2 * i + 1) & 1u ? x.y : 0.f;
-                    }
-                    const uint64_t p = f2(x.x, x.y);
+                    const float2 x = unf2(fma2(f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), k2, m2));
+                    const uint64_t p = f2(ex2(x.x), ex2(x.y));
                     sum = add2(sum, p);
                     split_h2(p, o[i], o[16 + i]);
                 }
@@ -384,7 +388,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         auto keys = [&](int j) {
             const uint8_t* tp = raw_step(j) + w * TB;
             const __half2 k2 = __float2half2_rn(0.125f);
-#pragma unroll
+#pragma unroll 1
             for (int h = 0; h < 2; ++h) {
                 uint32_t kw[NB], sw[NB / 2];
                 lane_words<HD>(tp, h, lane, kw);
@@ -434,52 +438,38 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             const StepCare<NB>& cr = care[j % PM_SLOTS];
             const __half2 vs2 = __float2half2_rn(cr.vs());
             const int any_nan = cr.any_nan, at = i0 + PM_TILES * j;
-            const int grp = w / 2, b0 = (w & 1) * (NB / 2);
-            uint32_t vw[4][NB / 2], dv[4][NB / 2];
+            const int grp = w / 2, ch = (grp & 1) * 4 + c;
+            uint32_t keep[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int t = 2 * grp + k / 2, h = k % 2;
-                const uint8_t* tp = rs + t * TB;
-                const uint8_t* vp = tp + 8 * HD + ((h * 32 + lane) * NB + b0) * 4;
-                uint32_t s[NB];
-                lane_scales<HD>(tp + 17 * HD, 8 * h + 2 * c, s);
-                const uint32_t keep = (live(at + t, 8 * h + 2 * c) ? 0xFFFFu : 0u) | (live(at + t, 8 * h + 2 * c + 1) ? 0xFFFF0000u : 0u);
-                if constexpr (NB == 4) {
-                    const uint2 x = lds64(vp);
-                    vw[k][0] = x.x;
-                    vw[k][1] = x.y;
-                    const uint32_t s0 = w & 1 ? s[1] : s[0], s1 = w & 1 ? s[3] : s[2];
-                    dv[k][0] = __byte_perm(s0, s1, 0x5410) & keep;
-                    dv[k][1] = __byte_perm(s0, s1, 0x7632) & keep;
-                } else {
-                    vw[k][0] = *reinterpret_cast<const uint32_t*>(vp);
-                    dv[k][0] = __byte_perm(s[0], s[1], w & 1 ? 0x7632 : 0x5410) & keep;
-                }
-#pragma unroll
-                for (int i = 0; i < NB / 2; ++i) {
-                    if (any_nan) {          // (a NaN scale, above infinity's bits, enters as zero)
-                        if ((dv[k][i] & 0x7FFFu) > 0x7C00u) dv[k][i] &= 0xFFFF0000u;
-                        if ((dv[k][i] & 0x7FFF0000u) > 0x7C000000u) dv[k][i] &= 0xFFFFu;
-                    }
-                    dv[k][i] = h2_bits(__hmul2(bits_h2(dv[k][i]), vs2));
-                }
+                const int it = at + 2 * grp + k / 2, r = 8 * (k & 1) + 2 * c;
+                keep[k] = (live(it, r) ? 0xFFFFu : 0u) | (live(it, r + 1) ? 0xFFFF0000u : 0u);
             }
-            const int ch = (grp & 1) * 4 + c;
+#pragma unroll 1
+            for (int b = (w & 1) * (NB / 2), e = b + NB / 2; b < e; ++b) {
+                uint32_t r[4][4], dv[4];
 #pragma unroll
-            for (int i = 0; i < NB / 2; ++i) {
-                uint32_t r[4][4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) unpack_signed(vw[k][i], r[k]);
+                for (int k = 0; k < 4; ++k) {
+                    const uint8_t* tp = rs + (2 * grp + k / 2) * TB;
+                    unpack_signed(*reinterpret_cast<const uint32_t*>(tp + 8 * HD + (((k & 1) * 32 + lane) * NB + b) * 4), r[k]);
+                    const uint16_t* sc = reinterpret_cast<const uint16_t*>(tp + 17 * HD) + (8 * (k & 1) + 2 * c) * NB + b;
+                    dv[k] = ((uint32_t)sc[0] | (uint32_t)sc[NB] << 16) & keep[k];
+                    if (any_nan) {          // (a NaN scale, above infinity's bits, enters as zero)
+                        if ((dv[k] & 0x7FFFu) > 0x7C00u) dv[k] &= 0xFFFF0000u;
+                        if ((dv[k] & 0x7FFF0000u) > 0x7C000000u) dv[k] &= 0xFFFFu;
+                    }
+                    dv[k] = h2_bits(__hmul2(bits_h2(dv[k]), vs2));
+                }
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const __half2 d = bits_h2(dv[k][i]), y = __hmul2(bits_h2(r[k][x]), d);
+                        const __half2 d = bits_h2(dv[k]), y = __hmul2(bits_h2(r[k][x]), d);
                         hi[k] = h2_bits(y);
                         lo[k] = h2_bits(__hfma2(bits_h2(r[k][x]), d, __hneg2(y)));
                     }
-                    const int dim = 32 * (b0 + i) + 4 * g + x;
+                    const int dim = 32 * b + 4 * g + x;
                     uint8_t* dst = vh + grp / 2 * (HD * 128) + dim / 8 * 1024 + dim % 8 * 128 + (ch ^ (dim % 8)) * 16;
                     *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     *reinterpret_cast<uint4*>(dst + PL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -558,16 +548,20 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 if (j > 0) pm_wait(&o_free, (uint32_t)(j - 1 & 1), a.err, abort);
                 tc_after();
                 const uint32_t p = tmem + TM_S + (j & 1) * 128;
+                uint64_t v = pm_desc(vh);           // (16-byte units: 2 a step of 16 positions, an atom's HD rows of 128 bytes a step of 64)
 #pragma unroll 1
-                for (int s = 0; s < PM_P / 16; ++s) {
-                    const uint64_t v = pm_desc(vh + s / 4 * (HD * 128) + s % 4 * 32);
-                    const uint32_t ph = p + s / 2 * 32 + s % 2 * 8;
-                    pm_mma(tmem + TM_O, ph, v + (PL >> 4), pm_idesc(HD), s > 0);
-                    pm_mma(tmem + TM_O, ph + 16, v, pm_idesc(HD), 1u);
-                }
+                for (int s = 0; s < PM_P / 64; ++s, v += HD * 8)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const uint32_t ph = p + 64 * s + x / 2 * 32 + x % 2 * 8;
+                        pm_mma(tmem + TM_O, ph, v + 2 * x + (PL >> 4), pm_idesc(HD), s > 0 || x > 0);
+                        pm_mma(tmem + TM_O, ph + 16, v + 2 * x, pm_idesc(HD), 1u);
+                    }
+                v = pm_desc(vh);
 #pragma unroll 1
-                for (int s = 0; s < PM_P / 16; ++s)
-                    pm_mma(tmem + TM_O, p + s / 2 * 32 + s % 2 * 8, pm_desc(vh + s / 4 * (HD * 128) + s % 4 * 32), pm_idesc(HD), 1u);
+                for (int s = 0; s < PM_P / 64; ++s, v += HD * 8)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) pm_mma(tmem + TM_O, p + 64 * s + x / 2 * 32 + x % 2 * 8, v + 2 * x, pm_idesc(HD), 1u);
                 pm_commit(&pv_done);
             };
             pm_wait(&q_full, 0u, a.err, abort);
@@ -576,15 +570,19 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 if (j > 1) pm_wait(&pv_done, (uint32_t)(j & 1), a.err, abort);      // the weights that this score buffer held are used
                 tc_after();
                 const uint32_t d = tmem + TM_S + (j & 1) * 128;
+                uint64_t k = pm_desc(kh);
 #pragma unroll 1
-                for (int s = 0; s < HD / 16; ++s) {
-                    const uint64_t k = pm_desc(kh + s / 4 * (PM_P * 128) + s % 4 * 32);
-                    pm_mma(d, tmem + TM_QH + 8 * s, k + (PL >> 4), pm_idesc(PM_P), s > 0);
-                    pm_mma(d, tmem + TM_QL + 8 * s, k, pm_idesc(PM_P), 1u);
-                }
+                for (int s = 0; s < HD / 64; ++s, k += PM_P * 8)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        pm_mma(d, tmem + TM_QH + 32 * s + 8 * x, k + 2 * x + (PL >> 4), pm_idesc(PM_P), s > 0 || x > 0);
+                        pm_mma(d, tmem + TM_QL + 32 * s + 8 * x, k + 2 * x, pm_idesc(PM_P), 1u);
+                    }
+                k = pm_desc(kh);
 #pragma unroll 1
-                for (int s = 0; s < HD / 16; ++s)
-                    pm_mma(d, tmem + TM_QH + 8 * s, pm_desc(kh + s / 4 * (PM_P * 128) + s % 4 * 32), pm_idesc(PM_P), 1u);
+                for (int s = 0; s < HD / 64; ++s, k += PM_P * 8)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) pm_mma(d, tmem + TM_QH + 32 * s + 8 * x, k + 2 * x, pm_idesc(PM_P), 1u);
                 pm_commit(&s_full[j & 1]);
                 pm_commit(&qk_done);
                 if (j > 0) pv(j - 1);
