@@ -266,7 +266,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             tc_before();
             pm_arrive(&q_full);
         }
-        const int w_min_n = __reduce_min_sync(0xffffffffu, vis.n), w_max_first = __reduce_max_sync(0xffffffffu, vis.first);
+        // (queries that see nothing, or are none, need no mask: their output is not read)
+        const int w_min_n = __reduce_min_sync(0xffffffffu, vis.n > 0 ? vis.n : INT_MAX), w_max_first = __reduce_max_sync(0xffffffffu, vis.first);
         float m = -INFINITY, l = 0.f;
         uint32_t poison = 0u;               // blocks of the output that a seen NaN reached
         for (int j = 0; j < steps; ++j) {
@@ -274,7 +275,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             pm_wait(&s_full[j & 1], (uint32_t)(j / 2 & 1), a.err, abort);
             tc_after();
             const int at = i0 + PM_TILES * j;
-            const bool full = at + PM_TILES <= i1 && tl.at(at) * KV4_P >= w_max_first && tl.at(at + PM_TILES - 1) * KV4_P + KV4_P <= w_min_n;
+            // every query of the warp sees all of column group g (two tiles)
+            auto full = [&](int g) {
+                const int it = at + 2 * g;
+                return it + 1 < i1 && tl.at(it) * KV4_P >= w_max_first && tl.at(it + 1) * KV4_P + KV4_P <= w_min_n;
+            };
             // bit n: this query sees column 32 g + n
             auto seen32 = [&](int g) {
                 uint32_t b = 0u;
@@ -289,7 +294,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             // the instruction caches and a step took twice as long)
             auto scores = [&](int g, uint32_t (&r)[32]) {
                 tmem_ld32(sbuf + 32 * g, r);
-                if (!full) {
+                if (!full(g)) {
                     const uint32_t b = seen32(g);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) r[i] = b >> i & 1u ? r[i] : 0xFF800000u;
@@ -315,7 +320,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             if (cr.any_nan) {
                 // a value row with a NaN enters as zeros: it reaches the rows that see it here, and no other
                 for (int g = 0; g < 4; ++g) {
-                    const uint32_t see = full ? 0xffffffffu : seen32(g);
+                    const uint32_t see = seen32(g);
                     for (int b = 0; b < NB; ++b)
                         if (cr.nan[b][g] & see) poison |= 1u << b;
                 }
@@ -341,9 +346,10 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             tc_before();
             pm_arrive(&p_full[j & 1]);
         }
-        fin_l[threadIdx.x] = state == 2 ? NAN : l;
+        if (state) l = state == 2 ? NAN : 0.f;
+        fin_l[threadIdx.x] = l;
         fin_poison[threadIdx.x] = poison;
-        if (a.S > 1 && th >= 0) reinterpret_cast<float2*>(a.ml)[th * a.S + sp] = make_float2(m, state == 2 ? NAN : l);
+        if (a.S > 1 && th >= 0) reinterpret_cast<float2*>(a.ml)[th * a.S + sp] = make_float2(state ? -INFINITY : m, l);
         asm volatile("bar.sync 2, 384;" ::: "memory");
     } else if (warp < PM_MMA_WARP) {
         // ---- codes to planes, and the output
