@@ -31,8 +31,8 @@ namespace k {
 namespace {
 
 constexpr int SR_THREADS = 512, SR_WARPS = SR_THREADS / 32;
-constexpr int SR_BINS = 2048;               // histogram bins
-constexpr int SR_CAP = 256;                 // ids ranked at once
+constexpr int SR_BINS = 2048;               // most histogram bins: 512 a CTA of the cluster, one a thread
+constexpr int SR_CAP = SR_THREADS;          // ids ranked at once, one a thread
 constexpr int SR_MAX_CLUSTER = 8;
 constexpr int SR_SLICE_MAX = 44 * 1024;     // logits a CTA keeps in shared memory; longer slices are read from L2
 
@@ -69,12 +69,20 @@ struct Item {               // a selected id: its key, id, and the sum up to and
     u64 cum;
 };
 
-struct RowShared {
+// A row's state in a CTA's shared memory (all of its scalars the same for all threads).
+struct Row {
     uint32_t lo[SR_BINS], hi[SR_BINS];      // per bin: a count (lo), or a 64-bit sum in two words
     double exp2_table[64];
     u64 scan[SR_WARPS], red[SR_WARPS];
+    const float* xs;                        // this CTA's slice
+    int n, id0, C, rank, bins, frac;        // its length and first id; the cluster; bins in use
+    float xmax, inv_w;                      // the histogram: bin = (xmax / 2 - x / 2) * inv_w
+    double inv_t, unit;                     // log2(e) / temperature, 2^F
+    int has_k;                              // a top-k cut: ids up to (k_key, k_id) in the order
+    uint32_t k_key, k_id;
     // published by every CTA of the cluster into each
-    u64 part[SR_MAX_CLUSTER], best[SR_MAX_CLUSTER], low[SR_MAX_CLUSTER], min_part[SR_MAX_CLUSTER];
+    u64 part[SR_MAX_CLUSTER], best[SR_MAX_CLUSTER], min_part[SR_MAX_CLUSTER];
+    uint32_t low[SR_MAX_CLUSTER];
     int bin;                                // the crossing bin and the sum before it
     u64 before;
     Item item;
@@ -83,31 +91,13 @@ struct RowShared {
     uint32_t kmin, kmax, imin, imax;
     uint32_t ckey[SR_CAP], cid[SR_CAP];
     u64 cval[SR_CAP];
-};
 
-__device__ __forceinline__ u64 warp_sum(u64 v)
-{
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
-struct Sampler {
-    RowShared& sh;
-    const float* xs;            // this CTA's slice
-    int n, id0, C, rank;        // its length and first id; the cluster
-    float xmax, inv_w;          // the histogram: bin = (xmax / 2 - x / 2) * inv_w
-    double inv_t;               // log2(e) / temperature
-    double unit;                // 2^F
-    bool has_k;                 // a top-k cut: ids up to (k_key, k_id) in the order
-    uint32_t k_key, k_id;
-    int frac;
-
-    __device__ __forceinline__ bool valid(float x) const { return x > -INFINITY; }
-    __device__ __forceinline__ bool kept(uint32_t key, uint32_t id) const
+    __device__ __forceinline__ bool kept(uint32_t key, uint32_t id) const { return !has_k || key > k_key || (key == k_key && id <= k_id); }
+    __device__ __forceinline__ int bin0(float x) const
     {
-        return !has_k || key > k_key || (key == k_key && id <= k_id);
+        return (int)fminf((xmax * 0.5f - x * 0.5f) * inv_w, (float)(bins - 1));     // (NaN, of infinities: the last bin)
     }
+    __device__ __forceinline__ u64 mass(double p) const { return (u64)(p * unit + 0.5); }
     // exp((x - xmax) / T) for a valid x: 2^y by table and polynomial (Tang's table-driven scheme: y = n + j/64 + r,
     // 2^(j/64) from the table, e^(r ln 2) to the fifth power, its remainder below 2^-54)
     __device__ __forceinline__ double prob(float x) const
@@ -123,259 +113,290 @@ struct Sampler {
         e = fma(t, e, 0.5);
         e = fma(t, e, 1.0);
         e = fma(t, e, 1.0);
-        const double m = sh.exp2_table[i & 63] * e;
+        const double m = exp2_table[i & 63] * e;
         return __longlong_as_double(__double_as_longlong(m) + ((long long)(i >> 6) << 52));
-    }
-    __device__ __forceinline__ u64 mass(double p) const { return (u64)(p * unit + 0.5); }
-
-    __device__ __forceinline__ int bin0(float x) const
-    {
-        return (int)fminf((xmax * 0.5f - x * 0.5f) * inv_w, (float)(SR_BINS - 1));     // (NaN, of infinities: bin 2047)
-    }
-
-    template <typename T> __device__ __forceinline__ void publish(T* p, T v)
-    {
-        for (int r = 0; r < C; ++r) *remote(p, r) = v;
-    }
-
-    __device__ __forceinline__ u64 block_sum(u64 v)
-    {
-        v = warp_sum(v);
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) sh.red[threadIdx.x >> 5] = v;
-        __syncthreads();
-        u64 s = 0;
-#pragma unroll
-        for (int w = 0; w < SR_WARPS; ++w) s += sh.red[w];
-        return s;
-    }
-
-    // Sum over the threads before this one.
-    __device__ __forceinline__ u64 block_before(u64 v, u64* total)
-    {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        u64 inc = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 u = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += u;
-        }
-        __syncthreads();
-        if (lane == 31) sh.scan[warp] = inc;
-        __syncthreads();
-        u64 b = 0, all = 0;
-#pragma unroll
-        for (int w = 0; w < SR_WARPS; ++w) {
-            if (w < warp) b += sh.scan[w];
-            all += sh.scan[w];
-        }
-        *total = all;
-        return b + inc - v;
-    }
-
-    __device__ __forceinline__ void clear_hist()
-    {
-        for (int b = threadIdx.x; b < SR_BINS; b += SR_THREADS) sh.lo[b] = sh.hi[b] = 0u;
-        __syncthreads();
     }
     __device__ __forceinline__ void add(int b, u64 v, bool count)
     {
         if (count) {
-            atomicAdd(&sh.lo[b], 1u);
+            atomicAdd(&lo[b], 1u);
         } else {
             // a 64-bit sum of two 32-bit words: the add that wraps the low word carries into the high one
-            const uint32_t l = (uint32_t)v, old = atomicAdd(&sh.lo[b], l);
+            const uint32_t l = (uint32_t)v, old = atomicAdd(&lo[b], l);
             const uint32_t h = (uint32_t)(v >> 32) + (old + l < old ? 1u : 0u);
-            if (h) atomicAdd(&sh.hi[b], h);
+            if (h) atomicAdd(&hi[b], h);
         }
     }
-
-    // The cluster's histogram: this CTA joins its share of the bins (thread t: `per` bins from first), and every CTA learns
-    // the shares' sums.
-    static constexpr int PER_MAX = SR_BINS / SR_THREADS;
-    struct Joined {
-        u64 v[PER_MAX], before, total;
-        int first, per;
-    };
-    __device__ __forceinline__ void join(Joined& j, bool count)
+    // (one thread)
+    template <typename T> __device__ __forceinline__ void publish(T* p, T v)
     {
-        cluster_sync();                     // every CTA's histogram is complete
-        const int share = SR_BINS / C;
-        j.per = share > SR_THREADS ? share / SR_THREADS : 1;
-        const int at = threadIdx.x * j.per;
-        j.first = rank * share + at;
-        u64 s = 0;
-#pragma unroll
-        for (int i = 0; i < PER_MAX; ++i) {
-            j.v[i] = 0;
-            if (i < j.per && at + i < share) {
-                for (int r = 0; r < C; ++r) {
-                    j.v[i] += *remote(&sh.lo[j.first + i], r);
-                    if (!count) j.v[i] += (u64)*remote(&sh.hi[j.first + i], r) << 32;
-                }
-                s += j.v[i];
-            }
-        }
-        u64 mine;
-        j.before = block_before(s, &mine);
-        if (threadIdx.x == 0) publish(&sh.part[rank], mine);
-        cluster_sync();
-        j.total = 0;
-        for (int r = 0; r < C; ++r) {
-            if (r < rank) j.before += sh.part[r];
-            j.total += sh.part[r];
-        }
-    }
-    // The bin in which base + the running sum first reaches target (1 <= target - base <= total), in sh.bin and sh.before of
-    // every CTA; clears the list of the gather that follows.
-    __device__ __forceinline__ void find(const Joined& j, u64 target, u64 base)
-    {
-        u64 b = base + j.before;
-#pragma unroll
-        for (int i = 0; i < PER_MAX; ++i) {
-            const u64 e = b + j.v[i];
-            if (b < target && e >= target) {
-                publish(&sh.bin, j.first + i);
-                publish(&sh.before, b);
-            }
-            b = e;
-        }
-        if (rank == 0 && threadIdx.x == 0) {
-            sh.n_cand = 0;
-            sh.kmin = sh.imin = UINT_MAX;
-            sh.kmax = sh.imax = 0u;
-        }
-        cluster_sync();
-    }
-
-    // The item at which the running sum (of ones, or of masses) reaches target; the level-0 histogram is joined in j.
-    __device__ Item select(const Joined& j0, u64 target, bool count)
-    {
-        find(j0, target, 0);
-        int bin = sh.bin;
-        u64 before = sh.before;
-        bool deep = false;                  // past level 0: the ids with keys [klo, khi] and ids [ilo, ihi]
-        uint32_t klo = 0u, khi = UINT_MAX, ilo = 0u, ihi = UINT_MAX;
-        RowShared* lead = remote(&sh, 0);
-        // (a cut by keys leaves 2^-11 of their range, one by ids of theirs: at most seven rounds)
-        for (int round = 0; round < 16; ++round) {
-            // gather the range's ids (with a mass) to CTA 0
-            auto each = [&](auto&& f) {
-                for (int i = threadIdx.x; i < n; i += SR_THREADS) {
-                    const float x = xs[i];
-                    if (!valid(x)) continue;
-                    const uint32_t key = order_key(x), id = (uint32_t)(id0 + i);
-                    if (deep ? key < klo || key > khi || id < ilo || id > ihi : bin0(x) != bin) continue;
-                    if (!kept(key, id)) continue;
-                    const u64 m = count ? 1ull : mass(prob(x));
-                    if (m) f(key, id, m);
-                }
-            };
-            each([&](uint32_t key, uint32_t id, u64 m) {
-                // one add for the lanes that are here together
-                const uint32_t here = __activemask(), lane = threadIdx.x & 31;
-                int at = 0;
-                if (lane == __ffs(here) - 1) at = atomicAdd(&lead->n_cand, __popc(here));
-                at = __shfl_sync(here, at, __ffs(here) - 1) + __popc(here & ((1u << lane) - 1u));
-                if (at < SR_CAP) {
-                    lead->ckey[at] = key;
-                    lead->cid[at] = id;
-                    lead->cval[at] = m;
-                }
-            });
-            cluster_sync();
-            const int nc = lead->n_cand;
-            if (nc <= SR_CAP) {
-                if (rank == 0 && (int)threadIdx.x < nc) {
-                    const uint32_t key = sh.ckey[threadIdx.x], id = sh.cid[threadIdx.x];
-                    u64 c = before;
-                    for (int q = 0; q < nc; ++q)
-                        if (sh.ckey[q] > key || (sh.ckey[q] == key && sh.cid[q] <= id)) c += sh.cval[q];
-                    if (c >= target && c - sh.cval[threadIdx.x] < target) publish(&sh.item, Item{key, id, c});
-                }
-                cluster_sync();
-                return sh.item;
-            }
-            // a crowded range: cut it by the bits of its keys, or, all keys equal, by ids
-            uint32_t k0 = UINT_MAX, k1 = 0u, d0 = UINT_MAX, d1 = 0u;
-            each([&](uint32_t key, uint32_t id, u64) {
-                k0 = min(k0, key);
-                k1 = max(k1, key);
-                d0 = min(d0, id);
-                d1 = max(d1, id);
-            });
-            k0 = __reduce_min_sync(0xffffffffu, k0);
-            k1 = __reduce_max_sync(0xffffffffu, k1);
-            d0 = __reduce_min_sync(0xffffffffu, d0);
-            d1 = __reduce_max_sync(0xffffffffu, d1);
-            if ((threadIdx.x & 31) == 0 && k0 <= k1) {
-                atomicMin(&lead->kmin, k0);
-                atomicMax(&lead->kmax, k1);
-                atomicMin(&lead->imin, d0);
-                atomicMax(&lead->imax, d1);
-            }
-            cluster_sync();
-            klo = lead->kmin; khi = lead->kmax; ilo = lead->imin; ihi = lead->imax;
-            deep = true;
-            const bool by_id = klo == khi;
-            const uint32_t width = by_id ? ihi - ilo : khi - klo;
-            const int shift = max(0, 32 - __clz(width) - 11);
-            clear_hist();
-            each([&](uint32_t key, uint32_t id, u64 m) { add((by_id ? id - ilo : khi - key) >> shift, m, count); });
-            Joined j;
-            join(j, count);
-            find(j, target, before);
-            before = sh.before;
-            const uint32_t from = (uint32_t)sh.bin << shift, upto = from + ((1u << shift) - 1u);
-            if (by_id) {
-                const uint32_t i0 = ilo;
-                ilo = i0 + from;
-                ihi = min(ihi, i0 + upto);
-            } else {
-                const uint32_t top = khi;
-                khi = top - from;
-                klo = top - klo > upto ? top - upto : klo;
-            }
-        }
-        return sh.item;
+        for (int r = 0; r < C; ++r) *remote(p, r) = v;
     }
 };
 
-__global__ void __launch_bounds__(SR_THREADS, 1) k_sample_rows(const float* logits, int64_t ld, int V, int frac,
-                                                            const wl_sample_opts* opts, int32_t* ids, int slice, int in_smem)
+__device__ __forceinline__ bool valid(float x) { return x > -INFINITY; }
+
+// Sum over the threads before this one, and over all.
+__device__ __noinline__ u64 block_before(Row& s, u64 v, u64* total)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    u64 inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
+    }
+    __syncthreads();
+    if (lane == 31) s.scan[warp] = inc;
+    __syncthreads();
+    u64 b = 0, all = 0;
+    for (int w = 0; w < SR_WARPS; ++w) {
+        const u64 x = s.scan[w];
+        if (w < warp) b += x;
+        all += x;
+    }
+    *total = all;
+    return b + inc - v;
+}
+
+__device__ __forceinline__ void clear_hist(Row& s)
+{
+    for (int b = threadIdx.x; b < s.bins; b += SR_THREADS) s.lo[b] = s.hi[b] = 0u;
+    __syncthreads();
+}
+
+// The cluster's histogram joined: this thread's bin (its CTA's share of bins, one a thread), the sum before it, and all.
+struct Joined {
+    u64 v, before, total;
+};
+__device__ __noinline__ Joined join(Row& s, bool count)
+{
+    cluster_sync();                         // every CTA's histogram is complete
+    const int share = s.bins / s.C, at = s.rank * share + threadIdx.x;
+    Joined j;
+    j.v = 0;
+    if ((int)threadIdx.x < share) {
+#pragma unroll 8
+        for (int r = 0; r < s.C; ++r) {
+            j.v += *remote(&s.lo[at], r);
+            if (!count) j.v += (u64)*remote(&s.hi[at], r) << 32;
+        }
+    }
+    u64 mine;
+    j.before = block_before(s, j.v, &mine);
+    if (threadIdx.x == 0) s.publish(&s.part[s.rank], mine);
+    cluster_sync();
+    j.total = 0;
+    for (int r = 0; r < s.C; ++r) {
+        if (r < s.rank) j.before += s.part[r];
+        j.total += s.part[r];
+    }
+    return j;
+}
+
+// The bin in which base + the running sum first reaches target (1 <= target - base <= total), in s.bin and s.before of every
+// CTA; clears the list of the gather that follows.
+__device__ __forceinline__ void find(Row& s, const Joined& j, u64 target, u64 base)
+{
+    const u64 b = base + j.before, e = b + j.v;
+    if (b < target && e >= target) {
+        s.publish(&s.bin, s.rank * (s.bins / s.C) + (int)threadIdx.x);
+        s.publish(&s.before, b);
+    }
+    if (s.rank == 0 && threadIdx.x == 0) {
+        s.n_cand = 0;
+        s.kmin = s.imin = UINT_MAX;
+        s.kmax = s.imax = 0u;
+    }
+    cluster_sync();
+}
+
+// f(key, id, mass or 1) for this CTA's ids that in(x, key, id) takes, that the top-k cut keeps and that have a mass.
+template <typename In, typename F> __device__ __forceinline__ void each(const Row& s, bool count, const In& in, const F& f)
+{
+    const float* xs = s.xs;
+    const int n = s.n;
+    for (int i = threadIdx.x; i < n; i += SR_THREADS) {
+        const float x = xs[i];
+        if (!valid(x)) continue;
+        const uint32_t key = order_key(x), id = (uint32_t)(s.id0 + i);
+        if (!in(x, key, id) || !s.kept(key, id)) continue;
+        const u64 m = count ? 1ull : s.mass(s.prob(x));
+        if (m) f(key, id, m);
+    }
+}
+
+// Those ids to CTA 0's list (up to SR_CAP of them; s.n_cand there counts all).
+template <typename In> __device__ __forceinline__ void gather(Row& s, bool count, const In& in)
+{
+    Row* lead = remote(&s, 0);
+    each(s, count, in, [&](uint32_t key, uint32_t id, u64 m) {
+        // one add for the lanes that are here together
+        const uint32_t here = __activemask(), lane = threadIdx.x & 31;
+        int at = 0;
+        if (lane == __ffs(here) - 1) at = atomicAdd(&lead->n_cand, __popc(here));
+        at = __shfl_sync(here, at, __ffs(here) - 1) + __popc(here & ((1u << lane) - 1u));
+        if (at < SR_CAP) {
+            lead->ckey[at] = key;
+            lead->cid[at] = id;
+            lead->cval[at] = m;
+        }
+    });
+    cluster_sync();
+}
+
+// The item at which the running sum (of ones, or of masses) reaches target; the level-0 histogram is joined in j.
+__device__ __noinline__ Item select(Row& s, const Joined j0, u64 target, bool count)
+{
+    find(s, j0, target, 0);
+    const int bin = s.bin;
+    u64 before = s.before;
+    bool deep = false;                      // past level 0: the ids with keys [klo, khi] and ids [ilo, ihi]
+    uint32_t klo = 0u, khi = UINT_MAX, ilo = 0u, ihi = UINT_MAX;
+    Row* lead = remote(&s, 0);
+    auto in = [&](float x, uint32_t key, uint32_t id) {
+        return deep ? key >= klo && key <= khi && id >= ilo && id <= ihi : s.bin0(x) == bin;
+    };
+    // (a cut by keys leaves 2^-9 of their range at most, one by ids of theirs: at most nine rounds)
+#pragma unroll 1
+    for (int round = 0; round < 16; ++round) {
+        gather(s, count, in);
+        const int nc = lead->n_cand;
+        if (nc <= SR_CAP) {
+            if (s.rank == 0 && (int)threadIdx.x < nc) {
+                const uint32_t key = s.ckey[threadIdx.x], id = s.cid[threadIdx.x];
+                u64 c = before;
+                for (int q = 0; q < nc; ++q)
+                    if (s.ckey[q] > key || (s.ckey[q] == key && s.cid[q] <= id)) c += s.cval[q];
+                if (c >= target && c - s.cval[threadIdx.x] < target) s.publish(&s.item, Item{key, id, c});
+            }
+            cluster_sync();
+            return s.item;
+        }
+        // a crowded range: cut it by the bits of its keys, or, all keys equal, by ids
+        uint32_t k0 = UINT_MAX, k1 = 0u, d0 = UINT_MAX, d1 = 0u;
+        each(s, count, in, [&](uint32_t key, uint32_t id, u64) {
+            k0 = min(k0, key);
+            k1 = max(k1, key);
+            d0 = min(d0, id);
+            d1 = max(d1, id);
+        });
+        k0 = __reduce_min_sync(0xffffffffu, k0);
+        k1 = __reduce_max_sync(0xffffffffu, k1);
+        d0 = __reduce_min_sync(0xffffffffu, d0);
+        d1 = __reduce_max_sync(0xffffffffu, d1);
+        if ((threadIdx.x & 31) == 0 && k0 <= k1) {
+            atomicMin(&lead->kmin, k0);
+            atomicMax(&lead->kmax, k1);
+            atomicMin(&lead->imin, d0);
+            atomicMax(&lead->imax, d1);
+        }
+        cluster_sync();
+        klo = lead->kmin; khi = lead->kmax; ilo = lead->imin; ihi = lead->imax;
+        deep = true;
+        const bool by_id = klo == khi;
+        const uint32_t width = by_id ? ihi - ilo : khi - klo;
+        const int shift = max(0, 32 - __clz(width) - (31 - __clz(s.bins)));
+        clear_hist(s);
+        each(s, count, in, [&](uint32_t key, uint32_t id, u64 m) { s.add((by_id ? id - ilo : khi - key) >> shift, m, count); });
+        const Joined j = join(s, count);
+        find(s, j, target, before);
+        before = s.before;
+        const uint32_t from = (uint32_t)s.bin << shift, upto = from + ((1u << shift) - 1u);
+        if (by_id) {
+            const uint32_t i0 = ilo;
+            ilo = i0 + from;
+            ihi = min(ihi, i0 + upto);
+        } else {
+            const uint32_t top = khi;
+            khi = top - from;
+            klo = top - klo > upto ? top - upto : klo;
+        }
+    }
+    return s.item;
+}
+
+__device__ __forceinline__ u64 share_of(double part, u64 sum)      // the sum that the running sum has to reach: 1 .. sum
+{
+    const double t = ceil(part * (double)sum);
+    return min(sum, t > 1.0 ? (u64)t : 1ull);
+}
+
+// CTA 0's list of n ids (one a thread, 0 < n <= SR_CAP), among them the first k of the order: its top-k, top-p, min-p and pick.
+__device__ __noinline__ void finish_list(Row& s, int n, int k, const wl_sample_opts& o, int32_t* out)
+{
+    const int tid = threadIdx.x;
+    uint32_t key = 0, id = 0;
+    int rank = 0;
+    if (tid < n) {
+        key = s.ckey[tid];
+        id = s.cid[tid];
+        for (int q = 0; q < n; ++q) rank += s.ckey[q] > key || (s.ckey[q] == key && s.cid[q] < id);
+    }
+    __syncthreads();
+    if (tid < n) {
+        s.ckey[rank] = key;
+        s.cid[rank] = id;
+    }
+    __syncthreads();
+    k = min(k, n);
+    double p = 0.0;
+    u64 m = 0, all;
+    if (tid < k) {
+        key = s.ckey[tid];
+        p = s.prob(__uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key));
+        m = s.mass(p);
+    }
+    const u64 cum = block_before(s, m, &all) + m;
+    u64 sum = all;
+    if (o.top_p < 1.0) {
+        const u64 t = share_of(o.top_p, sum);
+        if (cum >= t && cum - m < t) s.before = cum;        // (one thread: m > 0)
+        __syncthreads();
+        sum = s.before;
+    }
+    if (o.min_p > 0.0) {
+        const int above = __syncthreads_count(tid < k && p >= o.min_p);
+        if (tid == above - 1) s.red[0] = cum;
+        __syncthreads();
+        sum = max(1ull, min(sum, above ? s.red[0] : 0ull));
+    }
+    const u64 t = share_of(o.draw, sum);
+    if (cum >= t && cum - m < t) *out = (int32_t)s.cid[tid];
+}
+
+__global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logits, int64_t ld, int V, int frac,
+                                                               const wl_sample_opts* opts, int32_t* ids, int slice, int in_smem)
 {
     extern __shared__ __align__(16) uint8_t smem[];
-    RowShared& sh = *reinterpret_cast<RowShared*>(smem);
+    Row& s = *reinterpret_cast<Row*>(smem);
     pdl_trigger();
     pdl_wait();
-    const int row = blockIdx.y, C = gridDim.x, rank = (int)cluster_rank();
+    const int row = blockIdx.y, C = gridDim.x, rank = (int)cluster_rank(), tid = threadIdx.x;
     const float* x = logits + (int64_t)row * ld;
     const wl_sample_opts o = opts[row];
-    Sampler s{sh};
-    s.C = C;
-    s.rank = rank;
-    s.id0 = rank * slice;
-    s.n = max(0, min(slice, V - s.id0));
-    s.xs = x + s.id0;
-    const int tid = threadIdx.x;
-    if (tid < 64) sh.exp2_table[tid] = exp2(tid * 0.015625);
+    const int id0 = rank * slice, n = max(0, min(slice, V - id0));
+    const bool greedy = !(o.temperature > 0.0);
+    if (tid < 64) s.exp2_table[tid] = exp2(tid * 0.015625);
     // the slice, and its largest value (lowest id) and smallest value above -inf
+    float* keep = in_smem ? reinterpret_cast<float*>(smem + (sizeof(Row) + 15) / 16 * 16) : nullptr;
     u64 best = 0;
     uint32_t low = UINT_MAX;
     {
-        float* keep = in_smem ? reinterpret_cast<float*>(smem + (sizeof(RowShared) + 15) / 16 * 16) : nullptr;
+        const float* xs = x + id0;
         auto take = [&](int i, float v) {
-            if (!(v > -INFINITY)) return;
+            if (!valid(v)) return;
             const uint32_t key = order_key(v);
-            const u64 b = (u64)key << 32 | (uint32_t)~(uint32_t)(s.id0 + i);
+            const u64 b = (u64)key << 32 | (uint32_t)~(uint32_t)(id0 + i);
             best = b > best ? b : best;
             low = min(low, key);
         };
         int done = 0;
-        if (((uintptr_t)s.xs & 15) == 0) {
-            const int n4 = s.n / 4;
+        if (((uintptr_t)xs & 15) == 0) {
+            const int n4 = n / 4;
+#pragma unroll 4
             for (int i = tid; i < n4; i += SR_THREADS) {
-                const float4 v = reinterpret_cast<const float4*>(s.xs)[i];
+                const float4 v = reinterpret_cast<const float4*>(xs)[i];
                 if (keep) reinterpret_cast<float4*>(keep)[i] = v;
                 take(4 * i, v.x);
                 take(4 * i + 1, v.y);
@@ -384,12 +405,21 @@ __global__ void __launch_bounds__(SR_THREADS, 1) k_sample_rows(const float* logi
             }
             done = 4 * n4;
         }
-        for (int i = done + tid; i < s.n; i += SR_THREADS) {
-            const float v = s.xs[i];
+        for (int i = done + tid; i < n; i += SR_THREADS) {
+            const float v = xs[i];
             if (keep) keep[i] = v;
             take(i, v);
         }
-        if (keep) s.xs = keep;
+        if (tid == 0) {
+            s.xs = keep ? keep : xs;
+            s.n = n;
+            s.id0 = id0;
+            s.C = C;
+            s.rank = rank;
+            s.bins = min(SR_BINS, 512 * C);
+            s.frac = frac;
+            s.has_k = 0;
+        }
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) {
@@ -398,77 +428,94 @@ __global__ void __launch_bounds__(SR_THREADS, 1) k_sample_rows(const float* logi
         low = min(low, __shfl_xor_sync(0xffffffffu, low, d));
     }
     if ((tid & 31) == 0) {
-        sh.red[tid >> 5] = best;
-        sh.scan[tid >> 5] = low;
+        s.red[tid >> 5] = best;
+        s.scan[tid >> 5] = low;
     }
-    __syncthreads();
-    for (int w = 0; w < SR_WARPS; ++w) {
-        best = sh.red[w] > best ? sh.red[w] : best;
-        low = min(low, (uint32_t)sh.scan[w]);
-    }
-    cluster_sync();                         // every CTA of the cluster has started: its memory may be written
+    cluster_sync();                         // (also: every CTA of the cluster has started, its memory may be written)
     if (tid == 0) {
-        s.publish(&sh.best[rank], best);
-        s.publish(&sh.low[rank], (u64)low);
+        for (int w = 0; w < SR_WARPS; ++w) {
+            best = s.red[w] > best ? s.red[w] : best;
+            low = min(low, (uint32_t)s.scan[w]);
+        }
+        s.publish(&s.best[rank], best);
+        s.publish(&s.low[rank], low);
     }
     cluster_sync();
     for (int r = 0; r < C; ++r) {
-        best = sh.best[r] > best ? sh.best[r] : best;
-        low = min(low, (uint32_t)sh.low[r]);
+        best = s.best[r] > best ? s.best[r] : best;
+        low = min(low, s.low[r]);
     }
     const bool lead = rank == 0 && tid == 0;
     // nothing above -inf, or the greedy id. All CTAs take the same branch; nothing of another CTA is read after it.
-    const bool greedy = !(o.temperature > 0.0);
     if (best == 0 || greedy || !(o.draw >= 0.0 && o.draw < 1.0)) {
         if (lead) ids[row] = !greedy && !(o.draw >= 0.0 && o.draw < 1.0) ? -1 : best == 0 || (greedy && isnan(x[0])) ? 0 : (int32_t)~(uint32_t)best;
         return;
     }
-    const uint32_t kmax = (uint32_t)(best >> 32);
+    const bool with_k = o.top_k > 0 && o.top_k < V, sorted = with_k || o.top_p < 1.0 || o.min_p > 0.0;
     auto value = [](uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); };
-    s.xmax = value(kmax);
-    s.inv_t = 1.4426950408889634 / o.temperature;
-    s.frac = frac;
-    s.unit = ldexp(1.0, frac);
-    s.has_k = false;
+    const float xmax = value((uint32_t)(best >> 32));
     // the histogram's range: down to the smallest value, in halves so that no difference overflows
-    const float half_range = s.xmax * 0.5f - value(low) * 0.5f;
-    const bool with_k = o.top_k > 0 && o.top_k < V;
-    Sampler::Joined j;
-    if (with_k) {
-        s.inv_w = half_range > 0.f && half_range <= FLT_MAX ? (float)SR_BINS / half_range : 0.f;
-        s.clear_hist();
-        for (int i = tid; i < s.n; i += SR_THREADS)
-            if (s.valid(s.xs[i])) s.add(s.bin0(s.xs[i]), 0, true);
-        s.join(j, true);
-        if (j.total > (u64)o.top_k) {
-            const Item k = s.select(j, (u64)o.top_k, true);
-            s.has_k = true;
-            s.k_key = k.key;
-            s.k_id = k.id;
-        }
+    const float half_range = xmax * 0.5f - value(low) * 0.5f;
+    auto width = [&](float range) { return range > 0.f && range <= FLT_MAX ? (float)s.bins / range : 0.f; };
+    if (tid == 0) {
+        s.xmax = xmax;
+        s.inv_t = 1.4426950408889634 / o.temperature;
+        s.unit = ldexp(1.0, frac);
+        s.inv_w = width(half_range);
     }
-    if (!with_k && !(o.top_p < 1.0) && !(o.min_p > 0.0)) {
+    Joined j;
+    if (with_k) {
+        clear_hist(s);
+        for (int i = tid; i < n; i += SR_THREADS) {
+            const float v = s.xs[i];
+            if (valid(v)) s.add(s.bin0(v), 0, true);
+        }
+        j = join(s, true);
+        const int k = (int)min(j.total, (u64)o.top_k);
+        find(s, j, (u64)k, 0);
+        // few enough ids down to the k-th's bin: CTA 0 ends the row with them
+        const int bin = s.bin;
+        gather(s, true, [&](float v, uint32_t, uint32_t) { return s.bin0(v) <= bin; });
+        const int nc = remote(&s, 0)->n_cand;
+        cluster_sync();                     // (CTA 0's count has been read)
+        if (nc <= SR_CAP) {
+            if (rank == 0) finish_list(s, nc, k, o, ids + row);
+            return;
+        }
+        if (j.total > (u64)o.top_k) {
+            const Item it = select(s, j, (u64)k, true);
+            if (tid == 0) {
+                s.k_key = it.key;
+                s.k_id = it.id;
+                s.has_k = 1;
+            }
+        }
+        __syncthreads();
+    } else if (!sorted) {
         // id order: thread t has ids t per .. (an odd stride, so that a warp's reads fall in different banks)
-        const int per = ((s.n + SR_THREADS - 1) / SR_THREADS) | 1;
-        const int i0 = min(s.n, tid * per), i1 = min(s.n, i0 + per);
+        __syncthreads();
+        const int per = ((n + SR_THREADS - 1) / SR_THREADS) | 1;
+        const int i0 = min(n, tid * per), i1 = min(n, i0 + per);
         u64 sum = 0, mine;
-        for (int i = i0; i < i1; ++i)
-            if (s.valid(s.xs[i])) sum += s.mass(s.prob(s.xs[i]));
-        u64 before = s.block_before(sum, &mine);
-        if (tid == 0) s.publish(&sh.part[rank], mine);
+        for (int i = i0; i < i1; ++i) {
+            const float v = s.xs[i];
+            if (valid(v)) sum += s.mass(s.prob(v));
+        }
+        u64 before = block_before(s, sum, &mine);
+        if (tid == 0) s.publish(&s.part[rank], mine);
         cluster_sync();
         u64 total = 0;
         for (int r = 0; r < C; ++r) {
-            if (r < rank) before += sh.part[r];
-            total += sh.part[r];
+            if (r < rank) before += s.part[r];
+            total += s.part[r];
         }
-        const double want = ceil(o.draw * (double)total);
-        const u64 target = min(total, max(1ull, (u64)want));
+        const u64 target = share_of(o.draw, total);
         if (before < target && before + sum >= target) {
             for (int i = i0; i < i1; ++i) {
-                if (s.valid(s.xs[i])) before += s.mass(s.prob(s.xs[i]));
+                const float v = s.xs[i];
+                if (valid(v)) before += s.mass(s.prob(v));
                 if (before >= target) {
-                    ids[row] = s.id0 + i;
+                    ids[row] = id0 + i;
                     break;
                 }
             }
@@ -476,14 +523,12 @@ __global__ void __launch_bounds__(SR_THREADS, 1) k_sample_rows(const float* logi
         return;
     }
     // masses: below 2^-(F+1) of the largest nothing is left, so the histogram's range ends there
-    const float reach = (float)fmin((frac + 2) * 0.6931471805599453 * o.temperature * 0.5, (double)FLT_MAX);
-    const float range = fminf(half_range, reach);
-    s.inv_w = range > 0.f && range <= FLT_MAX ? (float)SR_BINS / range : 0.f;
-    s.clear_hist();
+    if (tid == 0) s.inv_w = width(fminf(half_range, (float)fmin((frac + 2) * 0.6931471805599453 * o.temperature * 0.5, (double)FLT_MAX)));
+    clear_hist(s);
     u64 over = 0;                           // the sum of the kept ids with p >= min_p
-    for (int i = tid; i < s.n; i += SR_THREADS) {
+    for (int i = tid; i < n; i += SR_THREADS) {
         const float v = s.xs[i];
-        if (!s.valid(v) || !s.kept(order_key(v), (uint32_t)(s.id0 + i))) continue;
+        if (!valid(v) || !s.kept(order_key(v), (uint32_t)(id0 + i))) continue;
         const double p = s.prob(v);
         const u64 m = s.mass(p);
         if (!m) continue;
@@ -491,22 +536,19 @@ __global__ void __launch_bounds__(SR_THREADS, 1) k_sample_rows(const float* logi
         if (p >= o.min_p) over += m;
     }
     if (o.min_p > 0.0) {
-        over = s.block_sum(over);
-        if (tid == 0) s.publish(&sh.min_part[rank], over);
+        u64 mine;
+        block_before(s, over, &mine);
+        if (tid == 0) s.publish(&s.min_part[rank], mine);
     }
-    s.join(j, false);
+    j = join(s, false);
     u64 sum = j.total;
-    if (o.top_p < 1.0) {
-        const double want = ceil(o.top_p * (double)sum);
-        sum = s.select(j, min(sum, want > 1.0 ? (u64)want : 1ull), false).cum;
-    }
+    if (o.top_p < 1.0) sum = select(s, j, share_of(o.top_p, sum), false).cum;
     if (o.min_p > 0.0) {
         u64 all = 0;
-        for (int r = 0; r < C; ++r) all += sh.min_part[r];
+        for (int r = 0; r < C; ++r) all += s.min_part[r];
         sum = max(1ull, min(sum, all));
     }
-    const double want = ceil(o.draw * (double)sum);
-    const Item it = s.select(j, min(sum, max(1ull, (u64)want)), false);
+    const Item it = select(s, j, share_of(o.draw, sum), false);
     if (lead) ids[row] = (int32_t)it.id;
 }
 
@@ -526,7 +568,7 @@ void sample_rows(const float* logits, int64_t ld, int V, int rows, const wl_samp
     const int C = cluster_for(V);
     const int slice = ((V + C - 1) / C + 3) / 4 * 4;
     const bool in_smem = slice <= SR_SLICE_MAX;
-    const size_t smem = (sizeof(RowShared) + 15) / 16 * 16 + (in_smem ? (size_t)slice * 4 : 0);
+    const size_t smem = (sizeof(Row) + 15) / 16 * 16 + (in_smem ? (size_t)slice * 4 : 0);
     int bits = 0;
     while ((1ll << bits) < V) ++bits;
     WL_CUDA(cudaFuncSetAttribute(k_sample_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
