@@ -64,9 +64,9 @@ def sample(wl, x, opts, ld=None, stream=None):
 
 def check(wl, x, opts, ld=None):
     got = sample(wl, x, opts, ld)
-    # rounding p to multiples of 2^-F moves a sum by at most V / 2 of them (F = 62 - log2 V); the reference's running sum
-    # by V of its own half steps
-    tol = 2 * x.shape[1] * (2.0 ** -(62 - int(np.ceil(np.log2(max(2, x.shape[1]))))) + 2.0 ** -53)
+    # rounding p to multiples of 2^-F moves a sum by at most V / 2 of them (F = 62 - log2 V, 51 at most); the reference's
+    # running sum by V of its own half steps
+    tol = 2 * x.shape[1] * (2.0 ** -min(51, 62 - int(np.ceil(np.log2(max(2, x.shape[1]))))) + 2.0 ** -53)
     near = 0
     for r in range(x.shape[0]):
         want, margin = reference(x[r], opts[r])

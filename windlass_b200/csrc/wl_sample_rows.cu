@@ -15,7 +15,7 @@
 // bin that the cut falls in, its few ids are gathered to one CTA and ranked by counting, each against each. A bin of more
 // than SR_CAP ids (ties, or a row whose values are far from evenly spread) is cut again by the bits of the logits and then
 // by ids. The probabilities are summed as 64-bit integers, multiples of 2^-F with F = 62 - ceil(log2 V) (44 for
-// 151936 ids), so that every sum is exact and does not depend on the order of the atomics; rounding them moves a
+// 151936 ids), 51 at most, so that every sum is exact and does not depend on the order of the atomics; rounding them moves a
 // boundary between two ids by at most V * 2^-(F+1), 4e-9 of the sum for the largest vocabulary, and by the square root of that many steps as a rule.
 #include <algorithm>
 #include <cfloat>
@@ -48,6 +48,8 @@ __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // The address of `p` (shared memory of this CTA) in CTA `rank` of the cluster.
 template <typename T> __device__ __forceinline__ T* remote(T* p, int rank)
 {
@@ -83,8 +85,8 @@ struct Row {
     // published by every CTA of the cluster into each
     u64 part[SR_MAX_CLUSTER], best[SR_MAX_CLUSTER], min_part[SR_MAX_CLUSTER];
     uint32_t low[SR_MAX_CLUSTER];
-    int bin;                                // the crossing bin and the sum before it
-    u64 before;
+    int bin, bin_hi;                        // the crossing bin, the sum before it and in it
+    u64 before, bin_sum;
     Item item;
     // in CTA 0: the gathered ids, and the range of keys and ids of a crowded bin
     int n_cand;
@@ -97,7 +99,11 @@ struct Row {
     {
         return (int)fminf((xmax * 0.5f - x * 0.5f) * inv_w, (float)(bins - 1));     // (NaN, of infinities: the last bin)
     }
-    __device__ __forceinline__ u64 mass(double p) const { return (u64)(p * unit + 0.5); }
+    // p 2^F, rounded (below 2^52: adding 2^52 leaves the integer in the sum's low bits)
+    __device__ __forceinline__ u64 mass(double p) const
+    {
+        return (u64)__double_as_longlong(fma(p, unit, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+    }
     // exp((x - xmax) / T) for a valid x: 2^y by table and polynomial (Tang's table-driven scheme: y = n + j/64 + r,
     // 2^(j/64) from the table, e^(r ln 2) to the fifth power, its remainder below 2^-54)
     __device__ __forceinline__ double prob(float x) const
@@ -105,16 +111,17 @@ struct Row {
         if (x == xmax) return 1.0;
         const double y = (double)__fsub_rn(x, xmax) * inv_t;
         if (!(y > -(double)(frac + 2))) return 0.0;
-        const double q = rint(y * 64.0);
-        const int i = (int)q;
-        const double t = (y - q * 0.015625) * 0.6931471805599453;
+        // y 64 to the nearest integer: the low bits of a sum with 1.5 2^52
+        const double z = fma(y, 64.0, 6755399441055744.0);
+        const int i = __double2loint(z);
+        const double t = fma(z - 6755399441055744.0, -0.015625, y) * 0.6931471805599453;
         double e = fma(t, 1.0 / 120, 1.0 / 24);
         e = fma(t, e, 1.0 / 6);
         e = fma(t, e, 0.5);
         e = fma(t, e, 1.0);
         e = fma(t, e, 1.0);
         const double m = exp2_table[i & 63] * e;
-        return __longlong_as_double(__double_as_longlong(m) + ((long long)(i >> 6) << 52));
+        return __hiloint2double(__double2hiint(m) + ((i >> 6) << 20), __double2loint(m));
     }
     __device__ __forceinline__ void add(int b, u64 v, bool count)
     {
@@ -202,6 +209,7 @@ __device__ __forceinline__ void find(Row& s, const Joined& j, u64 target, u64 ba
     if (b < target && e >= target) {
         s.publish(&s.bin, s.rank * (s.bins / s.C) + (int)threadIdx.x);
         s.publish(&s.before, b);
+        s.publish(&s.bin_sum, j.v);
     }
     if (s.rank == 0 && threadIdx.x == 0) {
         s.n_cand = 0;
@@ -211,26 +219,44 @@ __device__ __forceinline__ void find(Row& s, const Joined& j, u64 target, u64 ba
     cluster_sync();
 }
 
-// f(key, id, mass or 1) for this CTA's ids that in(x, key, id) takes, that the top-k cut keeps and that have a mass.
-template <typename In, typename F> __device__ __forceinline__ void each(const Row& s, bool count, const In& in, const F& f)
+// f(i, x) for this CTA's logits (xs is 16-byte aligned where it is shared memory; a slice is a multiple of 4 long but the last).
+template <typename F> __device__ __forceinline__ void each_logit(const Row& s, const F& f)
 {
     const float* xs = s.xs;
     const int n = s.n;
-    for (int i = threadIdx.x; i < n; i += SR_THREADS) {
-        const float x = xs[i];
-        if (!valid(x)) continue;
+    int done = 0;
+    if (((uintptr_t)xs & 15) == 0) {
+        for (int i = threadIdx.x; i < n / 4; i += SR_THREADS) {
+            const float4 v = reinterpret_cast<const float4*>(xs)[i];
+            f(4 * i, v.x);
+            f(4 * i + 1, v.y);
+            f(4 * i + 2, v.z);
+            f(4 * i + 3, v.w);
+        }
+        done = n & ~3;
+    }
+    for (int i = done + threadIdx.x; i < n; i += SR_THREADS) f(i, xs[i]);
+}
+
+// f(key, id, mass or 1) for this CTA's ids whose logit pre takes, that in(key, id) takes, that the top-k cut keeps and that
+// have a mass.
+template <typename Pre, typename In, typename F>
+__device__ __forceinline__ void each(const Row& s, bool count, const Pre& pre, const In& in, const F& f)
+{
+    each_logit(s, [&](int i, float x) {
+        if (!pre(x) || !valid(x)) return;
         const uint32_t key = order_key(x), id = (uint32_t)(s.id0 + i);
-        if (!in(x, key, id) || !s.kept(key, id)) continue;
+        if (!in(key, id) || !s.kept(key, id)) return;
         const u64 m = count ? 1ull : s.mass(s.prob(x));
         if (m) f(key, id, m);
-    }
+    });
 }
 
 // Those ids to CTA 0's list (up to SR_CAP of them; s.n_cand there counts all).
-template <typename In> __device__ __forceinline__ void gather(Row& s, bool count, const In& in)
+template <typename Pre, typename In> __device__ __forceinline__ void gather(Row& s, bool count, const Pre& pre, const In& in)
 {
     Row* lead = remote(&s, 0);
-    each(s, count, in, [&](uint32_t key, uint32_t id, u64 m) {
+    each(s, count, pre, in, [&](uint32_t key, uint32_t id, u64 m) {
         // one add for the lanes that are here together
         const uint32_t here = __activemask(), lane = threadIdx.x & 31;
         int at = 0;
@@ -254,13 +280,12 @@ __device__ __noinline__ Item select(Row& s, const Joined j0, u64 target, bool co
     bool deep = false;                      // past level 0: the ids with keys [klo, khi] and ids [ilo, ihi]
     uint32_t klo = 0u, khi = UINT_MAX, ilo = 0u, ihi = UINT_MAX;
     Row* lead = remote(&s, 0);
-    auto in = [&](float x, uint32_t key, uint32_t id) {
-        return deep ? key >= klo && key <= khi && id >= ilo && id <= ihi : s.bin0(x) == bin;
-    };
+    auto pre = [&](float x) { return deep || s.bin0(x) == bin; };
+    auto in = [&](uint32_t key, uint32_t id) { return key >= klo && key <= khi && id >= ilo && id <= ihi; };
     // (a cut by keys leaves 2^-9 of their range at most, one by ids of theirs: at most nine rounds)
 #pragma unroll 1
     for (int round = 0; round < 16; ++round) {
-        gather(s, count, in);
+        gather(s, count, pre, in);
         const int nc = lead->n_cand;
         if (nc <= SR_CAP) {
             if (s.rank == 0 && (int)threadIdx.x < nc) {
@@ -275,7 +300,7 @@ __device__ __noinline__ Item select(Row& s, const Joined j0, u64 target, bool co
         }
         // a crowded range: cut it by the bits of its keys, or, all keys equal, by ids
         uint32_t k0 = UINT_MAX, k1 = 0u, d0 = UINT_MAX, d1 = 0u;
-        each(s, count, in, [&](uint32_t key, uint32_t id, u64) {
+        each(s, count, pre, in, [&](uint32_t key, uint32_t id, u64) {
             k0 = min(k0, key);
             k1 = max(k1, key);
             d0 = min(d0, id);
@@ -298,7 +323,7 @@ __device__ __noinline__ Item select(Row& s, const Joined j0, u64 target, bool co
         const uint32_t width = by_id ? ihi - ilo : khi - klo;
         const int shift = max(0, 32 - __clz(width) - (31 - __clz(s.bins)));
         clear_hist(s);
-        each(s, count, in, [&](uint32_t key, uint32_t id, u64 m) { s.add((by_id ? id - ilo : khi - key) >> shift, m, count); });
+        each(s, count, pre, in, [&](uint32_t key, uint32_t id, u64 m) { s.add((by_id ? id - ilo : khi - key) >> shift, m, count); });
         const Joined j = join(s, count);
         find(s, j, target, before);
         before = s.before;
@@ -365,6 +390,42 @@ __device__ __noinline__ void finish_list(Row& s, int n, int k, const wl_sample_o
     if (cum >= t && cum - m < t) *out = (int32_t)s.cid[tid];
 }
 
+// CTA 0's list of n ids with their masses: those of the bin that the nucleus ends in (bin0 == nb, the sum before it nbefore;
+// nb < 0: no nucleus, the kept sum is `sum`), and of the bins p_lo .. p_hi that the pick falls in whichever id that is
+// (pbefore: the sum before p_lo). over: the sum of the ids with p >= min_p.
+__device__ __noinline__ void finish_bins(Row& s, int n, int nb, u64 nbefore, u64 ntarget, int p_lo, int p_hi, u64 pbefore, u64 sum, u64 over,
+                                         double draw, int32_t* out)
+{
+    const int tid = threadIdx.x;
+    uint32_t key = 0, id = 0;
+    int bin = -1;
+    u64 m = 0, cn = nbefore, cp = pbefore;
+    auto bin_of = [&](uint32_t k) { return s.bin0(__uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k)); };
+    if (tid < n) {
+        key = s.ckey[tid];
+        id = s.cid[tid];
+        m = s.cval[tid];
+        bin = bin_of(key);
+        for (int q = 0; q < n; ++q) {
+            const uint32_t k = s.ckey[q];
+            if (k > key || (k == key && s.cid[q] <= id)) {
+                const int b = bin_of(k);
+                const u64 v = s.cval[q];
+                if (b == nb) cn += v;
+                if (b >= p_lo && b <= p_hi) cp += v;
+            }
+        }
+    }
+    if (nb >= 0) {
+        if (bin == nb && cn >= ntarget && cn - m < ntarget) s.before = cn;
+        __syncthreads();
+        sum = s.before;
+    }
+    sum = max(1ull, min(sum, over));
+    const u64 t = share_of(draw, sum);
+    if (bin >= p_lo && bin <= p_hi && cp >= t && cp - m < t) *out = (int32_t)id;
+}
+
 __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logits, int64_t ld, int V, int frac,
                                                                const wl_sample_opts* opts, int32_t* ids, int slice, int in_smem)
 {
@@ -377,6 +438,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
     const wl_sample_opts o = opts[row];
     const int id0 = rank * slice, n = max(0, min(slice, V - id0));
     const bool greedy = !(o.temperature > 0.0);
+    cluster_arrive();                       // (waited for before another CTA's memory is written)
     if (tid < 64) s.exp2_table[tid] = exp2(tid * 0.015625);
     // the slice, and its largest value (lowest id) and smallest value above -inf
     float* keep = in_smem ? reinterpret_cast<float*>(smem + (sizeof(Row) + 15) / 16 * 16) : nullptr;
@@ -431,7 +493,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
         s.red[tid >> 5] = best;
         s.scan[tid >> 5] = low;
     }
-    cluster_sync();                         // (also: every CTA of the cluster has started, its memory may be written)
+    __syncthreads();
+    cluster_wait();
     if (tid == 0) {
         for (int w = 0; w < SR_WARPS; ++w) {
             best = s.red[w] > best ? s.red[w] : best;
@@ -466,16 +529,15 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
     Joined j;
     if (with_k) {
         clear_hist(s);
-        for (int i = tid; i < n; i += SR_THREADS) {
-            const float v = s.xs[i];
+        each_logit(s, [&](int, float v) {
             if (valid(v)) s.add(s.bin0(v), 0, true);
-        }
+        });
         j = join(s, true);
         const int k = (int)min(j.total, (u64)o.top_k);
         find(s, j, (u64)k, 0);
         // few enough ids down to the k-th's bin: CTA 0 ends the row with them
         const int bin = s.bin;
-        gather(s, true, [&](float v, uint32_t, uint32_t) { return s.bin0(v) <= bin; });
+        gather(s, true, [&](float v) { return s.bin0(v) <= bin; }, [](uint32_t, uint32_t) { return true; });
         const int nc = remote(&s, 0)->n_cand;
         cluster_sync();                     // (CTA 0's count has been read)
         if (nc <= SR_CAP) {
@@ -526,28 +588,56 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
     if (tid == 0) s.inv_w = width(fminf(half_range, (float)fmin((frac + 2) * 0.6931471805599453 * o.temperature * 0.5, (double)FLT_MAX)));
     clear_hist(s);
     u64 over = 0;                           // the sum of the kept ids with p >= min_p
-    for (int i = tid; i < n; i += SR_THREADS) {
-        const float v = s.xs[i];
-        if (!valid(v) || !s.kept(order_key(v), (uint32_t)(id0 + i))) continue;
+    each_logit(s, [&](int i, float v) {
+        if (!valid(v) || !s.kept(order_key(v), (uint32_t)(id0 + i))) return;
         const double p = s.prob(v);
         const u64 m = s.mass(p);
-        if (!m) continue;
+        if (!m) return;
         s.add(s.bin0(v), m, false);
         if (p >= o.min_p) over += m;
-    }
+    });
     if (o.min_p > 0.0) {
         u64 mine;
         block_before(s, over, &mine);
         if (tid == 0) s.publish(&s.min_part[rank], mine);
     }
     j = join(s, false);
-    u64 sum = j.total;
-    if (o.top_p < 1.0) sum = select(s, j, share_of(o.top_p, sum), false).cum;
+    over = ~0ull;
     if (o.min_p > 0.0) {
-        u64 all = 0;
-        for (int r = 0; r < C; ++r) all += s.min_part[r];
-        sum = max(1ull, min(sum, all));
+        over = 0;
+        for (int r = 0; r < C; ++r) over += s.min_part[r];
     }
+    // the nucleus's last bin, then the bins that the pick falls in whatever id of that bin ends the nucleus
+    int nb = -1;
+    u64 nbefore = 0, ntarget = 0, s_lo = j.total, s_hi = j.total;
+    if (o.top_p < 1.0) {
+        ntarget = share_of(o.top_p, j.total);
+        find(s, j, ntarget, 0);
+        nb = s.bin;
+        nbefore = s.before;
+        s_lo = nbefore + 1;
+        s_hi = nbefore + s.bin_sum;
+    }
+    const u64 t_lo = share_of(o.draw, max(1ull, min(s_lo, over))), t_hi = share_of(o.draw, max(1ull, min(s_hi, over)));
+    cluster_sync();                         // (s.bin and s.before have been read)
+    if (j.before < t_hi && j.before + j.v >= t_hi) s.publish(&s.bin_hi, rank * (s.bins / C) + tid);
+    find(s, j, t_lo, 0);
+    const int p_lo = s.bin, p_hi = s.bin_hi;
+    const u64 pbefore = s.before;
+    gather(s, false, [&](float v) {
+        const int b = s.bin0(v);
+        return b == nb || (b >= p_lo && b <= p_hi);
+    }, [](uint32_t, uint32_t) { return true; });
+    const int nc = remote(&s, 0)->n_cand;
+    cluster_sync();                         // (CTA 0's count has been read)
+    if (nc <= SR_CAP) {
+        if (rank == 0) finish_bins(s, nc, nb, nbefore, ntarget, p_lo, p_hi, pbefore, j.total, over, o.draw, ids + row);
+        return;
+    }
+    // crowded bins: one cut after the other
+    u64 sum = j.total;
+    if (nb >= 0) sum = select(s, j, ntarget, false).cum;
+    sum = max(1ull, min(sum, over));
     const Item it = select(s, j, share_of(o.draw, sum), false);
     if (lead) ids[row] = (int32_t)it.id;
 }
@@ -574,7 +664,7 @@ void sample_rows(const float* logits, int64_t ld, int V, int rows, const wl_samp
     WL_CUDA(cudaFuncSetAttribute(k_sample_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     for (int r0 = 0; r0 < rows; r0 += 65535) {
         launch_cluster(k_sample_rows, dim3(C, std::min(rows - r0, 65535)), dim3(SR_THREADS), smem, s, C, logits + (int64_t)r0 * ld, ld, V,
-                       62 - bits, opts + r0, ids + r0, slice, in_smem ? 1 : 0);
+                       std::min(51, 62 - bits), opts + r0, ids + r0, slice, in_smem ? 1 : 0);
         note_launch();
     }
 }
