@@ -71,33 +71,18 @@ struct Item {               // a selected id: its key, id, and the sum up to and
     u64 cum;
 };
 
-// A row's state in a CTA's shared memory (all of its scalars the same for all threads).
-struct Row {
-    uint32_t lo[SR_BINS], hi[SR_BINS];      // per bin: a count (lo), or a 64-bit sum in two words
-    double exp2_table[64];
-    u64 scan[SR_WARPS], red[SR_WARPS];
-    const float* xs;                        // this CTA's slice
-    int n, id0, C, rank, bins, frac;        // its length and first id; the cluster; bins in use
-    float xmax, inv_w;                      // the histogram: bin = (xmax / 2 - x / 2) * inv_w
+// What a row's loops need of it, in registers while they run.
+struct RowConst {
+    float xmax, inv_w, last_bin;            // the histogram: bin = (xmax / 2 - x / 2) * inv_w
+    int frac;
     double inv_t, unit;                     // log2(e) / temperature, 2^F
     int has_k;                              // a top-k cut: ids up to (k_key, k_id) in the order
     uint32_t k_key, k_id;
-    // published by every CTA of the cluster into each
-    u64 part[SR_MAX_CLUSTER], best[SR_MAX_CLUSTER], min_part[SR_MAX_CLUSTER];
-    uint32_t low[SR_MAX_CLUSTER];
-    int bin, bin_hi;                        // the crossing bin, the sum before it and in it
-    u64 before, bin_sum;
-    Item item;
-    // in CTA 0: the gathered ids, and the range of keys and ids of a crowded bin
-    int n_cand;
-    uint32_t kmin, kmax, imin, imax;
-    uint32_t ckey[SR_CAP], cid[SR_CAP];
-    u64 cval[SR_CAP];
 
     __device__ __forceinline__ bool kept(uint32_t key, uint32_t id) const { return !has_k || key > k_key || (key == k_key && id <= k_id); }
     __device__ __forceinline__ int bin0(float x) const
     {
-        return (int)fminf((xmax * 0.5f - x * 0.5f) * inv_w, (float)(bins - 1));     // (NaN, of infinities: the last bin)
+        return (int)fminf((xmax * 0.5f - x * 0.5f) * inv_w, last_bin);      // (NaN, of infinities: the last bin)
     }
     // p 2^F, rounded (below 2^52: adding 2^52 leaves the integer in the sum's low bits)
     __device__ __forceinline__ u64 mass(double p) const
@@ -106,7 +91,7 @@ struct Row {
     }
     // exp((x - xmax) / T) for a valid x: 2^y by table and polynomial (Tang's table-driven scheme: y = n + j/64 + r,
     // 2^(j/64) from the table, e^(r ln 2) to the fifth power, its remainder below 2^-54)
-    __device__ __forceinline__ double prob(float x) const
+    __device__ __forceinline__ double prob(float x, const double* exp2_table) const
     {
         if (x == xmax) return 1.0;
         const double y = (double)__fsub_rn(x, xmax) * inv_t;
@@ -123,6 +108,32 @@ struct Row {
         const double m = exp2_table[i & 63] * e;
         return __hiloint2double(__double2hiint(m) + ((i >> 6) << 20), __double2loint(m));
     }
+};
+
+// A row's state in a CTA's shared memory (all of its scalars the same for all threads).
+struct Row {
+    uint32_t lo[SR_BINS], hi[SR_BINS];      // per bin: a count (lo), or a 64-bit sum in two words
+    double exp2_table[64];
+    u64 scan[SR_WARPS];
+    const float* xs;                        // this CTA's slice
+    int n, id0, C, rank, bins;              // its length and first id; the cluster; bins in use
+    RowConst c;
+    // published by every CTA of the cluster into each
+    u64 part[SR_MAX_CLUSTER], best[SR_MAX_CLUSTER], min_part[SR_MAX_CLUSTER];
+    uint32_t low[SR_MAX_CLUSTER];
+    struct Cut {                            // a crossing bin, the sum before it and in it
+        int bin, bin_hi;
+        u64 before, sum;
+    } cut[2];
+    Item item;
+    u64 found[2];
+    // in CTA 0: the gathered ids, and the range of keys and ids of a crowded bin
+    int n_cand;
+    uint32_t kmin, kmax, imin, imax;
+    uint32_t ckey[SR_CAP], cid[SR_CAP];
+    u64 cval[SR_CAP];
+    int cbin[SR_CAP];
+
     __device__ __forceinline__ void add(int b, u64 v, bool count)
     {
         if (count) {
@@ -141,6 +152,7 @@ struct Row {
     }
 };
 
+__device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
 __device__ __forceinline__ bool valid(float x) { return x > -INFINITY; }
 
 // Sum over the threads before this one, and over all.
@@ -179,15 +191,18 @@ struct Joined {
 __device__ __noinline__ Joined join(Row& s, bool count)
 {
     cluster_sync();                         // every CTA's histogram is complete
-    const int share = s.bins / s.C, at = s.rank * share + threadIdx.x;
+    const int share = s.bins / s.C, at = s.rank * share + threadIdx.x, C = s.C;
     Joined j;
     j.v = 0;
     if ((int)threadIdx.x < share) {
-#pragma unroll 8
-        for (int r = 0; r < s.C; ++r) {
-            j.v += *remote(&s.lo[at], r);
-            if (!count) j.v += (u64)*remote(&s.hi[at], r) << 32;
+        uint32_t l[SR_MAX_CLUSTER], h[SR_MAX_CLUSTER];      // (all CTAs' loads in flight together)
+#pragma unroll
+        for (int r = 0; r < SR_MAX_CLUSTER; ++r) {
+            l[r] = r < C ? *remote(&s.lo[at], r) : 0u;
+            h[r] = r < C && !count ? *remote(&s.hi[at], r) : 0u;
         }
+#pragma unroll
+        for (int r = 0; r < SR_MAX_CLUSTER; ++r) j.v += (u64)l[r] + ((u64)h[r] << 32);
     }
     u64 mine;
     j.before = block_before(s, j.v, &mine);
@@ -201,15 +216,15 @@ __device__ __noinline__ Joined join(Row& s, bool count)
     return j;
 }
 
-// The bin in which base + the running sum first reaches target (1 <= target - base <= total), in s.bin and s.before of every
-// CTA; clears the list of the gather that follows.
-__device__ __forceinline__ void find(Row& s, const Joined& j, u64 target, u64 base)
+// The bin in which base + the running sum first reaches target (1 <= target - base <= total), in s.cut[which] of every CTA;
+// clears the list of the gather that follows.
+__device__ __forceinline__ void find(Row& s, const Joined& j, u64 target, u64 base, int which = 0)
 {
     const u64 b = base + j.before, e = b + j.v;
     if (b < target && e >= target) {
-        s.publish(&s.bin, s.rank * (s.bins / s.C) + (int)threadIdx.x);
-        s.publish(&s.before, b);
-        s.publish(&s.bin_sum, j.v);
+        s.publish(&s.cut[which].bin, s.rank * (s.bins / s.C) + (int)threadIdx.x);
+        s.publish(&s.cut[which].before, b);
+        s.publish(&s.cut[which].sum, j.v);
     }
     if (s.rank == 0 && threadIdx.x == 0) {
         s.n_cand = 0;
@@ -241,22 +256,23 @@ template <typename F> __device__ __forceinline__ void each_logit(const Row& s, c
 // f(key, id, mass or 1) for this CTA's ids whose logit pre takes, that in(key, id) takes, that the top-k cut keeps and that
 // have a mass.
 template <typename Pre, typename In, typename F>
-__device__ __forceinline__ void each(const Row& s, bool count, const Pre& pre, const In& in, const F& f)
+__device__ __forceinline__ void each(const Row& s, const RowConst& c, bool count, const Pre& pre, const In& in, const F& f)
 {
+    const int id0 = s.id0;
     each_logit(s, [&](int i, float x) {
         if (!pre(x) || !valid(x)) return;
-        const uint32_t key = order_key(x), id = (uint32_t)(s.id0 + i);
-        if (!in(key, id) || !s.kept(key, id)) return;
-        const u64 m = count ? 1ull : s.mass(s.prob(x));
+        const uint32_t key = order_key(x), id = (uint32_t)(id0 + i);
+        if (!in(key, id) || !c.kept(key, id)) return;
+        const u64 m = count ? 1ull : c.mass(c.prob(x, s.exp2_table));
         if (m) f(key, id, m);
     });
 }
 
 // Those ids to CTA 0's list (up to SR_CAP of them; s.n_cand there counts all).
-template <typename Pre, typename In> __device__ __forceinline__ void gather(Row& s, bool count, const Pre& pre, const In& in)
+template <typename Pre, typename In> __device__ __forceinline__ void gather(Row& s, const RowConst& c, bool count, const Pre& pre, const In& in)
 {
     Row* lead = remote(&s, 0);
-    each(s, count, pre, in, [&](uint32_t key, uint32_t id, u64 m) {
+    each(s, c, count, pre, in, [&](uint32_t key, uint32_t id, u64 m) {
         // one add for the lanes that are here together
         const uint32_t here = __activemask(), lane = threadIdx.x & 31;
         int at = 0;
@@ -275,32 +291,33 @@ template <typename Pre, typename In> __device__ __forceinline__ void gather(Row&
 __device__ __noinline__ Item select(Row& s, const Joined j0, u64 target, bool count)
 {
     find(s, j0, target, 0);
-    const int bin = s.bin;
-    u64 before = s.before;
+    const RowConst c = s.c;
+    const int bin = s.cut[0].bin;
+    u64 before = s.cut[0].before;
     bool deep = false;                      // past level 0: the ids with keys [klo, khi] and ids [ilo, ihi]
     uint32_t klo = 0u, khi = UINT_MAX, ilo = 0u, ihi = UINT_MAX;
     Row* lead = remote(&s, 0);
-    auto pre = [&](float x) { return deep || s.bin0(x) == bin; };
+    auto pre = [&](float x) { return deep || c.bin0(x) == bin; };
     auto in = [&](uint32_t key, uint32_t id) { return key >= klo && key <= khi && id >= ilo && id <= ihi; };
     // (a cut by keys leaves 2^-9 of their range at most, one by ids of theirs: at most nine rounds)
 #pragma unroll 1
     for (int round = 0; round < 16; ++round) {
-        gather(s, count, pre, in);
+        gather(s, c, count, pre, in);
         const int nc = lead->n_cand;
         if (nc <= SR_CAP) {
             if (s.rank == 0 && (int)threadIdx.x < nc) {
                 const uint32_t key = s.ckey[threadIdx.x], id = s.cid[threadIdx.x];
-                u64 c = before;
+                u64 cum = before;
                 for (int q = 0; q < nc; ++q)
-                    if (s.ckey[q] > key || (s.ckey[q] == key && s.cid[q] <= id)) c += s.cval[q];
-                if (c >= target && c - s.cval[threadIdx.x] < target) s.publish(&s.item, Item{key, id, c});
+                    if (s.ckey[q] > key || (s.ckey[q] == key && s.cid[q] <= id)) cum += s.cval[q];
+                if (cum >= target && cum - s.cval[threadIdx.x] < target) s.publish(&s.item, Item{key, id, cum});
             }
             cluster_sync();
             return s.item;
         }
         // a crowded range: cut it by the bits of its keys, or, all keys equal, by ids
         uint32_t k0 = UINT_MAX, k1 = 0u, d0 = UINT_MAX, d1 = 0u;
-        each(s, count, pre, in, [&](uint32_t key, uint32_t id, u64) {
+        each(s, c, count, pre, in, [&](uint32_t key, uint32_t id, u64) {
             k0 = min(k0, key);
             k1 = max(k1, key);
             d0 = min(d0, id);
@@ -323,11 +340,11 @@ __device__ __noinline__ Item select(Row& s, const Joined j0, u64 target, bool co
         const uint32_t width = by_id ? ihi - ilo : khi - klo;
         const int shift = max(0, 32 - __clz(width) - (31 - __clz(s.bins)));
         clear_hist(s);
-        each(s, count, pre, in, [&](uint32_t key, uint32_t id, u64 m) { s.add((by_id ? id - ilo : khi - key) >> shift, m, count); });
+        each(s, c, count, pre, in, [&](uint32_t key, uint32_t id, u64 m) { s.add((by_id ? id - ilo : khi - key) >> shift, m, count); });
         const Joined j = join(s, count);
         find(s, j, target, before);
-        before = s.before;
-        const uint32_t from = (uint32_t)s.bin << shift, upto = from + ((1u << shift) - 1u);
+        before = s.cut[0].before;
+        const uint32_t from = (uint32_t)s.cut[0].bin << shift, upto = from + ((1u << shift) - 1u);
         if (by_id) {
             const uint32_t i0 = ilo;
             ilo = i0 + from;
@@ -347,19 +364,39 @@ __device__ __forceinline__ u64 share_of(double part, u64 sum)      // the sum th
     return min(sum, t > 1.0 ? (u64)t : 1ull);
 }
 
-// CTA 0's list of n ids (one a thread, 0 < n <= SR_CAP), among them the first k of the order: its top-k, top-p, min-p and pick.
+// f(i, q) for every pair of list items i < n and q < n, the q's of an i shared by a group of g lanes (whose lane 0 gets true
+// from owner()): g so that the pairs spread over the CTA.
+struct Pairs {
+    int i, sub, g;
+    __device__ __forceinline__ explicit Pairs(int n)
+    {
+        g = n <= 16 ? 32 : n <= 32 ? 16 : n <= 64 ? 8 : n <= 128 ? 4 : n <= 256 ? 2 : 1;
+        i = threadIdx.x / g;
+        sub = threadIdx.x & (g - 1);
+    }
+    template <typename T> __device__ __forceinline__ T sum(T v) const
+    {
+        for (int o = 1; o < g; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    }
+};
+
+// CTA 0's list of n ids (0 < n <= SR_CAP), among them the first k of the order: its top-k, top-p, min-p and pick.
 __device__ __noinline__ void finish_list(Row& s, int n, int k, const wl_sample_opts& o, int32_t* out)
 {
     const int tid = threadIdx.x;
+    const RowConst c = s.c;
+    const Pairs pr(n);
     uint32_t key = 0, id = 0;
     int rank = 0;
-    if (tid < n) {
-        key = s.ckey[tid];
-        id = s.cid[tid];
-        for (int q = 0; q < n; ++q) rank += s.ckey[q] > key || (s.ckey[q] == key && s.cid[q] < id);
+    if (pr.i < n) {
+        key = s.ckey[pr.i];
+        id = s.cid[pr.i];
+        for (int q = pr.sub; q < n; q += pr.g) rank += s.ckey[q] > key || (s.ckey[q] == key && s.cid[q] < id);
     }
+    rank = pr.sum(rank);
     __syncthreads();
-    if (tid < n) {
+    if (pr.i < n && pr.sub == 0) {
         s.ckey[rank] = key;
         s.cid[rank] = id;
     }
@@ -368,58 +405,61 @@ __device__ __noinline__ void finish_list(Row& s, int n, int k, const wl_sample_o
     double p = 0.0;
     u64 m = 0, all;
     if (tid < k) {
-        key = s.ckey[tid];
-        p = s.prob(__uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key));
-        m = s.mass(p);
+        p = c.prob(key_value(s.ckey[tid]), s.exp2_table);
+        m = c.mass(p);
     }
     const u64 cum = block_before(s, m, &all) + m;
     u64 sum = all;
     if (o.top_p < 1.0) {
         const u64 t = share_of(o.top_p, sum);
-        if (cum >= t && cum - m < t) s.before = cum;        // (one thread: m > 0)
+        if (cum >= t && cum - m < t) s.found[0] = cum;      // (one thread: m > 0)
         __syncthreads();
-        sum = s.before;
+        sum = s.found[0];
     }
     if (o.min_p > 0.0) {
         const int above = __syncthreads_count(tid < k && p >= o.min_p);
-        if (tid == above - 1) s.red[0] = cum;
+        if (tid == above - 1) s.found[1] = cum;
         __syncthreads();
-        sum = max(1ull, min(sum, above ? s.red[0] : 0ull));
+        sum = max(1ull, min(sum, above ? s.found[1] : 0ull));
     }
     const u64 t = share_of(o.draw, sum);
     if (cum >= t && cum - m < t) *out = (int32_t)s.cid[tid];
 }
 
-// CTA 0's list of n ids with their masses: those of the bin that the nucleus ends in (bin0 == nb, the sum before it nbefore;
-// nb < 0: no nucleus, the kept sum is `sum`), and of the bins p_lo .. p_hi that the pick falls in whichever id that is
-// (pbefore: the sum before p_lo). over: the sum of the ids with p >= min_p.
+// CTA 0's list of n ids with their masses: those of the bin that the nucleus ends in (nb, the sum before it nbefore; nb < 0:
+// no nucleus, the kept sum is `sum`), and of the bins p_lo .. p_hi that the pick falls in whichever id that is (pbefore: the
+// sum before p_lo). over: the sum of the ids with p >= min_p.
 __device__ __noinline__ void finish_bins(Row& s, int n, int nb, u64 nbefore, u64 ntarget, int p_lo, int p_hi, u64 pbefore, u64 sum, u64 over,
                                          double draw, int32_t* out)
 {
-    const int tid = threadIdx.x;
+    const RowConst c = s.c;
+    for (int i = threadIdx.x; i < n; i += SR_THREADS) s.cbin[i] = c.bin0(key_value(s.ckey[i]));
+    __syncthreads();
+    const Pairs pr(n);
     uint32_t key = 0, id = 0;
     int bin = -1;
-    u64 m = 0, cn = nbefore, cp = pbefore;
-    auto bin_of = [&](uint32_t k) { return s.bin0(__uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k)); };
-    if (tid < n) {
-        key = s.ckey[tid];
-        id = s.cid[tid];
-        m = s.cval[tid];
-        bin = bin_of(key);
-        for (int q = 0; q < n; ++q) {
+    u64 m = 0, cn = 0, cp = 0;
+    if (pr.i < n) {
+        key = s.ckey[pr.i];
+        id = s.cid[pr.i];
+        m = s.cval[pr.i];
+        bin = s.cbin[pr.i];
+        for (int q = pr.sub; q < n; q += pr.g) {
             const uint32_t k = s.ckey[q];
             if (k > key || (k == key && s.cid[q] <= id)) {
-                const int b = bin_of(k);
+                const int b = s.cbin[q];
                 const u64 v = s.cval[q];
-                if (b == nb) cn += v;
-                if (b >= p_lo && b <= p_hi) cp += v;
+                cn += b == nb ? v : 0ull;
+                cp += b >= p_lo && b <= p_hi ? v : 0ull;
             }
         }
     }
+    cn = nbefore + pr.sum(cn);
+    cp = pbefore + pr.sum(cp);
     if (nb >= 0) {
-        if (bin == nb && cn >= ntarget && cn - m < ntarget) s.before = cn;
+        if (bin == nb && cn >= ntarget && cn - m < ntarget) s.found[0] = cn;
         __syncthreads();
-        sum = s.before;
+        sum = s.found[0];
     }
     sum = max(1ull, min(sum, over));
     const u64 t = share_of(draw, sum);
@@ -446,18 +486,34 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
     uint32_t low = UINT_MAX;
     {
         const float* xs = x + id0;
-        auto take = [&](int i, float v) {
-            if (!valid(v)) return;
-            const uint32_t key = order_key(v);
-            const u64 b = (u64)key << 32 | (uint32_t)~(uint32_t)(id0 + i);
-            best = b > best ? b : best;
-            low = min(low, key);
+        float top = -INFINITY, bottom = INFINITY;
+        int top_i = -1;
+        auto take = [&](int i, float v) {   // (a thread's i ascend: the first of equal values stays)
+            if (v > top) {
+                top = v;
+                top_i = i;
+            }
+            if (v > -INFINITY) bottom = fminf(bottom, v);
         };
         int done = 0;
         if (((uintptr_t)xs & 15) == 0) {
             const int n4 = n / 4;
-#pragma unroll 4
-            for (int i = tid; i < n4; i += SR_THREADS) {
+            int i = tid;
+            for (; i + 3 * SR_THREADS < n4; i += 4 * SR_THREADS) {
+                float4 v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = reinterpret_cast<const float4*>(xs)[i + k * SR_THREADS];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int at = i + k * SR_THREADS;
+                    if (keep) reinterpret_cast<float4*>(keep)[at] = v[k];
+                    take(4 * at, v[k].x);
+                    take(4 * at + 1, v[k].y);
+                    take(4 * at + 2, v[k].z);
+                    take(4 * at + 3, v[k].w);
+                }
+            }
+            for (; i < n4; i += SR_THREADS) {
                 const float4 v = reinterpret_cast<const float4*>(xs)[i];
                 if (keep) reinterpret_cast<float4*>(keep)[i] = v;
                 take(4 * i, v.x);
@@ -472,6 +528,10 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
             if (keep) keep[i] = v;
             take(i, v);
         }
+        if (top_i >= 0) {
+            best = (u64)order_key(top) << 32 | (uint32_t)~(uint32_t)(id0 + top_i);
+            low = order_key(bottom);
+        }
         if (tid == 0) {
             s.xs = keep ? keep : xs;
             s.n = n;
@@ -479,31 +539,38 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
             s.C = C;
             s.rank = rank;
             s.bins = min(SR_BINS, 512 * C);
-            s.frac = frac;
-            s.has_k = 0;
+            s.c.frac = frac;
+            s.c.last_bin = (float)(s.bins - 1);
+            s.c.has_k = 0;
         }
     }
+    auto reduce = [&] {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        const u64 b = __shfl_xor_sync(0xffffffffu, best, d);
-        best = b > best ? b : best;
-        low = min(low, __shfl_xor_sync(0xffffffffu, low, d));
-    }
+        for (int d = 16; d > 0; d >>= 1) {
+            const u64 b = __shfl_xor_sync(0xffffffffu, best, d);
+            best = b > best ? b : best;
+        }
+        low = __reduce_min_sync(0xffffffffu, low);
+    };
+    reduce();
     if ((tid & 31) == 0) {
-        s.red[tid >> 5] = best;
-        s.scan[tid >> 5] = low;
+        s.scan[tid >> 5] = best;
+        s.cid[tid >> 5] = low;
     }
     __syncthreads();
-    cluster_wait();
-    if (tid == 0) {
-        for (int w = 0; w < SR_WARPS; ++w) {
-            best = s.red[w] > best ? s.red[w] : best;
-            low = min(low, (uint32_t)s.scan[w]);
+    cluster_wait();                         // (every CTA of the cluster has started: its memory may be written)
+    if (tid < 32) {
+        best = tid < SR_WARPS ? s.scan[tid] : 0;
+        low = tid < SR_WARPS ? s.cid[tid] : UINT_MAX;
+        reduce();
+        if (tid < C) {
+            *remote(&s.best[rank], tid) = best;
+            *remote(&s.low[rank], tid) = low;
         }
-        s.publish(&s.best[rank], best);
-        s.publish(&s.low[rank], low);
     }
     cluster_sync();
+    best = 0;
+    low = UINT_MAX;
     for (int r = 0; r < C; ++r) {
         best = s.best[r] > best ? s.best[r] : best;
         low = min(low, s.low[r]);
@@ -515,41 +582,41 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
         return;
     }
     const bool with_k = o.top_k > 0 && o.top_k < V, sorted = with_k || o.top_p < 1.0 || o.min_p > 0.0;
-    auto value = [](uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); };
-    const float xmax = value((uint32_t)(best >> 32));
+    const float xmax = key_value((uint32_t)(best >> 32));
     // the histogram's range: down to the smallest value, in halves so that no difference overflows
-    const float half_range = xmax * 0.5f - value(low) * 0.5f;
+    const float half_range = xmax * 0.5f - key_value(low) * 0.5f;
     auto width = [&](float range) { return range > 0.f && range <= FLT_MAX ? (float)s.bins / range : 0.f; };
     if (tid == 0) {
-        s.xmax = xmax;
-        s.inv_t = 1.4426950408889634 / o.temperature;
-        s.unit = ldexp(1.0, frac);
-        s.inv_w = width(half_range);
+        s.c.xmax = xmax;
+        s.c.inv_t = 1.4426950408889634 / o.temperature;
+        s.c.unit = ldexp(1.0, frac);
+        s.c.inv_w = width(half_range);
     }
     Joined j;
     if (with_k) {
         clear_hist(s);
+        const RowConst c = s.c;
         each_logit(s, [&](int, float v) {
-            if (valid(v)) s.add(s.bin0(v), 0, true);
+            if (valid(v)) s.add(c.bin0(v), 0, true);
         });
         j = join(s, true);
         const int k = (int)min(j.total, (u64)o.top_k);
         find(s, j, (u64)k, 0);
-        // few enough ids down to the k-th's bin: CTA 0 ends the row with them
-        const int bin = s.bin;
-        gather(s, true, [&](float v) { return s.bin0(v) <= bin; }, [](uint32_t, uint32_t) { return true; });
-        const int nc = remote(&s, 0)->n_cand;
-        cluster_sync();                     // (CTA 0's count has been read)
+        const int bin = s.cut[0].bin;
+        const u64 nc = s.cut[0].before + s.cut[0].sum;
         if (nc <= SR_CAP) {
-            if (rank == 0) finish_list(s, nc, k, o, ids + row);
+            // few enough ids down to the k-th's bin: CTA 0 ends the row with them
+            gather(s, c, true, [&](float v) { return c.bin0(v) <= bin; }, [](uint32_t, uint32_t) { return true; });
+            if (rank == 0) finish_list(s, (int)nc, k, o, ids + row);
             return;
         }
         if (j.total > (u64)o.top_k) {
+            cluster_sync();                 // (s.cut has been read)
             const Item it = select(s, j, (u64)k, true);
             if (tid == 0) {
-                s.k_key = it.key;
-                s.k_id = it.id;
-                s.has_k = 1;
+                s.c.k_key = it.key;
+                s.c.k_id = it.id;
+                s.c.has_k = 1;
             }
         }
         __syncthreads();
@@ -558,10 +625,12 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
         __syncthreads();
         const int per = ((n + SR_THREADS - 1) / SR_THREADS) | 1;
         const int i0 = min(n, tid * per), i1 = min(n, i0 + per);
+        const RowConst c = s.c;
+        const float* xs = s.xs;
         u64 sum = 0, mine;
         for (int i = i0; i < i1; ++i) {
-            const float v = s.xs[i];
-            if (valid(v)) sum += s.mass(s.prob(v));
+            const float v = xs[i];
+            if (valid(v)) sum += c.mass(c.prob(v, s.exp2_table));
         }
         u64 before = block_before(s, sum, &mine);
         if (tid == 0) s.publish(&s.part[rank], mine);
@@ -574,8 +643,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
         const u64 target = share_of(o.draw, total);
         if (before < target && before + sum >= target) {
             for (int i = i0; i < i1; ++i) {
-                const float v = s.xs[i];
-                if (valid(v)) before += s.mass(s.prob(v));
+                const float v = xs[i];
+                if (valid(v)) before += c.mass(c.prob(v, s.exp2_table));
                 if (before >= target) {
                     ids[row] = id0 + i;
                     break;
@@ -585,16 +654,18 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
         return;
     }
     // masses: below 2^-(F+1) of the largest nothing is left, so the histogram's range ends there
-    if (tid == 0) s.inv_w = width(fminf(half_range, (float)fmin((frac + 2) * 0.6931471805599453 * o.temperature * 0.5, (double)FLT_MAX)));
+    if (tid == 0) s.c.inv_w = width(fminf(half_range, (float)fmin((frac + 2) * 0.6931471805599453 * o.temperature * 0.5, (double)FLT_MAX)));
     clear_hist(s);
+    const RowConst c = s.c;
     u64 over = 0;                           // the sum of the kept ids with p >= min_p
+    const double min_p = o.min_p;
     each_logit(s, [&](int i, float v) {
-        if (!valid(v) || !s.kept(order_key(v), (uint32_t)(id0 + i))) return;
-        const double p = s.prob(v);
-        const u64 m = s.mass(p);
+        if (!valid(v) || (c.has_k && !c.kept(order_key(v), (uint32_t)(id0 + i)))) return;
+        const double p = c.prob(v, s.exp2_table);
+        const u64 m = c.mass(p);
         if (!m) return;
-        s.add(s.bin0(v), m, false);
-        if (p >= o.min_p) over += m;
+        s.add(c.bin0(v), m, false);
+        if (p >= min_p) over += m;
     });
     if (o.min_p > 0.0) {
         u64 mine;
@@ -613,27 +684,29 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
     if (o.top_p < 1.0) {
         ntarget = share_of(o.top_p, j.total);
         find(s, j, ntarget, 0);
-        nb = s.bin;
-        nbefore = s.before;
+        nb = s.cut[0].bin;
+        nbefore = s.cut[0].before;
         s_lo = nbefore + 1;
-        s_hi = nbefore + s.bin_sum;
+        s_hi = nbefore + s.cut[0].sum;
     }
     const u64 t_lo = share_of(o.draw, max(1ull, min(s_lo, over))), t_hi = share_of(o.draw, max(1ull, min(s_hi, over)));
-    cluster_sync();                         // (s.bin and s.before have been read)
-    if (j.before < t_hi && j.before + j.v >= t_hi) s.publish(&s.bin_hi, rank * (s.bins / C) + tid);
-    find(s, j, t_lo, 0);
-    const int p_lo = s.bin, p_hi = s.bin_hi;
-    const u64 pbefore = s.before;
-    gather(s, false, [&](float v) {
-        const int b = s.bin0(v);
+    if (j.before < t_hi && j.before + j.v >= t_hi) s.publish(&s.cut[1].bin_hi, rank * (s.bins / C) + tid);
+    find(s, j, t_lo, 0, 1);
+    const int p_lo = s.cut[1].bin, p_hi = s.cut[1].bin_hi;
+    const u64 pbefore = s.cut[1].before;
+    gather(s, c, false, [&](float v) {
+        const int b = c.bin0(v);
         return b == nb || (b >= p_lo && b <= p_hi);
     }, [](uint32_t, uint32_t) { return true; });
     const int nc = remote(&s, 0)->n_cand;
-    cluster_sync();                         // (CTA 0's count has been read)
+    // CTA 0 ends the row; it leaves once the others have read its count
+    cluster_arrive();
     if (nc <= SR_CAP) {
         if (rank == 0) finish_bins(s, nc, nb, nbefore, ntarget, p_lo, p_hi, pbefore, j.total, over, o.draw, ids + row);
+        cluster_wait();
         return;
     }
+    cluster_wait();
     // crowded bins: one cut after the other
     u64 sum = j.total;
     if (nb >= 0) sum = select(s, j, ntarget, false).cum;
