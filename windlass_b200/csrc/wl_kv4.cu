@@ -472,16 +472,29 @@ constexpr int ATT_TPS = 48;
 constexpr int ATT_STAGES = 2;               // ring stages a warp, of two tiles each
 constexpr int att_ctas(int HD) { return HD <= 128 ? 2 : 1; }
 
-// Rows on their own (decode): CTA (range, KV head and tile of 8 query heads, row); each warp streams its own tiles, every
-// fourth pair of the range, through its ring of bulk copies, and the warps' sums are joined in warp order. The ranges follow
-// from the row's own length, so a row's bits do not depend on the other rows.
-template <int HD>
+// Rows on their own (decode). A row's tiles are cut into ranges of att_range() tiles, from the row's own length; a CTA
+// (range, KV head and tile of 8 query heads, row) gives a range's maximum, sum and output. Each warp streams its own tiles,
+// every eighth pair of the range, through its ring of bulk copies, and the warps' sums are joined in warp order. The last
+// CTA of a row joins the ranges, or, where there are rows enough to fill the SMs (ALONE: rows of up to a.alone ranges), one
+// CTA walks a row's ranges: a row's bits do not depend on that, nor on the other rows.
+__device__ __forceinline__ int att_range(int tiles, int s_max)
+{
+    constexpr int step = 2 * ATT_WARPS;     // a pair of tiles for each warp
+    return max(ATT_TPS, ((tiles + s_max - 1) / s_max + step - 1) / step * step);
+}
+
+template <int HD, bool ALONE>
 __global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const Kv4Att a)
 {
     constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD), ST = ATT_STAGES, NT = 32 * ATT_WARPS;
+    constexpr int IT = (8 * (HD / 4) + NT - 1) / NT;        // 4-value items of the output a thread joins
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[ATT_WARPS][ST];
     __shared__ float sm_m[ATT_WARPS][8], sm_l[ATT_WARPS][8];
+    // the queries' fragments and terms, made by one warp
+    __shared__ __align__(16) uint4 sq[NB * 2 * 32];
+    __shared__ float sqt[(NB + 1) * 32];
+    float* so = reinterpret_cast<float*>(smem + ATT_WARPS * ST * 2 * TB);       // [warp][8][HD]
     pdl_trigger();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -499,19 +512,21 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const
     }
     const Vis vis[1] = {visible(p, a.window, a.sinks)};
     const TileList tl = tile_list(vis[0].n, vis[0].first, vis[0].sink);
-    const int S = min(a.s_max, (tl.count + ATT_TPS - 1) / ATT_TPS);
-    if (sp >= S) return;
-    const int i0 = (int)((int64_t)tl.count * sp / S), i1 = (int)((int64_t)tl.count * (sp + 1) / S);
-    // the warp's steps of two tiles: items i0 + 2 (warp + 4 i) and the next of the list
-    const int steps = ((i1 - i0 + 1) / 2 - warp + ATT_WARPS - 1) / ATT_WARPS;
+    const int range = att_range(tl.count, a.s_max), S = (tl.count + range - 1) / range;
+    const bool alone = ALONE && S <= a.alone;
+    if (sp >= (alone ? 1 : S)) return;
+    const int i0 = sp * range, i1 = alone ? tl.count : min(tl.count, i0 + range);
+    // step i of the warp: the pair of tiles at list item at(i) and the next (a range holds whole rounds of the warps' pairs)
+    auto at = [&](int i) { return i0 + 2 * (i * ATT_WARPS + warp); };
+    const int steps = max(0, (i1 - i0 - 2 * warp + 2 * ATT_WARPS - 1) / (2 * ATT_WARPS));
     uint8_t* ring = smem + warp * ST * 2 * TB;
     const uint8_t* src = base + (int64_t)kvh * TB;
     auto issue = [&](int i) {
         uint64_t* bar = &bars[warp][i % ST];
-        const int at = i0 + 2 * (warp + ATT_WARPS * i), two = at + 1 < i1;
+        const int x = at(i), two = x + 1 < i1;
         mbar_expect_tx(bar, two ? 2 * TB : TB);
-        bulk_load(ring + i % ST * 2 * TB, src + (int64_t)tl.at(at) * a.kv_heads * TB, TB, bar);
-        if (two) bulk_load(ring + i % ST * 2 * TB + TB, src + (int64_t)tl.at(at + 1) * a.kv_heads * TB, TB, bar);
+        bulk_load(ring + i % ST * 2 * TB, src + (int64_t)tl.at(x) * a.kv_heads * TB, TB, bar);
+        if (two) bulk_load(ring + i % ST * 2 * TB + TB, src + (int64_t)tl.at(x + 1) * a.kv_heads * TB, TB, bar);
     };
     if (lane == 0) {
         for (int s = 0; s < ST; ++s) mbar_init(&bars[warp][s], 1);
@@ -519,9 +534,6 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const
         for (int s = 0; s < ST && s < steps; ++s) issue(s);
     }
     QueryTerms<NB> qt[1];
-    // the queries' fragments and terms, made by one warp
-    __shared__ __align__(16) uint4 sq[NB * 2 * 32];
-    __shared__ float sqt[(NB + 1) * 32];
     if (warp == 0) {
         uint4 qa[NB][2];
         load_query<HD>(g < nh ? a.q + ((int64_t)t * a.heads + head0 + g) * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa, qt[0]);
@@ -538,71 +550,84 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const
     for (int b = 0; b < NB; ++b) qt[0].off[b] = sqt[b * 32 + lane];
     qt[0].ks = sqt[NB * 32 + lane];
     auto qf = [&](int, int b, int s) { return sq[b * 64 + s * 32 + lane]; };
-    AttState<HD, 1> st;
-    st.init();
-    for (int i = 0; i < steps; ++i) {
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bars[warp][i % ST], (uint32_t)(i / ST & 1), a.err, 21))) break;
-        const int at = i0 + 2 * (warp + ATT_WARPS * i);
-        // (of an odd range's last step the second tile is not there: a position that no row sees)
-        const int tile0[2] = {tl.at(at) * KV4_P, at + 1 < i1 ? tl.at(at + 1) * KV4_P : INT_MAX - KV4_P};
-        const bool full = tile0[0] >= vis[0].first && tile0[1] < vis[0].n - KV4_P + 1;
-        kv4_tiles<HD, 1, 2>(ring + i % ST * 2 * TB, lane, tile0, vis, full, qf, qt, st);
-        __syncwarp();
-        if (lane == 0 && i + ST < steps) issue(i + ST);
-    }
-    // the warps' sums, joined through the ring's memory (every copy has landed and been read)
-    st.l[0] += __shfl_xor_sync(0xffffffffu, st.l[0], 1);
-    st.l[0] += __shfl_xor_sync(0xffffffffu, st.l[0], 2);
-    __syncthreads();
-    float* so = reinterpret_cast<float*>(smem);
-    const float undo = 1.f / st.vs;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float4 v;
-            v.x = (st.o[0][4 * b][e] + st.o[0][4 * b][e + 2]) * undo;
-            v.y = (st.o[0][4 * b + 1][e] + st.o[0][4 * b + 1][e + 2]) * undo;
-            v.z = (st.o[0][4 * b + 2][e] + st.o[0][4 * b + 2][e + 2]) * undo;
-            v.w = (st.o[0][4 * b + 3][e] + st.o[0][4 * b + 3][e + 2]) * undo;
-            *reinterpret_cast<float4*>(so + (warp * 8 + g) * HD + 32 * b + 8 * c + 4 * e) = v;
+    JoinState js[IT];
+    int i = 0;
+    bool ok = true;
+    for (int r0 = i0; r0 < i1 && ok; r0 += range) {
+        const int r1 = ALONE ? min(i1, r0 + range) : i1;
+        AttState<HD, 1> st;
+        st.init();
+        for (; i < steps && (!ALONE || at(i) < r1); ++i) {
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars[warp][i % ST], (uint32_t)(i / ST & 1), a.err, 21));
+            if (!ok) break;
+            const int x = at(i);
+            // (of an odd range's last step the second tile is not there: a position that no row sees)
+            const int tile0[2] = {tl.at(x) * KV4_P, x + 1 < i1 ? tl.at(x + 1) * KV4_P : INT_MAX - KV4_P};
+            const bool full = tile0[0] >= vis[0].first && tile0[1] < vis[0].n - KV4_P + 1;
+            kv4_tiles<HD, 1, 2>(ring + i % ST * 2 * TB, lane, tile0, vis, full, qf, qt, st);
+            __syncwarp();
+            if (lane == 0 && i + ST < steps) issue(i + ST);
         }
-    if (c == 0) {
-        sm_m[warp][g] = st.m[0];
-        sm_l[warp][g] = st.l[0];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < nh * HD / 4; i += NT) {
-        const int h = i / (HD / 4), d = i % (HD / 4) * 4;
-        float M = sm_m[0][h];
+        // the warps' sums of the range
+        st.l[0] += __shfl_xor_sync(0xffffffffu, st.l[0], 1);
+        st.l[0] += __shfl_xor_sync(0xffffffffu, st.l[0], 2);
+        const float undo = 1.f / st.vs;
 #pragma unroll
-        for (int w = 1; w < ATT_WARPS; ++w) M = fmaxf(M, sm_m[w][h]);
-        const float mu = M == -INFINITY ? 0.f : M;
-        float L = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int w = 0; w < ATT_WARPS; ++w) {
-            const float f = ex2(sm_m[w][h] - mu);
-            const float4 x = *reinterpret_cast<const float4*>(so + (w * 8 + h) * HD + d);
-            L += f * sm_l[w][h];
-            o.x += f * x.x;
-            o.y += f * x.y;
-            o.z += f * x.z;
-            o.w += f * x.w;
+            for (int e = 0; e < 2; ++e) {
+                float4 v;
+                v.x = (st.o[0][4 * b][e] + st.o[0][4 * b][e + 2]) * undo;
+                v.y = (st.o[0][4 * b + 1][e] + st.o[0][4 * b + 1][e + 2]) * undo;
+                v.z = (st.o[0][4 * b + 2][e] + st.o[0][4 * b + 2][e + 2]) * undo;
+                v.w = (st.o[0][4 * b + 3][e] + st.o[0][4 * b + 3][e + 2]) * undo;
+                *reinterpret_cast<float4*>(so + (warp * 8 + g) * HD + 32 * b + 8 * c + 4 * e) = v;
+            }
+        if (c == 0) {
+            sm_m[warp][g] = st.m[0];
+            sm_l[warp][g] = st.l[0];
         }
+        ok = __syncthreads_and(ok);         // (a wait that gave up ends the row for all warps)
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+            const int it = threadIdx.x + NT * k, h = it / (HD / 4), d = it % (HD / 4) * 4;
+            if (h >= 8) break;
+            float M = sm_m[0][h];
+#pragma unroll
+            for (int w = 1; w < ATT_WARPS; ++w) M = fmaxf(M, sm_m[w][h]);
+            const float mu = M == -INFINITY ? 0.f : M;
+            float L = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < ATT_WARPS; ++w) {
+                const float f = ex2(sm_m[w][h] - mu);
+                const float4 x = *reinterpret_cast<const float4*>(so + (w * 8 + h) * HD + d);
+                L = __fmaf_rn(f, sm_l[w][h], L);
+                o.x = __fmaf_rn(f, x.x, o.x);
+                o.y = __fmaf_rn(f, x.y, o.y);
+                o.z = __fmaf_rn(f, x.z, o.z);
+                o.w = __fmaf_rn(f, x.w, o.w);
+            }
+            js[k].add(M, L, o, r0 == i0);
+        }
+        if (!ALONE) break;
+        if (r1 < i1) __syncthreads();       // (the next range's sums go to the same place)
+    }
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+        const int it = threadIdx.x + NT * k, h = it / (HD / 4), d = it % (HD / 4) * 4;
+        if (h >= nh) continue;
         const int64_t th = (int64_t)t * a.heads + head0 + h;
-        if (S == 1) {
-            const float inv = 1.f / L;
-            *reinterpret_cast<float4*>(a.out + th * HD + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        if (S == 1 || alone) {
+            *reinterpret_cast<float4*>(a.out + th * HD + d) = js[k].out();
         } else {
-            *reinterpret_cast<float4*>(a.part + (th * a.S + sp) * HD + d) = o;
-            if (d == 0) reinterpret_cast<float2*>(a.ml)[th * a.S + sp] = make_float2(M, L);
+            *reinterpret_cast<float4*>(a.part + (th * a.S + sp) * HD + d) = js[k].o;
+            if (d == 0) reinterpret_cast<float2*>(a.ml)[th * a.S + sp] = make_float2(js[k].M, js[k].L);
         }
     }
-    if (S == 1) return;
+    if (S == 1 || alone) return;
     if (!last_ticket(a.tickets + t * gridDim.y + blockIdx.y, S)) return;
-    const int64_t th0 = (int64_t)t * a.heads + head0;
-    join_ranges<HD, NT>(a, nh, S, so, [&](int h) { return th0 + h; });
+    join_ranges<HD, NT>(a.ml, a.part, a.out, a.S, nh, S, so, RowMap{(int64_t)t * a.heads + head0, 0, 8, 8});
 }
 
 // Runs of R rows that read one cache (prompts): the (row, head) pairs of a run and KV head are queries 0 .. R G - 1; a CTA
@@ -747,9 +772,8 @@ __global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att
     }
     if (S == 1) return;
     if (!last_ticket(a.tickets + ((int64_t)run * a.kv_heads + kvh) * q_blocks + qb, S)) return;
-    join_ranges<HD, 32 * RUN_WARPS>(a, min(QB, nq - q0), S, reinterpret_cast<float*>(smem), [&](int i) {
-        return ((int64_t)run * a.R + (q0 + i) / G) * a.heads + kvh * G + (q0 + i) % G;
-    });
+    join_ranges<HD, 32 * RUN_WARPS>(a.ml, a.part, a.out, S, min(QB, nq - q0), S, reinterpret_cast<float*>(smem),
+                                    RowMap{(int64_t)run * a.R * a.heads + kvh * G, q0, G, a.heads});
 }
 
 constexpr int64_t KV4_TICKETS = 1 << 18;    // tickets at the head of a workspace (zero between calls)
@@ -760,7 +784,7 @@ constexpr int MMA_MIN_QUERIES = 96;
 // How a call is cut.
 struct Kv4Plan {
     bool runs, mma;         // the rows' runs share their cache's tiles: on the tensor cores (k_kv4_attn_mma) or k_kv4_attn_run
-    int S, s_max, q_blocks, MT, MG;
+    int S, s_max, alone, q_blocks, MT, MG;
     int64_t part_floats;
 };
 
@@ -797,8 +821,15 @@ Kv4Plan kv4_plan(int T, int R, int heads, int kv_heads, int head_dim, int64_t ca
         ctas = (int64_t)T * kv_heads * p.MG;
         p.s_max = T > 64 ? 1 : std::max(1, std::min(ATT_MAX_RANGES, 2 * 148 / (kv_heads * p.MG)));
         p.S = (int)std::max<int64_t>(1, std::min<int64_t>(p.s_max, (tiles + ATT_TPS - 1) / ATT_TPS));
+        // enough rows for the SMs: short ones are walked by one CTA each (64 rows with a window of 1024: 49.7 us with a CTA a
+        // range); a row of more than 8 ranges among them is still spread, so that the call does not wait for it
+        p.alone = ctas >= 2 * 148 ? 8 : 0;
+        if (p.alone >= p.S) p.S = 1;
     }
-    if (ctas > KV4_TICKETS) p.S = p.s_max = 1;
+    if (ctas > KV4_TICKETS) {
+        p.S = p.s_max = 1;
+        p.alone = 1;
+    }
     p.part_floats = p.S > 1 ? (int64_t)T * heads * p.S * (head_dim + 2) : 0;
     return p;
 }
@@ -812,17 +843,19 @@ template <typename K> void set_smem(K kern, size_t bytes)
 
 template <int HD> void attn_rows(const Kv4Att& a, const Kv4Plan& p, cudaStream_t s)
 {
-    const size_t smem = (size_t)ATT_WARPS * ATT_STAGES * 2 * kv4_tile_bytes(HD);
-    static_assert(ATT_WARPS * ATT_STAGES * 2 * kv4_tile_bytes(HD) >= ATT_WARPS * 8 * HD * 4, "the warps' sums fit the ring");
-    set_smem(k_kv4_attn<HD>, smem);
-    launch(k_kv4_attn<HD>, dim3(p.S, a.kv_heads * p.MG, a.T), dim3(32 * ATT_WARPS), smem, s, a);
+    const size_t smem = (size_t)ATT_WARPS * ATT_STAGES * 2 * kv4_tile_bytes(HD) + ATT_WARPS * 8 * HD * 4;
+    auto kern = p.alone ? k_kv4_attn<HD, true> : k_kv4_attn<HD, false>;
+    set_smem(kern, smem);
+    launch(kern, dim3(p.S, a.kv_heads * p.MG, a.T), dim3(32 * ATT_WARPS), smem, s, a);
     note_launch();
 }
 
 template <int HD> void attn_runs(const Kv4Att& a, const Kv4Plan& p, cudaStream_t s)
 {
     constexpr int MT = HD <= 128 ? 2 : 1;
-    const size_t smem = 4 * kv4_tile_bytes(HD) + (size_t)RUN_WARPS * MT * (HD / 32) * 2 * 512;
+    // the ring and the queries' fragments; then the join's factors in their place
+    const size_t smem = std::max(4 * kv4_tile_bytes(HD) + (size_t)RUN_WARPS * MT * (HD / 32) * 2 * 512,
+                                 (size_t)RUN_WARPS * 8 * MT * (3 * p.S + 1) * 4);
     set_smem(k_kv4_attn_run<HD, MT>, smem);
     launch(k_kv4_attn_run<HD, MT>, dim3(p.q_blocks * p.S, a.kv_heads, a.T / a.R), dim3(32 * RUN_WARPS), smem, s, a, p.q_blocks);
     note_launch();
@@ -920,7 +953,7 @@ void kv4_attention(const float* q, int T, int R, int heads, int kv_heads, int he
         a.rows = Kv4Rows{(const uint8_t*)cache.rows + t0 * cache.pitch, cache.pitch, cache.layer};
         a.pos = pos + t0;
         a.T = (int)std::min<int64_t>(T - t0, (int64_t)65535 * unit);
-        a.capacity = capacity; a.R = R; a.heads = heads; a.kv_heads = kv_heads; a.S = p.S; a.s_max = p.s_max;
+        a.capacity = capacity; a.R = R; a.heads = heads; a.kv_heads = kv_heads; a.S = p.S; a.s_max = p.s_max; a.alone = p.alone;
         a.scale = scale; a.window = window; a.sinks = sinks;
         a.tickets = (int*)ws;
         a.part = (float*)((uint8_t*)ws + KV4_TICKETS * 4);

@@ -32,6 +32,7 @@ struct Kv4Att {
     const int32_t* pos;
     int64_t capacity;
     int T, R, heads, kv_heads, S, s_max;    // S: ranges a row may be cut into (the stride of the partials)
+    int alone;                              // rows of up to this many ranges are walked by one CTA
     float scale;
     int window, sinks;
     float* part;                            // [T][heads][S][HD]
@@ -234,43 +235,85 @@ constexpr float ATT_SLACK = 6.f;
 
 constexpr int ATT_MAX_RANGES = 96;          // ranges a row may be cut into
 
-// Joins the n ranges of nh rows of heads (the i-th at (row, head) index row(i)) in range order, by a CTA of NT threads:
-// a warp takes a head's weights at a time, then every thread takes 4 output values at a time, its loads of 8 ranges in
-// flight together. w: nh * n floats of shared memory.
-template <int HD, int NT, class F> __device__ __forceinline__ void join_ranges(const Kv4Att& a, int nh, int n, float* w, const F& row)
+// A row's ranges are joined one after the other: (M, L, o) and the next range's (m, l, p) give M' = max(M, m),
+// L e^(M - M') + l e^(m - M') and the same of o. The order and the operations are the same whether one CTA walks all ranges
+// (JoinState) or the last of several CTAs joins what the others left (join_ranges), so a row's bits are too.
+struct JoinState {
+    float M, L;
+    float4 o;
+    __device__ __forceinline__ void add(float m, float l, const float4& p, bool first)
+    {
+        if (first) {
+            M = m;
+            L = l;
+            o = p;
+            return;
+        }
+        const float mn = fmaxf(M, m), mu = mn == -INFINITY ? 0.f : mn, a = ex2(M - mu), b = ex2(m - mu);
+        M = mn;
+        L = __fmaf_rn(l, b, __fmul_rn(L, a));
+        o.x = __fmaf_rn(p.x, b, __fmul_rn(o.x, a));
+        o.y = __fmaf_rn(p.y, b, __fmul_rn(o.y, a));
+        o.z = __fmaf_rn(p.z, b, __fmul_rn(o.z, a));
+        o.w = __fmaf_rn(p.w, b, __fmul_rn(o.w, a));
+    }
+    __device__ __forceinline__ float4 out() const
+    {
+        const float inv = L != 0.f ? __fdiv_rn(1.f, L) : 0.f;      // (a NaN sum stays NaN; no visible position: zeros)
+        return make_float4(__fmul_rn(o.x, inv), __fmul_rn(o.y, inv), __fmul_rn(o.z, inv), __fmul_rn(o.w, inv));
+    }
+};
+
+// Where the queries of a join are: query i is at (row, head) index base + (q0 + i) / G * heads + (q0 + i) % G.
+struct RowMap {
+    int64_t base;
+    int q0, G, heads;
+    __device__ __forceinline__ int64_t at(int i) const { return base + (int64_t)((q0 + i) / G) * heads + (q0 + i) % G; }
+};
+
+// Joins the n ranges (of S places for partials) of nh queries, by a CTA of NT threads: a warp takes a head's
+// factors at a time (the running maxima by a scan), then every thread 4 output values, its loads of 8 ranges in flight
+// together. w: nh * (3 n + 1) floats of shared memory.
+template <int HD, int NT>
+__device__ __noinline__ void join_ranges(const float* ml_, const float* part, float* out, int S, int nh, int n, float* w, RowMap row)
 {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int h = warp; h < nh; h += NT / 32) {
-        const float2* ml = reinterpret_cast<const float2*>(a.ml) + row(h) * a.S;
-        float2 x[ATT_MAX_RANGES / 32];
-        float M = -INFINITY;
+        const float2* ml = reinterpret_cast<const float2*>(ml_) + row.at(h) * S;
+        float* wh = w + h * (3 * n + 1);    // of range s: what the ranges before it are scaled by, what it is, its sum
+        float M = -INFINITY;                // the maximum of the ranges before this lane's
 #pragma unroll
         for (int i = 0; i < ATT_MAX_RANGES / 32; ++i) {
             const int s = lane + 32 * i;
-            x[i] = s < n ? __ldcg(ml + s) : make_float2(-INFINITY, 0.f);
-            M = fmaxf(M, x[i].x);
+            const float2 x = s < n ? __ldcg(ml + s) : make_float2(-INFINITY, 0.f);
+            float inc = x.x;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const float y = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc = fmaxf(inc, y);
+            }
+            float before = __shfl_up_sync(0xffffffffu, inc, 1);
+            before = lane ? fmaxf(before, M) : M;
+            const float mn = fmaxf(before, x.x), mu = mn == -INFINITY ? 0.f : mn;
+            if (s < n) {
+                wh[3 * s] = ex2(before - mu);
+                wh[3 * s + 1] = ex2(x.x - mu);
+                wh[3 * s + 2] = x.y;
+            }
+            M = fmaxf(M, __shfl_sync(0xffffffffu, inc, 31));
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        const float mu = M == -INFINITY ? 0.f : M;
-        float L = 0.f;
-#pragma unroll
-        for (int i = 0; i < ATT_MAX_RANGES / 32; ++i) {
-            x[i].x = ex2(x[i].x - mu);
-            L += x[i].x * x[i].y;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        const float inv = L != 0.f ? 1.f / L : 0.f;     // (a NaN sum stays NaN; no visible position: zeros)
-#pragma unroll
-        for (int i = 0; i < ATT_MAX_RANGES / 32; ++i)
-            if (lane + 32 * i < n) w[h * n + lane + 32 * i] = x[i].x * inv;
+        __syncwarp();
+        float L = wh[2];
+#pragma unroll 8
+        for (int s = 1; s < n; ++s) L = __fmaf_rn(wh[3 * s + 2], wh[3 * s + 1], __fmul_rn(L, wh[3 * s]));
+        __syncwarp();
+        if (lane == 0) wh[3 * n] = L != 0.f ? __fdiv_rn(1.f, L) : 0.f;      // (as JoinState::out)
     }
     __syncthreads();
     for (int i = threadIdx.x; i < nh * (HD / 4); i += NT) {
         const int h = i / (HD / 4), d = i % (HD / 4) * 4;
-        const float4* pp = reinterpret_cast<const float4*>(a.part + row(h) * a.S * HD + d);
-        const float* wh = w + h * n;
+        const float4* pp = reinterpret_cast<const float4*>(part + row.at(h) * S * HD + d);
+        const float* wh = w + h * (3 * n + 1);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int s0 = 0; s0 < n; s0 += 8) {
             float4 p[8];
@@ -278,14 +321,18 @@ template <int HD, int NT, class F> __device__ __forceinline__ void join_ranges(c
             for (int k = 0; k < 8; ++k) p[k] = s0 + k < n ? __ldcg(pp + (int64_t)(s0 + k) * (HD / 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float f = s0 + k < n ? wh[s0 + k] : 0.f;
-                o.x += f * p[k].x;
-                o.y += f * p[k].y;
-                o.z += f * p[k].z;
-                o.w += f * p[k].w;
+                const int s = s0 + k;
+                if (s >= n) break;
+                const float fa = wh[3 * s], fb = wh[3 * s + 1];
+                o.x = s ? __fmaf_rn(p[k].x, fb, __fmul_rn(o.x, fa)) : p[k].x;
+                o.y = s ? __fmaf_rn(p[k].y, fb, __fmul_rn(o.y, fa)) : p[k].y;
+                o.z = s ? __fmaf_rn(p[k].z, fb, __fmul_rn(o.z, fa)) : p[k].z;
+                o.w = s ? __fmaf_rn(p[k].w, fb, __fmul_rn(o.w, fa)) : p[k].w;
             }
         }
-        *reinterpret_cast<float4*>(a.out + row(h) * HD + d) = o;
+        const float inv = wh[3 * n];
+        *reinterpret_cast<float4*>(out + row.at(h) * HD + d) =
+            make_float4(__fmul_rn(o.x, inv), __fmul_rn(o.y, inv), __fmul_rn(o.z, inv), __fmul_rn(o.w, inv));
     }
 }
 

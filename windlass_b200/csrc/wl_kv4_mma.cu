@@ -617,7 +617,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
     }
     if (a.S == 1) return;
     if (!last_ticket(a.tickets + ((int64_t)run * a.kv_heads + kvh) * q_blocks + qb, a.S)) return;
-    join_ranges<HD, PM_THREADS>(a, min(PM_Q, nq - q0), a.S, reinterpret_cast<float*>(smem), [&](int i) { return query(q0 + i); });
+    join_ranges<HD, PM_THREADS>(a.ml, a.part, a.out, a.S, min(PM_Q, nq - q0), a.S, reinterpret_cast<float*>(smem),
+                                RowMap{(int64_t)run * a.R * a.heads + kvh * G, q0, G, a.heads});
 }
 
 template <int HD> void launch_mma(const Kv4Att& a, int q_blocks, cudaStream_t s)
