@@ -533,22 +533,19 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const
         fence_mbar_init();
         for (int s = 0; s < ST && s < steps; ++s) issue(s);
     }
-    QueryTerms<NB> qt[1];
     if (warp == 0) {
         uint4 qa[NB][2];
-        load_query<HD>(g < nh ? a.q + ((int64_t)t * a.heads + head0 + g) * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa, qt[0]);
+        QueryTerms<NB> qt;
+        load_query<HD>(g < nh ? a.q + ((int64_t)t * a.heads + head0 + g) * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa, qt);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             sq[b * 64 + lane] = qa[b][0];
             sq[b * 64 + 32 + lane] = qa[b][1];
-            sqt[b * 32 + lane] = qt[0].off[b];
+            sqt[b * 32 + lane] = qt.off[b];
         }
-        sqt[NB * 32 + lane] = qt[0].ks;
+        sqt[NB * 32 + lane] = qt.ks;
     }
     __syncthreads();
-#pragma unroll
-    for (int b = 0; b < NB; ++b) qt[0].off[b] = sqt[b * 32 + lane];
-    qt[0].ks = sqt[NB * 32 + lane];
     auto qf = [&](int, int b, int s) { return sq[b * 64 + s * 32 + lane]; };
     JoinState js[IT];
     int i = 0;
@@ -564,6 +561,10 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const
             // (of an odd range's last step the second tile is not there: a position that no row sees)
             const int tile0[2] = {tl.at(x) * KV4_P, x + 1 < i1 ? tl.at(x + 1) * KV4_P : INT_MAX - KV4_P};
             const bool full = tile0[0] >= vis[0].first && tile0[1] < vis[0].n - KV4_P + 1;
+            QueryTerms<NB> qt[1];           // (from shared memory at each step: registers are short in the values' part)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) qt[0].off[b] = sqt[b * 32 + lane];
+            qt[0].ks = sqt[NB * 32 + lane];
             kv4_tiles<HD, 1, 2>(ring + i % ST * 2 * TB, lane, tile0, vis, full, qf, qt, st);
             __syncwarp();
             if (lane == 0 && i + ST < steps) issue(i + ST);
