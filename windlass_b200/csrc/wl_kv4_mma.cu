@@ -73,8 +73,19 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
                    "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
                    "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+// Waits for this thread's loads; the values of r come out of it, so that none is used before.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                   "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                   "+r"(r[28]), "+r"(r[29])
+                 :: "memory");
+    asm volatile("" : "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32])
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -85,7 +96,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
                    "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
                    "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
                  : "memory");
-    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -263,6 +273,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 tmem_st32(row + TM_QH + 32 * i, hi);
                 tmem_st32(row + TM_QL + 32 * i, lo);
             }
+            tmem_st_wait();
             tc_before();
             pm_arrive(&q_full);
         }
@@ -290,24 +301,29 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 }
                 return b;
             };
-            // a group's scores, those not seen at -inf (the loops are kept rolled: unrolled, the three roles' code outgrew
-            // the instruction caches and a step took twice as long)
-            auto scores = [&](int g, uint32_t (&r)[32]) {
-                tmem_ld32(sbuf + 32 * g, r);
+            // a group's scores: those not seen to -inf (the loops are kept rolled: unrolled, the three roles' code outgrew the
+            // instruction caches and a step took twice as long; two groups at a time, one's load behind the other's work)
+            auto mask = [&](int g, uint32_t (&r)[32]) {
                 if (!full(g)) {
                     const uint32_t b = seen32(g);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) r[i] = b >> i & 1u ? r[i] : 0xFF800000u;
                 }
             };
+            uint32_t ra[32], rb[32];
             float mx = -INFINITY;
 #pragma unroll 1
-            for (int g = 0; g < 4; ++g) {
-                uint32_t r[32];
-                scores(g, r);
+            for (int g = 0; g < 4; g += 2) {
+                tmem_ld32(sbuf + 32 * g, ra);
+                tmem_ld32(sbuf + 32 * g + 32, rb);
+                tmem_ld_wait(ra);
+                tmem_ld_wait(rb);
+                mask(g, ra);
+                mask(g + 1, rb);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
+                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(ra[i]), __uint_as_float(rb[i])));
             }
+            tmem_ld32(sbuf, ra);            // the first group again, behind the maximum's work
             mx *= ks;
             float f = 1.f;
             if (mx > m + ATT_SLACK) {
@@ -328,19 +344,31 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             const float mu = m == -INFINITY ? 0.f : m;
             const uint64_t k2 = f2(ks, ks), m2 = f2(-mu, -mu);
             uint64_t sum = f2(0.f, 0.f);
-#pragma unroll 1
-            for (int g = 0; g < 4; ++g) {
-                uint32_t r[32], o[32];
-                scores(g, r);
+            // a group's weights in place of its scores: 16 columns of their roundings, 16 of what those left
+            auto weights = [&](int g, uint32_t (&r)[32]) {
+                uint32_t lo[16];
+                mask(g, r);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float2 x = unf2(fma2(f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), k2, m2));
                     const uint64_t p = f2(ex2(x.x), ex2(x.y));
                     sum = add2(sum, p);
-                    split_h2(p, o[i], o[16 + i]);
+                    split_h2(p, r[i], lo[i]);
                 }
-                tmem_st32(sbuf + 32 * g, o);        // in place: 16 columns of P's roundings, 16 of what they left
+#pragma unroll
+                for (int i = 0; i < 16; ++i) r[16 + i] = lo[i];
+                tmem_st32(sbuf + 32 * g, r);
+            };
+#pragma unroll 1
+            for (int g = 0; g < 4; g += 2) {
+                tmem_ld_wait(ra);
+                tmem_ld32(sbuf + 32 * g + 32, rb);
+                weights(g, ra);
+                tmem_ld_wait(rb);
+                if (g == 0) tmem_ld32(sbuf + 64, ra);
+                weights(g + 1, rb);
             }
+            tmem_st_wait();
             const float2 x = unf2(sum);
             l += x.x + x.y;
             tc_before();
@@ -359,14 +387,24 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             return it < i1 && seen(tl.at(it) * KV4_P + r);
         };
         auto raw_step = [&](int j) -> const uint8_t* { return raw + j % PM_RAW * PM_TILES * TB; };
-        // step j's raw tiles are there; what its values' scales call for is known to all warps
+        // step j's raw tiles are there; what its values' scales call for is known to all warps. Each warp looks at all of them:
+        // only a scale of 2 or more (or what lies in unseen places) makes the warps meet.
+        uint32_t used = 0u;                 // care slots that are not clear (the same in all warps)
         auto survey = [&](int j) {
-            const int at = i0 + PM_TILES * j;
+            const int at = i0 + PM_TILES * j, slot = j % PM_SLOTS;
             pm_wait(&raw_full[j % PM_RAW], (uint32_t)(j / PM_RAW & 1), a.err, abort);
-            StepCare<NB>& cr = care[j % PM_SLOTS];
+            const int words = KV4_P * NB / 2;       // of two fp16 scales, of a tile
+            uint32_t any = 0u;
+            for (int t = 0; t < min(PM_TILES, i1 - at); ++t)
+                if (lane < words) any |= reinterpret_cast<const uint32_t*>(raw_step(j) + t * TB + 17 * HD)[lane];
+            if (!__any_sync(0xffffffffu, any & 0x40004000u) && !(used >> slot & 1u)) return;
+            StepCare<NB>& cr = care[slot];
+            asm volatile("bar.sync 1, 256;" ::: "memory");      // (step j - 8, whose slot this was, is behind every warp)
+            if (threadIdx.x == 32 * PM_DQ_WARP) cr.clear();
+            asm volatile("bar.sync 1, 256;" ::: "memory");
             uint32_t big = 0u, nan = 0u;
-            const int i = 2 * lane;         // two fp16 scales of tile w a lane
-            if (i < KV4_P * NB) {
+            const int i = 2 * lane;
+            if (lane < words && at + w < i1) {
                 const uint32_t x = reinterpret_cast<const uint32_t*>(raw_step(j) + w * TB + 17 * HD)[lane];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
@@ -376,19 +414,16 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                     else big = max(big, __float_as_uint(__half2float(__ushort_as_half((unsigned short)d))));
                 }
             }
-            if (__any_sync(0xffffffffu, big | nan)) {
-                if (big) atomicMax(&cr.vmax, big);
+            if (big) atomicMax(&cr.vmax, big);
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    if (nan >> e & 1u) {
-                        const int r = (i + e) / NB;
-                        cr.any_nan = 1;
-                        atomicOr(&cr.nan[(i + e) % NB][w / 2], 1u << (8 * (r % 8 / 2) + 2 * (2 * (w & 1) + r / 8) + r % 2));
-                    }
-            }
-            // (the next step's slot held step j - 3's, which every warp here has seen used: it has waited for that step's PV)
-            if (threadIdx.x == 32 * PM_DQ_WARP) care[(j + 1) % PM_SLOTS].clear();
+            for (int e = 0; e < 2; ++e)
+                if (nan >> e & 1u) {
+                    const int r = (i + e) / NB;
+                    cr.any_nan = 1;
+                    atomicOr(&cr.nan[(i + e) % NB][w / 2], 1u << (8 * (r % 8 / 2) + 2 * (2 * (w & 1) + r / 8) + r % 2));
+                }
             asm volatile("bar.sync 1, 256;" ::: "memory");
+            used = cr.vmax || cr.any_nan ? used | 1u << slot : used & ~(1u << slot);
         };
         // K' of step j: two (tile, half) units a warp, a position's 8 dims x NB a lane
         auto keys = [&](int j) {
@@ -507,6 +542,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             for (int x = 0; x < HD / 64; ++x) {
                 uint32_t r[32];
                 tmem_ld32(otm + 32 * x, r);
+                tmem_ld_wait(r);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     o[16 * x + i] = fma2(f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), u1, o[16 * x + i]);
