@@ -89,24 +89,21 @@ struct RowConst {
     {
         return (u64)__double_as_longlong(fma(p, unit, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
     }
-    // exp((x - xmax) / T) for a valid x: 2^y by table and polynomial (Tang's table-driven scheme: y = n + j/64 + r,
-    // 2^(j/64) from the table, e^(r ln 2) to the fifth power, its remainder below 2^-54)
+    // exp((x - xmax) / T), 0 for a NaN or -inf x: 2^y by table and polynomial (Tang's table-driven scheme: y = n + j/64 + r,
+    // 2^(j/64) from the table, e^(r ln 2) to the fifth power, its remainder below 2^-54). No branch, so that several run
+    // side by side.
     __device__ __forceinline__ double prob(float x, const double* exp2_table) const
     {
-        if (x == xmax) return 1.0;
         const double y = (double)__fsub_rn(x, xmax) * inv_t;
-        if (!(y > -(double)(frac + 2))) return 0.0;
+        const bool some = y > -(double)(frac + 2);
         // y 64 to the nearest integer: the low bits of a sum with 1.5 2^52
-        const double z = fma(y, 64.0, 6755399441055744.0);
+        const double yy = some ? y : 0.0, z = fma(yy, 64.0, 6755399441055744.0);
         const int i = __double2loint(z);
-        const double t = fma(z - 6755399441055744.0, -0.015625, y) * 0.6931471805599453;
-        double e = fma(t, 1.0 / 120, 1.0 / 24);
-        e = fma(t, e, 1.0 / 6);
-        e = fma(t, e, 0.5);
-        e = fma(t, e, 1.0);
-        e = fma(t, e, 1.0);
+        const double t = fma(z - 6755399441055744.0, -0.015625, yy) * 0.6931471805599453, t2 = t * t;
+        const double e = fma(t2, fma(t2, fma(t, 1.0 / 120, 1.0 / 24), fma(t, 1.0 / 6, 0.5)), 1.0 + t);
         const double m = exp2_table[i & 63] * e;
-        return __hiloint2double(__double2hiint(m) + ((i >> 6) << 20), __double2loint(m));
+        const double p = __hiloint2double(__double2hiint(m) + ((i >> 6) << 20), __double2loint(m));
+        return x == xmax ? 1.0 : some ? p : 0.0;    // (some is false for a NaN and for -inf)
     }
 };
 
@@ -169,6 +166,7 @@ __device__ __noinline__ u64 block_before(Row& s, u64 v, u64* total)
     if (lane == 31) s.scan[warp] = inc;
     __syncthreads();
     u64 b = 0, all = 0;
+#pragma unroll
     for (int w = 0; w < SR_WARPS; ++w) {
         const u64 x = s.scan[w];
         if (w < warp) b += x;
@@ -206,12 +204,14 @@ __device__ __noinline__ Joined join(Row& s, bool count)
     }
     u64 mine;
     j.before = block_before(s, j.v, &mine);
-    if (threadIdx.x == 0) s.publish(&s.part[s.rank], mine);
+    if ((int)threadIdx.x < C) *remote(&s.part[s.rank], threadIdx.x) = mine;
     cluster_sync();
     j.total = 0;
-    for (int r = 0; r < s.C; ++r) {
-        if (r < s.rank) j.before += s.part[r];
-        j.total += s.part[r];
+#pragma unroll
+    for (int r = 0; r < SR_MAX_CLUSTER; ++r) {
+        const u64 x = r < C ? s.part[r] : 0ull;
+        if (r < s.rank) j.before += x;
+        j.total += x;
     }
     return j;
 }
@@ -220,11 +220,18 @@ __device__ __noinline__ Joined join(Row& s, bool count)
 // clears the list of the gather that follows.
 __device__ __forceinline__ void find(Row& s, const Joined& j, u64 target, u64 base, int which = 0)
 {
+    // (the lanes of the warp that has it write one CTA each)
     const u64 b = base + j.before, e = b + j.v;
-    if (b < target && e >= target) {
-        s.publish(&s.cut[which].bin, s.rank * (s.bins / s.C) + (int)threadIdx.x);
-        s.publish(&s.cut[which].before, b);
-        s.publish(&s.cut[which].sum, j.v);
+    const uint32_t who = __ballot_sync(0xffffffffu, b < target && e >= target);
+    if (who) {
+        const int src = __ffs(who) - 1, lane = threadIdx.x & 31;
+        const u64 cb = __shfl_sync(0xffffffffu, b, src), cv = __shfl_sync(0xffffffffu, j.v, src);
+        if (lane < s.C) {
+            Row::Cut* cut = remote(&s.cut[which], lane);
+            cut->bin = s.rank * (s.bins / s.C) + (int)threadIdx.x - lane + src;
+            cut->before = cb;
+            cut->sum = cv;
+        }
     }
     if (s.rank == 0 && threadIdx.x == 0) {
         s.n_cand = 0;
@@ -234,23 +241,22 @@ __device__ __forceinline__ void find(Row& s, const Joined& j, u64 target, u64 ba
     cluster_sync();
 }
 
-// f(i, x) for this CTA's logits (xs is 16-byte aligned where it is shared memory; a slice is a multiple of 4 long but the last).
-template <typename F> __device__ __forceinline__ void each_logit(const Row& s, const F& f)
+// f(i, x) for this CTA's logits, four (i .. i + 3, -inf past the end) at a time.
+template <typename F> __device__ __forceinline__ void each_four(const Row& s, const F& f)
 {
     const float* xs = s.xs;
     const int n = s.n;
-    int done = 0;
-    if (((uintptr_t)xs & 15) == 0) {
-        for (int i = threadIdx.x; i < n / 4; i += SR_THREADS) {
-            const float4 v = reinterpret_cast<const float4*>(xs)[i];
-            f(4 * i, v.x);
-            f(4 * i + 1, v.y);
-            f(4 * i + 2, v.z);
-            f(4 * i + 3, v.w);
+    const bool aligned = ((uintptr_t)xs & 15) == 0;
+    for (int i = 4 * threadIdx.x; i < n; i += 4 * SR_THREADS) {
+        float x[4];
+        if (aligned && i + 4 <= n) {
+            *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(xs + i);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = i + k < n ? xs[i + k] : -INFINITY;
         }
-        done = n & ~3;
+        f(i, x);
     }
-    for (int i = done + threadIdx.x; i < n; i += SR_THREADS) f(i, xs[i]);
 }
 
 // f(key, id, mass or 1) for this CTA's ids whose logit pre takes, that in(key, id) takes, that the top-k cut keeps and that
@@ -259,12 +265,21 @@ template <typename Pre, typename In, typename F>
 __device__ __forceinline__ void each(const Row& s, const RowConst& c, bool count, const Pre& pre, const In& in, const F& f)
 {
     const int id0 = s.id0;
-    each_logit(s, [&](int i, float x) {
-        if (!pre(x) || !valid(x)) return;
-        const uint32_t key = order_key(x), id = (uint32_t)(id0 + i);
-        if (!in(key, id) || !c.kept(key, id)) return;
-        const u64 m = count ? 1ull : c.mass(c.prob(x, s.exp2_table));
-        if (m) f(key, id, m);
+    each_four(s, [&](int i, const float (&x)[4]) {
+        bool take[4], any = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            take[k] = pre(x[k]) && valid(x[k]);
+            any |= take[k];
+        }
+        if (!any) return;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t key = order_key(x[k]), id = (uint32_t)(id0 + i + k);
+            if (!take[k] || !in(key, id) || !c.kept(key, id)) continue;
+            const u64 m = count ? 1ull : c.mass(c.prob(x[k], s.exp2_table));
+            if (m) f(key, id, m);
+        }
     });
 }
 
@@ -596,8 +611,12 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
     if (with_k) {
         clear_hist(s);
         const RowConst c = s.c;
-        each_logit(s, [&](int, float v) {
-            if (valid(v)) s.add(c.bin0(v), 0, true);
+        each_four(s, [&](int, const float (&v)[4]) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int b = c.bin0(v[k]);
+                if (valid(v[k])) s.add(b, 0, true);
+            }
         });
         j = join(s, true);
         const int k = (int)min(j.total, (u64)o.top_k);
@@ -628,12 +647,10 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
         const RowConst c = s.c;
         const float* xs = s.xs;
         u64 sum = 0, mine;
-        for (int i = i0; i < i1; ++i) {
-            const float v = xs[i];
-            if (valid(v)) sum += c.mass(c.prob(v, s.exp2_table));
-        }
+#pragma unroll 4
+        for (int i = i0; i < i1; ++i) sum += c.mass(c.prob(xs[i], s.exp2_table));
         u64 before = block_before(s, sum, &mine);
-        if (tid == 0) s.publish(&s.part[rank], mine);
+        if (tid < C) *remote(&s.part[rank], tid) = mine;
         cluster_sync();
         u64 total = 0;
         for (int r = 0; r < C; ++r) {
@@ -643,8 +660,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
         const u64 target = share_of(o.draw, total);
         if (before < target && before + sum >= target) {
             for (int i = i0; i < i1; ++i) {
-                const float v = xs[i];
-                if (valid(v)) before += c.mass(c.prob(v, s.exp2_table));
+                before += c.mass(c.prob(xs[i], s.exp2_table));
                 if (before >= target) {
                     ids[row] = id0 + i;
                     break;
@@ -659,18 +675,25 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
     const RowConst c = s.c;
     u64 over = 0;                           // the sum of the kept ids with p >= min_p
     const double min_p = o.min_p;
-    each_logit(s, [&](int i, float v) {
-        if (!valid(v) || (c.has_k && !c.kept(order_key(v), (uint32_t)(id0 + i)))) return;
-        const double p = c.prob(v, s.exp2_table);
-        const u64 m = c.mass(p);
-        if (!m) return;
-        s.add(c.bin0(v), m, false);
-        if (p >= min_p) over += m;
+    each_four(s, [&](int i, const float (&v)[4]) {
+        double p[4];
+        u64 m[4];
+        int b[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            p[k] = c.prob(v[k], s.exp2_table);
+            b[k] = c.bin0(v[k]);
+            m[k] = c.has_k && !c.kept(order_key(v[k]), (uint32_t)(id0 + i + k)) ? 0ull : c.mass(p[k]);
+            over += p[k] >= min_p ? m[k] : 0ull;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (m[k]) s.add(b[k], m[k], false);
     });
     if (o.min_p > 0.0) {
         u64 mine;
         block_before(s, over, &mine);
-        if (tid == 0) s.publish(&s.min_part[rank], mine);
+        if (tid < C) *remote(&s.min_part[rank], tid) = mine;
     }
     j = join(s, false);
     over = ~0ull;
@@ -690,7 +713,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const float* logi
         s_hi = nbefore + s.cut[0].sum;
     }
     const u64 t_lo = share_of(o.draw, max(1ull, min(s_lo, over))), t_hi = share_of(o.draw, max(1ull, min(s_hi, over)));
-    if (j.before < t_hi && j.before + j.v >= t_hi) s.publish(&s.cut[1].bin_hi, rank * (s.bins / C) + tid);
+    const uint32_t hi_in = __ballot_sync(0xffffffffu, j.before < t_hi && j.before + j.v >= t_hi);
+    if (hi_in && (tid & 31) < C) remote(&s.cut[1], tid & 31)->bin_hi = rank * (s.bins / C) + (tid & ~31) + __ffs(hi_in) - 1;
     find(s, j, t_lo, 0, 1);
     const int p_lo = s.cut[1].bin, p_hi = s.cut[1].bin_hi;
     const u64 pbefore = s.cut[1].before;
