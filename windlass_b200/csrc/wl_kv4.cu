@@ -784,7 +784,7 @@ constexpr int MMA_MIN_QUERIES = 96;
 
 // How a call is cut.
 struct Kv4Plan {
-    bool runs, mma;         // the rows' runs share their cache's tiles: on the tensor cores (k_kv4_attn_mma) or k_kv4_attn_run
+    bool runs, mma, pairs;  // the rows' runs share their cache's tiles: on the tensor cores (k_kv4_attn_mma) or k_kv4_attn_run
     int S, s_max, alone, q_blocks, MT, MG;
     int64_t part_floats;
 };
@@ -801,6 +801,8 @@ Kv4Plan kv4_plan(int T, int R, int heads, int kv_heads, int head_dim, int64_t ca
     p.MT = head_dim <= 128 ? 2 : 1;
     const int QB = p.mma ? 128 : RUN_WARPS * 8 * p.MT;
     p.q_blocks = (int)(((int64_t)R * G + QB - 1) / QB);
+    p.pairs = p.mma && p.q_blocks > 1;
+    if (p.pairs) p.q_blocks += p.q_blocks & 1;
     int64_t ctas;
     if (p.runs) {
         // as many ranges as end soonest: waves of CTAs over the SMs (two an SM, with CTAs of four warps), each of a range's
@@ -960,7 +962,7 @@ void kv4_attention(const float* q, int T, int R, int heads, int kv_heads, int he
         a.part = (float*)((uint8_t*)ws + KV4_TICKETS * 4);
         a.ml = a.part + (int64_t)T * heads * p.S * head_dim;
         a.err = err;
-        if (p.mma) kv4_attention_mma(a, head_dim, p.q_blocks, s);
+        if (p.mma) kv4_attention_mma(a, head_dim, p.q_blocks, p.pairs, s);
         else switch (head_dim) {
         case 64: p.runs ? attn_runs<64>(a, p, s) : attn_rows<64>(a, p, s); break;
         case 96: p.runs ? attn_runs<96>(a, p, s) : attn_rows<96>(a, p, s); break;

@@ -41,8 +41,9 @@ struct Kv4Att {
     int* err;
 };
 
-// wl_kv4_mma.cu's kernel (head_dim 64 and 128): q_blocks CTAs of 128 queries a run and KV head, a.S ranges each.
-void kv4_attention_mma(const Kv4Att& a, int head_dim, int q_blocks, cudaStream_t s);
+// wl_kv4_mma.cu's kernel (head_dim 64 and 128): q_blocks CTAs of 128 queries a run and KV head (an even number of pairs'), a.S
+// ranges each.
+void kv4_attention_mma(const Kv4Att& a, int head_dim, int q_blocks, bool pairs, cudaStream_t s);
 
 namespace {
 

@@ -38,15 +38,23 @@ constexpr int PM_SLOTS = 8;                 // steps whose care and factors are 
 constexpr int TM_S = 0, TM_O = 256, TM_QH = 384, TM_QL = 448;
 
 constexpr int pm_plane(int HD) { return HD * 256; }             // one fp16 plane of a step: 128 x HD
-constexpr int pm_smem(int HD) { return 4 * pm_plane(HD) + PM_RAW * PM_TILES * kv4_tile_bytes(HD) + 1024; }
+constexpr int pm_smem(int HD, int NC) { return 4 * pm_plane(HD) / NC + PM_RAW * PM_TILES * kv4_tile_bytes(HD) + 1024; }
 
+// (acquires from the whole cluster: the other CTA of a pair arrives too)
+__device__ __forceinline__ bool pm_try_wait(uint64_t* bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok;
+}
 // A wait bounded by time (2 s); after one gives up, all of the CTA's waits return at once.
 __device__ __forceinline__ bool pm_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort)
 {
     if (*abort) return false;
-    if (mbar_try_wait(bar, parity)) return true;
+    if (pm_try_wait(bar, parity)) return true;
     const unsigned long long t0 = globaltimer_ns();
-    while (!mbar_try_wait(bar, parity)) {
+    while (!pm_try_wait(bar, parity)) {
         if (*abort) return false;
         if (globaltimer_ns() - t0 > MBAR_WAIT_NS) {
             atomicExch(err, 24);
@@ -60,6 +68,23 @@ __device__ __forceinline__ void pm_arrive(uint64_t* bar)
 {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// The same at the barrier of the CTA that issues the MMAs.
+template <int NC> __device__ __forceinline__ void pm_arrive_lead(uint64_t* bar)
+{
+    if constexpr (NC == 1) {
+        pm_arrive(bar);
+    } else {
+        asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}\n"
+                     ::"r"(smem_u32(bar)) : "memory");
+    }
+}
+template <int NC> __device__ __forceinline__ void pm_sync()     // all threads of the CTA or pair
+{
+    if constexpr (NC == 1) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// (all address spaces: the pair's MMA reads both CTAs' shared memory)
+__device__ __forceinline__ void pm_fence_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
@@ -107,18 +132,28 @@ __device__ __forceinline__ uint64_t pm_desc(const void* p)
     const uint64_t addr = smem_u32(p);
     return ((addr & 0x3FFFFull) >> 4) | (1ull << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// kind::f16 with fp16 operands, fp32 sums, M = 128.
-constexpr uint32_t pm_idesc(int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
+// kind::f16 with fp16 operands, fp32 sums, M = 128 queries a CTA.
+constexpr uint32_t pm_idesc(int N, int NC) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 * NC >> 4) << 24); }
 
-__device__ __forceinline__ void pm_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+template <int NC> __device__ __forceinline__ void pm_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
 {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    if constexpr (NC == 1)
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                     " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+                     ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                     " tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+                     ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void pm_commit(uint64_t* bar)
+// Arrives at the barrier (of both CTAs of a pair) when the MMAs before it are done.
+template <int NC> __device__ __forceinline__ void pm_commit(uint64_t* bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    if constexpr (NC == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
 }
 
 // Bits [0, 16) of the positions p0 .. p0 + 15 that v sees.
@@ -154,10 +189,11 @@ template <int NB> struct StepCare {
     }
 };
 
-template <int HD>
+template <int HD, int NC>
 __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, int q_blocks)
 {
-    constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD), PL = pm_plane(HD);
+    constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD), PL = pm_plane(HD) / NC;
+    constexpr int KP = PM_P / NC, VD = HD / NC;             // rows of K' (positions) and V' (dims) that this CTA makes
     static_assert(HD == 64 || HD == 128, "planes of whole 64-value swizzle atoms");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -173,7 +209,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.heads / a.kv_heads, kvh = blockIdx.y;
     // the last queries (of a prompt: those that see most) first
-    const int qb = q_blocks - 1 - (int)blockIdx.x / a.S, sp = blockIdx.x % a.S, run = blockIdx.z;
+    const int cta = NC == 1 ? 0 : (int)blockIdx.x % NC, group = (int)blockIdx.x / NC;
+    const int qg = q_blocks / NC - 1 - group / a.S, sp = group % a.S, qb = qg * NC + cta, run = blockIdx.z;
     const int nq = a.R * G, q0 = qb * PM_Q;
     const uint8_t* base = a.rows.base(run * a.R);
     if (threadIdx.x == 0) {
@@ -181,15 +218,15 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             mbar_init(&raw_full[s], 1);
             mbar_init(&raw_empty[s], PM_DQ);
         }
-        mbar_init(&q_full, 128);
-        mbar_init(&k_full, PM_DQ);
-        mbar_init(&v_full, PM_DQ);
-        mbar_init(&o_free, PM_DQ);
+        mbar_init(&q_full, 4 * NC);
+        mbar_init(&k_full, PM_DQ * NC);
+        mbar_init(&v_full, PM_DQ * NC);
+        mbar_init(&o_free, PM_DQ * NC);
         mbar_init(&qk_done, 1);
         mbar_init(&pv_done, 1);
         for (int s = 0; s < 2; ++s) {
             mbar_init(&s_full[s], 1);
-            mbar_init(&p_full[s], 128);
+            mbar_init(&p_full[s], 4 * NC);
         }
         abort_flag = 0;
         rng[0] = 0;
@@ -199,13 +236,18 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         fence_mbar_init();
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (NC == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
     }
     __syncthreads();
     {
-        // the positions that the CTA's rows see together
-        const int r0 = q0 / G, r1 = min(a.R - 1, (min(q0 + PM_Q, nq) - 1) / G);
+        // the positions that the CTA's (both CTAs') rows see together
+        const int p0 = qg * NC * PM_Q, r0 = p0 / G, r1 = min(a.R - 1, (min(p0 + NC * PM_Q, nq) - 1) / G);
         for (int r = r0 + threadIdx.x; r <= r1; r += PM_THREADS) {
             const int p = a.pos[run * a.R + r];
             if (kv4_row_state(base, p, a.capacity)) continue;
@@ -216,7 +258,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         }
     }
     tc_before();
-    __syncthreads();
+    pm_sync<NC>();
     tc_after();
     const uint32_t tmem = tmem_base;
     const Vis seen{rng[0], rng[1], rng[2]};
@@ -275,7 +317,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             }
             tmem_st_wait();
             tc_before();
-            pm_arrive(&q_full);
+            __syncwarp();
+            if (lane == 0) pm_arrive_lead<NC>(&q_full);
         }
         // (queries that see nothing, or are none, need no mask: their output is not read)
         const int w_min_n = __reduce_min_sync(0xffffffffu, vis.n > 0 ? vis.n : INT_MAX), w_max_first = __reduce_max_sync(0xffffffffu, vis.first);
@@ -372,7 +415,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             const float2 x = unf2(sum);
             l += x.x + x.y;
             tc_before();
-            pm_arrive(&p_full[j & 1]);
+            __syncwarp();
+            if (lane == 0) pm_arrive_lead<NC>(&p_full[j & 1]);
         }
         if (state) l = state == 2 ? NAN : 0.f;
         fin_l[threadIdx.x] = l;
@@ -425,12 +469,13 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             asm volatile("bar.sync 1, 256;" ::: "memory");
             used = cr.vmax || cr.any_nan ? used | 1u << slot : used & ~(1u << slot);
         };
-        // K' of step j: two (tile, half) units a warp, a position's 8 dims x NB a lane
+        // K' of step j (a CTA of a pair: its half of the positions): (tile, half) units, a position's 8 dims x NB a lane
         auto keys = [&](int j) {
-            const uint8_t* tp = raw_step(j) + w * TB;
             const __half2 k2 = __float2half2_rn(0.125f);
 #pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
+            for (int u = 0; u < 2 / NC; ++u) {
+                const int tile = NC == 1 ? w : 4 * cta + w / 2, h = NC == 1 ? u : w & 1;
+                const uint8_t* tp = raw_step(j) + tile * TB;
                 uint32_t kw[NB], sw[NB / 2];
                 lane_words<HD>(tp, h, lane, kw);
                 const uint8_t* sc = tp + 16 * HD + (8 * h + g) * NB * 2;
@@ -441,11 +486,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 } else {
                     sw[0] = *reinterpret_cast<const uint32_t*>(sc);
                 }
-                if (!live(i0 + PM_TILES * j + w, 8 * h + g)) {
+                if (!live(i0 + PM_TILES * j + tile, 8 * h + g)) {
 #pragma unroll
                     for (int i = 0; i < NB / 2; ++i) sw[i] = 0u;
                 }
-                const int n = w / 2 * 32 + g / 2 * 8 + (2 * (w & 1) + h) * 2 + (g & 1);
+                const int n = tile / 2 * 32 - KP * cta + g / 2 * 8 + (2 * (tile & 1) + h) * 2 + (g & 1);
                 const int off = n / 8 * 1024 + n % 8 * 128;
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
@@ -464,17 +509,19 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                         lo[x] = h2_bits(__hfma2(bits_h2(r[x]), d, __hneg2(y)));
                     }
                     const int ch = 4 * b + c;
-                    uint8_t* dst = kh + ch / 8 * (PM_P * 128) + off + ((ch % 8) ^ (n % 8)) * 16;
+                    uint8_t* dst = kh + ch / 8 * (KP * 128) + off + ((ch % 8) ^ (n % 8)) * 16;
                     *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     *reinterpret_cast<uint4*>(dst + PL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             }
-            fence_proxy_async();
+            pm_fence_async();
             __syncwarp();
-            if (lane == 0) pm_arrive(&k_full);
+            if (lane == 0) pm_arrive_lead<NC>(&k_full);
         };
-        // V' of step j: 32 positions (two tiles) and half the blocks a warp; a lane 8 positions of 4 dims a block
+        // V' of step j (a CTA of a pair: its half of the dims): 32 positions (two tiles) and half the blocks, or half of the one
+        // block, a warp; a lane 8 positions of 4 dims a block
         auto values = [&](int j) {
+            constexpr int VB = NB / NC;
             const uint8_t* rs = raw_step(j);
             const StepCare<NB>& cr = care[j % PM_SLOTS];
             const __half2 vs2 = __float2half2_rn(cr.vs());
@@ -487,7 +534,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 keep[k] = (live(it, r) ? 0xFFFFu : 0u) | (live(it, r + 1) ? 0xFFFF0000u : 0u);
             }
 #pragma unroll 1
-            for (int b = (w & 1) * (NB / 2), e = b + NB / 2; b < e; ++b) {
+            for (int vb = VB > 1 ? (w & 1) * (VB / 2) : 0, e = vb + (VB > 1 ? VB / 2 : 1); vb < e; ++vb) {
+                const int b = VB * cta + vb;
                 uint32_t r[4][4], dv[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -503,6 +551,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 }
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
+                    if (VB == 1 && x / 2 != (w & 1)) continue;
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -510,16 +559,16 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                         hi[k] = h2_bits(y);
                         lo[k] = h2_bits(__hfma2(bits_h2(r[k][x]), d, __hneg2(y)));
                     }
-                    const int dim = 32 * b + 4 * g + x;
-                    uint8_t* dst = vh + grp / 2 * (HD * 128) + dim / 8 * 1024 + dim % 8 * 128 + (ch ^ (dim % 8)) * 16;
+                    const int dim = 32 * vb + 4 * g + x;
+                    uint8_t* dst = vh + grp / 2 * (VD * 128) + dim / 8 * 1024 + dim % 8 * 128 + (ch ^ (dim % 8)) * 16;
                     *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     *reinterpret_cast<uint4*>(dst + PL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             }
-            fence_proxy_async();
+            pm_fence_async();
             __syncwarp();
             if (lane == 0) {
-                pm_arrive(&v_full);
+                pm_arrive_lead<NC>(&v_full);
                 pm_arrive(&raw_empty[j % PM_RAW]);
             }
         };
@@ -549,7 +598,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             }
             tc_before();
             __syncwarp();
-            if (lane == 0) pm_arrive(&o_free);
+            if (lane == 0) pm_arrive_lead<NC>(&o_free);
         };
         if (steps > 0) {
             survey(0);
@@ -582,8 +631,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         }
     } else {
         regs_dec<24>();
-        if (warp == PM_MMA_WARP && lane == 0 && steps > 0) {
-            // ---- one thread issues the MMAs. The products with remainders come first: sums are cut off at their size.
+        if (warp == PM_MMA_WARP && cta == 0 && lane == 0 && steps > 0) {
+            // ---- one thread (of a pair: for both) issues the MMAs. The products with remainders come first: sums are cut off at their size.
             auto pv = [&](int j) {
                 pm_wait(&p_full[j & 1], (uint32_t)(j / 2 & 1), a.err, abort);
                 pm_wait(&v_full, (uint32_t)(j & 1), a.err, abort);
@@ -592,19 +641,19 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 const uint32_t p = tmem + TM_S + (j & 1) * 128;
                 uint64_t v = pm_desc(vh);           // (16-byte units: 2 a step of 16 positions, an atom's HD rows of 128 bytes a step of 64)
 #pragma unroll 1
-                for (int s = 0; s < PM_P / 64; ++s, v += HD * 8)
+                for (int s = 0; s < PM_P / 64; ++s, v += VD * 8)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         const uint32_t ph = p + 64 * s + x / 2 * 32 + x % 2 * 8;
-                        pm_mma(tmem + TM_O, ph, v + 2 * x + (PL >> 4), pm_idesc(HD), s > 0 || x > 0);
-                        pm_mma(tmem + TM_O, ph + 16, v + 2 * x, pm_idesc(HD), 1u);
+                        pm_mma<NC>(tmem + TM_O, ph, v + 2 * x + (PL >> 4), pm_idesc(HD, NC), s > 0 || x > 0);
+                        pm_mma<NC>(tmem + TM_O, ph + 16, v + 2 * x, pm_idesc(HD, NC), 1u);
                     }
                 v = pm_desc(vh);
 #pragma unroll 1
-                for (int s = 0; s < PM_P / 64; ++s, v += HD * 8)
+                for (int s = 0; s < PM_P / 64; ++s, v += VD * 8)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) pm_mma(tmem + TM_O, p + 64 * s + x / 2 * 32 + x % 2 * 8, v + 2 * x, pm_idesc(HD), 1u);
-                pm_commit(&pv_done);
+                    for (int x = 0; x < 4; ++x) pm_mma<NC>(tmem + TM_O, p + 64 * s + x / 2 * 32 + x % 2 * 8, v + 2 * x, pm_idesc(HD, NC), 1u);
+                pm_commit<NC>(&pv_done);
             };
             pm_wait(&q_full, 0u, a.err, abort);
             for (int j = 0; j < steps; ++j) {
@@ -614,19 +663,19 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 const uint32_t d = tmem + TM_S + (j & 1) * 128;
                 uint64_t k = pm_desc(kh);
 #pragma unroll 1
-                for (int s = 0; s < HD / 64; ++s, k += PM_P * 8)
+                for (int s = 0; s < HD / 64; ++s, k += KP * 8)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        pm_mma(d, tmem + TM_QH + 32 * s + 8 * x, k + 2 * x + (PL >> 4), pm_idesc(PM_P), s > 0 || x > 0);
-                        pm_mma(d, tmem + TM_QL + 32 * s + 8 * x, k + 2 * x, pm_idesc(PM_P), 1u);
+                        pm_mma<NC>(d, tmem + TM_QH + 32 * s + 8 * x, k + 2 * x + (PL >> 4), pm_idesc(PM_P, NC), s > 0 || x > 0);
+                        pm_mma<NC>(d, tmem + TM_QL + 32 * s + 8 * x, k + 2 * x, pm_idesc(PM_P, NC), 1u);
                     }
                 k = pm_desc(kh);
 #pragma unroll 1
-                for (int s = 0; s < HD / 64; ++s, k += PM_P * 8)
+                for (int s = 0; s < HD / 64; ++s, k += KP * 8)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) pm_mma(d, tmem + TM_QH + 32 * s + 8 * x, k + 2 * x, pm_idesc(PM_P), 1u);
-                pm_commit(&s_full[j & 1]);
-                pm_commit(&qk_done);
+                    for (int x = 0; x < 4; ++x) pm_mma<NC>(d, tmem + TM_QH + 32 * s + 8 * x, k + 2 * x, pm_idesc(PM_P, NC), 1u);
+                pm_commit<NC>(&s_full[j & 1]);
+                pm_commit<NC>(&qk_done);
                 if (j > 0) pv(j - 1);
             }
             pv(steps - 1);
@@ -646,31 +695,46 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         }
     }
     tc_before();
-    __syncthreads();
+    __syncwarp();
+    pm_sync<NC>();                          // (nothing arrives at a pair's other CTA, and no MMA uses it, after this)
     if (warp == 0) {
         tc_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        if constexpr (NC == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
-    if (a.S == 1) return;
+    if (a.S == 1 || q0 >= nq) return;
     if (!last_ticket(a.tickets + ((int64_t)run * a.kv_heads + kvh) * q_blocks + qb, a.S)) return;
     join_ranges<HD, PM_THREADS>(a.ml, a.part, a.out, a.S, min(PM_Q, nq - q0), a.S, reinterpret_cast<float*>(smem),
                                 RowMap{(int64_t)run * a.R * a.heads + kvh * G, q0, G, a.heads});
 }
 
-template <int HD> void launch_mma(const Kv4Att& a, int q_blocks, cudaStream_t s)
+template <int HD, int NC> void launch_mma(const Kv4Att& a, int q_blocks, cudaStream_t s)
 {
-    WL_CUDA(cudaFuncSetAttribute(k_kv4_attn_mma<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, pm_smem(HD)));
+    auto kern = k_kv4_attn_mma<HD, NC>;
+    constexpr int smem = pm_smem(HD, NC);
+    WL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     // (launched plainly: it takes all of an SM's tensor memory, so it does not start beside another kernel's end)
-    k_kv4_attn_mma<HD><<<dim3(q_blocks * a.S, a.kv_heads, a.T / a.R), PM_THREADS, pm_smem(HD), s>>>(a, q_blocks);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(q_blocks * a.S, a.kv_heads, a.T / a.R);
+    cfg.blockDim = dim3(PM_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = NC;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    WL_CUDA(cudaLaunchKernelEx(&cfg, kern, a, q_blocks));
     note_launch();
 }
 
 }  // namespace
 
-void kv4_attention_mma(const Kv4Att& a, int head_dim, int q_blocks, cudaStream_t s)
+void kv4_attention_mma(const Kv4Att& a, int head_dim, int q_blocks, bool pairs, cudaStream_t s)
 {
-    if (head_dim == 64) launch_mma<64>(a, q_blocks, s);
-    else launch_mma<128>(a, q_blocks, s);
+    if (head_dim == 64) pairs ? launch_mma<64, 2>(a, q_blocks, s) : launch_mma<64, 1>(a, q_blocks, s);
+    else pairs ? launch_mma<128, 2>(a, q_blocks, s) : launch_mma<128, 1>(a, q_blocks, s);
 }
 
 }  // namespace k
