@@ -38,7 +38,10 @@ constexpr int PM_SLOTS = 8;                 // steps whose care and factors are 
 constexpr int TM_S = 0, TM_O = 256, TM_QH = 384, TM_QL = 448;
 
 constexpr int pm_plane(int HD) { return HD * 256; }             // one fp16 plane of a step: 128 x HD
-constexpr int pm_smem(int HD, int NC) { return 4 * pm_plane(HD) / NC + PM_RAW * PM_TILES * kv4_tile_bytes(HD) + 1024; }
+constexpr int pm_q_row(int HD) { return HD * 4 + 16; }          // a staged query's bytes (16 more: no bank conflicts)
+constexpr int pm_o_row(int HD) { return HD * 2 + 16; }          // half a staged output row's
+constexpr int pm_v_bufs(int NC) { return NC; }                  // steps of V' in shared memory: a pair's CTA has room for two
+constexpr int pm_smem(int HD, int NC) { return (2 + 2 * pm_v_bufs(NC)) * pm_plane(HD) / NC + PM_RAW * PM_TILES * kv4_tile_bytes(HD) + 1024; }
 
 // (acquires from the whole cluster: the other CTA of a pair arrives too)
 __device__ __forceinline__ bool pm_try_wait(uint64_t* bar, uint32_t parity)
@@ -68,23 +71,23 @@ __device__ __forceinline__ void pm_arrive(uint64_t* bar)
 {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// The same at the barrier of the CTA that issues the MMAs.
-template <int NC> __device__ __forceinline__ void pm_arrive_lead(uint64_t* bar)
+// The same at the barrier of a pair's first CTA, which issues the MMAs.
+__device__ __forceinline__ void pm_arrive_lead(uint64_t* bar)
 {
-    if constexpr (NC == 1) {
-        pm_arrive(bar);
-    } else {
-        asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}\n"
-                     ::"r"(smem_u32(bar)) : "memory");
-    }
+    asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}\n"
+                 ::"r"(smem_u32(bar)) : "memory");
 }
-template <int NC> __device__ __forceinline__ void pm_sync()     // all threads of the CTA or pair
+// All threads of a pair meet.
+template <int NC> __device__ __forceinline__ void pm_pair_arrive()
 {
-    if constexpr (NC == 1) __syncthreads();
-    else asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if constexpr (NC == 2) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
-// (all address spaces: the pair's MMA reads both CTAs' shared memory)
-__device__ __forceinline__ void pm_fence_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
+template <int NC> __device__ __forceinline__ void pm_pair_wait()
+{
+    if constexpr (NC == 2) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// (a pair's MMA reads both CTAs' shared memory)
+__device__ __forceinline__ void pm_fence_async() { asm volatile("fence.proxy.async.shared::cluster;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
@@ -193,12 +196,16 @@ template <int HD, int NC>
 __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, int q_blocks)
 {
     constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD), PL = pm_plane(HD) / NC;
-    constexpr int KP = PM_P / NC, VD = HD / NC;             // rows of K' (positions) and V' (dims) that this CTA makes
+    constexpr int NV = pm_v_bufs(NC), KP = PM_P / NC, VD = HD / NC;             // rows of K' (positions) and V' (dims) that this CTA makes
     static_assert(HD == 64 || HD == 128, "planes of whole 64-value swizzle atoms");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint8_t *kh = smem, *vh = smem + 2 * PL, *raw = smem + 4 * PL;      // (each plane's remainder PL behind it)
-    __shared__ __align__(8) uint64_t raw_full[PM_RAW], raw_empty[PM_RAW], q_full, k_full, qk_done, v_full, pv_done, o_free, s_full[2],
+    uint8_t *kh = smem, *raw = smem + 2 * PL, *vh = raw + PM_RAW * PM_TILES * TB;      // (each plane's remainder PL behind it)
+    // the queries before the first V' and the raw steps 2 and 3; the output after the last raw step
+    uint8_t *qs = raw + 2 * PM_TILES * TB, *os = raw;
+    static_assert(PM_RAW == 4 && PM_Q * pm_q_row(HD) <= 2 * PM_TILES * TB + 2 * PL, "the queries end before V' does");
+    static_assert(PM_DQ * 32 * pm_o_row(HD) <= PM_RAW * PM_TILES * TB && PM_RAW * PM_TILES * TB % 1024 == 0, "the output fits; V' is aligned");
+    __shared__ __align__(8) uint64_t raw_full[PM_RAW], raw_empty[PM_RAW], q_raw, q_read, q_full, k_full, qk_done, v_full[NV], pv_done, o_free, s_full[2],
         p_full[2];
     __shared__ StepCare<NB> care[PM_SLOTS];
     __shared__ float factor[PM_SLOTS][PM_Q];        // e^(old - new reference maximum) of a step and query
@@ -212,29 +219,36 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
     const int cta = NC == 1 ? 0 : (int)blockIdx.x % NC, group = (int)blockIdx.x / NC;
     const int qg = q_blocks / NC - 1 - group / a.S, sp = group % a.S, qb = qg * NC + cta, run = blockIdx.z;
     const int nq = a.R * G, q0 = qb * PM_Q;
+    // the rows that the CTA (both CTAs) takes; their positions and cache are on their way while the rest is set up
+    const int p0 = qg * NC * PM_Q, r0 = p0 / G, r1 = min(a.R - 1, (min(p0 + NC * PM_Q, nq) - 1) / G);
+    const int pos0 = r0 + (int)threadIdx.x <= r1 ? a.pos[run * a.R + r0 + threadIdx.x] : -1;
     const uint8_t* base = a.rows.base(run * a.R);
     if (threadIdx.x == 0) {
         for (int s = 0; s < PM_RAW; ++s) {
             mbar_init(&raw_full[s], 1);
             mbar_init(&raw_empty[s], PM_DQ);
         }
-        mbar_init(&q_full, 4 * NC);
-        mbar_init(&k_full, PM_DQ * NC);
-        mbar_init(&v_full, PM_DQ * NC);
-        mbar_init(&o_free, PM_DQ * NC);
+        // the first CTA of a pair counts the other's warps as one: that CTA's forwarding thread
+        const int more = NC == 2 && cta == 0;
+        mbar_init(&q_raw, 4);
+        mbar_init(&q_read, 4);
+        mbar_init(&q_full, 4 + more);
+        mbar_init(&k_full, PM_DQ + more);
+        for (int s = 0; s < NV; ++s) mbar_init(&v_full[s], PM_DQ + more);
+        mbar_init(&o_free, PM_DQ + more);
         mbar_init(&qk_done, 1);
         mbar_init(&pv_done, 1);
         for (int s = 0; s < 2; ++s) {
             mbar_init(&s_full[s], 1);
-            mbar_init(&p_full[s], 4 * NC);
+            mbar_init(&p_full[s], 4 + more);
         }
         abort_flag = 0;
         rng[0] = 0;
         rng[1] = INT_MAX;
         rng[2] = 0;
-        for (int i = 0; i < PM_SLOTS; ++i) care[i].clear();
         fence_mbar_init();
     }
+    if (warp == 1 && lane < PM_SLOTS) care[lane].clear();
     if (warp == 0) {
         if constexpr (NC == 1) {
             asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(512) : "memory");
@@ -245,29 +259,40 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         }
     }
     __syncthreads();
-    {
-        // the positions that the CTA's (both CTAs') rows see together
-        const int p0 = qg * NC * PM_Q, r0 = p0 / G, r1 = min(a.R - 1, (min(p0 + NC * PM_Q, nq) - 1) / G);
-        for (int r = r0 + threadIdx.x; r <= r1; r += PM_THREADS) {
-            const int p = a.pos[run * a.R + r];
-            if (kv4_row_state(base, p, a.capacity)) continue;
-            const Vis v = visible(p, a.window, a.sinks);
-            atomicMax(&rng[0], v.n);
-            atomicMin(&rng[1], v.first);
-            atomicMax(&rng[2], v.sink);
-        }
+    pm_pair_arrive<NC>();                   // (this CTA's barriers are there)
+    // a query's index in the call's queries, or -1 past the run
+    auto query = [&](int qi) -> int64_t { return qi < nq ? (int64_t)(run * a.R + qi / G) * a.heads + kvh * G + qi % G : -1; };
+    if (warp < 4) {
+        // the queries, rows of HD floats far from one another, by bulk copies
+        const int64_t th = query(q0 + threadIdx.x);
+        const uint32_t rows = __ballot_sync(0xffffffffu, th >= 0);
+        if (lane == 0) mbar_expect_tx(&q_raw, __popc(rows) * HD * 4);
+        __syncwarp();
+        if (th >= 0) bulk_load(qs + threadIdx.x * pm_q_row(HD), a.q + th * HD, HD * 4, &q_raw);
+    }
+    // the positions that the CTA's (both CTAs') rows see together
+    for (int r = r0 + threadIdx.x; r <= r1; r += PM_THREADS) {
+        const int p = r < r0 + PM_THREADS ? pos0 : a.pos[run * a.R + r];
+        if (kv4_row_state(base, p, a.capacity)) continue;
+        const Vis v = visible(p, a.window, a.sinks);
+        atomicMax(&rng[0], v.n);
+        atomicMin(&rng[1], v.first);
+        atomicMax(&rng[2], v.sink);
     }
     tc_before();
-    pm_sync<NC>();
+    pm_pair_wait<NC>();
+    __syncthreads();
     tc_after();
     const uint32_t tmem = tmem_base;
     const Vis seen{rng[0], rng[1], rng[2]};
     const TileList tl = seen.n > 0 ? tile_list(seen.n, seen.first, seen.sink) : TileList{0, 0, 0};
-    const int i0 = (int)((int64_t)tl.count * sp / a.S), i1 = (int)((int64_t)tl.count * (sp + 1) / a.S);
+    int i0 = 0, i1 = tl.count;
+    if (a.S > 1) {
+        i0 = (int)((int64_t)tl.count * sp / a.S);
+        i1 = (int)((int64_t)tl.count * (sp + 1) / a.S);
+    }
     const int steps = (i1 - i0 + PM_TILES - 1) / PM_TILES;
     volatile int* abort = &abort_flag;
-    // a query's (row, head), or -1 past the run
-    auto query = [&](int qi) -> int64_t { return qi < nq ? (int64_t)(run * a.R + qi / G) * a.heads + kvh * G + qi % G : -1; };
 
     // Registers: 512 threads of 128 at launch; 176 + 2 * 152 + 24 a thread of the four warpgroups = 504 of these 512.
     if (warp < 4) {
@@ -278,7 +303,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         Vis vis{0, 0, 0};
         int state = 1;
         if (th >= 0) {
-            const int p = a.pos[th / a.heads];
+            const int p = a.pos[run * a.R + (q0 + (int)threadIdx.x) / G];
             state = kv4_row_state(base, p, a.capacity);
             if (!state) vis = visible(p, a.window, a.sinks);
         }
@@ -286,9 +311,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         {
             // Q's planes: 2^13..2^14 at the row's largest value, dims in the order 0 4 1 5 2 6 3 7
             const float f = a.scale * 1.4426950408889634f;
-            const float4* x = reinterpret_cast<const float4*>(a.q + th * HD);
+            const float4* x = reinterpret_cast<const float4*>(qs + threadIdx.x * pm_q_row(HD));
             float mx = 0.f;
+            pm_wait(&q_raw, 0u, a.err, abort);
             if (th >= 0)
+#pragma unroll 8
                 for (int i = 0; i < HD / 4; ++i) {
                     const float4 v = x[i];
                     mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x * f), fabsf(v.y * f)), fmaxf(fabsf(v.z * f), fabsf(v.w * f))));
@@ -318,7 +345,10 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             tmem_st_wait();
             tc_before();
             __syncwarp();
-            if (lane == 0) pm_arrive_lead<NC>(&q_full);
+            if (lane == 0) {
+                pm_arrive(&q_read);
+                pm_arrive(&q_full);
+            }
         }
         // (queries that see nothing, or are none, need no mask: their output is not read)
         const int w_min_n = __reduce_min_sync(0xffffffffu, vis.n > 0 ? vis.n : INT_MAX), w_max_first = __reduce_max_sync(0xffffffffu, vis.first);
@@ -416,7 +446,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             l += x.x + x.y;
             tc_before();
             __syncwarp();
-            if (lane == 0) pm_arrive_lead<NC>(&p_full[j & 1]);
+            if (lane == 0) pm_arrive(&p_full[j & 1]);
         }
         if (state) l = state == 2 ? NAN : 0.f;
         fin_l[threadIdx.x] = l;
@@ -430,6 +460,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         auto live = [&](int it, int r) {    // position r of list item it is seen by some row of the CTA
             return it < i1 && seen(tl.at(it) * KV4_P + r);
         };
+        auto all_live = [&](int at) {       // every position of a step's tiles is seen by some row
+            return at + PM_TILES <= i1 && tl.at(at) * KV4_P >= seen.first && (tl.at(at + PM_TILES - 1) + 1) * KV4_P <= seen.n;
+        };
         auto raw_step = [&](int j) -> const uint8_t* { return raw + j % PM_RAW * PM_TILES * TB; };
         // step j's raw tiles are there; what its values' scales call for is known to all warps. Each warp looks at all of them:
         // only a scale of 2 or more (or what lies in unseen places) makes the warps meet.
@@ -439,8 +472,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             pm_wait(&raw_full[j % PM_RAW], (uint32_t)(j / PM_RAW & 1), a.err, abort);
             const int words = KV4_P * NB / 2;       // of two fp16 scales, of a tile
             uint32_t any = 0u;
-            for (int t = 0; t < min(PM_TILES, i1 - at); ++t)
-                if (lane < words) any |= reinterpret_cast<const uint32_t*>(raw_step(j) + t * TB + 17 * HD)[lane];
+#pragma unroll
+            for (int t = 0; t < PM_TILES; ++t)
+                if (lane < words && at + t < i1) any |= reinterpret_cast<const uint32_t*>(raw_step(j) + t * TB + 17 * HD)[lane];
             if (!__any_sync(0xffffffffu, any & 0x40004000u) && !(used >> slot & 1u)) return;
             StepCare<NB>& cr = care[slot];
             asm volatile("bar.sync 1, 256;" ::: "memory");      // (step j - 8, whose slot this was, is behind every warp)
@@ -472,6 +506,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         // K' of step j (a CTA of a pair: its half of the positions): (tile, half) units, a position's 8 dims x NB a lane
         auto keys = [&](int j) {
             const __half2 k2 = __float2half2_rn(0.125f);
+            const bool whole = all_live(i0 + PM_TILES * j);
 #pragma unroll 1
             for (int u = 0; u < 2 / NC; ++u) {
                 const int tile = NC == 1 ? w : 4 * cta + w / 2, h = NC == 1 ? u : w & 1;
@@ -486,7 +521,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 } else {
                     sw[0] = *reinterpret_cast<const uint32_t*>(sc);
                 }
-                if (!live(i0 + PM_TILES * j + tile, 8 * h + g)) {
+                if (!whole && !live(i0 + PM_TILES * j + tile, 8 * h + g)) {
 #pragma unroll
                     for (int i = 0; i < NB / 2; ++i) sw[i] = 0u;
                 }
@@ -516,23 +551,27 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             }
             pm_fence_async();
             __syncwarp();
-            if (lane == 0) pm_arrive_lead<NC>(&k_full);
+            if (lane == 0) pm_arrive(&k_full);
         };
         // V' of step j (a CTA of a pair: its half of the dims): 32 positions (two tiles) and half the blocks, or half of the one
         // block, a warp; a lane 8 positions of 4 dims a block
         auto values = [&](int j) {
             constexpr int VB = NB / NC;
             const uint8_t* rs = raw_step(j);
+            uint8_t* vj = vh + j % NV * 2 * PL;
             const StepCare<NB>& cr = care[j % PM_SLOTS];
             const __half2 vs2 = __float2half2_rn(cr.vs());
             const int any_nan = cr.any_nan, at = i0 + PM_TILES * j;
             const int grp = w / 2, ch = (grp & 1) * 4 + c;
             uint32_t keep[4];
+            const bool whole = all_live(at);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int it = at + 2 * grp + k / 2, r = 8 * (k & 1) + 2 * c;
-                keep[k] = (live(it, r) ? 0xFFFFu : 0u) | (live(it, r + 1) ? 0xFFFF0000u : 0u);
+                keep[k] = 0xFFFFFFFFu;
+                if (!whole) keep[k] = (live(it, r) ? 0xFFFFu : 0u) | (live(it, r + 1) ? 0xFFFF0000u : 0u);
             }
+            if (j == 0) pm_wait(&q_read, 0u, a.err, abort);     // (V' takes the place of the staged queries)
 #pragma unroll 1
             for (int vb = VB > 1 ? (w & 1) * (VB / 2) : 0, e = vb + (VB > 1 ? VB / 2 : 1); vb < e; ++vb) {
                 const int b = VB * cta + vb;
@@ -560,7 +599,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                         lo[k] = h2_bits(__hfma2(bits_h2(r[k][x]), d, __hneg2(y)));
                     }
                     const int dim = 32 * vb + 4 * g + x;
-                    uint8_t* dst = vh + grp / 2 * (VD * 128) + dim / 8 * 1024 + dim % 8 * 128 + (ch ^ (dim % 8)) * 16;
+                    uint8_t* dst = vj + grp / 2 * (VD * 128) + dim / 8 * 1024 + dim % 8 * 128 + (ch ^ (dim % 8)) * 16;
                     *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     *reinterpret_cast<uint4*>(dst + PL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
@@ -568,7 +607,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             pm_fence_async();
             __syncwarp();
             if (lane == 0) {
-                pm_arrive_lead<NC>(&v_full);
+                pm_arrive(&v_full[j % NV]);
                 pm_arrive(&raw_empty[j % PM_RAW]);
             }
         };
@@ -598,11 +637,12 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             }
             tc_before();
             __syncwarp();
-            if (lane == 0) pm_arrive_lead<NC>(&o_free);
+            if (lane == 0) pm_arrive(&o_free);
         };
         if (steps > 0) {
             survey(0);
             keys(0);
+            if (NV == 2) values(0);
         }
         for (int j = 0; j < steps; ++j) {
             if (j + 1 < steps) {
@@ -610,23 +650,34 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 pm_wait(&qk_done, (uint32_t)(j & 1), a.err, abort);
                 keys(j + 1);
             }
-            if (j > 0) collect(j - 1);
-            values(j);
+            if (j > 0) collect(j - 1);      // (its product is done: its V' may be written over)
+            if (NV == 1) values(j);
+            else if (j + 1 < steps) values(j + 1);
         }
         if (steps > 0) collect(steps - 1);
         asm volatile("bar.sync 2, 384;" ::: "memory");
-        const int64_t th = query(q0 + qr);
-        if (th >= 0) {
+        {
+            // the warp's 32 half rows by way of shared memory (a thread's own would go out 16 bytes a line at a time)
             const bool whole = a.S == 1;
             const float l = fin_l[qr];
             const float f = !whole ? 1.f : l != 0.f ? 1.f / l : 0.f;    // (a refused row's NaN stays; nothing visible: zeros)
             const uint32_t poison = fin_poison[qr];
-            float* dst = (whole ? a.out + th * HD : a.part + (th * a.S + sp) * HD) + d0;
+            uint8_t* st = os + w * 32 * pm_o_row(HD);
 #pragma unroll
             for (int i = 0; i < HD / 4; i += 2) {
                 const float g1 = poison >> ((d0 + 2 * i) / 32) & 1u ? NAN : f;
                 const float2 x = unf2(o[i]), y = unf2(o[i + 1]);
-                *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(x.x * g1, x.y * g1, y.x * g1, y.y * g1);
+                *reinterpret_cast<float4*>(st + lane * pm_o_row(HD) + 8 * i) = make_float4(x.x * g1, x.y * g1, y.x * g1, y.y * g1);
+            }
+            __syncwarp();
+            constexpr int L = HD / 8;           // lanes a half row
+            const int64_t mine = query(q0 + qr);
+#pragma unroll 4
+            for (int r = lane / L; r < 32; r += 32 / L) {
+                const int64_t th = __shfl_sync(0xffffffffu, mine, r);
+                if (th < 0) continue;
+                float* dst = (whole ? a.out + th * HD : a.part + (th * a.S + sp) * HD) + d0;
+                *reinterpret_cast<float4*>(dst + 4 * (lane % L)) = *reinterpret_cast<const float4*>(st + r * pm_o_row(HD) + 16 * (lane % L));
             }
         }
     } else {
@@ -635,11 +686,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             // ---- one thread (of a pair: for both) issues the MMAs. The products with remainders come first: sums are cut off at their size.
             auto pv = [&](int j) {
                 pm_wait(&p_full[j & 1], (uint32_t)(j / 2 & 1), a.err, abort);
-                pm_wait(&v_full, (uint32_t)(j & 1), a.err, abort);
                 if (j > 0) pm_wait(&o_free, (uint32_t)(j - 1 & 1), a.err, abort);
+                pm_wait(&v_full[j % NV], (uint32_t)(j / NV & 1), a.err, abort);
                 tc_after();
                 const uint32_t p = tmem + TM_S + (j & 1) * 128;
-                uint64_t v = pm_desc(vh);           // (16-byte units: 2 a step of 16 positions, an atom's HD rows of 128 bytes a step of 64)
+                uint64_t v = pm_desc(vh + j % NV * 2 * PL);           // (16-byte units: 2 a step of 16 positions, an atom's HD rows of 128 bytes a step of 64)
 #pragma unroll 1
                 for (int s = 0; s < PM_P / 64; ++s, v += VD * 8)
 #pragma unroll
@@ -648,7 +699,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                         pm_mma<NC>(tmem + TM_O, ph, v + 2 * x + (PL >> 4), pm_idesc(HD, NC), s > 0 || x > 0);
                         pm_mma<NC>(tmem + TM_O, ph + 16, v + 2 * x, pm_idesc(HD, NC), 1u);
                     }
-                v = pm_desc(vh);
+                v = pm_desc(vh + j % NV * 2 * PL);
 #pragma unroll 1
                 for (int s = 0; s < PM_P / 64; ++s, v += VD * 8)
 #pragma unroll
@@ -679,6 +730,26 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 if (j > 0) pv(j - 1);
             }
             pv(steps - 1);
+        } else if (NC == 2 && warp == PM_MMA_WARP && lane == 0 && steps > 0) {
+            // ---- a pair's other CTA: what the MMAs wait for, on to the first CTA in the order of its waits (one arrival across
+            // the pair each; made by the warps themselves, each across the pair, it cost them 400 cycles a time)
+            auto forward = [&](uint64_t* bar, int n) {
+                pm_wait(bar, (uint32_t)(n & 1), a.err, abort);
+                tc_after();
+                tc_before();
+                pm_arrive_lead(bar);
+            };
+            auto pv = [&](int j) {
+                forward(&p_full[j & 1], j / 2);
+                if (j > 0) forward(&o_free, j - 1);
+                forward(&v_full[j % NV], j / NV);
+            };
+            forward(&q_full, 0);
+            for (int j = 0; j < steps; ++j) {
+                forward(&k_full, j);
+                if (j > 0) pv(j - 1);
+            }
+            pv(steps - 1);
         } else if (warp == PM_RAW_WARP && lane == 0) {
             // ---- raw tiles
             const uint8_t* src = base + (int64_t)kvh * TB;
@@ -686,6 +757,10 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 const int s = j % PM_RAW, at = i0 + PM_TILES * j, n = min(PM_TILES, i1 - at);
                 if (j >= PM_RAW) {
                     pm_wait(&raw_empty[s], (uint32_t)((j / PM_RAW + 1) & 1), a.err, abort);
+                    fence_proxy_async();
+                }
+                if (j == 2) {               // (its place held the staged queries)
+                    pm_wait(&q_read, 0u, a.err, abort);
                     fence_proxy_async();
                 }
                 mbar_expect_tx(&raw_full[s], n * TB);
@@ -696,7 +771,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
     }
     tc_before();
     __syncwarp();
-    pm_sync<NC>();                          // (nothing arrives at a pair's other CTA, and no MMA uses it, after this)
+    pm_pair_arrive<NC>();
+    pm_pair_wait<NC>();                     // (nothing arrives at a pair's other CTA, and no MMA uses it, after this)
+    __syncthreads();
     if (warp == 0) {
         tc_after();
         if constexpr (NC == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
