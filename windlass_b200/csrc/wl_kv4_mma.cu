@@ -40,8 +40,8 @@ constexpr int TM_S = 0, TM_O = 256, TM_QH = 384, TM_QL = 448;
 constexpr int pm_plane(int HD) { return HD * 256; }             // one fp16 plane of a step: 128 x HD
 constexpr int pm_q_row(int HD) { return HD * 4 + 16; }          // a staged query's bytes (16 more: no bank conflicts)
 constexpr int pm_o_row(int HD) { return HD * 2 + 16; }          // half a staged output row's
-constexpr int pm_v_bufs(int NC) { return NC; }                  // steps of V' in shared memory: a pair's CTA has room for two
-constexpr int pm_smem(int HD, int NC) { return (2 + 2 * pm_v_bufs(NC)) * pm_plane(HD) / NC + PM_RAW * PM_TILES * kv4_tile_bytes(HD) + 1024; }
+constexpr int pm_bufs(int NC) { return NC; }                    // steps of K' and V' in shared memory: a pair's CTA has room for two
+constexpr int pm_smem(int HD, int NC) { return 4 * pm_bufs(NC) * pm_plane(HD) / NC + PM_RAW * PM_TILES * kv4_tile_bytes(HD) + 1024; }
 
 // (acquires from the whole cluster: the other CTA of a pair arrives too)
 __device__ __forceinline__ bool pm_try_wait(uint64_t* bar, uint32_t parity)
@@ -196,16 +196,16 @@ template <int HD, int NC>
 __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, int q_blocks)
 {
     constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD), PL = pm_plane(HD) / NC;
-    constexpr int NV = pm_v_bufs(NC), KP = PM_P / NC, VD = HD / NC;             // rows of K' (positions) and V' (dims) that this CTA makes
+    constexpr int NP = pm_bufs(NC), KP = PM_P / NC, VD = HD / NC;             // rows of K' (positions) and V' (dims) that this CTA makes
     static_assert(HD == 64 || HD == 128, "planes of whole 64-value swizzle atoms");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint8_t *kh = smem, *raw = smem + 2 * PL, *vh = raw + PM_RAW * PM_TILES * TB;      // (each plane's remainder PL behind it)
+    uint8_t *kh = smem, *raw = smem + NP * 2 * PL, *vh = raw + PM_RAW * PM_TILES * TB;      // (each plane's remainder PL behind it)
     // the queries before the first V' and the raw steps 2 and 3; the output after the last raw step
     uint8_t *qs = raw + 2 * PM_TILES * TB, *os = raw;
     static_assert(PM_RAW == 4 && PM_Q * pm_q_row(HD) <= 2 * PM_TILES * TB + 2 * PL, "the queries end before V' does");
     static_assert(PM_DQ * 32 * pm_o_row(HD) <= PM_RAW * PM_TILES * TB && PM_RAW * PM_TILES * TB % 1024 == 0, "the output fits; V' is aligned");
-    __shared__ __align__(8) uint64_t raw_full[PM_RAW], raw_empty[PM_RAW], q_raw, q_read, q_full, k_full, qk_done, v_full[NV], pv_done, o_free, s_full[2],
+    __shared__ __align__(8) uint64_t raw_full[PM_RAW], raw_empty[PM_RAW], q_raw, q_read, q_full, k_full[NP], v_full[NP], pv_done, o_free, s_full[2],
         p_full[2];
     __shared__ StepCare<NB> care[PM_SLOTS];
     __shared__ float factor[PM_SLOTS][PM_Q];        // e^(old - new reference maximum) of a step and query
@@ -233,10 +233,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         mbar_init(&q_raw, 4);
         mbar_init(&q_read, 4);
         mbar_init(&q_full, 4 + more);
-        mbar_init(&k_full, PM_DQ + more);
-        for (int s = 0; s < NV; ++s) mbar_init(&v_full[s], PM_DQ + more);
+        for (int s = 0; s < NP; ++s) {
+            mbar_init(&k_full[s], PM_DQ + more);
+            mbar_init(&v_full[s], PM_DQ + more);
+        }
         mbar_init(&o_free, PM_DQ + more);
-        mbar_init(&qk_done, 1);
         mbar_init(&pv_done, 1);
         for (int s = 0; s < 2; ++s) {
             mbar_init(&s_full[s], 1);
@@ -505,6 +506,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         };
         // K' of step j (a CTA of a pair: its half of the positions): (tile, half) units, a position's 8 dims x NB a lane
         auto keys = [&](int j) {
+            uint8_t* kj = kh + j % NP * 2 * PL;
             const __half2 k2 = __float2half2_rn(0.125f);
             const bool whole = all_live(i0 + PM_TILES * j);
 #pragma unroll 1
@@ -544,21 +546,21 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                         lo[x] = h2_bits(__hfma2(bits_h2(r[x]), d, __hneg2(y)));
                     }
                     const int ch = 4 * b + c;
-                    uint8_t* dst = kh + ch / 8 * (KP * 128) + off + ((ch % 8) ^ (n % 8)) * 16;
+                    uint8_t* dst = kj + ch / 8 * (KP * 128) + off + ((ch % 8) ^ (n % 8)) * 16;
                     *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     *reinterpret_cast<uint4*>(dst + PL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             }
             pm_fence_async();
             __syncwarp();
-            if (lane == 0) pm_arrive(&k_full);
+            if (lane == 0) pm_arrive(&k_full[j % NP]);
         };
         // V' of step j (a CTA of a pair: its half of the dims): 32 positions (two tiles) and half the blocks, or half of the one
         // block, a warp; a lane 8 positions of 4 dims a block
         auto values = [&](int j) {
             constexpr int VB = NB / NC;
             const uint8_t* rs = raw_step(j);
-            uint8_t* vj = vh + j % NV * 2 * PL;
+            uint8_t* vj = vh + j % NP * 2 * PL;
             const StepCare<NB>& cr = care[j % PM_SLOTS];
             const __half2 vs2 = __float2half2_rn(cr.vs());
             const int any_nan = cr.any_nan, at = i0 + PM_TILES * j;
@@ -607,7 +609,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             pm_fence_async();
             __syncwarp();
             if (lane == 0) {
-                pm_arrive(&v_full[j % NV]);
+                pm_arrive(&v_full[j % NP]);
                 pm_arrive(&raw_empty[j % PM_RAW]);
             }
         };
@@ -642,16 +644,17 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         if (steps > 0) {
             survey(0);
             keys(0);
-            if (NV == 2) values(0);
+            if (NP == 2) values(0);
         }
         for (int j = 0; j < steps; ++j) {
             if (j + 1 < steps) {
                 survey(j + 1);
-                pm_wait(&qk_done, (uint32_t)(j & 1), a.err, abort);
+                const int u = j + 1 - NP;   // (the step whose K' this takes the place of: its scores are there)
+                if (u >= 0) pm_wait(&s_full[u & 1], (uint32_t)(u / 2 & 1), a.err, abort);
                 keys(j + 1);
             }
             if (j > 0) collect(j - 1);      // (its product is done: its V' may be written over)
-            if (NV == 1) values(j);
+            if (NP == 1) values(j);
             else if (j + 1 < steps) values(j + 1);
         }
         if (steps > 0) collect(steps - 1);
@@ -687,10 +690,10 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             auto pv = [&](int j) {
                 pm_wait(&p_full[j & 1], (uint32_t)(j / 2 & 1), a.err, abort);
                 if (j > 0) pm_wait(&o_free, (uint32_t)(j - 1 & 1), a.err, abort);
-                pm_wait(&v_full[j % NV], (uint32_t)(j / NV & 1), a.err, abort);
+                pm_wait(&v_full[j % NP], (uint32_t)(j / NP & 1), a.err, abort);
                 tc_after();
                 const uint32_t p = tmem + TM_S + (j & 1) * 128;
-                uint64_t v = pm_desc(vh + j % NV * 2 * PL);           // (16-byte units: 2 a step of 16 positions, an atom's HD rows of 128 bytes a step of 64)
+                uint64_t v = pm_desc(vh + j % NP * 2 * PL);           // (16-byte units: 2 a step of 16 positions, an atom's HD rows of 128 bytes a step of 64)
 #pragma unroll 1
                 for (int s = 0; s < PM_P / 64; ++s, v += VD * 8)
 #pragma unroll
@@ -699,7 +702,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                         pm_mma<NC>(tmem + TM_O, ph, v + 2 * x + (PL >> 4), pm_idesc(HD, NC), s > 0 || x > 0);
                         pm_mma<NC>(tmem + TM_O, ph + 16, v + 2 * x, pm_idesc(HD, NC), 1u);
                     }
-                v = pm_desc(vh + j % NV * 2 * PL);
+                v = pm_desc(vh + j % NP * 2 * PL);
 #pragma unroll 1
                 for (int s = 0; s < PM_P / 64; ++s, v += VD * 8)
 #pragma unroll
@@ -708,11 +711,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             };
             pm_wait(&q_full, 0u, a.err, abort);
             for (int j = 0; j < steps; ++j) {
-                pm_wait(&k_full, (uint32_t)(j & 1), a.err, abort);
+                pm_wait(&k_full[j % NP], (uint32_t)(j / NP & 1), a.err, abort);
                 if (j > 1) pm_wait(&pv_done, (uint32_t)(j & 1), a.err, abort);      // the weights that this score buffer held are used
                 tc_after();
                 const uint32_t d = tmem + TM_S + (j & 1) * 128;
-                uint64_t k = pm_desc(kh);
+                uint64_t k = pm_desc(kh + j % NP * 2 * PL);
 #pragma unroll 1
                 for (int s = 0; s < HD / 64; ++s, k += KP * 8)
 #pragma unroll
@@ -720,13 +723,12 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                         pm_mma<NC>(d, tmem + TM_QH + 32 * s + 8 * x, k + 2 * x + (PL >> 4), pm_idesc(PM_P, NC), s > 0 || x > 0);
                         pm_mma<NC>(d, tmem + TM_QL + 32 * s + 8 * x, k + 2 * x, pm_idesc(PM_P, NC), 1u);
                     }
-                k = pm_desc(kh);
+                k = pm_desc(kh + j % NP * 2 * PL);
 #pragma unroll 1
                 for (int s = 0; s < HD / 64; ++s, k += KP * 8)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) pm_mma<NC>(d, tmem + TM_QH + 32 * s + 8 * x, k + 2 * x, pm_idesc(PM_P, NC), 1u);
                 pm_commit<NC>(&s_full[j & 1]);
-                pm_commit<NC>(&qk_done);
                 if (j > 0) pv(j - 1);
             }
             pv(steps - 1);
@@ -742,11 +744,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             auto pv = [&](int j) {
                 forward(&p_full[j & 1], j / 2);
                 if (j > 0) forward(&o_free, j - 1);
-                forward(&v_full[j % NV], j / NV);
+                forward(&v_full[j % NP], j / NP);
             };
             forward(&q_full, 0);
             for (int j = 0; j < steps; ++j) {
-                forward(&k_full, j);
+                forward(&k_full[j % NP], j / NP);
                 if (j > 0) pv(j - 1);
             }
             pv(steps - 1);
