@@ -32,7 +32,7 @@ namespace {
 constexpr int PM_Q = 128, PM_P = 128;       // queries of a CTA, positions of a step
 constexpr int PM_TILES = PM_P / KV4_P;
 constexpr int PM_RAW = 4;                   // raw steps in flight
-constexpr int PM_DQ_WARP = 4, PM_DQ = 8, PM_MMA_WARP = 12, PM_RAW_WARP = 13, PM_THREADS = 512;
+constexpr int PM_DQ_WARP = 4, PM_DQ = 8, PM_MMA_WARP = 12, PM_RAW_WARP = 13, PM_CARE_WARP = 14, PM_THREADS = 512;
 constexpr int PM_SLOTS = 8;                 // steps whose care and factors are kept
 // tensor memory columns
 constexpr int TM_S = 0, TM_O = 256, TM_QH = 384, TM_QL = 448;
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
     uint8_t *qs = raw + 2 * PM_TILES * TB, *os = raw;
     static_assert(PM_RAW == 4 && PM_Q * pm_q_row(HD) <= 2 * PM_TILES * TB + 2 * PL, "the queries end before V' does");
     static_assert(PM_DQ * 32 * pm_o_row(HD) <= PM_RAW * PM_TILES * TB && PM_RAW * PM_TILES * TB % 1024 == 0, "the output fits; V' is aligned");
-    __shared__ __align__(8) uint64_t raw_full[PM_RAW], raw_empty[PM_RAW], q_raw, q_read, q_full, k_full[NP], v_full[NP], pv_done, o_free, s_full[2],
+    __shared__ __align__(8) uint64_t raw_full[PM_RAW], raw_empty[PM_RAW], care_full[PM_RAW], q_raw, q_read, q_full, k_full[NP], v_full[NP], pv_done, o_free, s_full[2],
         p_full[2];
     __shared__ StepCare<NB> care[PM_SLOTS];
     __shared__ float factor[PM_SLOTS][PM_Q];        // e^(old - new reference maximum) of a step and query
@@ -222,22 +222,24 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
     // the rows that the CTA (both CTAs) takes; their positions and cache are on their way while the rest is set up
     const int p0 = qg * NC * PM_Q, r0 = p0 / G, r1 = min(a.R - 1, (min(p0 + NC * PM_Q, nq) - 1) / G);
     const int pos0 = r0 + (int)threadIdx.x <= r1 ? a.pos[run * a.R + r0 + threadIdx.x] : -1;
+    const int qpos = warp < 4 && q0 + (int)threadIdx.x < nq ? a.pos[run * a.R + (q0 + (int)threadIdx.x) / G] : -1;
     const uint8_t* base = a.rows.base(run * a.R);
     if (threadIdx.x == 0) {
         for (int s = 0; s < PM_RAW; ++s) {
             mbar_init(&raw_full[s], 1);
             mbar_init(&raw_empty[s], PM_DQ);
+            mbar_init(&care_full[s], 1);
         }
         // the first CTA of a pair counts the other's warps as one: that CTA's forwarding thread
         const int more = NC == 2 && cta == 0;
         mbar_init(&q_raw, 4);
         mbar_init(&q_read, 4);
-        mbar_init(&q_full, 4 + more);
+        mbar_init(&q_full, 4);
         for (int s = 0; s < NP; ++s) {
             mbar_init(&k_full[s], PM_DQ + more);
-            mbar_init(&v_full[s], PM_DQ + more);
+            mbar_init(&v_full[s], PM_DQ);
         }
-        mbar_init(&o_free, PM_DQ + more);
+        mbar_init(&o_free, PM_DQ);
         mbar_init(&pv_done, 1);
         for (int s = 0; s < 2; ++s) {
             mbar_init(&s_full[s], 1);
@@ -295,6 +297,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
     const int steps = (i1 - i0 + PM_TILES - 1) / PM_TILES;
     volatile int* abort = &abort_flag;
 
+    auto live = [&](int it, int r) {        // position r of list item it is seen by some row of the CTA (of the pair)
+        return it < i1 && seen(tl.at(it) * KV4_P + r);
+    };
+    auto raw_step = [&](int j) -> const uint8_t* { return raw + j % PM_RAW * PM_TILES * TB; };
+
     // Registers: 512 threads of 128 at launch; 176 + 2 * 152 + 24 a thread of the four warpgroups = 504 of these 512.
     if (warp < 4) {
         // ---- a query a thread
@@ -304,9 +311,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         Vis vis{0, 0, 0};
         int state = 1;
         if (th >= 0) {
-            const int p = a.pos[run * a.R + (q0 + (int)threadIdx.x) / G];
-            state = kv4_row_state(base, p, a.capacity);
-            if (!state) vis = visible(p, a.window, a.sinks);
+            state = kv4_row_state(base, qpos, a.capacity);
+            if (!state) vis = visible(qpos, a.window, a.sinks);
         }
         float ks;
         {
@@ -458,51 +464,12 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         // ---- codes to planes, and the output
         regs_inc<152>();
         const int w = warp - PM_DQ_WARP, g = lane >> 2, c = lane & 3;
-        auto live = [&](int it, int r) {    // position r of list item it is seen by some row of the CTA
-            return it < i1 && seen(tl.at(it) * KV4_P + r);
-        };
         auto all_live = [&](int at) {       // every position of a step's tiles is seen by some row
             return at + PM_TILES <= i1 && tl.at(at) * KV4_P >= seen.first && (tl.at(at + PM_TILES - 1) + 1) * KV4_P <= seen.n;
         };
-        auto raw_step = [&](int j) -> const uint8_t* { return raw + j % PM_RAW * PM_TILES * TB; };
-        // step j's raw tiles are there; what its values' scales call for is known to all warps. Each warp looks at all of them:
-        // only a scale of 2 or more (or what lies in unseen places) makes the warps meet.
-        uint32_t used = 0u;                 // care slots that are not clear (the same in all warps)
-        auto survey = [&](int j) {
-            const int at = i0 + PM_TILES * j, slot = j % PM_SLOTS;
+        auto arrived = [&](int j) {         // step j's raw tiles, and what its values' scales call for
             pm_wait(&raw_full[j % PM_RAW], (uint32_t)(j / PM_RAW & 1), a.err, abort);
-            const int words = KV4_P * NB / 2;       // of two fp16 scales, of a tile
-            uint32_t any = 0u;
-#pragma unroll
-            for (int t = 0; t < PM_TILES; ++t)
-                if (lane < words && at + t < i1) any |= reinterpret_cast<const uint32_t*>(raw_step(j) + t * TB + 17 * HD)[lane];
-            if (!__any_sync(0xffffffffu, any & 0x40004000u) && !(used >> slot & 1u)) return;
-            StepCare<NB>& cr = care[slot];
-            asm volatile("bar.sync 1, 256;" ::: "memory");      // (step j - 8, whose slot this was, is behind every warp)
-            if (threadIdx.x == 32 * PM_DQ_WARP) cr.clear();
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            uint32_t big = 0u, nan = 0u;
-            const int i = 2 * lane;
-            if (lane < words && at + w < i1) {
-                const uint32_t x = reinterpret_cast<const uint32_t*>(raw_step(j) + w * TB + 17 * HD)[lane];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t d = (x >> (16 * e)) & 0x7FFFu;
-                    if (d < 0x4000u || !live(at + w, (i + e) / NB)) continue;
-                    if (d > 0x7C00u) nan |= 1u << e;
-                    else big = max(big, __float_as_uint(__half2float(__ushort_as_half((unsigned short)d))));
-                }
-            }
-            if (big) atomicMax(&cr.vmax, big);
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (nan >> e & 1u) {
-                    const int r = (i + e) / NB;
-                    cr.any_nan = 1;
-                    atomicOr(&cr.nan[(i + e) % NB][w / 2], 1u << (8 * (r % 8 / 2) + 2 * (2 * (w & 1) + r / 8) + r % 2));
-                }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            used = cr.vmax || cr.any_nan ? used | 1u << slot : used & ~(1u << slot);
+            pm_wait(&care_full[j % PM_RAW], (uint32_t)(j / PM_RAW & 1), a.err, abort);
         };
         // K' of step j (a CTA of a pair: its half of the positions): (tile, half) units, a position's 8 dims x NB a lane
         auto keys = [&](int j) {
@@ -551,67 +518,70 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                     *reinterpret_cast<uint4*>(dst + PL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             }
+        };
+        auto keys_done = [&](int j) {
             pm_fence_async();
             __syncwarp();
             if (lane == 0) pm_arrive(&k_full[j % NP]);
         };
         // V' of step j (a CTA of a pair: its half of the dims): 32 positions (two tiles) and half the blocks, or half of the one
-        // block, a warp; a lane 8 positions of 4 dims a block
-        auto values = [&](int j) {
-            constexpr int VB = NB / NC;
+        // block, a warp; a lane 8 positions of 4 dims a block. Made in registers, and put in place.
+        constexpr int VB = NB / NC;
+        const int grp = w / 2, vb0 = VB > 1 ? (w & 1) * (VB / 2) : 0, vbs = VB > 1 ? VB / 2 : 1;
+        auto make = [&](int j, int vb, uint32_t (&hi)[4][4], uint32_t (&lo)[4][4]) {
             const uint8_t* rs = raw_step(j);
-            uint8_t* vj = vh + j % NP * 2 * PL;
             const StepCare<NB>& cr = care[j % PM_SLOTS];
             const __half2 vs2 = __float2half2_rn(cr.vs());
-            const int any_nan = cr.any_nan, at = i0 + PM_TILES * j;
-            const int grp = w / 2, ch = (grp & 1) * 4 + c;
-            uint32_t keep[4];
+            const int any_nan = cr.any_nan, at = i0 + PM_TILES * j, b = VB * cta + vb;
             const bool whole = all_live(at);
+            uint32_t r[4][4], dv[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int it = at + 2 * grp + k / 2, r = 8 * (k & 1) + 2 * c;
-                keep[k] = 0xFFFFFFFFu;
-                if (!whole) keep[k] = (live(it, r) ? 0xFFFFu : 0u) | (live(it, r + 1) ? 0xFFFF0000u : 0u);
+                const uint8_t* tp = rs + (2 * grp + k / 2) * TB;
+                unpack_signed(*reinterpret_cast<const uint32_t*>(tp + 8 * HD + (((k & 1) * 32 + lane) * NB + b) * 4), r[k]);
+                const uint16_t* sc = reinterpret_cast<const uint16_t*>(tp + 17 * HD) + (8 * (k & 1) + 2 * c) * NB + b;
+                dv[k] = (uint32_t)sc[0] | (uint32_t)sc[NB] << 16;
+                if (!whole) {
+                    const int it = at + 2 * grp + k / 2, r0 = 8 * (k & 1) + 2 * c;
+                    dv[k] &= (live(it, r0) ? 0xFFFFu : 0u) | (live(it, r0 + 1) ? 0xFFFF0000u : 0u);
+                }
+                if (any_nan) {              // (a NaN scale, above infinity's bits, enters as zero)
+                    if ((dv[k] & 0x7FFFu) > 0x7C00u) dv[k] &= 0xFFFF0000u;
+                    if ((dv[k] & 0x7FFF0000u) > 0x7C000000u) dv[k] &= 0xFFFFu;
+                }
+                dv[k] = h2_bits(__hmul2(bits_h2(dv[k]), vs2));
             }
-            if (j == 0) pm_wait(&q_read, 0u, a.err, abort);     // (V' takes the place of the staged queries)
-#pragma unroll 1
-            for (int vb = VB > 1 ? (w & 1) * (VB / 2) : 0, e = vb + (VB > 1 ? VB / 2 : 1); vb < e; ++vb) {
-                const int b = VB * cta + vb;
-                uint32_t r[4][4], dv[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                if (VB == 1 && x / 2 != (w & 1)) continue;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const uint8_t* tp = rs + (2 * grp + k / 2) * TB;
-                    unpack_signed(*reinterpret_cast<const uint32_t*>(tp + 8 * HD + (((k & 1) * 32 + lane) * NB + b) * 4), r[k]);
-                    const uint16_t* sc = reinterpret_cast<const uint16_t*>(tp + 17 * HD) + (8 * (k & 1) + 2 * c) * NB + b;
-                    dv[k] = ((uint32_t)sc[0] | (uint32_t)sc[NB] << 16) & keep[k];
-                    if (any_nan) {          // (a NaN scale, above infinity's bits, enters as zero)
-                        if ((dv[k] & 0x7FFFu) > 0x7C00u) dv[k] &= 0xFFFF0000u;
-                        if ((dv[k] & 0x7FFF0000u) > 0x7C000000u) dv[k] &= 0xFFFFu;
-                    }
-                    dv[k] = h2_bits(__hmul2(bits_h2(dv[k]), vs2));
-                }
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    if (VB == 1 && x / 2 != (w & 1)) continue;
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const __half2 d = bits_h2(dv[k]), y = __hmul2(bits_h2(r[k][x]), d);
-                        hi[k] = h2_bits(y);
-                        lo[k] = h2_bits(__hfma2(bits_h2(r[k][x]), d, __hneg2(y)));
-                    }
-                    const int dim = 32 * vb + 4 * g + x;
-                    uint8_t* dst = vj + grp / 2 * (VD * 128) + dim / 8 * 1024 + dim % 8 * 128 + (ch ^ (dim % 8)) * 16;
-                    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(dst + PL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    const __half2 d = bits_h2(dv[k]), y = __hmul2(bits_h2(r[k][x]), d);
+                    hi[x][k] = h2_bits(y);
+                    lo[x][k] = h2_bits(__hfma2(bits_h2(r[k][x]), d, __hneg2(y)));
                 }
             }
+        };
+        auto put = [&](int j, int vb, const uint32_t (&hi)[4][4], const uint32_t (&lo)[4][4]) {
+            if (j == 0) pm_wait(&q_read, 0u, a.err, abort);     // (V' takes the place of the staged queries)
+            const int ch = (grp & 1) * 4 + c;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                if (VB == 1 && x / 2 != (w & 1)) continue;
+                const int dim = 32 * vb + 4 * g + x;
+                uint8_t* dst = vh + j % NP * 2 * PL + grp / 2 * (VD * 128) + dim / 8 * 1024 + dim % 8 * 128 + (ch ^ (dim % 8)) * 16;
+                *reinterpret_cast<uint4*>(dst) = make_uint4(hi[x][0], hi[x][1], hi[x][2], hi[x][3]);
+                *reinterpret_cast<uint4*>(dst + PL) = make_uint4(lo[x][0], lo[x][1], lo[x][2], lo[x][3]);
+            }
+        };
+        auto values_done = [&](int j) {
             pm_fence_async();
             __syncwarp();
-            if (lane == 0) {
-                pm_arrive(&v_full[j % NP]);
-                pm_arrive(&raw_empty[j % PM_RAW]);
-            }
+            if (lane == 0) pm_arrive(&v_full[j % NP]);
+        };
+        auto raw_done = [&](int j) {
+            __syncwarp();
+            if (lane == 0) pm_arrive(&raw_empty[j % PM_RAW]);
         };
         // the warp's part of the output: queries 32 (w % 4) + lane, dims HD / 2 * (w / 4) ..
         const int qr = 32 * (w & 3) + lane, d0 = HD / 2 * (w / 4);
@@ -641,21 +611,48 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             __syncwarp();
             if (lane == 0) pm_arrive(&o_free);
         };
-        if (steps > 0) {
-            survey(0);
-            keys(0);
-            if (NP == 2) values(0);
-        }
-        for (int j = 0; j < steps; ++j) {
-            if (j + 1 < steps) {
-                survey(j + 1);
-                const int u = j + 1 - NP;   // (the step whose K' this takes the place of: its scores are there)
-                if (u >= 0) pm_wait(&s_full[u & 1], (uint32_t)(u / 2 & 1), a.err, abort);
-                keys(j + 1);
+        if constexpr (NC == 1) {
+            uint32_t hi[4][4], lo[4][4];
+            if (steps > 0) {
+                arrived(0);
+                keys(0);
+                keys_done(0);
             }
-            if (j > 0) collect(j - 1);      // (its product is done: its V' may be written over)
-            if (NP == 1) values(j);
-            else if (j + 1 < steps) values(j + 1);
+            for (int j = 0; j < steps; ++j) {
+                if (j + 1 < steps) {
+                    arrived(j + 1);
+                    pm_wait(&s_full[j & 1], (uint32_t)(j / 2 & 1), a.err, abort);       // (step j's K' is used)
+                    keys(j + 1);
+                    keys_done(j + 1);
+                }
+                if (j > 0) collect(j - 1);
+#pragma unroll 1
+                for (int vb = vb0; vb < vb0 + vbs; ++vb) {
+                    make(j, vb, hi, lo);
+                    put(j, vb, hi, lo);
+                }
+                values_done(j);
+                raw_done(j);
+            }
+        } else {
+            // two steps of K' and V' each: step j + 1 is made while the product of step j - 1 runs (the fence that K' needs comes
+            // after V' is made: its writes have drained by then), and its V' put in the place of that product's
+            uint32_t hi[4][4], lo[4][4];
+            for (int j = -1; j < steps; ++j) {
+                if (j + 1 < steps) {
+                    arrived(j + 1);
+                    if (j > 0) pm_wait(&s_full[(j - 1) & 1], (uint32_t)((j - 1) / 2 & 1), a.err, abort);        // (step j - 1's K' is used)
+                    keys(j + 1);
+                    make(j + 1, vb0, hi, lo);
+                    keys_done(j + 1);
+                    raw_done(j + 1);
+                }
+                if (j > 0) collect(j - 1);
+                if (j + 1 < steps) {
+                    put(j + 1, vb0, hi, lo);
+                    values_done(j + 1);
+                }
+            }
         }
         if (steps > 0) collect(steps - 1);
         asm volatile("bar.sync 2, 384;" ::: "memory");
@@ -688,9 +685,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         if (warp == PM_MMA_WARP && cta == 0 && lane == 0 && steps > 0) {
             // ---- one thread (of a pair: for both) issues the MMAs. The products with remainders come first: sums are cut off at their size.
             auto pv = [&](int j) {
-                pm_wait(&p_full[j & 1], (uint32_t)(j / 2 & 1), a.err, abort);
                 if (j > 0) pm_wait(&o_free, (uint32_t)(j - 1 & 1), a.err, abort);
                 pm_wait(&v_full[j % NP], (uint32_t)(j / NP & 1), a.err, abort);
+                pm_wait(&p_full[j & 1], (uint32_t)(j / 2 & 1), a.err, abort);
                 tc_after();
                 const uint32_t p = tmem + TM_S + (j & 1) * 128;
                 uint64_t v = pm_desc(vh + j % NP * 2 * PL);           // (16-byte units: 2 a step of 16 positions, an atom's HD rows of 128 bytes a step of 64)
@@ -733,22 +730,24 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             }
             pv(steps - 1);
         } else if (NC == 2 && warp == PM_MMA_WARP && lane == 0 && steps > 0) {
-            // ---- a pair's other CTA: what the MMAs wait for, on to the first CTA in the order of its waits (one arrival across
-            // the pair each; made by the warps themselves, each across the pair, it cost them 400 cycles a time)
-            auto forward = [&](uint64_t* bar, int n) {
-                pm_wait(bar, (uint32_t)(n & 1), a.err, abort);
+            // ---- a pair's other CTA: what the MMAs wait for, on to the first CTA in the order of its waits, one arrival for all
+            // that a product waits for (made by the warps themselves, each across the pair, they cost them 400 cycles a time)
+            auto wait = [&](uint64_t* bar, int n) { pm_wait(bar, (uint32_t)(n & 1), a.err, abort); };
+            auto forward = [&](uint64_t* bar) {
                 tc_after();
                 tc_before();
                 pm_arrive_lead(bar);
             };
             auto pv = [&](int j) {
-                forward(&p_full[j & 1], j / 2);
-                if (j > 0) forward(&o_free, j - 1);
-                forward(&v_full[j % NP], j / NP);
+                if (j > 0) wait(&o_free, j - 1);
+                wait(&v_full[j % NP], j / NP);
+                wait(&p_full[j & 1], j / 2);
+                forward(&p_full[j & 1]);
             };
-            forward(&q_full, 0);
+            wait(&q_full, 0);
             for (int j = 0; j < steps; ++j) {
-                forward(&k_full[j % NP], j / NP);
+                wait(&k_full[j % NP], j / NP);
+                forward(&k_full[j % NP]);
                 if (j > 0) pv(j - 1);
             }
             pv(steps - 1);
@@ -768,6 +767,49 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 mbar_expect_tx(&raw_full[s], n * TB);
                 for (int i = 0; i < n; ++i)
                     bulk_load(raw + (s * PM_TILES + i) * TB, src + (int64_t)tl.at(at + i) * a.kv_heads * TB, TB, &raw_full[s]);
+            }
+        } else if (warp == PM_CARE_WARP) {
+            // ---- what the values' scales of a step call for: nothing, unless one is 2 or more or NaN (or what lies in unseen
+            // places looks so). A slot's step of PM_SLOTS before is behind every warp: its raw tiles' place was given up twice.
+            constexpr int words = KV4_P * NB / 2;           // of two fp16 scales, of a tile
+            uint32_t used = 0u;                             // slots that are not clear
+            for (int j = 0; j < steps; ++j) {
+                const int at = i0 + PM_TILES * j, slot = j % PM_SLOTS;
+                pm_wait(&raw_full[j % PM_RAW], (uint32_t)(j / PM_RAW & 1), a.err, abort);
+                uint32_t any = 0u;
+                for (int t = 0; t < PM_TILES; ++t)
+                    if (lane < words && at + t < i1) any |= reinterpret_cast<const uint32_t*>(raw_step(j) + t * TB + 17 * HD)[lane];
+                if (__any_sync(0xffffffffu, any & 0x40004000u) || (used >> slot & 1u)) {
+                    StepCare<NB>& cr = care[slot];
+                    if (lane == 0) cr.clear();
+                    __syncwarp();
+                    uint32_t big = 0u;
+                    bool nans = false;
+                    for (int t = 0; t < PM_TILES; ++t) {
+                        if (lane >= words || at + t >= i1) continue;
+                        const uint32_t x = reinterpret_cast<const uint32_t*>(raw_step(j) + t * TB + 17 * HD)[lane];
+                        for (int e = 0; e < 2; ++e) {
+                            const int r = (2 * lane + e) / NB, b = (2 * lane + e) % NB;
+                            const uint32_t d = (x >> (16 * e)) & 0x7FFFu;
+                            if (d < 0x4000u || !live(at + t, r)) continue;
+                            if (d > 0x7C00u) {
+                                nans = true;
+                                atomicOr(&cr.nan[b][t / 2], 1u << (8 * (r % 8 / 2) + 2 * (2 * (t & 1) + r / 8) + r % 2));
+                            } else {
+                                big = max(big, __float_as_uint(__half2float(__ushort_as_half((unsigned short)d))));
+                            }
+                        }
+                    }
+                    big = __reduce_max_sync(0xffffffffu, big);
+                    nans = __any_sync(0xffffffffu, nans);
+                    if (lane == 0) {
+                        cr.vmax = big;
+                        cr.any_nan = nans;
+                    }
+                    used = big || nans ? used | 1u << slot : used & ~(1u << slot);
+                }
+                __syncwarp();
+                if (lane == 0) pm_arrive(&care_full[j % PM_RAW]);
             }
         }
     }
