@@ -8,7 +8,8 @@
 // bits; vs a power of two). Each product is three MMAs, hi hi + lo hi + hi lo; the dropped lo lo is below 2^-22 of it, so
 // the result is as exact as fp32 arithmetic. Q and P are the MMA's A operand in tensor memory (P in the place of the
 // scores it came from), K' and V' its B operand in shared memory.
-//   - warp 13 copies a step's cache tiles (contiguous 18 HD bytes each) into a ring of raw steps with bulk copies;
+//   - warp 13 copies a step's cache tiles (contiguous 18 HD bytes each) into a ring of raw steps with bulk copies, warp 14
+//     looks their value scales over;
 //   - warps 4-11 turn codes into the planes of K' and V' in the 128-byte-swizzled K-major layout. The order of a step's
 //     positions is chosen so that a thread's codes are whole 16-byte chunks of it: within 32 positions, slot 8 c + 2 (2 t + h)
 //     + e is position 16 t + 8 h + 2 c + e; within 8 dims, 0 4 1 5 2 6 3 7. Both products use the same order;
@@ -18,9 +19,16 @@
 //   - warps 4-11 also keep the output in registers (32 queries by HD / 2 dims a warp): a step's product starts from zero in
 //     tensor memory and is added here in fp32 (the tensor core's sums are cut off, not rounded: over 768 of them in one
 //     place the output was 8e-6 off, added step by step 1e-6), scaled by what the step changed in the query's maximum.
-// Order of the products: scores of step j + 1, output of step j - 1, scores of j + 2, ... While the output of j - 1 runs, K' of
-// j + 1 is made; while the scores of j + 1 run, V' of j, and the weights of j from the scores before: two score buffers,
-// one of K' and of V'. Tensor memory: scores 2 x 128 columns, the step's output 128, Q 128 (at HD = 128): all 512.
+// Order of the products: scores of step j + 1, output of step j - 1, scores of j + 2, ... with two score buffers. Tensor
+// memory: scores 2 x 128 columns, the step's output 128, Q 128 (at HD = 128): all 512.
+// Two blocks of queries or more go in pairs of CTAs (cta_group::2): the pair walks the positions that its 256 queries see, each
+// CTA makes half of K' (64 positions) and of V' (half the dims) and the MMAs read both halves, so that a CTA unpacks half as
+// much and has room for two steps of both planes. One block goes by a CTA of its own. What that gave (1500 rows of a prompt,
+// 64 heads on 8 of 128 dims): 194 us by single CTAs, 195 by pairs with one step of planes, 172 with two of V' and the queries
+// and outputs copied by way of shared memory (a thread's own loads of its query took 11000 cycles of a CTA's start), 162.7
+// with two of K', the scales' warp and the positions' range found by each warp for itself. That is 0.74 PFLOP/s of MMAs; a
+// step takes 5000 cycles, of them 3700 of MMAs and as much of each other role, and starting and ending a CTA as much as 5
+// steps. 512 rows behind a window of 4096 positions (32 heads on 4): 119 us, 0.89 PFLOP/s.
 #include <algorithm>
 #include "wl_kv4.cuh"
 
@@ -43,8 +51,8 @@ constexpr int pm_o_row(int HD) { return HD * 2 + 16; }          // half a staged
 constexpr int pm_bufs(int NC) { return NC; }                    // steps of K' and V' in shared memory: a pair's CTA has room for two
 constexpr int pm_smem(int HD, int NC) { return 4 * pm_bufs(NC) * pm_plane(HD) / NC + PM_RAW * PM_TILES * kv4_tile_bytes(HD) + 1024; }
 
-// (acquires from the whole cluster: the other CTA of a pair arrives too)
-__device__ __forceinline__ bool pm_try_wait(uint64_t* bar, uint32_t parity)
+// (where the other CTA of a pair arrives)
+__device__ __forceinline__ bool pm_try_wait_cluster(uint64_t* bar, uint32_t parity)
 {
     uint32_t ok;
     asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
@@ -52,12 +60,13 @@ __device__ __forceinline__ bool pm_try_wait(uint64_t* bar, uint32_t parity)
     return ok;
 }
 // A wait bounded by time (2 s); after one gives up, all of the CTA's waits return at once.
-__device__ __forceinline__ bool pm_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort)
+template <bool CLUSTER = false> __device__ __forceinline__ bool pm_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort)
 {
+    auto ready = [&] { return CLUSTER ? pm_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
     if (*abort) return false;
-    if (pm_try_wait(bar, parity)) return true;
+    if (ready()) return true;
     const unsigned long long t0 = globaltimer_ns();
-    while (!pm_try_wait(bar, parity)) {
+    while (!ready()) {
         if (*abort) return false;
         if (globaltimer_ns() - t0 > MBAR_WAIT_NS) {
             atomicExch(err, 24);
@@ -66,6 +75,13 @@ __device__ __forceinline__ bool pm_wait(uint64_t* bar, uint32_t parity, int* err
         }
     }
     return true;
+}
+// After a wait gave up: what is still in flight ends before the CTA does (bounded as well).
+__device__ __forceinline__ void pm_drain(uint64_t* bar, uint32_t parity)
+{
+    const unsigned long long t0 = globaltimer_ns();
+    while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 <= MBAR_WAIT_NS) {
+    }
 }
 __device__ __forceinline__ void pm_arrive(uint64_t* bar)
 {
@@ -86,8 +102,6 @@ template <int NC> __device__ __forceinline__ void pm_pair_wait()
 {
     if constexpr (NC == 2) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// (a pair's MMA reads both CTAs' shared memory)
-__device__ __forceinline__ void pm_fence_async() { asm volatile("fence.proxy.async.shared::cluster;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
@@ -205,50 +219,52 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
     uint8_t *qs = raw + 2 * PM_TILES * TB, *os = raw;
     static_assert(PM_RAW == 4 && PM_Q * pm_q_row(HD) <= 2 * PM_TILES * TB + 2 * PL, "the queries end before V' does");
     static_assert(PM_DQ * 32 * pm_o_row(HD) <= PM_RAW * PM_TILES * TB && PM_RAW * PM_TILES * TB % 1024 == 0, "the output fits; V' is aligned");
-    __shared__ __align__(8) uint64_t raw_full[PM_RAW], raw_empty[PM_RAW], care_full[PM_RAW], q_raw, q_read, q_full, k_full[NP], v_full[NP], pv_done, o_free, s_full[2],
+    __shared__ __align__(8) uint64_t raw_full[PM_RAW], raw_empty[PM_RAW], care_full[PM_RAW], q_raw, q_read, drained, q_full, k_full[NP], v_full[NP], pv_done, o_free, s_full[2],
         p_full[2];
     __shared__ StepCare<NB> care[PM_SLOTS];
     __shared__ float factor[PM_SLOTS][PM_Q];        // e^(old - new reference maximum) of a step and query
     __shared__ float fin_l[PM_Q];
     __shared__ uint32_t fin_poison[PM_Q];
     __shared__ uint32_t tmem_base;
-    __shared__ int abort_flag, rng[3];
+    __shared__ int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.heads / a.kv_heads, kvh = blockIdx.y;
     // the last queries (of a prompt: those that see most) first
     const int cta = NC == 1 ? 0 : (int)blockIdx.x % NC, group = (int)blockIdx.x / NC;
     const int qg = q_blocks / NC - 1 - group / a.S, sp = group % a.S, qb = qg * NC + cta, run = blockIdx.z;
     const int nq = a.R * G, q0 = qb * PM_Q;
-    // the rows that the CTA (both CTAs) takes; their positions and cache are on their way while the rest is set up
+    // the rows that the CTA (both CTAs) takes: each warp finds the positions that they see together (the loads are on their way
+    // while the rest is set up)
     const int p0 = qg * NC * PM_Q, r0 = p0 / G, r1 = min(a.R - 1, (min(p0 + NC * PM_Q, nq) - 1) / G);
-    const int pos0 = r0 + (int)threadIdx.x <= r1 ? a.pos[run * a.R + r0 + threadIdx.x] : -1;
+    const int pos0 = r0 + lane <= r1 ? a.pos[run * a.R + r0 + lane] : -1;
     const int qpos = warp < 4 && q0 + (int)threadIdx.x < nq ? a.pos[run * a.R + (q0 + (int)threadIdx.x) / G] : -1;
     const uint8_t* base = a.rows.base(run * a.R);
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < PM_RAW; ++s) {
-            mbar_init(&raw_full[s], 1);
-            mbar_init(&raw_empty[s], PM_DQ);
-            mbar_init(&care_full[s], 1);
-        }
-        // the first CTA of a pair counts the other's warps as one: that CTA's forwarding thread
+    if (warp == 2) {
+        // (the first CTA of a pair counts the other's warps as one: that CTA's forwarding thread)
         const int more = NC == 2 && cta == 0;
-        mbar_init(&q_raw, 4);
-        mbar_init(&q_read, 4);
-        mbar_init(&q_full, 4);
-        for (int s = 0; s < NP; ++s) {
-            mbar_init(&k_full[s], PM_DQ + more);
-            mbar_init(&v_full[s], PM_DQ);
+        if (lane < PM_RAW) {
+            mbar_init(&raw_full[lane], 1);
+            mbar_init(&raw_empty[lane], PM_DQ);
+            mbar_init(&care_full[lane], 1);
+        } else if (lane < 8) {
+            const int s = lane & 1;
+            if (lane < 6) {
+                mbar_init(&s_full[s], 1);
+                mbar_init(&p_full[s], 4 + more);
+            } else if (s < NP) {
+                mbar_init(&k_full[s], PM_DQ + more);
+                mbar_init(&v_full[s], PM_DQ);
+            }
+        } else if (lane == 8) {
+            mbar_init(&q_raw, 4);
+            mbar_init(&q_read, 4);
+            mbar_init(&drained, 1);
+            mbar_init(&q_full, 4);
+        } else if (lane == 9) {
+            mbar_init(&o_free, PM_DQ);
+            mbar_init(&pv_done, 1);
+            abort_flag = 0;
         }
-        mbar_init(&o_free, PM_DQ);
-        mbar_init(&pv_done, 1);
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(&s_full[s], 1);
-            mbar_init(&p_full[s], 4 + more);
-        }
-        abort_flag = 0;
-        rng[0] = 0;
-        rng[1] = INT_MAX;
-        rng[2] = 0;
         fence_mbar_init();
     }
     if (warp == 1 && lane < PM_SLOTS) care[lane].clear();
@@ -261,8 +277,36 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         }
     }
+    Vis seen{0, INT_MAX, 0};
+    for (int r = r0 + lane; r <= r1; r += 32) {
+        const int p = r < r0 + 32 ? pos0 : a.pos[run * a.R + r];
+        if (kv4_row_state(base, p, a.capacity)) continue;
+        const Vis v = visible(p, a.window, a.sinks);
+        seen.n = max(seen.n, v.n);
+        seen.first = min(seen.first, v.first);
+        seen.sink = max(seen.sink, v.sink);
+    }
+    seen.n = __reduce_max_sync(0xffffffffu, seen.n);
+    seen.first = __reduce_min_sync(0xffffffffu, seen.first);
+    seen.sink = __reduce_max_sync(0xffffffffu, seen.sink);
+    const TileList tl = seen.n > 0 ? tile_list(seen.n, seen.first, seen.sink) : TileList{0, 0, 0};
+    int i0 = 0, i1 = tl.count;
+    if (a.S > 1) {
+        i0 = (int)((int64_t)tl.count * sp / a.S);
+        i1 = (int)((int64_t)tl.count * (sp + 1) / a.S);
+    }
+    const int steps = (i1 - i0 + PM_TILES - 1) / PM_TILES;
+    tc_before();
     __syncthreads();
-    pm_pair_arrive<NC>();                   // (this CTA's barriers are there)
+    tc_after();
+    pm_pair_arrive<NC>();                   // (this CTA's barriers and tensor memory are there)
+    volatile int* abort = &abort_flag;
+    auto raw_load = [&](int j) {            // (one thread) step j's cache tiles
+        const int s = j % PM_RAW, at = i0 + PM_TILES * j, n = min(PM_TILES, i1 - at);
+        mbar_expect_tx(&raw_full[s], n * TB);
+        for (int i = 0; i < n; ++i)
+            bulk_load(raw + (s * PM_TILES + i) * TB, base + ((int64_t)tl.at(at + i) * a.kv_heads + kvh) * TB, TB, &raw_full[s]);
+    };
     // a query's index in the call's queries, or -1 past the run
     auto query = [&](int qi) -> int64_t { return qi < nq ? (int64_t)(run * a.R + qi / G) * a.heads + kvh * G + qi % G : -1; };
     if (warp < 4) {
@@ -272,40 +316,21 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         if (lane == 0) mbar_expect_tx(&q_raw, __popc(rows) * HD * 4);
         __syncwarp();
         if (th >= 0) bulk_load(qs + threadIdx.x * pm_q_row(HD), a.q + th * HD, HD * 4, &q_raw);
+    } else if (warp == PM_RAW_WARP && lane == 0) {
+        for (int j = 0; j < min(steps, 2); ++j) raw_load(j);
     }
-    // the positions that the CTA's (both CTAs') rows see together
-    for (int r = r0 + threadIdx.x; r <= r1; r += PM_THREADS) {
-        const int p = r < r0 + PM_THREADS ? pos0 : a.pos[run * a.R + r];
-        if (kv4_row_state(base, p, a.capacity)) continue;
-        const Vis v = visible(p, a.window, a.sinks);
-        atomicMax(&rng[0], v.n);
-        atomicMin(&rng[1], v.first);
-        atomicMax(&rng[2], v.sink);
-    }
-    tc_before();
+    __syncwarp();
     pm_pair_wait<NC>();
-    __syncthreads();
-    tc_after();
     const uint32_t tmem = tmem_base;
-    const Vis seen{rng[0], rng[1], rng[2]};
-    const TileList tl = seen.n > 0 ? tile_list(seen.n, seen.first, seen.sink) : TileList{0, 0, 0};
-    int i0 = 0, i1 = tl.count;
-    if (a.S > 1) {
-        i0 = (int)((int64_t)tl.count * sp / a.S);
-        i1 = (int)((int64_t)tl.count * (sp + 1) / a.S);
-    }
-    const int steps = (i1 - i0 + PM_TILES - 1) / PM_TILES;
-    volatile int* abort = &abort_flag;
-
     auto live = [&](int it, int r) {        // position r of list item it is seen by some row of the CTA (of the pair)
         return it < i1 && seen(tl.at(it) * KV4_P + r);
     };
     auto raw_step = [&](int j) -> const uint8_t* { return raw + j % PM_RAW * PM_TILES * TB; };
 
-    // Registers: 512 threads of 128 at launch; 176 + 2 * 152 + 24 a thread of the four warpgroups = 504 of these 512.
+    // Registers: 512 threads of 128 at launch; 168 + 2 * 152 + 40 a thread of the four warpgroups = these 512.
     if (warp < 4) {
         // ---- a query a thread
-        regs_inc<176>();
+        regs_inc<168>();
         const uint32_t row = tmem + ((uint32_t)(32 * warp) << 16);
         const int64_t th = query(q0 + threadIdx.x);
         Vis vis{0, 0, 0};
@@ -520,7 +545,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             }
         };
         auto keys_done = [&](int j) {
-            pm_fence_async();
+            fence_proxy_async();
             __syncwarp();
             if (lane == 0) pm_arrive(&k_full[j % NP]);
         };
@@ -575,7 +600,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             }
         };
         auto values_done = [&](int j) {
-            pm_fence_async();
+            fence_proxy_async();
             __syncwarp();
             if (lane == 0) pm_arrive(&v_full[j % NP]);
         };
@@ -589,9 +614,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         uint64_t o[HD / 4];
 #pragma unroll
         for (int i = 0; i < HD / 4; ++i) o[i] = f2(0.f, 0.f);
-        auto collect = [&](int j) {         // step j's product into the output
+        auto product = [&](int j) {         // step j's product is there
             pm_wait(&pv_done, (uint32_t)(j & 1), a.err, abort);
             tc_after();
+        };
+        auto collect = [&](int j) {         // and goes into the output
             const float f = factor[j % PM_SLOTS][qr], u = 1.f / care[j % PM_SLOTS].vs();
             const uint64_t f1 = f2(f, f), u1 = f2(u, u);
             if (__any_sync(0xffffffffu, f != 1.f)) {
@@ -625,7 +652,10 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                     keys(j + 1);
                     keys_done(j + 1);
                 }
-                if (j > 0) collect(j - 1);
+                if (j > 0) {
+                    product(j - 1);
+                    collect(j - 1);
+                }
 #pragma unroll 1
                 for (int vb = vb0; vb < vb0 + vbs; ++vb) {
                     make(j, vb, hi, lo);
@@ -635,8 +665,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 raw_done(j);
             }
         } else {
-            // two steps of K' and V' each: step j + 1 is made while the product of step j - 1 runs (the fence that K' needs comes
-            // after V' is made: its writes have drained by then), and its V' put in the place of that product's
+            // two steps of K' and V' each: step j + 1 is made while the product of step j - 1 runs (the fences come after
+            // other work: the writes have drained by then), and its V' put in the place of that product's
             uint32_t hi[4][4], lo[4][4];
             for (int j = -1; j < steps; ++j) {
                 if (j + 1 < steps) {
@@ -647,18 +677,21 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                     keys_done(j + 1);
                     raw_done(j + 1);
                 }
+                if (j > 0) product(j - 1);
+                if (j + 1 < steps) put(j + 1, vb0, hi, lo);
                 if (j > 0) collect(j - 1);
-                if (j + 1 < steps) {
-                    put(j + 1, vb0, hi, lo);
-                    values_done(j + 1);
-                }
+                if (j + 1 < steps) values_done(j + 1);
             }
         }
-        if (steps > 0) collect(steps - 1);
+        if (steps > 0) {
+            product(steps - 1);
+            collect(steps - 1);
+        }
         asm volatile("bar.sync 2, 384;" ::: "memory");
         {
             // the warp's 32 half rows by way of shared memory (a thread's own would go out 16 bytes a line at a time)
             const bool whole = a.S == 1;
+            const int r_first = q0 / G;
             const float l = fin_l[qr];
             const float f = !whole ? 1.f : l != 0.f ? 1.f / l : 0.f;    // (a refused row's NaN stays; nothing visible: zeros)
             const uint32_t poison = fin_poison[qr];
@@ -671,23 +704,26 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             }
             __syncwarp();
             constexpr int L = HD / 8;           // lanes a half row
-            const int64_t mine = query(q0 + qr);
-#pragma unroll 4
-            for (int r = lane / L; r < 32; r += 32 / L) {
-                const int64_t th = __shfl_sync(0xffffffffu, mine, r);
-                if (th < 0) continue;
-                float* dst = (whole ? a.out + th * HD : a.part + (th * a.S + sp) * HD) + d0;
-                *reinterpret_cast<float4*>(dst + 4 * (lane % L)) = *reinterpret_cast<const float4*>(st + r * pm_o_row(HD) + 16 * (lane % L));
+            const int qi = q0 + qr, mine = qi < nq ? (qi / G - r_first) * a.heads + qi % G : -1;     // (its row and head from the CTA's first row's)
+            const int64_t th0 = (int64_t)(run * a.R + r_first) * a.heads + kvh * G;
+            float* dst = (whole ? a.out + th0 * HD : a.part + (th0 * a.S + sp) * HD) + d0 + 4 * (lane % L);
+            const int64_t pitch = whole ? HD : (int64_t)a.S * HD;
+#pragma unroll
+            for (int r = 0; r < 32; r += 32 / L) {
+                const int th = __shfl_sync(0xffffffffu, mine, r + lane / L);
+                const float4 v = *reinterpret_cast<const float4*>(st + (r + lane / L) * pm_o_row(HD) + 16 * (lane % L));
+                if (th >= 0) *reinterpret_cast<float4*>(dst + th * pitch) = v;
             }
         }
     } else {
-        regs_dec<24>();
+        regs_dec<40>();
         if (warp == PM_MMA_WARP && cta == 0 && lane == 0 && steps > 0) {
             // ---- one thread (of a pair: for both) issues the MMAs. The products with remainders come first: sums are cut off at their size.
             auto pv = [&](int j) {
                 if (j > 0) pm_wait(&o_free, (uint32_t)(j - 1 & 1), a.err, abort);
                 pm_wait(&v_full[j % NP], (uint32_t)(j / NP & 1), a.err, abort);
-                pm_wait(&p_full[j & 1], (uint32_t)(j / 2 & 1), a.err, abort);
+                pm_wait<NC == 2>(&p_full[j & 1], (uint32_t)(j / 2 & 1), a.err, abort);
+                if (*abort) return;
                 tc_after();
                 const uint32_t p = tmem + TM_S + (j & 1) * 128;
                 uint64_t v = pm_desc(vh + j % NP * 2 * PL);           // (16-byte units: 2 a step of 16 positions, an atom's HD rows of 128 bytes a step of 64)
@@ -708,8 +744,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             };
             pm_wait(&q_full, 0u, a.err, abort);
             for (int j = 0; j < steps; ++j) {
-                pm_wait(&k_full[j % NP], (uint32_t)(j / NP & 1), a.err, abort);
+                pm_wait<NC == 2>(&k_full[j % NP], (uint32_t)(j / NP & 1), a.err, abort);
                 if (j > 1) pm_wait(&pv_done, (uint32_t)(j & 1), a.err, abort);      // the weights that this score buffer held are used
+                if (*abort) break;
                 tc_after();
                 const uint32_t d = tmem + TM_S + (j & 1) * 128;
                 uint64_t k = pm_desc(kh + j % NP * 2 * PL);
@@ -729,6 +766,10 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 if (j > 0) pv(j - 1);
             }
             pv(steps - 1);
+            if (*abort) {
+                pm_commit<NC>(&drained);
+                pm_drain(&drained, 0u);
+            }
         } else if (NC == 2 && warp == PM_MMA_WARP && lane == 0 && steps > 0) {
             // ---- a pair's other CTA: what the MMAs wait for, on to the first CTA in the order of its waits, one arrival for all
             // that a product waits for (made by the warps themselves, each across the pair, they cost them 400 cycles a time)
@@ -753,20 +794,19 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             pv(steps - 1);
         } else if (warp == PM_RAW_WARP && lane == 0) {
             // ---- raw tiles
-            const uint8_t* src = base + (int64_t)kvh * TB;
-            for (int j = 0; j < steps; ++j) {
-                const int s = j % PM_RAW, at = i0 + PM_TILES * j, n = min(PM_TILES, i1 - at);
-                if (j >= PM_RAW) {
-                    pm_wait(&raw_empty[s], (uint32_t)((j / PM_RAW + 1) & 1), a.err, abort);
-                    fence_proxy_async();
-                }
-                if (j == 2) {               // (its place held the staged queries)
-                    pm_wait(&q_read, 0u, a.err, abort);
-                    fence_proxy_async();
-                }
-                mbar_expect_tx(&raw_full[s], n * TB);
-                for (int i = 0; i < n; ++i)
-                    bulk_load(raw + (s * PM_TILES + i) * TB, src + (int64_t)tl.at(at + i) * a.kv_heads * TB, TB, &raw_full[s]);
+            int issued = min(steps, 2);
+            for (int j = 2; j < steps; ++j) {
+                // (the places of steps 2 and 3 held the staged queries)
+                if (j >= PM_RAW) pm_wait(&raw_empty[j % PM_RAW], (uint32_t)((j / PM_RAW + 1) & 1), a.err, abort);
+                else if (j == 2) pm_wait(&q_read, 0u, a.err, abort);
+                if (*abort) break;
+                fence_proxy_async();
+                raw_load(j);
+                issued = j + 1;
+            }
+            if (*abort) {
+                pm_drain(&q_raw, 0u);
+                for (int j = max(0, issued - PM_RAW); j < issued; ++j) pm_drain(&raw_full[j % PM_RAW], (uint32_t)(j / PM_RAW & 1));
             }
         } else if (warp == PM_CARE_WARP) {
             // ---- what the values' scales of a step call for: nothing, unless one is 2 or more or NaN (or what lies in unseen
