@@ -279,12 +279,36 @@ template <int HD, int NT>
 __device__ __noinline__ void join_ranges(const float* ml_, const float* part, float* out, int S, int nh, int n, float* w, RowMap row)
 {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (n <= 8) {
+        // few ranges: every thread makes the factors of its output values itself
+        for (int i = threadIdx.x; i < nh * (HD / 4); i += NT) {
+            const int64_t at = row.at(i / (HD / 4));
+            const int d = i % (HD / 4) * 4;
+            const float2* ml = reinterpret_cast<const float2*>(ml_) + at * S;
+            const float4* pp = reinterpret_cast<const float4*>(part + at * S * HD + d);
+            float2 x[8];
+            float4 p[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < n) {
+                    x[k] = __ldcg(ml + k);
+                    p[k] = __ldcg(pp + (int64_t)k * (HD / 4));
+                }
+            JoinState j;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < n) j.add(x[k].x, x[k].y, p[k], k == 0);
+            *reinterpret_cast<float4*>(out + at * HD + d) = j.out();
+        }
+        return;
+    }
     for (int h = warp; h < nh; h += NT / 32) {
         const float2* ml = reinterpret_cast<const float2*>(ml_) + row.at(h) * S;
         float* wh = w + h * (3 * n + 1);    // of range s: what the ranges before it are scaled by, what it is, its sum
         float M = -INFINITY;                // the maximum of the ranges before this lane's
 #pragma unroll
         for (int i = 0; i < ATT_MAX_RANGES / 32; ++i) {
+            if (32 * i >= n) break;
             const int s = lane + 32 * i;
             const float2 x = s < n ? __ldcg(ml + s) : make_float2(-INFINITY, 0.f);
             float inc = x.x;

@@ -864,6 +864,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
     if (a.S == 1 || q0 >= nq) return;
+    // (128 registers for all again: the join compiled for the fewest kept its partials in local memory)
+    if (warp < PM_MMA_WARP) regs_dec<128>();
+    else regs_inc<128>();
     if (!last_ticket(a.tickets + ((int64_t)run * a.kv_heads + kvh) * q_blocks + qb, a.S)) return;
     join_ranges<HD, PM_THREADS>(a.ml, a.part, a.out, a.S, min(PM_Q, nq - q0), a.S, reinterpret_cast<float*>(smem),
                                 RowMap{(int64_t)run * a.R * a.heads + kvh * G, q0, G, a.heads});
