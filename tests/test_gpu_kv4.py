@@ -179,6 +179,23 @@ def test_attention_of_runs(wl, heads, kv_heads, hd, window, sinks):
     assert wl.lib().wl_kernel_status(0) == 0
 
 
+@pytest.mark.parametrize("rows", [16, 17, 31, 64, 129, 257])
+@pytest.mark.parametrize("heads,kv_heads,hd,window", [(4, 4, 64, 0), (8, 1, 128, 0), (3, 3, 128, 130), (12, 2, 64, 50), (4, 2, 96, 0),
+                                                      (2, 2, 256, 90)])
+def test_attention_of_runs_of_every_kernel(wl, rows, heads, kv_heads, hd, window):
+    """Rows by themselves, one block of queries, blocks in pairs with and without a last one of its own; no, one and many steps."""
+    rng = np.random.default_rng(rows * 7 + hd + heads)
+    for start in (0, 700):
+        c, raw = filled(rng, 2, kv_heads, hd, 1024, [start + rows, 1000])
+        seq = [0] * rows + [1] * rows
+        pos = [start + r for r in range(rows)] + [int(p) for p in rng.integers(0, 1000, rows)]
+        pos[rows + 1] = -1
+        q = rng.standard_normal((2 * rows, heads, hd)).astype(np.float32) * 2
+        out = attend(wl, c, seq, pos, q, window, 3, runs=rows)
+        check(out, q, raw, kv_heads, hd, seq, pos, window, 3)
+    assert wl.lib().wl_kernel_status(0) == 0
+
+
 @pytest.mark.parametrize("heads,kv_heads,hd", [(16, 2, 128), (8, 2, 64), (20, 4, 128), (7, 7, 64)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (200, 17)])
 def test_attention_of_long_runs(wl, heads, kv_heads, hd, window, sinks):

@@ -779,12 +779,14 @@ __global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att
 
 constexpr int64_t KV4_TICKETS = 1 << 18;    // tickets at the head of a workspace (zero between calls)
 
-// Queries of a run and KV head from which the tensor-core kernel is taken (its CTAs hold 128).
-constexpr int MMA_MIN_QUERIES = 96;
+// Rows of a run up to which each is attended to by itself. 9 rows, 32 heads on 4, 4000 positions: 15 us so, 37 by tensor
+// cores and 67 by k_kv4_attn_run; 12 rows of 500 positions: 9, 21 and 34; 16 rows of 3000: 27, 32 and 64; the other way
+// round where runs are few and long (10 rows, 64 heads on 8, 20000 positions: 96, 65 and 161), which the shape does not tell.
+constexpr int RUN_MIN_ROWS = 17;
 
 // How a call is cut.
 struct Kv4Plan {
-    bool runs, mma, pairs;  // the rows' runs share their cache's tiles: on the tensor cores (k_kv4_attn_mma) or k_kv4_attn_run
+    bool runs, mma, pairs;  // the rows' runs share their cache's tiles: on the tensor cores (k_kv4_attn_mma, in pairs of CTAs) or k_kv4_attn_run
     int S, s_max, alone, q_blocks, MT, MG;
     int64_t part_floats;
 };
@@ -796,8 +798,9 @@ Kv4Plan kv4_plan(int T, int R, int heads, int kv_heads, int head_dim, int64_t ca
     p.MG = (G + 7) / 8;
     int64_t tiles = (capacity + KV4_P - 1) / KV4_P;
     if (window > 0) tiles = std::min<int64_t>(tiles, ((int64_t)window + 15) / 16 + 1 + ((int64_t)sinks + 15) / 16);
-    p.runs = R > 8;
-    p.mma = p.runs && (head_dim == 64 || head_dim == 128) && (int64_t)R * G >= MMA_MIN_QUERIES;
+    p.runs = R >= RUN_MIN_ROWS;
+    // (32 and 64 rows of one query each, 5000 positions: 30 and 37 us by tensor cores, 54 and 75 by k_kv4_attn_run)
+    p.mma = p.runs && (head_dim == 64 || head_dim == 128);
     p.MT = head_dim <= 128 ? 2 : 1;
     const int QB = p.mma ? 128 : RUN_WARPS * 8 * p.MT;
     p.q_blocks = (int)(((int64_t)R * G + QB - 1) / QB);
@@ -806,7 +809,7 @@ Kv4Plan kv4_plan(int T, int R, int heads, int kv_heads, int head_dim, int64_t ca
     int64_t ctas;
     if (p.runs) {
         // as many ranges as end soonest: waves of CTAs over the SMs (two an SM, with CTAs of four warps), each of a range's
-        // share of the tiles and 12 tiles' time to start and end (measured: 8000 cycles against 5000 for 8 tiles)
+        // share of the tiles and 12 tiles' time to start and end (measured of k_kv4_attn_run: 8000 cycles against 5000 for 8 tiles)
         ctas = (int64_t)(T / R) * p.q_blocks * kv_heads;
         const int64_t slots = p.mma ? 148 : 2 * 148;
         double least = 1e30;
@@ -964,9 +967,9 @@ void kv4_attention(const float* q, int T, int R, int heads, int kv_heads, int he
         a.err = err;
         if (p.mma) kv4_attention_mma(a, head_dim, p.q_blocks, p.pairs, s);
         else switch (head_dim) {
-        case 64: p.runs ? attn_runs<64>(a, p, s) : attn_rows<64>(a, p, s); break;
+        case 64: attn_rows<64>(a, p, s); break;
         case 96: p.runs ? attn_runs<96>(a, p, s) : attn_rows<96>(a, p, s); break;
-        case 128: p.runs ? attn_runs<128>(a, p, s) : attn_rows<128>(a, p, s); break;
+        case 128: attn_rows<128>(a, p, s); break;
         default: p.runs ? attn_runs<256>(a, p, s) : attn_rows<256>(a, p, s); break;
         }
     }
