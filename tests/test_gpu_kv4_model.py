@@ -133,6 +133,22 @@ def test_growing_and_streamed_sequences_keep_their_bits(wl):
         assert got == list(ids)
 
 
+def test_prompts_of_any_length_have_the_workspace_they_need(wl):
+    """The ranges that a prompt is cut into, and so what its partial results take, do not fall steadily with its length (64
+    heads on 8, a cache of 2048: 193 rows need none, 289 more than all shorter ones)."""
+    rng = np.random.default_rng(7)
+    spec = synth_spec("llama", 1, 256, 64, 8, 64, 256, 1024, 2048, rope_base=10000.0, type_ffn_down=8, seed=1)
+    with CudaTransformer(synthetic=spec, max_context=2048, kv_type=Q4) as m:
+        for n in (193, 289, 400):
+            prompt = rng.integers(0, 1024, n).astype(np.int32)
+            a, b = m.new_sequence(), m.new_sequence()
+            one = m.forward(prompt, seq=a)
+            for i in range(0, n, 97):
+                parts = m.forward(prompt[i:i + 97], pos0=i, seq=b)
+            # (as in the mixed steps below: two paths' flips)
+            assert np.abs(one - parts).max() < 0.058 * one.std(), n
+
+
 def test_mixed_steps_and_a_sampled_serving_run(wl):
     """Prompts of many lengths join in mixed steps, then a batch decodes with every row's own sampling options: each id is
     the sampler's choice on that row's own logits, taken from a model that runs the row alone."""

@@ -316,8 +316,8 @@ void kv4_read(const Kv4Cache& cache, const int32_t* pos, int T, int kv_heads, in
 // Attention of T rows, R consecutive rows reading one cache (1: each its own). ws: kv4_workspace_bytes, its first
 // kv4_ticket_bytes() zero before the first call.
 int64_t kv4_workspace_bytes(int T, int R, int heads, int kv_heads, int head_dim, int64_t capacity, int window, int sinks);
-// The most that calls of up to T rows, in runs of any length, need.
-int64_t kv4_workspace_max(int T, int heads, int kv_heads, int head_dim, int64_t capacity, int window, int sinks);
+// The most that calls of above + 1 .. T rows need, each row alone or all one run.
+int64_t kv4_workspace_max(int above, int T, int heads, int kv_heads, int head_dim, int64_t capacity, int window, int sinks);
 size_t kv4_ticket_bytes();
 void kv4_attention(const float* q, int T, int R, int heads, int kv_heads, int head_dim, float scale, const Kv4Cache& cache,
                    const int32_t* pos, int64_t capacity, int window, int sinks, float* out, void* ws, int* err, cudaStream_t s);

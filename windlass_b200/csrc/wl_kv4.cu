@@ -905,13 +905,13 @@ int64_t kv4_workspace_bytes(int T, int R, int heads, int kv_heads, int head_dim,
     return KV4_TICKETS * 4 + 4 * kv4_plan(T, R, heads, kv_heads, head_dim, capacity, window, sinks).part_floats;
 }
 
-int64_t kv4_workspace_max(int T, int heads, int kv_heads, int head_dim, int64_t capacity, int window, int sinks)
+int64_t kv4_workspace_max(int above, int T, int heads, int kv_heads, int head_dim, int64_t capacity, int window, int sinks)
 {
-    int64_t most = kv4_workspace_bytes(std::min(T, 64), 1, heads, kv_heads, head_dim, capacity, window, sinks);
-    // (long runs have one range: their CTAs fill the SMs)
-    for (int r = 9; r <= T; ++r) {
-        if (kv4_plan(r, r, heads, kv_heads, head_dim, capacity, window, sinks).S == 1 && r > 64) break;
-        most = std::max(most, kv4_workspace_bytes(r, r, heads, kv_heads, head_dim, capacity, window, sinks));
+    // (every length: the ranges of neither kind fall steadily with it)
+    int64_t most = 0;
+    for (int t = above + 1; t <= T; ++t) {
+        if (t <= 64) most = std::max(most, kv4_workspace_bytes(t, 1, heads, kv_heads, head_dim, capacity, window, sinks));
+        most = std::max(most, kv4_workspace_bytes(t, t, heads, kv_heads, head_dim, capacity, window, sinks));
     }
     return most;
 }

@@ -962,7 +962,11 @@ void Model::ensure_workspace(int T, int logit_rows)
         drop_graphs();
     }
     if (kv4_) {
-        const int64_t need = k::kv4_workspace_max(T, c_.heads, c_.kv_heads, c_.head_dim, max_context_, window_, sinks_);
+        if (T > kv4_ws_T_) {
+            kv4_ws_need_ = std::max(kv4_ws_need_, k::kv4_workspace_max(kv4_ws_T_, T, c_.heads, c_.kv_heads, c_.head_dim, max_context_, window_, sinks_));
+            kv4_ws_T_ = T;
+        }
+        const int64_t need = kv4_ws_need_;
         if (need > kv4_ws_bytes_) {
             WL_CUDA(cudaStreamSynchronize(stream_));
             if (kv4_ws_) cudaFree(kv4_ws_);
@@ -1435,6 +1439,8 @@ void Model::kv4_layer(int l, int T, float scale)
     for (size_t i = 0; i < std::max<size_t>(1, segs_.size()); ++i) {
         const AttnSeg& g = segs[i];
         const k::Kv4Cache c{rows_d_ + g.start, (int)sizeof(RowKV), l};
+        if (k::kv4_workspace_bytes(g.count, g.run, c_.heads, c_.kv_heads, HD, max_context_, window_, sinks_) > kv4_ws_bytes_)
+            WL_THROW(WL_ENOMEM, "attention of " + std::to_string(g.count) + " rows: the workspace is too small");
         k::kv4_attention(q_ + (int64_t)g.start * QD, g.count, g.run, c_.heads, c_.kv_heads, HD, scale, c, pos_d_ + g.start, max_context_,
                          window_, sinks_, att_ + (int64_t)g.start * QD, kv4_ws_, err_d_, stream_);
     }

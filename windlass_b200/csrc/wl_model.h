@@ -254,7 +254,8 @@ private:
     bool kv4_ = false;
     int window_ = 0, sinks_ = 0;
     void* kv4_ws_ = nullptr;
-    int64_t kv4_ws_bytes_ = 0;
+    int64_t kv4_ws_bytes_ = 0, kv4_ws_need_ = 0;    // held, and needed by passes of up to kv4_ws_T_ rows
+    int kv4_ws_T_ = 0;
     // a pass's rows in runs that share a cache: rows [start, start + count) in runs of `run` (empty: every row alone)
     struct AttnSeg {
         int start, count, run;
