@@ -335,9 +335,9 @@ int32_t wl_kv4_read(void* const* dev_caches, const int32_t* dev_pos, int32_t T, 
 /* Attention (src/Transformer.cs:351-395) over the caches: row t attends to positions j <= dev_pos[t]; with window > 0 only
  * to those with j > dev_pos[t] - window or j < sinks (the first tokens stay visible). dev_out [T][heads * head_dim]. The
  * rows come in runs of rows_per_seq consecutive rows that read the same cache (T a multiple of it; 1 = every row may
- * have its own): runs of more than 8 rows (prompts) share the cache's tiles, and only a run's first cache pointer is
- * read. With runs of up to 8 rows a row's result does not depend on the other rows of a call of up to 64 rows.
- * dev_workspace (256-byte aligned, wl_kv4_workspace_bytes of the same arguments) is initialised once with
+ * have its own): runs of more than 16 rows (prompts) share the cache's tiles, and only a run's first cache pointer is
+ * read. With runs of up to 16 rows a row's result does not depend on the other rows of a call of up to 64 rows.
+ * dev_workspace (16-byte aligned, wl_kv4_workspace_bytes of the same arguments) is initialised once with
  * wl_kv4_workspace_init and then kept for any calls that are ordered after one another; calls that may overlap (two
  * streams, two graphs in flight) need a workspace each. */
 int32_t wl_kv4_attention(const float* dev_q, int32_t T, int32_t rows_per_seq, int32_t heads, int32_t kv_heads,
@@ -356,7 +356,7 @@ int32_t wl_sample_rows(const float* dev_logits, int64_t ld, int32_t V, int32_t r
                        int32_t* dev_ids, void* stream);
 
 /* Synchronises `device` and reports whether a device-side wait of a kernel-level export (wl_matvec, wl_matvec_tiles,
- * wl_matvec_static, wl_gemm_tiles, wl_matmul) gave up since the last report: WL_ETIMEDOUT (and the code) if one did,
+ * wl_matvec_static, wl_gemm_tiles, wl_matmul, wl_kv4_attention) gave up since the last report: WL_ETIMEDOUT (and the code) if one did,
  * else WL_OK. The waits are bounded at 2 s of device time, so this is a stalled copy, not a slow one. The model's own
  * calls report such a wait themselves. */
 int32_t wl_kernel_status(int32_t device);

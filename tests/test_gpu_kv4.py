@@ -350,6 +350,40 @@ def test_captured_and_replayed_on_a_stream_of_its_own(wl):
             check(host(d["o"]), host(d["qr"]), raw, kv_heads, hd, [0], [p])
 
 
+def test_prompts_on_two_streams_and_replayed(wl):
+    """Prompts of two shapes (pairs of CTAs and single ones, several ranges each) and a decode step captured on streams of their
+    own and replayed at once, a workspace each: the bits of calls made alone."""
+    torch = torch_cuda()
+    rng = np.random.default_rng(21)
+    lib, sets = wl.lib(), []
+    for rows, heads, kv_heads, hd, start, window in ((130, 8, 2, 128, 1500, 0), (40, 2, 2, 64, 900, 300), (1, 8, 2, 128, 1700, 0)):
+        c, raw = filled(rng, 1, kv_heads, hd, 1800, [start + rows])
+        pos = [start + r for r in range(rows)]
+        q = rng.standard_normal((rows, heads, hd)).astype(np.float32)
+        want = attend(wl, c, [0] * rows, pos, q, window, 4, runs=rows)
+        check(want, q, raw, kv_heads, hd, [0] * rows, pos, window, 4)
+        st = torch.cuda.Stream()
+        d = dict(c=c, q=dev(q), o=empty((rows, heads, hd)), rows=c.rows([0] * rows), pos=dev(np.array(pos, np.int32)), st=st, want=want,
+                 ws=workspace(wl, rows, rows, heads, kv_heads, hd, 1800, window, 4), g=torch.cuda.CUDAGraph())
+        torch.cuda.synchronize()
+        with torch.cuda.graph(d["g"], stream=st):
+            for _ in range(3):
+                wl.check(lib.wl_kv4_attention(ptr(d["q"]), rows, rows, heads, kv_heads, hd, hd ** -0.5, ptr(d["rows"]), ptr(d["pos"]), 1800,
+                                              window, 4, ptr(d["o"]), ptr(d["ws"]), d["ws"].numel(), C.c_void_p(st.cuda_stream)))
+        sets.append(d)
+    for _ in range(5):
+        for d in sets:
+            d["o"].zero_()
+        torch.cuda.synchronize()
+        for d in sets:
+            with torch.cuda.stream(d["st"]):
+                d["g"].replay()
+        torch.cuda.synchronize()
+        for d in sets:
+            assert np.array_equal(host(d["o"]).view(np.uint32), d["want"].view(np.uint32))
+    assert lib.wl_kernel_status(0) == 0
+
+
 def test_one_workspace_serves_calls_of_different_shapes(wl):
     rng = np.random.default_rng(15)
     n = C.c_int64()
