@@ -14,9 +14,9 @@
 //
 // Attention. The query heads of one KV head share its codes: a tile of 8 queries (heads of a row, or rows of a prompt)
 // is the 16-row side of m16n8k16 MMAs, each query twice: rows 0-7 its values' fp16 roundings, rows 8-15 what the
-// roundings left (together 22 bits of the row's largest value). Keys enter the MMA as their codes 0..15, which are fp16
-// subnormals once a mask has cut them out (c 2^-24, or 16 c 2^-24 with the query's share divided by 16), and 8 times the
-// sum of the query's block is taken off; values enter as fp16 integers -8..7. All products are exact, sums are fp32; the
+// roundings left (together 22 bits of the row's largest value). Keys and values enter as fp16 integers -8..7. (Keys as
+// fp16 subnormals, their codes cut out by a mask, with 8 times the query's sum taken off, took 4 % less time and lost bits in
+// the MMA's sums: 2.3e-6 to 2.8e-6 of the output, against 2.5e-7 to 4.3e-7 so.) All products are exact, sums are fp32; the
 // block scales are applied outside: to each block's fp32 sums for the scores, and to the weights before they are split
 // for the values (p * d, per block). So the codes' rounding is the only one below fp32.
 #include <algorithm>
@@ -267,17 +267,12 @@ template <int HD, int MT> struct AttState {
     }
 };
 
-// What a lane keeps of its queries besides their fragments: ks undoes the query's power of two (and the codes' 2^-24);
-// off[b] = 8 * 2^-24 * (the sum of block b's dims), what codes of 0..15 give too much.
-template <int NB> struct QueryTerms {
-    float ks, off[NB];
-};
-
 // NT tiles of 16 positions (from positions tile0[.], one behind the other at sm) for MT query tiles. qf(i, b, s) gives the A
-// fragment of query tile i, block b, step s (dims 32 b + 8 c + {2s, 2s + 4} of lane c, and, divided by 16, {2s + 1, 2s + 5}).
+// fragment of query tile i, block b, step s (dims 32 b + 8 c + {2s, 2s + 4}, {2s + 1, 2s + 5} of lane c); ks undoes the
+// queries' powers of two.
 template <int HD, int MT, int NT, class QF>
 __device__ __forceinline__ void kv4_tiles(const uint8_t* sm, int lane, const int (&tile0)[NT], const Vis (&vis)[MT], bool full,
-                                          const QF& qf, const QueryTerms<HD / 32> (&qt)[MT], AttState<HD, MT>& st)
+                                          const QF& qf, const float (&ks)[MT], AttState<HD, MT>& st)
 {
     constexpr int NB = HD / 32, TB = kv4_tile_bytes(HD);
     const int c = lane & 3;
@@ -293,15 +288,14 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* sm, int lane, const int
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             uint32_t r[4];
-            unpack_raw(kw[b], r);
+            unpack_signed(kw[b], r);
             const uint64_t d01 = f2(scale_of<NB>(dw, 0, b), scale_of<NB>(dw, 1, b));
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 float d[4];
                 mma_zero(d, qf(i, b, 0), r[0], r[1]);
                 mma_add(d, qf(i, b, 1), r[2], r[3]);
-                const uint64_t u = add2(add2(f2(d[0], d[1]), f2(d[2], d[3])), f2(-qt[i].off[b], -qt[i].off[b]));
-                s2[i][h] = fma2(d01, u, s2[i][h]);
+                s2[i][h] = fma2(d01, add2(f2(d[0], d[1]), f2(d[2], d[3])), s2[i][h]);
             }
         }
     }
@@ -329,7 +323,7 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* sm, int lane, const int
             mx = fmaxf(mx, fmaxf(x.x, x.y));
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * qt[i].ks;
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * ks[i];
         if (__any_sync(0xffffffffu, mx > st.m[i] + ATT_SLACK)) {
             const float mn = mx > st.m[i] ? mx : st.m[i], a = st.m[i] == -INFINITY ? 0.f : ex2(st.m[i] - mn);
             st.l[i] *= a;
@@ -340,7 +334,7 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* sm, int lane, const int
             st.m[i] = mn;
         }
         const float mu = st.m[i] == -INFINITY ? 0.f : st.m[i];
-        const uint64_t k2 = f2(qt[i].ks, qt[i].ks), m2 = f2(-mu, -mu);
+        const uint64_t k2 = f2(ks[i], ks[i]), m2 = f2(-mu, -mu);
 #pragma unroll
         for (int h = 0; h < 2 * NT; ++h) {
             const float2 x = unf2(fma2(s2[i][h], k2, m2));
@@ -422,7 +416,7 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* sm, int lane, const int
 // The A fragments qa[b][s] of lane (g, c)'s query row (nullptr: zeros) and its terms. A power of two brings the row's largest
 // value to 2^13..2^14, where fp16 and its remainder keep 22 bits.
 template <int HD>
-__device__ __forceinline__ void load_query(const float* x, int lane, float f, uint4 (&qa)[HD / 32][2], QueryTerms<HD / 32>& qt)
+__device__ __forceinline__ void load_query(const float* x, int lane, float f, uint4 (&qa)[HD / 32][2], float& ks)
 {
     constexpr int NB = HD / 32;
     const int c = lane & 3;
@@ -446,23 +440,16 @@ __device__ __forceinline__ void load_query(const float* x, int lane, float f, ui
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     int e = mx > 0.f && mx <= 3e38f ? 13 - ilogbf(mx) : 0;
     e = e > 100 ? 100 : e < -100 ? -100 : e;
-    const float up = ldexpf(1.f, e), up16 = up * 0.0625f;
+    const float up = ldexpf(1.f, e);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        float sum = 0.f;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             split_h2(f2(v[b][2 * s] * up, v[b][2 * s + 4] * up), qa[b][s].x, qa[b][s].y);
-            split_h2(f2(v[b][2 * s + 1] * up16, v[b][2 * s + 5] * up16), qa[b][s].z, qa[b][s].w);
-            const float2 h0 = __half22float2(bits_h2(qa[b][s].x)), l0 = __half22float2(bits_h2(qa[b][s].y));
-            const float2 h1 = __half22float2(bits_h2(qa[b][s].z)), l1 = __half22float2(bits_h2(qa[b][s].w));
-            sum += ((h0.x + h0.y) + (l0.x + l0.y)) + 16.f * ((h1.x + h1.y) + (l1.x + l1.y));
+            split_h2(f2(v[b][2 * s + 1] * up, v[b][2 * s + 5] * up), qa[b][s].z, qa[b][s].w);
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        qt.off[b] = sum * (8.f / 16777216.f);
     }
-    qt.ks = ldexpf(1.f, 24 - e);
+    ks = ldexpf(1.f, -e);
 }
 
 // A CTA of 8 warps, two an SM (128 registers, the queries' fragments in shared memory): against three CTAs of 4 warps with the
@@ -479,9 +466,9 @@ constexpr int att_ctas(int HD) { return HD <= 128 ? 2 : 1; }
 // every eighth pair of the range, through its ring of bulk copies, and the warps' sums are joined in warp order. The last
 // CTA of a row joins the ranges, or, where there are rows enough to fill the SMs (ALONE: rows of up to a.alone ranges), one
 // CTA walks a row's ranges: a row's bits do not depend on that, nor on the other rows.
-// Measured: 64 heads on 8 of 128 dims over 131001 positions 54 us (151 MB, 2.8 TB/s, 0.43 of a copy's rate), 8 such rows of up
-// to 4100 15.2 us, 64 rows of 32 on 8 behind a window of 1024 39.7 us (78 MB, 2.0 TB/s), 8 heads of 64 dims over 300
-// positions 4.6 us. Bound by the warps' instructions: about 370 a tile of 16 positions and warp (the codes' masks, the scales'
+// Measured: 64 heads on 8 of 128 dims over 131001 positions 56.7 us (151 MB, 2.7 TB/s, 0.41 of a copy's rate), 8 such rows of up
+// to 4100 15.8 us, 64 rows of 32 on 8 behind a window of 1024 41.0 us (78 MB, 1.9 TB/s), 8 heads of 64 dims over 300
+// positions 4.6 us. Bound by the warps' instructions: about 380 a tile of 16 positions and warp (the codes' masks, the scales'
 // products, weights split in two), with the loads always two tiles ahead.
 __device__ __forceinline__ int att_range(int tiles, int s_max)
 {
@@ -499,7 +486,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const
     __shared__ float sm_m[ATT_WARPS][8], sm_l[ATT_WARPS][8];
     // the queries' fragments and terms, made by one warp
     __shared__ __align__(16) uint4 sq[NB * 2 * 32];
-    __shared__ float sqt[(NB + 1) * 32];
+    __shared__ float sks[32];
     float* so = reinterpret_cast<float*>(smem + ATT_WARPS * ST * 2 * TB);       // [warp][8][HD]
     pdl_trigger();
     pdl_wait();
@@ -541,15 +528,14 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const
     }
     if (warp == 0) {
         uint4 qa[NB][2];
-        QueryTerms<NB> qt;
-        load_query<HD>(g < nh ? a.q + ((int64_t)t * a.heads + head0 + g) * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa, qt);
+        float ks;
+        load_query<HD>(g < nh ? a.q + ((int64_t)t * a.heads + head0 + g) * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa, ks);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             sq[b * 64 + lane] = qa[b][0];
             sq[b * 64 + 32 + lane] = qa[b][1];
-            sqt[b * 32 + lane] = qt.off[b];
         }
-        sqt[NB * 32 + lane] = qt.ks;
+        sks[lane] = ks;
     }
     __syncthreads();
     auto qf = [&](int, int b, int s) { return sq[b * 64 + s * 32 + lane]; };
@@ -567,11 +553,8 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const
             // (of an odd range's last step the second tile is not there: a position that no row sees)
             const int tile0[2] = {tl.at(x) * KV4_P, x + 1 < i1 ? tl.at(x + 1) * KV4_P : INT_MAX - KV4_P};
             const bool full = tile0[0] >= vis[0].first && tile0[1] < vis[0].n - KV4_P + 1;
-            QueryTerms<NB> qt[1];           // (from shared memory at each step: registers are short in the values' part)
-#pragma unroll
-            for (int b = 0; b < NB; ++b) qt[0].off[b] = sqt[b * 32 + lane];
-            qt[0].ks = sqt[NB * 32 + lane];
-            kv4_tiles<HD, 1, 2>(ring + i % ST * 2 * TB, lane, tile0, vis, full, qf, qt, st);
+            const float ks[1] = {sks[lane]};
+            kv4_tiles<HD, 1, 2>(ring + i % ST * 2 * TB, lane, tile0, vis, full, qf, ks, st);
             __syncwarp();
             if (lane == 0 && i + ST < steps) issue(i + ST);
         }
@@ -640,7 +623,8 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const
 // Runs of R rows that read one cache (prompts): the (row, head) pairs of a run and KV head are queries 0 .. R G - 1; a CTA
 // takes QB of them, each warp MT tiles of 8, and all warps share each tile of the cache (one ring of bulk copies), so
 // a tile's codes are unpacked once for 8 MT queries. Only for head sizes that wl_kv4_mma.cu does not take (96 and 256).
-// RUNFIG
+// Measured: 500 rows behind 4000 positions, 32 heads on 8 of 96 dims 373 us, 16 on 8 of 256 446 us: bound by mma.sync's rate
+// and the unpacking (32 rows of 8 heads of 128 dims, 5000 positions: 54 us so, 30 by wl_kv4_mma.cu).
 template <int HD, int MT>
 __global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att a, int q_blocks)
 {
@@ -695,7 +679,7 @@ __global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att
     if (threadIdx.x == 0)
         for (int s = 0; s < ST && s < nt; ++s) issue(s);
     Vis vis[MT];
-    QueryTerms<NB> qt[MT];
+    float ks[MT];
     int state[MT];
     int64_t th[MT];             // (row, head) of the lane's query, or -1
     int w_n = 0, w_min_n = INT_MAX, w_first = INT_MAX, w_max_first = 0, w_sink = 0;
@@ -714,7 +698,7 @@ __global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att
             if (!state[i]) vis[i] = visible(p, a.window, a.sinks);
         }
         uint4 qa[NB][2];
-        load_query<HD>(th[i] >= 0 ? a.q + th[i] * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa, qt[i]);
+        load_query<HD>(th[i] >= 0 ? a.q + th[i] * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa, ks[i]);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -743,7 +727,7 @@ __global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att
         if (tile0 < w_n && (tile0 + KV4_P > w_first || tile0 < w_sink)) {
             const bool full = tile0 + KV4_P <= w_min_n && tile0 >= w_max_first;
             const int t0[1] = {tile0};
-            kv4_tiles<HD, MT, 1>(smem + i % ST * TB, lane, t0, vis, full, qf, qt, st);
+            kv4_tiles<HD, MT, 1>(smem + i % ST * TB, lane, t0, vis, full, qf, ks, st);
         }
         __syncwarp();
         bool ok = true;

@@ -107,16 +107,6 @@ __device__ __forceinline__ void unpack_signed(uint32_t w, uint32_t (&r)[4])
     r[3] = h2_bits(__hfma2(bits_h2(and_or(w8, 0x00F000F0u, 0x64006400u)), s16, m72));
 }
 
-// The same as fp16 subnormals c 2^-24 (pairs 0 and 2) and 16 c 2^-24 (pairs 1 and 3): masks only.
-__device__ __forceinline__ void unpack_raw(uint32_t w, uint32_t (&r)[4])
-{
-    const uint32_t w8 = w >> 8;
-    r[0] = w & 0x000F000Fu;
-    r[1] = w & 0x00F000F0u;
-    r[2] = w8 & 0x000F000Fu;
-    r[3] = w8 & 0x00F000F0u;
-}
-
 // Pairs of floats in one instruction.
 __device__ __forceinline__ uint64_t f2(float lo, float hi)
 {
