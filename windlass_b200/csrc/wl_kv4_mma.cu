@@ -30,6 +30,7 @@
 // step takes 5000 cycles, of them 3700 of MMAs and as much of each other role, and starting and ending a CTA as much as 5
 // steps. 512 rows behind a window of 4096 positions (32 heads on 4): 119 us, 0.89 PFLOP/s.
 #include <algorithm>
+#include <type_traits>
 #include "wl_kv4.cuh"
 
 namespace wl {
@@ -406,74 +407,83 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 }
                 return b;
             };
-            // a group's scores: those not seen to -inf (the loops are kept rolled: unrolled, the three roles' code outgrew the
-            // instruction caches and a step took twice as long; two groups at a time, one's load behind the other's work)
-            auto mask = [&](int g, uint32_t (&r)[32]) {
-                if (!full(g)) {
-                    const uint32_t b = seen32(g);
+            // every query of the warp sees all of the step (most steps): a form without masks, so that what most steps run is
+            // short (the roles' code outgrows the instruction caches: no instruction was a warp's most frequent wait)
+            const bool clear = at + PM_TILES <= i1 && tl.at(at) * KV4_P >= w_max_first && (tl.at(at + PM_TILES - 1) + 1) * KV4_P <= w_min_n;
+            uint64_t sum;
+            auto step = [&](auto masked) {
+                constexpr bool MASKED = decltype(masked)::value;
+                // a group's scores: those not seen to -inf (the loops are kept rolled: unrolled, the three roles' code outgrew the
+                // instruction caches and a step took twice as long; two groups at a time, one's load behind the other's work)
+                auto mask = [&](int g, uint32_t (&r)[32]) {
+                    if (MASKED && !full(g)) {
+                        const uint32_t b = seen32(g);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) r[i] = b >> i & 1u ? r[i] : 0xFF800000u;
-                }
-            };
-            uint32_t ra[32], rb[32];
-            float mx = -INFINITY;
+                        for (int i = 0; i < 32; ++i) r[i] = b >> i & 1u ? r[i] : 0xFF800000u;
+                    }
+                };
+                uint32_t ra[32], rb[32];
+                float mx = -INFINITY;
 #pragma unroll 1
-            for (int g = 0; g < 4; g += 2) {
-                tmem_ld32(sbuf + 32 * g, ra);
-                tmem_ld32(sbuf + 32 * g + 32, rb);
-                tmem_ld_wait(ra);
-                tmem_ld_wait(rb);
-                mask(g, ra);
-                mask(g + 1, rb);
+                for (int g = 0; g < 4; g += 2) {
+                    tmem_ld32(sbuf + 32 * g, ra);
+                    tmem_ld32(sbuf + 32 * g + 32, rb);
+                    tmem_ld_wait(ra);
+                    tmem_ld_wait(rb);
+                    mask(g, ra);
+                    mask(g + 1, rb);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(ra[i]), __uint_as_float(rb[i])));
-            }
-            tmem_ld32(sbuf, ra);            // the first group again, behind the maximum's work
-            mx *= ks;
-            float f = 1.f;
-            if (mx > m + ATT_SLACK) {
-                f = m == -INFINITY ? 0.f : ex2(m - mx);
-                l *= f;
-                m = mx;
-            }
-            factor[j % PM_SLOTS][threadIdx.x] = f;
-            const StepCare<NB>& cr = care[j % PM_SLOTS];
-            if (cr.any_nan) {
-                // a value row with a NaN enters as zeros: it reaches the rows that see it here, and no other
-                for (int g = 0; g < 4; ++g) {
-                    const uint32_t see = seen32(g);
-                    for (int b = 0; b < NB; ++b)
-                        if (cr.nan[b][g] & see) poison |= 1u << b;
+                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(ra[i]), __uint_as_float(rb[i])));
                 }
-            }
-            const float mu = m == -INFINITY ? 0.f : m;
-            const uint64_t k2 = f2(ks, ks), m2 = f2(-mu, -mu);
-            uint64_t sum = f2(0.f, 0.f);
-            // a group's weights in place of its scores: 16 columns of their roundings, 16 of what those left
-            auto weights = [&](int g, uint32_t (&r)[32]) {
-                uint32_t lo[16];
-                mask(g, r);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float2 x = unf2(fma2(f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), k2, m2));
-                    const uint64_t p = f2(ex2(x.x), ex2(x.y));
-                    sum = add2(sum, p);
-                    split_h2(p, r[i], lo[i]);
+                tmem_ld32(sbuf, ra);            // the first group again, behind the maximum's work
+                mx *= ks;
+                float f = 1.f;
+                if (mx > m + ATT_SLACK) {
+                    f = m == -INFINITY ? 0.f : ex2(m - mx);
+                    l *= f;
+                    m = mx;
                 }
+                factor[j % PM_SLOTS][threadIdx.x] = f;
+                const StepCare<NB>& cr = care[j % PM_SLOTS];
+                if (cr.any_nan) {
+                    // a value row with a NaN enters as zeros: it reaches the rows that see it here, and no other
+                    for (int g = 0; g < 4; ++g) {
+                        const uint32_t see = seen32(g);
+                        for (int b = 0; b < NB; ++b)
+                            if (cr.nan[b][g] & see) poison |= 1u << b;
+                    }
+                }
+                const float mu = m == -INFINITY ? 0.f : m;
+                const uint64_t k2 = f2(ks, ks), m2 = f2(-mu, -mu);
+                sum = f2(0.f, 0.f);
+                // a group's weights in place of its scores: 16 columns of their roundings, 16 of what those left
+                auto weights = [&](int g, uint32_t (&r)[32]) {
+                    uint32_t lo[16];
+                    mask(g, r);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) r[16 + i] = lo[i];
-                tmem_st32(sbuf + 32 * g, r);
-            };
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 x = unf2(fma2(f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), k2, m2));
+                        const uint64_t p = f2(ex2(x.x), ex2(x.y));
+                        sum = add2(sum, p);
+                        split_h2(p, r[i], lo[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) r[16 + i] = lo[i];
+                    tmem_st32(sbuf + 32 * g, r);
+                };
 #pragma unroll 1
-            for (int g = 0; g < 4; g += 2) {
-                tmem_ld_wait(ra);
-                tmem_ld32(sbuf + 32 * g + 32, rb);
-                weights(g, ra);
-                tmem_ld_wait(rb);
-                if (g == 0) tmem_ld32(sbuf + 64, ra);
-                weights(g + 1, rb);
-            }
-            tmem_st_wait();
+                for (int g = 0; g < 4; g += 2) {
+                    tmem_ld_wait(ra);
+                    tmem_ld32(sbuf + 32 * g + 32, rb);
+                    weights(g, ra);
+                    tmem_ld_wait(rb);
+                    if (g == 0) tmem_ld32(sbuf + 64, ra);
+                    weights(g + 1, rb);
+                }
+                tmem_st_wait();
+            };
+            if (clear) step(std::false_type{});
+            else step(std::true_type{});
             const float2 x = unf2(sum);
             l += x.x + x.y;
             tc_before();
@@ -553,12 +563,12 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         // block, a warp; a lane 8 positions of 4 dims a block. Made in registers, and put in place.
         constexpr int VB = NB / NC;
         const int grp = w / 2, vb0 = VB > 1 ? (w & 1) * (VB / 2) : 0, vbs = VB > 1 ? VB / 2 : 1;
-        auto make = [&](int j, int vb, uint32_t (&hi)[4][4], uint32_t (&lo)[4][4]) {
+        auto make_as = [&](auto plain, int j, int vb, uint32_t (&hi)[4][4], uint32_t (&lo)[4][4]) {
+            constexpr bool PLAIN = decltype(plain)::value;      // all positions live, no scale that calls for care
             const uint8_t* rs = raw_step(j);
             const StepCare<NB>& cr = care[j % PM_SLOTS];
-            const __half2 vs2 = __float2half2_rn(cr.vs());
-            const int any_nan = cr.any_nan, at = i0 + PM_TILES * j, b = VB * cta + vb;
-            const bool whole = all_live(at);
+            const __half2 vs2 = __float2half2_rn(PLAIN ? 256.f : cr.vs());
+            const int any_nan = PLAIN ? 0 : cr.any_nan, at = i0 + PM_TILES * j, b = VB * cta + vb;
             uint32_t r[4][4], dv[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -566,7 +576,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 unpack_signed(*reinterpret_cast<const uint32_t*>(tp + 8 * HD + (((k & 1) * 32 + lane) * NB + b) * 4), r[k]);
                 const uint16_t* sc = reinterpret_cast<const uint16_t*>(tp + 17 * HD) + (8 * (k & 1) + 2 * c) * NB + b;
                 dv[k] = (uint32_t)sc[0] | (uint32_t)sc[NB] << 16;
-                if (!whole) {
+                if (!PLAIN) {
                     const int it = at + 2 * grp + k / 2, r0 = 8 * (k & 1) + 2 * c;
                     dv[k] &= (live(it, r0) ? 0xFFFFu : 0u) | (live(it, r0 + 1) ? 0xFFFF0000u : 0u);
                 }
@@ -586,6 +596,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                     lo[x][k] = h2_bits(__hfma2(bits_h2(r[k][x]), d, __hneg2(y)));
                 }
             }
+        };
+        auto make = [&](int j, int vb, uint32_t (&hi)[4][4], uint32_t (&lo)[4][4]) {
+            const StepCare<NB>& cr = care[j % PM_SLOTS];
+            if (all_live(i0 + PM_TILES * j) && !cr.vmax && !cr.any_nan) make_as(std::true_type{}, j, vb, hi, lo);
+            else make_as(std::false_type{}, j, vb, hi, lo);
         };
         auto put = [&](int j, int vb, const uint32_t (&hi)[4][4], const uint32_t (&lo)[4][4]) {
             if (j == 0) pm_wait(&q_read, 0u, a.err, abort);     // (V' takes the place of the staged queries)
@@ -619,7 +634,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             tc_after();
         };
         auto collect = [&](int j) {         // and goes into the output
-            const float f = factor[j % PM_SLOTS][qr], u = 1.f / care[j % PM_SLOTS].vs();
+            const StepCare<NB>& cr = care[j % PM_SLOTS];
+            const float f = factor[j % PM_SLOTS][qr], u = cr.vmax ? 1.f / cr.vs() : 1.f / 256.f;
             const uint64_t f1 = f2(f, f), u1 = f2(u, u);
             if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll
