@@ -26,9 +26,12 @@
 // much and has room for two steps of both planes. One block goes by a CTA of its own. What that gave (1500 rows of a prompt,
 // 64 heads on 8 of 128 dims): 194 us by single CTAs, 195 by pairs with one step of planes, 172 with two of V' and the queries
 // and outputs copied by way of shared memory (a thread's own loads of its query took 11000 cycles of a CTA's start), 162.7
-// with two of K', the scales' warp and the positions' range found by each warp for itself. That is 0.74 PFLOP/s of MMAs; a
-// step takes 5000 cycles, of them 3700 of MMAs and as much of each other role, and starting and ending a CTA as much as 5
-// steps. 512 rows behind a window of 4096 positions (32 heads on 4): 119 us, 0.89 PFLOP/s.
+// with two of K', the scales' warp and the positions' range found by each warp for itself, 160.6 with forms of their own for
+// steps without masks and scales without care (less code in the instruction caches; 512 rows behind a window of 4096
+// positions, 32 heads on 4: 130.7 to 108.2 us). That is 0.75 and 0.98 PFLOP/s of MMAs, of 1.65 measured. A step takes 5000 to
+// 6000 cycles, of them 3700 and more of MMAs, and each other role about as long; starting and ending a CTA takes as long as 4
+// or 5 steps. One thread's issue of the MMAs is close to the bound: with its loops rolled up 177 and 123 us, with
+// all 48 products unrolled 159 and 111.
 #include <algorithm>
 #include <type_traits>
 #include "wl_kv4.cuh"
