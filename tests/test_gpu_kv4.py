@@ -350,6 +350,23 @@ def test_captured_and_replayed_on_a_stream_of_its_own(wl):
             check(host(d["o"]), host(d["qr"]), raw, kv_heads, hd, [0], [p])
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd", [(8, 2, 64), (8, 2, 128), (4, 2, 96), (4, 2, 256)])
+@pytest.mark.parametrize("rows,start,cap", [(20, 200, 220), (40, 900, 1024), (80, 1900, 2000), (9, 50, 64)])
+def test_padding_rows_that_hold_nan_give_zeros(wl, heads, kv_heads, hd, rows, start, cap):
+    """The queries of padding rows may hold anything, whatever kernel and number of ranges; a refused row's stays NaN."""
+    rng = np.random.default_rng(hd + rows)
+    c, raw = filled(rng, 1, kv_heads, hd, cap, [start + rows])
+    pos = [start + r for r in range(rows)]
+    pos[0] = pos[5] = pos[rows - 1] = -1
+    pos[7] = cap
+    q = rng.standard_normal((rows, heads, hd)).astype(np.float32)
+    q[[0, 7]], q[5], q[rows - 1] = np.nan, np.inf, 3e38
+    out = attend(wl, c, [0] * rows, pos, q, runs=rows)
+    keep = [t for t in range(rows) if t != 7]
+    check(out[keep], q[keep], raw, kv_heads, hd, [0] * len(keep), [pos[t] for t in keep])
+    assert np.isnan(out[7]).all()
+
+
 def test_prompts_on_two_streams_and_replayed(wl):
     """Prompts of two shapes (pairs of CTAs and single ones, several ranges each) and a decode step captured on streams of their
     own and replayed at once, a workspace each: the bits of calls made alone."""

@@ -698,7 +698,8 @@ __global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att
             if (!state[i]) vis[i] = visible(p, a.window, a.sinks);
         }
         uint4 qa[NB][2];
-        load_query<HD>(th[i] >= 0 ? a.q + th[i] * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa, ks[i]);
+        // (a padding row's query may hold anything: it enters as zeros, and its sums are zeros)
+        load_query<HD>(!state[i] ? a.q + th[i] * HD : nullptr, lane, a.scale * 1.4426950408889634f, qa, ks[i]);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll

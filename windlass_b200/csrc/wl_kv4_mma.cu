@@ -350,7 +350,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             const float4* x = reinterpret_cast<const float4*>(qs + threadIdx.x * pm_q_row(HD));
             float mx = 0.f;
             pm_wait(&q_raw, 0u, a.err, abort);
-            if (th >= 0)
+            const bool use = !state;        // (a padding row's query may hold anything: it enters as zeros)
+            if (use)
 #pragma unroll 8
                 for (int i = 0; i < HD / 4; ++i) {
                     const float4 v = x[i];
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f), w = v;
-                    if (th >= 0) {
+                    if (use) {
                         v = x[16 * i + 2 * c];
                         w = x[16 * i + 2 * c + 1];
                     }
@@ -712,14 +713,15 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             const bool whole = a.S == 1;
             const int r_first = q0 / G;
             const float l = fin_l[qr];
-            const float f = !whole ? 1.f : l != 0.f ? 1.f / l : 0.f;    // (a refused row's NaN stays; nothing visible: zeros)
+            const float f = l == 0.f ? 0.f : !whole ? 1.f : 1.f / l;    // (a refused row's NaN stays; nothing visible: zeros)
             const uint32_t poison = fin_poison[qr];
             uint8_t* st = os + w * 32 * pm_o_row(HD);
 #pragma unroll
             for (int i = 0; i < HD / 4; i += 2) {
                 const float g1 = poison >> ((d0 + 2 * i) / 32) & 1u ? NAN : f;
                 const float2 x = unf2(o[i]), y = unf2(o[i + 1]);
-                *reinterpret_cast<float4*>(st + lane * pm_o_row(HD) + 8 * i) = make_float4(x.x * g1, x.y * g1, y.x * g1, y.y * g1);
+                *reinterpret_cast<float4*>(st + lane * pm_o_row(HD) + 8 * i) =
+                    g1 == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x * g1, x.y * g1, y.x * g1, y.y * g1);
             }
             __syncwarp();
             constexpr int L = HD / 8;           // lanes a half row
