@@ -5,8 +5,11 @@
 //   S[128 queries][128 positions] = Q K',    O[128 queries][HD] += P V'.
 // Everything enters as two fp16 planes, a value's rounding and what it left: Q (scaled by a power of two a row) and the
 // weights P 22 bits, K' = (c - 8) d 2^-3 and V' = (c - 8) d vs exactly (a 4-bit code times an 11-bit scale has at most 15
-// bits; vs a power of two). Each product is three MMAs, hi hi + lo hi + hi lo; the dropped lo lo is below 2^-22 of it, so
-// the result is as exact as fp32 arithmetic. Q and P are the MMA's A operand in tensor memory (P in the place of the
+// bits; vs a power of two). A query's weights of a step are scaled by a power of two of their own that brings the step's
+// largest to 2^14..2^15: fp16 has no steps below 2^-24, so beside weights left as they are, at most 1, one of 2^-25 would be
+// lost, and of a few thousand positions 12 nats below a sink the output lost 2e-3. So scaled, weights keep 22 bits down to
+// 2^-16 of their step's largest, and what is lost below is at most 2^-39 of it. Each product is three MMAs, hi hi + lo hi +
+// hi lo; the dropped lo lo is below 2^-22 of it, so the result is as exact as fp32 arithmetic. Q and P are the MMA's A operand in tensor memory (P in the place of the
 // scores it came from), K' and V' its B operand in shared memory.
 //   - warp 13 copies a step's cache tiles (contiguous 18 HD bytes each) into a ring of raw steps with bulk copies, warp 14
 //     looks their value scales over;
@@ -46,6 +49,7 @@ constexpr int PM_TILES = PM_P / KV4_P;
 constexpr int PM_RAW = 4;                   // raw steps in flight
 constexpr int PM_DQ_WARP = 4, PM_DQ = 8, PM_MMA_WARP = 12, PM_RAW_WARP = 13, PM_CARE_WARP = 14, PM_THREADS = 512;
 constexpr int PM_SLOTS = 8;                 // steps whose care and factors are kept
+constexpr float PM_WEIGHT_BITS = 15.f;      // a step's weights are multiplied by 2^(15 - its reference maximum)
 // tensor memory columns
 constexpr int TM_S = 0, TM_O = 256, TM_QH = 384, TM_QL = 448;
 
@@ -177,6 +181,9 @@ template <int NC> __device__ __forceinline__ void pm_commit(uint64_t* bar)
                      ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
 }
 
+// 2^k of a whole k <= 127; 0 below 2^-126, and of -inf and NaN.
+__device__ __forceinline__ float pow2i(float k) { return __int_as_float(((int)fmaxf(k, -127.f) + 127) << 23); }
+
 // Bits [0, 16) of the positions p0 .. p0 + 15 that v sees.
 __device__ __forceinline__ uint32_t seen16(const Vis& v, int p0)
 {
@@ -226,7 +233,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
     __shared__ __align__(8) uint64_t raw_full[PM_RAW], raw_empty[PM_RAW], care_full[PM_RAW], q_raw, q_read, drained, q_full, k_full[NP], v_full[NP], pv_done, o_free, s_full[2],
         p_full[2];
     __shared__ StepCare<NB> care[PM_SLOTS];
-    __shared__ float factor[PM_SLOTS][PM_Q];        // e^(old - new reference maximum) of a step and query
+    // of a step and query: e^(old - new reference maximum), and the power of two that its weights' product is multiplied by
+    __shared__ float2 factor[PM_SLOTS][PM_Q];
     __shared__ float fin_l[PM_Q];
     __shared__ uint32_t fin_poison[PM_Q];
     __shared__ uint32_t tmem_base;
@@ -414,7 +422,6 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             // every query of the warp sees all of the step (most steps): a form without masks, so that what most steps run is
             // short (the roles' code outgrows the instruction caches: no instruction was a warp's most frequent wait)
             const bool clear = at + PM_TILES <= i1 && tl.at(at) * KV4_P >= w_max_first && (tl.at(at + PM_TILES - 1) + 1) * KV4_P <= w_min_n;
-            uint64_t sum;
             auto step = [&](auto masked) {
                 constexpr bool MASKED = decltype(masked)::value;
                 // a group's scores: those not seen to -inf (the loops are kept rolled: unrolled, the three roles' code outgrew the
@@ -440,14 +447,18 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                     for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(ra[i]), __uint_as_float(rb[i])));
                 }
                 tmem_ld32(sbuf, ra);            // the first group again, behind the maximum's work
-                mx *= ks;
+                // reference maxima are whole (in log2 units), so that these factors are exact powers of two
+                mx = ceilf(mx * ks);
                 float f = 1.f;
                 if (mx > m + ATT_SLACK) {
-                    f = m == -INFINITY ? 0.f : ex2(m - mx);
+                    f = pow2i(m - mx);
                     l *= f;
                     m = mx;
                 }
-                factor[j % PM_SLOTS][threadIdx.x] = f;
+                float mu = mx == -INFINITY ? 0.f : mx - PM_WEIGHT_BITS;
+                if (mx - mu > PM_WEIGHT_BITS) mu = mx;          // (a maximum past 2^24: the difference was rounded up)
+                const float back = mx == -INFINITY ? 0.f : pow2i(mu - m);
+                factor[j % PM_SLOTS][threadIdx.x] = make_float2(f, back);
                 const StepCare<NB>& cr = care[j % PM_SLOTS];
                 if (cr.any_nan) {
                     // a value row with a NaN enters as zeros: it reaches the rows that see it here, and no other
@@ -457,9 +468,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                             if (cr.nan[b][g] & see) poison |= 1u << b;
                     }
                 }
-                const float mu = m == -INFINITY ? 0.f : m;
                 const uint64_t k2 = f2(ks, ks), m2 = f2(-mu, -mu);
-                sum = f2(0.f, 0.f);
+                uint64_t sum = f2(0.f, 0.f);
                 // a group's weights in place of its scores: 16 columns of their roundings, 16 of what those left
                 auto weights = [&](int g, uint32_t (&r)[32]) {
                     uint32_t lo[16];
@@ -484,12 +494,12 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                     if (g == 0) tmem_ld32(sbuf + 64, ra);
                     weights(g + 1, rb);
                 }
+                const float2 x = unf2(sum);
+                l = __fmaf_rn(x.x + x.y, back, l);
                 tmem_st_wait();
             };
             if (clear) step(std::false_type{});
             else step(std::true_type{});
-            const float2 x = unf2(sum);
-            l += x.x + x.y;
             tc_before();
             __syncwarp();
             if (lane == 0) pm_arrive(&p_full[j & 1]);
@@ -639,7 +649,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         };
         auto collect = [&](int j) {         // and goes into the output
             const StepCare<NB>& cr = care[j % PM_SLOTS];
-            const float f = factor[j % PM_SLOTS][qr], u = cr.vmax ? 1.f / cr.vs() : 1.f / 256.f;
+            const float2 fb = factor[j % PM_SLOTS][qr];
+            const float f = fb.x, u = (cr.vmax ? 1.f / cr.vs() : 1.f / 256.f) * fb.y;
             const uint64_t f1 = f2(f, f), u1 = f2(u, u);
             if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll
