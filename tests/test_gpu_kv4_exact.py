@@ -8,8 +8,10 @@ from test_gpu_kv4 import Cache, append, attend
 
 pytestmark = pytest.mark.gpu
 
-# heads, KV heads, head size, rows of the run: one block of 128 queries, two and more (pairs)
-SHAPES = [(4, 1, 64, 24), (4, 1, 128, 24), (8, 1, 64, 40), (16, 2, 128, 300)]
+# heads, KV heads, head size, rows of the run: rows by themselves; one block of 128 queries, two and more (pairs); the runs of
+# the other head sizes
+SHAPES = [(8, 2, 64, 1), (4, 2, 96, 1), (8, 1, 128, 1), (4, 1, 256, 1), (4, 1, 64, 24), (4, 1, 128, 24), (8, 1, 64, 40), (16, 2, 128, 300),
+          (4, 2, 96, 24), (2, 1, 256, 24)]
 
 
 def held(wl, k, v):

@@ -18,7 +18,11 @@
 // fp16 subnormals, their codes cut out by a mask, with 8 times the query's sum taken off, took 4 % less time and lost bits in
 // the MMA's sums: 2.3e-6 to 2.8e-6 of the output, against 2.5e-7 to 4.3e-7 so.) All products are exact, sums are fp32; the
 // block scales are applied outside: to each block's fp32 sums for the scores, and to the weights before they are split
-// for the values (p * d, per block). So the codes' rounding is the only one below fp32.
+// for the values (p * d, per block, times a power of two vs for fp16's range). fp16 has no steps below 2^-24, so the remainders
+// of those weights enter times 2^11 (their products have sums of their own): 22 bits down to p d = 2^-14 / vs, and at most
+// 2^-36 / vs lost below. vs is 2^8 where no value's scale reaches 2, so that is 2^-44 beside weights of up to 1, and a
+// position 26 nats below the largest still counts. (Without the 2^11, positions 15 nats below a sink lost a tenth of
+// their weight where the values are small; it costs 2 % of a row's time.)
 #include <algorithm>
 #include "wl_kv4.cuh"
 
@@ -250,7 +254,7 @@ __global__ void __launch_bounds__(128) k_kv4_read(Kv4Rows rows, const int32_t* p
 // ------------------------------------------------------------------------------------------------------------------
 
 // Running softmax of MT tiles of 8 queries: lane (g, c) keeps query g's reference maximum (in log2 units), its own share of
-// the sum, and the output's fragments (o[.][0,1] the rows of the weights' roundings, [2,3] of what they left).
+// the sum, and the output's fragments (o[.][0,1] the rows of the weights' roundings, [2,3] of what they left, times 2^11).
 template <int HD, int MT> struct AttState {
     float m[MT], l[MT], o[MT][HD / 8][4];
     float vs;                   // the values' scales are multiplied by vs = 2^k, so that a weight's product stays below 2^15
@@ -265,6 +269,8 @@ template <int HD, int MT> struct AttState {
         }
         vs = 256.f;
     }
+    // Output fragment j's value e (0, 1), times vs.
+    __device__ __forceinline__ float sum(int i, int j, int e) const { return fmaf(o[i][j][e + 2], 1.f / REM_UP, o[i][j][e]); }
 };
 
 // NT tiles of 16 positions (from positions tile0[.], one behind the other at sm) for MT query tiles. qf(i, b, s) gives the A
@@ -404,8 +410,8 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* sm, int lane, const int
                     p01 = f2(see & 1u ? x.x : 0.f, see & 2u ? x.y : 0.f);
                     p23 = f2(see & 4u ? y.x : 0.f, see & 8u ? y.y : 0.f);
                 }
-                split_h2(p01, a.x, a.y);
-                split_h2(p23, a.z, a.w);
+                split_h2_up(p01, a.x, a.y);
+                split_h2_up(p23, a.z, a.w);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) mma_add(st.o[i][4 * b + j], a, r0[j], r1[j]);
             }
@@ -567,10 +573,10 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float4 v;
-                v.x = (st.o[0][4 * b][e] + st.o[0][4 * b][e + 2]) * undo;
-                v.y = (st.o[0][4 * b + 1][e] + st.o[0][4 * b + 1][e + 2]) * undo;
-                v.z = (st.o[0][4 * b + 2][e] + st.o[0][4 * b + 2][e + 2]) * undo;
-                v.w = (st.o[0][4 * b + 3][e] + st.o[0][4 * b + 3][e + 2]) * undo;
+                v.x = st.sum(0, 4 * b, e) * undo;
+                v.y = st.sum(0, 4 * b + 1, e) * undo;
+                v.z = st.sum(0, 4 * b + 2, e) * undo;
+                v.w = st.sum(0, 4 * b + 3, e) * undo;
                 *reinterpret_cast<float4*>(so + (warp * 8 + g) * HD + 32 * b + 8 * c + 4 * e) = v;
             }
         if (c == 0) {
@@ -755,10 +761,10 @@ __global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float4 v;
-                v.x = (st.o[i][4 * b][e] + st.o[i][4 * b][e + 2]) * f;
-                v.y = (st.o[i][4 * b + 1][e] + st.o[i][4 * b + 1][e + 2]) * f;
-                v.z = (st.o[i][4 * b + 2][e] + st.o[i][4 * b + 2][e + 2]) * f;
-                v.w = (st.o[i][4 * b + 3][e] + st.o[i][4 * b + 3][e + 2]) * f;
+                v.x = st.sum(i, 4 * b, e) * f;
+                v.y = st.sum(i, 4 * b + 1, e) * f;
+                v.z = st.sum(i, 4 * b + 2, e) * f;
+                v.w = st.sum(i, 4 * b + 3, e) * f;
                 *reinterpret_cast<float4*>(dst + 32 * b + 8 * c + 4 * e) = v;
             }
         if (!whole && c == 0) reinterpret_cast<float2*>(a.ml)[th[i] * S + sp] = make_float2(st.m[i], state[i] == 2 ? NAN : st.l[i]);

@@ -151,6 +151,19 @@ __device__ __forceinline__ void split_h2(uint64_t ab, uint32_t& hi, uint32_t& lo
 }
 
 // The words of one lane's fragments: NB consecutive (planes of 4) 32-bit words.
+// The same with the remainders times 2^11: a remainder is 2^-11 of its value at most, so it is brought to the value's size, and
+// keeps its bits where the value is near fp16's smallest (for remainders whose products have sums of their own).
+constexpr float REM_UP = 2048.f;
+__device__ __forceinline__ void split_h2_up(uint64_t ab, uint32_t& hi, uint32_t& lo)
+{
+    const float2 v = unf2(ab);
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    const float2 f = __half22float2(h);
+    const float2 d = unf2(mul2(fma2(f2(f.x, f.y), f2(-1.f, -1.f), ab), f2(REM_UP, REM_UP)));
+    hi = h2_bits(h);
+    lo = h2_bits(__floats2half2_rn(d.x, d.y));
+}
+
 template <int HD> __device__ __forceinline__ void lane_words(const uint8_t* area, int half, int lane, uint32_t (&w)[HD / 32])
 {
     constexpr int NB = HD / 32;
