@@ -77,3 +77,45 @@ def test_weights_far_below_a_sink_keep_their_precision(wl, heads, kv_heads, hd, 
         off = np.abs(out[t] - want)
         assert (off <= bound).all(), (t, float((off / bound).max()), float(off.max() / np.abs(want).max()))
     assert wl.lib().wl_kernel_status(0) == 0
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,rows", SHAPES)
+@pytest.mark.parametrize("kscale", [1e-6, 1e-5, 2e-4, 1e-3, 1e5])
+def test_keys_of_any_scale(wl, heads, kv_heads, hd, rows, kscale):
+    """Keys whose scales are subnormal in fp16, or near its largest value, under queries that are large or small in return."""
+    rng = np.random.default_rng(heads * hd + rows)
+    n, scale = 700, hd ** -0.5
+    k, v = (rng.standard_normal((n, kv_heads, hd)) for _ in range(2))
+    c, hk, hv = held(wl, k * kscale, v)
+    q = (rng.standard_normal((rows, heads, hd)) * 2 / kscale).astype(np.float32)
+    pos = list(range(n - rows, n))
+    out = attend(wl, c, [0] * rows, pos, q, runs=rows)
+    for t in list(range(0, rows, 23)) + [rows - 1]:
+        want, bound = by_terms(q[t], hk, hv, pos[t], scale)
+        off = np.abs(out[t] - want)
+        assert (off <= bound).all(), (t, float((off / bound).max()))
+    assert wl.lib().wl_kernel_status(0) == 0
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,rows", SHAPES)
+def test_steps_with_keys_of_two_scales(wl, heads, kv_heads, hd, rows):
+    """Keys of 60000 and more among small ones, in steps of their own and beside them: the small ones keep what 2^-24 of a
+    step's largest key scale leaves them."""
+    rng = np.random.default_rng(heads * hd + rows)
+    n, scale = 700, hd ** -0.5
+    k, v = (rng.standard_normal((n, kv_heads, hd)) for _ in range(2))
+    k *= 0.05
+    big = [130, 131, 300, 690]
+    k[:, :, 0] = 0
+    k[big] = 0
+    k[big, :, 0] = -8.0 * 10240                         # (scales of 10240: held exactly)
+    c, hk, hv = held(wl, k, v)
+    q = rng.standard_normal((rows, heads, hd)).astype(np.float32)
+    q[:, :, 0] = 1e-4
+    q[:, ::2, 0] = -1e-4
+    pos = list(range(n - rows, n))
+    out = attend(wl, c, [0] * rows, pos, q, runs=rows)
+    for t in list(range(0, rows, 23)) + [rows - 1]:
+        want, bound = by_terms(q[t], hk, hv, pos[t], scale)
+        off = np.abs(out[t] - want)
+        assert (off <= bound).all(), (t, float((off / bound).max()))

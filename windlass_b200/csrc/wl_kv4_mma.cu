@@ -4,13 +4,17 @@
 // positions in steps of 128 (8 cache tiles). Scores and output are tcgen05 products with fp32 sums in tensor memory:
 //   S[128 queries][128 positions] = Q K',    O[128 queries][HD] += P V'.
 // Everything enters as two fp16 planes, a value's rounding and what it left: Q (scaled by a power of two a row) and the
-// weights P 22 bits, K' = (c - 8) d 2^-3 and V' = (c - 8) d vs exactly (a 4-bit code times an 11-bit scale has at most 15
-// bits; vs a power of two). A query's weights of a step are scaled by a power of two of their own that brings the step's
-// largest to 2^14..2^15: fp16 has no steps below 2^-24, so beside weights left as they are, at most 1, one of 2^-25 would be
-// lost, and of a few thousand positions 12 nats below a sink the output lost 2e-3. So scaled, weights keep 22 bits down to
-// 2^-16 of their step's largest, and what is lost below is at most 2^-39 of it. Each product is three MMAs, hi hi + lo hi +
-// hi lo; the dropped lo lo is below 2^-22 of it, so the result is as exact as fp32 arithmetic. Q and P are the MMA's A operand in tensor memory (P in the place of the
-// scores it came from), K' and V' its B operand in shared memory.
+// weights P 22 bits, K' = (c - 8) d and V' = (c - 8) d vs exactly (a 4-bit code times an 11-bit scale has at most 15 bits; vs
+// is a power of two, 2^8 unless a step has a value scale of 2 or more). Only in a step with a key scale of 2^13 or more, whose
+// products would pass fp16's largest, is K' (c - 8) d 2^-3; key scales below 2^-11 beside it lose bits, and so do value scales
+// below 2^-14 / vs: less than 2^-22 of the step's largest, both.
+// A query's weights of a step are scaled by a power of two of their own that brings the step's largest to 2^14..2^15: fp16
+// has no steps below 2^-24, so beside weights left as they are, at most 1, one of 2^-25 would be lost, and of a few
+// thousand positions 12 nats below a sink the output lost 2e-3. So scaled, weights keep 22 bits down to 2^-16 of their
+// step's largest, and what is lost below is at most 2^-39 of it.
+// Each product is three MMAs, hi hi + lo hi + hi lo; the dropped lo lo is below 2^-22 of it, so the result is as exact as fp32
+// arithmetic. Q and P are the MMA's A operand in tensor memory (P in the place of the scores it came from), K' and V' its B
+// operand in shared memory.
 //   - warp 13 copies a step's cache tiles (contiguous 18 HD bytes each) into a ring of raw steps with bulk copies, warp 14
 //     looks their value scales over;
 //   - warps 4-11 turn codes into the planes of K' and V' in the 128-byte-swizzled K-major layout. The order of a step's
@@ -202,6 +206,7 @@ __device__ __forceinline__ uint32_t slots16(uint32_t x)
 template <int NB> struct StepCare {
     uint32_t vmax;              // its float's bits; 0: all below 2
     int any_nan;
+    int big_keys;               // K' = (c - 8) d 2^-3
     uint32_t nan[NB][PM_P / 32];
     __device__ __forceinline__ float vs() const
     {
@@ -211,7 +216,7 @@ template <int NB> struct StepCare {
     __device__ __forceinline__ void clear()
     {
         vmax = 0u;
-        any_nan = 0;
+        any_nan = big_keys = 0;
         for (int b = 0; b < NB; ++b)
             for (int i = 0; i < PM_P / 32; ++i) nan[b][i] = 0u;
     }
@@ -368,7 +373,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             int e = mx > 0.f && mx <= 3e38f ? 13 - ilogbf(mx) : 0;
             e = e > 100 ? 100 : e < -100 ? -100 : e;
             const float up = ldexpf(1.f, e);
-            ks = ldexpf(1.f, 3 - e);
+            ks = ldexpf(1.f, -e);
 #pragma unroll 1
             for (int i = 0; i < HD / 64; ++i) {
                 uint32_t hi[32], lo[32];
@@ -447,8 +452,10 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                     for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(ra[i]), __uint_as_float(rb[i])));
                 }
                 tmem_ld32(sbuf, ra);            // the first group again, behind the maximum's work
+                const StepCare<NB>& cr = care[j % PM_SLOTS];
+                const float kj = cr.big_keys ? 8.f * ks : ks;
                 // reference maxima are whole (in log2 units), so that these factors are exact powers of two
-                mx = ceilf(mx * ks);
+                mx = ceilf(mx * kj);
                 float f = 1.f;
                 if (mx > m + ATT_SLACK) {
                     f = pow2i(m - mx);
@@ -459,7 +466,6 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 if (mx - mu > PM_WEIGHT_BITS) mu = mx;          // (a maximum past 2^24: the difference was rounded up)
                 const float back = mx == -INFINITY ? 0.f : pow2i(mu - m);
                 factor[j % PM_SLOTS][threadIdx.x] = make_float2(f, back);
-                const StepCare<NB>& cr = care[j % PM_SLOTS];
                 if (cr.any_nan) {
                     // a value row with a NaN enters as zeros: it reaches the rows that see it here, and no other
                     for (int g = 0; g < 4; ++g) {
@@ -468,7 +474,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                             if (cr.nan[b][g] & see) poison |= 1u << b;
                     }
                 }
-                const uint64_t k2 = f2(ks, ks), m2 = f2(-mu, -mu);
+                const uint64_t k2 = f2(kj, kj), m2 = f2(-mu, -mu);
                 uint64_t sum = f2(0.f, 0.f);
                 // a group's weights in place of its scores: 16 columns of their roundings, 16 of what those left
                 auto weights = [&](int g, uint32_t (&r)[32]) {
@@ -523,7 +529,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
         // K' of step j (a CTA of a pair: its half of the positions): (tile, half) units, a position's 8 dims x NB a lane
         auto keys = [&](int j) {
             uint8_t* kj = kh + j % NP * 2 * PL;
-            const __half2 k2 = __float2half2_rn(0.125f);
+            const __half2 k2 = __float2half2_rn(care[j % PM_SLOTS].big_keys ? 0.125f : 1.f);
             const bool whole = all_live(i0 + PM_TILES * j);
 #pragma unroll 1
             for (int u = 0; u < 2 / NC; ++u) {
@@ -841,8 +847,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 for (int j = max(0, issued - PM_RAW); j < issued; ++j) pm_drain(&raw_full[j % PM_RAW], (uint32_t)(j / PM_RAW & 1));
             }
         } else if (warp == PM_CARE_WARP) {
-            // ---- what the values' scales of a step call for: nothing, unless one is 2 or more or NaN (or what lies in unseen
-            // places looks so). A slot's step of PM_SLOTS before is behind every warp: its raw tiles' place was given up twice.
+            // ---- what the scales of a step call for: nothing, unless a value's is 2 or more, a key's 2^13 or more, or one NaN (or
+            // what lies in unseen places looks so). A slot's step of PM_SLOTS before is behind every warp: its raw tiles' place
+            // was given up twice.
             constexpr int words = KV4_P * NB / 2;           // of two fp16 scales, of a tile
             uint32_t used = 0u;                             // slots that are not clear
             for (int j = 0; j < steps; ++j) {
@@ -850,20 +857,27 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 pm_wait(&raw_full[j % PM_RAW], (uint32_t)(j / PM_RAW & 1), a.err, abort);
                 uint32_t any = 0u;
                 for (int t = 0; t < PM_TILES; ++t)
-                    if (lane < words && at + t < i1) any |= reinterpret_cast<const uint32_t*>(raw_step(j) + t * TB + 17 * HD)[lane];
+                    if (lane < words && at + t < i1) {
+                        const uint32_t k = reinterpret_cast<const uint32_t*>(raw_step(j) + t * TB + 16 * HD)[lane];
+                        any |= reinterpret_cast<const uint32_t*>(raw_step(j) + t * TB + 17 * HD)[lane];
+                        any |= k & k << 1 & k << 2;             // (the exponent's top three bits: 2^13, infinity or NaN)
+                    }
                 if (__any_sync(0xffffffffu, any & 0x40004000u) || (used >> slot & 1u)) {
                     StepCare<NB>& cr = care[slot];
                     if (lane == 0) cr.clear();
                     __syncwarp();
                     uint32_t big = 0u;
-                    bool nans = false;
+                    bool nans = false, big_keys = false;
                     for (int t = 0; t < PM_TILES; ++t) {
                         if (lane >= words || at + t >= i1) continue;
                         const uint32_t x = reinterpret_cast<const uint32_t*>(raw_step(j) + t * TB + 17 * HD)[lane];
+                        const uint32_t k = reinterpret_cast<const uint32_t*>(raw_step(j) + t * TB + 16 * HD)[lane];
                         for (int e = 0; e < 2; ++e) {
                             const int r = (2 * lane + e) / NB, b = (2 * lane + e) % NB;
-                            const uint32_t d = (x >> (16 * e)) & 0x7FFFu;
-                            if (d < 0x4000u || !live(at + t, r)) continue;
+                            const uint32_t d = (x >> (16 * e)) & 0x7FFFu, kd = (k >> (16 * e)) & 0x7FFFu;
+                            if (!live(at + t, r)) continue;
+                            big_keys |= kd >= 0x7000u && kd <= 0x7C00u;
+                            if (d < 0x4000u) continue;
                             if (d > 0x7C00u) {
                                 nans = true;
                                 atomicOr(&cr.nan[b][t / 2], 1u << (8 * (r % 8 / 2) + 2 * (2 * (t & 1) + r / 8) + r % 2));
@@ -874,11 +888,13 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                     }
                     big = __reduce_max_sync(0xffffffffu, big);
                     nans = __any_sync(0xffffffffu, nans);
+                    big_keys = __any_sync(0xffffffffu, big_keys);
                     if (lane == 0) {
                         cr.vmax = big;
                         cr.any_nan = nans;
+                        cr.big_keys = big_keys;
                     }
-                    used = big || nans ? used | 1u << slot : used & ~(1u << slot);
+                    used = big || nans || big_keys ? used | 1u << slot : used & ~(1u << slot);
                 }
                 __syncwarp();
                 if (lane == 0) pm_arrive(&care_full[j % PM_RAW]);
