@@ -119,3 +119,22 @@ def test_steps_with_keys_of_two_scales(wl, heads, kv_heads, hd, rows):
         want, bound = by_terms(q[t], hk, hv, pos[t], scale)
         off = np.abs(out[t] - want)
         assert (off <= bound).all(), (t, float((off / bound).max()))
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,rows", SHAPES)
+@pytest.mark.parametrize("size", [1e8, 1e9, 8e9, 1e33, 1e36, 3e38])
+def test_queries_of_any_finite_size(wl, heads, kv_heads, hd, rows, size):
+    """Finite scores of finite queries, up to the largest floats: one position has a key where the queries are that large, and takes
+    all of the weight."""
+    rng = np.random.default_rng(hd + rows)
+    n, scale, kv = 60, hd ** -0.5, 2.0 ** -6
+    k, v = np.zeros((n, kv_heads, hd)), rng.standard_normal((n, kv_heads, hd))
+    k[7, :, 3] = -8 * kv
+    c, hk, hv = held(wl, k, v)
+    q = np.zeros((rows, heads, hd), np.float32)
+    q[:, :, 3] = -size
+    pos = list(range(n - rows, n)) if rows <= 40 else [n - 1] * rows
+    out = attend(wl, c, [0] * rows, pos, q, runs=rows)
+    # a weight of 1 times an exact value, divided by the sum 1: a few roundings of 2^-22
+    want = np.repeat(hv[7], heads // kv_heads, 0)
+    assert (np.abs(out - want) <= 2.0 ** -20 * np.abs(want)).all()

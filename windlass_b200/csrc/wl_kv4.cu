@@ -444,8 +444,7 @@ __device__ __forceinline__ void load_query(const float* x, int lane, float f, ui
     }
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    int e = mx > 0.f && mx <= 3e38f ? 13 - ilogbf(mx) : 0;
-    e = e > 100 ? 100 : e < -100 ? -100 : e;
+    const int e = mx > 0.f && mx <= FLT_MAX ? min(100, 13 - ilogbf(mx)) : 0;      // (-114 at least)
     const float up = ldexpf(1.f, e);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {

@@ -1,6 +1,7 @@
 // Device code shared by the kernels of the 4-bit KV cache (wl_kv4.cu, wl_kv4_mma.cu): the cache's layout, the codes' way into
 // fp16, visible positions, and the join of ranges.
 #pragma once
+#include <cfloat>
 #include <climits>
 #include <cstdint>
 #include <cuda_fp16.h>

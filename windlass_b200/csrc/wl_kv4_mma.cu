@@ -370,8 +370,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                     const float4 v = x[i];
                     mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x * f), fabsf(v.y * f)), fmaxf(fabsf(v.z * f), fabsf(v.w * f))));
                 }
-            int e = mx > 0.f && mx <= 3e38f ? 13 - ilogbf(mx) : 0;
-            e = e > 100 ? 100 : e < -100 ? -100 : e;
+            const int e = mx > 0.f && mx <= FLT_MAX ? min(100, 13 - ilogbf(mx)) : 0;      // (-114 at least)
             const float up = ldexpf(1.f, e);
             ks = ldexpf(1.f, -e);
 #pragma unroll 1
