@@ -336,7 +336,7 @@ int32_t wl_kv4_read(void* const* dev_caches, const int32_t* dev_pos, int32_t T, 
  * to those with j > dev_pos[t] - window or j < sinks (the first tokens stay visible). dev_out [T][heads * head_dim]. The
  * rows come in runs of rows_per_seq consecutive rows that read the same cache (T a multiple of it; 1 = every row may
  * have its own): runs of more than 16 rows (prompts) share the cache's tiles, and only a run's first cache pointer is
- * read. With runs of up to 16 rows a row's result does not depend on the other rows of a call of up to 64 rows.
+ * read. With runs of up to 16 rows a row's result does not depend on the other rows of the call.
  * dev_workspace (16-byte aligned, wl_kv4_workspace_bytes of the same arguments) is initialised once with
  * wl_kv4_workspace_init and then kept for any calls that are ordered after one another; calls that may overlap (two
  * streams, two graphs in flight) need a workspace each. */

@@ -820,19 +820,18 @@ Kv4Plan kv4_plan(int T, int R, int heads, int kv_heads, int head_dim, int64_t ca
         p.S = p.s_max;
     } else {
         // the most ranges of one row, from the shape alone (a row's bits must not depend on the others): one row's
-        // CTAs fill the SMs two deep. Beyond 64 rows the rows alone do.
+        // CTAs fill the SMs two deep.
         ctas = (int64_t)T * kv_heads * p.MG;
-        p.s_max = T > 64 ? 1 : std::max(1, std::min(ATT_MAX_RANGES, 2 * 148 / (kv_heads * p.MG)));
+        p.s_max = std::max(1, std::min(ATT_MAX_RANGES, 2 * 148 / (kv_heads * p.MG)));
         p.S = (int)std::max<int64_t>(1, std::min<int64_t>(p.s_max, (tiles + ATT_TPS - 1) / ATT_TPS));
         // enough rows for the SMs: short ones are walked by one CTA each (64 rows with a window of 1024: 49.7 us with a CTA a
-        // range); a row of more than 8 ranges among them is still spread, so that the call does not wait for it
-        p.alone = ctas >= 2 * 148 ? 8 : 0;
+        // range); a row of more than 8 ranges among them is still spread, so that the call does not wait for it. Beyond 64
+        // rows every row is walked by one CTA a KV head, whatever its length, so that calls of any size need no partials: the
+        // same ranges joined in the same order, so the same bits, but the call does wait for its longest row.
+        p.alone = T > 64 || ctas > KV4_TICKETS ? INT_MAX : ctas >= 2 * 148 ? 8 : 0;
         if (p.alone >= p.S) p.S = 1;
     }
-    if (ctas > KV4_TICKETS) {
-        p.S = p.s_max = 1;
-        p.alone = 1;
-    }
+    if (p.runs && ctas > KV4_TICKETS) p.S = p.s_max = 1;
     p.part_floats = p.S > 1 ? (int64_t)T * heads * p.S * (head_dim + 2) : 0;
     return p;
 }
