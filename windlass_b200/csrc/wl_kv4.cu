@@ -780,6 +780,7 @@ constexpr int64_t KV4_TICKETS = 1 << 18;    // tickets at the head of a workspac
 // cores and 67 by k_kv4_attn_run; 12 rows of 500 positions: 9, 21 and 34; 16 rows of 3000: 27, 32 and 64; the other way
 // round where runs are few and long (10 rows, 64 heads on 8, 20000 positions: 96, 65 and 161), which the shape does not tell.
 constexpr int RUN_MIN_ROWS = 17;
+constexpr int RUN_MAX_RANGES = 32;          // ranges a run may be cut into
 
 // How a call is cut.
 struct Kv4Plan {
@@ -810,7 +811,7 @@ Kv4Plan kv4_plan(int T, int R, int heads, int kv_heads, int head_dim, int64_t ca
         ctas = (int64_t)(T / R) * p.q_blocks * kv_heads;
         const int64_t slots = p.mma ? 148 : 2 * 148;
         double least = 1e30;
-        for (int S = 1; S <= std::max<int64_t>(1, std::min<int64_t>(32, tiles / 16)); ++S) {
+        for (int S = 1; S <= std::max<int64_t>(1, std::min<int64_t>(RUN_MAX_RANGES, tiles / 16)); ++S) {
             const double cost = (double)((ctas * S + slots - 1) / slots) * ((double)tiles / S + 12.0);
             if (cost < least) {
                 least = cost;
@@ -836,29 +837,28 @@ Kv4Plan kv4_plan(int T, int R, int heads, int kv_heads, int head_dim, int64_t ca
     return p;
 }
 
-template <typename K> void set_smem(K kern, size_t bytes)
+template <int HD, bool ALONE> void attn_rows(const Kv4Att& a, const Kv4Plan& p, cudaStream_t s)
 {
-    // (an attribute of the function on the current device; setting it again costs under a microsecond and is allowed
-    // during a capture)
-    if (bytes > 48 * 1024) WL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    constexpr int smem = ATT_WARPS * ATT_STAGES * 2 * kv4_tile_bytes(HD) + ATT_WARPS * 8 * HD * 4;
+    static std::atomic<bool> done[64];
+    ensure_smem_attr(k_kv4_attn<HD, ALONE>, smem, done);
+    launch(k_kv4_attn<HD, ALONE>, dim3(p.S, a.kv_heads * p.MG, a.T), dim3(32 * ATT_WARPS), smem, s, a);
+    note_launch();
 }
 
 template <int HD> void attn_rows(const Kv4Att& a, const Kv4Plan& p, cudaStream_t s)
 {
-    const size_t smem = (size_t)ATT_WARPS * ATT_STAGES * 2 * kv4_tile_bytes(HD) + ATT_WARPS * 8 * HD * 4;
-    auto kern = p.alone ? k_kv4_attn<HD, true> : k_kv4_attn<HD, false>;
-    set_smem(kern, smem);
-    launch(kern, dim3(p.S, a.kv_heads * p.MG, a.T), dim3(32 * ATT_WARPS), smem, s, a);
-    note_launch();
+    p.alone ? attn_rows<HD, true>(a, p, s) : attn_rows<HD, false>(a, p, s);
 }
 
 template <int HD> void attn_runs(const Kv4Att& a, const Kv4Plan& p, cudaStream_t s)
 {
     constexpr int MT = HD <= 128 ? 2 : 1;
     // the ring and the queries' fragments; then the join's factors in their place
-    const size_t smem = std::max(4 * kv4_tile_bytes(HD) + (size_t)RUN_WARPS * MT * (HD / 32) * 2 * 512,
-                                 (size_t)RUN_WARPS * 8 * MT * (3 * p.S + 1) * 4);
-    set_smem(k_kv4_attn_run<HD, MT>, smem);
+    constexpr int smem = 4 * kv4_tile_bytes(HD) + RUN_WARPS * MT * (HD / 32) * 2 * 512;
+    static_assert(smem >= RUN_WARPS * 8 * MT * (3 * RUN_MAX_RANGES + 1) * 4, "the join's factors fit");
+    static std::atomic<bool> done[64];
+    ensure_smem_attr(k_kv4_attn_run<HD, MT>, smem, done);
     launch(k_kv4_attn_run<HD, MT>, dim3(p.q_blocks * p.S, a.kv_heads, a.T / a.R), dim3(32 * RUN_WARPS), smem, s, a, p.q_blocks);
     note_launch();
 }

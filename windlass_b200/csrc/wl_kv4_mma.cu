@@ -923,7 +923,8 @@ template <int HD, int NC> void launch_mma(const Kv4Att& a, int q_blocks, cudaStr
 {
     auto kern = k_kv4_attn_mma<HD, NC>;
     constexpr int smem = pm_smem(HD, NC);
-    WL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static std::atomic<bool> done[64];
+    ensure_smem_attr(kern, smem, done);
     // (launched plainly: it takes all of an SM's tensor memory, so it does not start beside another kernel's end)
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(q_blocks * a.S, a.kv_heads, a.T / a.R);

@@ -8,6 +8,8 @@
 // matvec kernels). Because every kernel waits, the ordering stays transitive: kernel N+1 cannot complete before
 // kernel N has. Outside a PDL launch (or after a memcpy/memset node) the two instructions are no-ops.
 #pragma once
+#include <atomic>
+#include <mutex>
 #include <utility>
 #include <cuda_runtime.h>
 #include "wl_common.h"
@@ -54,6 +56,22 @@ inline void launch_cluster(void (*kern)(P...), dim3 grid, dim3 block, size_t sme
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     WL_CUDA(cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...));
+}
+
+// Raises a kernel's dynamic shared-memory limit once per device; `done` is that kernel's own per-device flags (one
+// set per template instantiation, so kernels of the same signature do not share them). Safe from several host threads.
+template <typename Kernel>
+inline void ensure_smem_attr(Kernel kernel, int bytes, std::atomic<bool> (&done)[64])
+{
+    static std::mutex mu;
+    int dev = 0;
+    WL_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) WL_THROW(WL_EINVAL, "device ordinal out of range");
+    if (done[dev].load(std::memory_order_acquire)) return;
+    std::lock_guard<std::mutex> lock(mu);
+    if (done[dev].load(std::memory_order_relaxed)) return;
+    WL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done[dev].store(true, std::memory_order_release);
 }
 
 }  // namespace k

@@ -1266,22 +1266,6 @@ void make_weight_map(int type, const uint8_t* w, int64_t rows_total, int64_t row
     out->valid = true;
 }
 
-// Raises a kernel's dynamic shared-memory limit once per device; `done` is that kernel's own per-device flags (one
-// set per template instantiation, so kernels of the same signature do not share them). Safe from several host threads.
-template <typename Kernel>
-static void ensure_smem_attr(Kernel kernel, int bytes, std::atomic<bool> (&done)[64])
-{
-    static std::mutex mu;
-    int dev = 0;
-    WL_CUDA(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64) WL_THROW(WL_EINVAL, "device ordinal out of range");
-    if (done[dev].load(std::memory_order_acquire)) return;
-    std::lock_guard<std::mutex> lock(mu);
-    if (done[dev].load(std::memory_order_relaxed)) return;
-    WL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    done[dev].store(true, std::memory_order_release);
-}
-
 template <int NC, bool TILED, bool PAIRS, int NW = 8, bool AR = false> struct Q4Attr {
     static std::atomic<bool> done[64];
     static void ensure() { ensure_smem_attr(k_mmv_q4k<NC, TILED, PAIRS, NW, AR>, Q4Layout<NC, NW>::SMEM, done); }

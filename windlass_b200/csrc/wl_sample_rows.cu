@@ -766,7 +766,10 @@ void sample_rows(const float* logits, int64_t ld, int V, int rows, const wl_samp
     const size_t smem = (sizeof(Row) + 15) / 16 * 16 + (in_smem ? (size_t)slice * 4 : 0);
     int bits = 0;
     while ((1ll << bits) < V) ++bits;
-    WL_CUDA(cudaFuncSetAttribute(k_sample_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // (the limit is the function's, not the launch's: the largest of all vocabularies, so that no other thread's call lowers it
+    // between this one's limit and its launch)
+    static std::atomic<bool> done[64];
+    ensure_smem_attr(k_sample_rows, (int)((sizeof(Row) + 15) / 16 * 16 + SR_SLICE_MAX * 4), done);
     for (int r0 = 0; r0 < rows; r0 += 65535) {
         launch_cluster(k_sample_rows, dim3(C, std::min(rows - r0, 65535)), dim3(SR_THREADS), smem, s, C, logits + (int64_t)r0 * ld, ld, V,
                        std::min(51, 62 - bits), opts + r0, ids + r0, slice, in_smem ? 1 : 0);
