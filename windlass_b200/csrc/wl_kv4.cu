@@ -608,6 +608,9 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const
         if (!ALONE) break;
         if (r1 < i1) __syncthreads();       // (the next range's sums go to the same place)
     }
+    // (after a wait that gave up, the warp's copies from step i on are still in flight; else none is)
+    if (!ok && lane == 0)
+        for (int x = i; x < min(steps, i + ST); ++x) mbar_drain(&bars[warp][x % ST], (uint32_t)(x / ST & 1));
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
         const int it = threadIdx.x + NT * k, h = it / (HD / 4), d = it % (HD / 4) * 4;
@@ -727,7 +730,8 @@ __global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att
     AttState<HD, MT> st;
     st.init();
     auto qf = [&](int i, int b, int s) { return wq[((i * NB + b) * 2 + s) * 32 + lane]; };
-    for (int i = 0; i < nt; ++i) {
+    int i = 0;
+    for (; i < nt; ++i) {
         if (!__all_sync(0xffffffffu, mbar_wait_bounded(&fullb[i % ST], (uint32_t)(i / ST & 1), a.err, 22))) break;
         const int tile0 = tl.at(i0 + i) * KV4_P;
         if (tile0 < w_n && (tile0 + KV4_P > w_first || tile0 < w_sink)) {
@@ -746,6 +750,9 @@ __global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att
         }
         if (!__all_sync(0xffffffffu, ok)) break;
     }
+    // (after a wait that gave up, the copies from tile i on are still in flight; else none is)
+    if (threadIdx.x == 0)
+        for (int x = i; x < min(nt, i + ST); ++x) mbar_drain(&fullb[x % ST], (uint32_t)(x / ST & 1));
     const float undo = 1.f / st.vs;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {

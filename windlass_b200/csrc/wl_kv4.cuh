@@ -151,7 +151,6 @@ __device__ __forceinline__ void split_h2(uint64_t ab, uint32_t& hi, uint32_t& lo
     lo = h2_bits(__floats2half2_rn(d.x, d.y));
 }
 
-// The words of one lane's fragments: NB consecutive (planes of 4) 32-bit words.
 // The same with the remainders times 2^11: a remainder is 2^-11 of its value at most, so it is brought to the value's size, and
 // keeps its bits where the value is near fp16's smallest (for remainders whose products have sums of their own).
 constexpr float REM_UP = 2048.f;
@@ -165,6 +164,7 @@ __device__ __forceinline__ void split_h2_up(uint64_t ab, uint32_t& hi, uint32_t&
     lo = h2_bits(__floats2half2_rn(d.x, d.y));
 }
 
+// The words of one lane's fragments: NB consecutive (planes of 4) 32-bit words.
 template <int HD> __device__ __forceinline__ void lane_words(const uint8_t* area, int half, int lane, uint32_t (&w)[HD / 32])
 {
     constexpr int NB = HD / 32;
@@ -362,6 +362,14 @@ __device__ __noinline__ void join_ranges(const float* ml_, const float* part, fl
         const float inv = wh[3 * n];
         *reinterpret_cast<float4*>(out + row.at(h) * HD + d) =
             make_float4(__fmul_rn(o.x, inv), __fmul_rn(o.y, inv), __fmul_rn(o.z, inv), __fmul_rn(o.w, inv));
+    }
+}
+
+// After a wait gave up: what is still in flight ends before the CTA does (bounded as well).
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity)
+{
+    const unsigned long long t0 = globaltimer_ns();
+    while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 <= MBAR_WAIT_NS) {
     }
 }
 

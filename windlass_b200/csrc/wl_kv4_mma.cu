@@ -88,13 +88,6 @@ template <bool CLUSTER = false> __device__ __forceinline__ bool pm_wait(uint64_t
     }
     return true;
 }
-// After a wait gave up: what is still in flight ends before the CTA does (bounded as well).
-__device__ __forceinline__ void pm_drain(uint64_t* bar, uint32_t parity)
-{
-    const unsigned long long t0 = globaltimer_ns();
-    while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 <= MBAR_WAIT_NS) {
-    }
-}
 __device__ __forceinline__ void pm_arrive(uint64_t* bar)
 {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -805,7 +798,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
             pv(steps - 1);
             if (*abort) {
                 pm_commit<NC>(&drained);
-                pm_drain(&drained, 0u);
+                mbar_drain(&drained, 0u);
             }
         } else if (NC == 2 && warp == PM_MMA_WARP && lane == 0 && steps > 0) {
             // ---- a pair's other CTA: what the MMAs wait for, on to the first CTA in the order of its waits, one arrival for all
@@ -842,8 +835,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
                 issued = j + 1;
             }
             if (*abort) {
-                pm_drain(&q_raw, 0u);
-                for (int j = max(0, issued - PM_RAW); j < issued; ++j) pm_drain(&raw_full[j % PM_RAW], (uint32_t)(j / PM_RAW & 1));
+                mbar_drain(&q_raw, 0u);
+                for (int j = max(0, issued - PM_RAW); j < issued; ++j) mbar_drain(&raw_full[j % PM_RAW], (uint32_t)(j / PM_RAW & 1));
             }
         } else if (warp == PM_CARE_WARP) {
             // ---- what the scales of a step call for: nothing, unless a value's is 2 or more, a key's 2^13 or more, or one NaN (or
