@@ -320,8 +320,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_kv4_attn_mma(const Kv4Att a, 
     // a query's index in the call's queries, or -1 past the run
     auto query = [&](int qi) -> int64_t { return qi < nq ? (int64_t)(run * a.R + qi / G) * a.heads + kvh * G + qi % G : -1; };
     if (warp < 4) {
-        // the queries, rows of HD floats far from one another, by bulk copies
-        const int64_t th = query(q0 + threadIdx.x);
+        // the queries, rows of HD floats far from one another, by bulk copies (none of a padding or refused row)
+        const int64_t th = kv4_row_state(base, qpos, a.capacity) ? -1 : query(q0 + threadIdx.x);
         const uint32_t rows = __ballot_sync(0xffffffffu, th >= 0);
         if (lane == 0) mbar_expect_tx(&q_raw, __popc(rows) * HD * 4);
         __syncwarp();
