@@ -313,8 +313,9 @@ int32_t wl_sample(const float* dev_logits, int32_t V, double temperature, double
  * padding: nothing is read or written for it (its attention and read-back give zeros). A row whose position is not
  * below capacity, or whose cache is null or not 16-byte aligned, is refused on the device: nothing is written to a
  * cache, its attention and read-back give NaN. head_dim is 64, 96, 128 or 256, heads a multiple of kv_heads; other
- * shapes return WL_EUNSUPPORTED. Float buffers are 16-byte aligned, contiguous, and on the current device (WL_EINVAL
- * otherwise). The calls enqueue on `stream` and return; they allocate nothing and may be captured into a graph. ---- */
+ * shapes return WL_EUNSUPPORTED. Float buffers are 16-byte aligned (the rope table 4), contiguous, and on the current
+ * device; dev_caches and dev_pos are aligned to their elements, on the current device or in pinned host memory (WL_EINVAL
+ * otherwise: the calls look at every pointer that they are given, not at the caches behind dev_caches). The calls enqueue on `stream` and return; they allocate nothing and may be captured into a graph. ---- */
 
 /* Bytes of the cache of one layer of one sequence with room for `positions` positions. */
 int32_t wl_kv4_bytes(int32_t kv_heads, int32_t head_dim, int64_t positions, int64_t* bytes);
@@ -349,8 +350,8 @@ int32_t wl_kv4_workspace_bytes(int32_t T, int32_t rows_per_seq, int32_t heads, i
 int32_t wl_kv4_workspace_init(void* dev_workspace, int64_t workspace_bytes, void* stream);
 
 /* The choice of wl_forward_batch_sample_opts on `rows` rows of V device floats, row r at dev_logits + r * ld (ld >= V), with
- * the options dev_opts[r] (device memory, 8-byte aligned): dev_ids[r] = the chosen id, or -1 where temperature > 0 and
- * the draw is not in [0, 1). Enqueues one launch on `stream`; needs no workspace and may be captured into a graph, whose
+ * the options dev_opts[r] (device memory, 8-byte aligned): dev_ids[r] (device or pinned host memory) = the chosen id, or -1
+ * where temperature > 0 and the draw is not in [0, 1). Enqueues one launch on `stream`; needs no workspace and may be captured into a graph, whose
  * replays read the options anew. */
 int32_t wl_sample_rows(const float* dev_logits, int64_t ld, int32_t V, int32_t rows, const wl_sample_opts* dev_opts,
                        int32_t* dev_ids, void* stream);

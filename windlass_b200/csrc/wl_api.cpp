@@ -2,10 +2,10 @@
 // kernel-level test exports. No function aborts or exits; failures return a status and set wl_last_error().
 #include <algorithm>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <string>
-#include <utility>
 #include <vector>
 #include "../../include/windlass.h"
 #include "wl_common.h"
@@ -715,19 +715,32 @@ int32_t wl_sample(const float* dev_logits, int32_t V, double temperature, double
 }
 
 namespace {
-// Empty when `p` is 16-byte aligned memory of the current device (or managed memory); else what is wrong with it.
-std::string device_buffer_fault(const void* p, const char* what, size_t align = 16)
+// A buffer of a call: aligned memory of the current device, or managed memory; with `table` set also pinned host memory that
+// the device reads at the same address (pointers, positions, ids).
+struct DevBuffer {
+    const void* p;
+    const char* what;
+    size_t align = 16;
+    bool table = false;
+};
+// What is wrong with the first of the buffers that is not as it says; empty when all are. Null pointers and alignments come
+// first: they need no device.
+std::string device_buffers_fault(std::initializer_list<DevBuffer> list)
 {
-    if (!p) return std::string(what) + " is null";
-    if ((uintptr_t)p % align) return std::string(what) + " must be " + std::to_string(align) + "-byte aligned";
-    cudaPointerAttributes a{};
+    for (const DevBuffer& b : list) {
+        if (!b.p) return std::string(b.what) + " is null";
+        if ((uintptr_t)b.p % b.align) return std::string(b.what) + " must be " + std::to_string(b.align) + "-byte aligned";
+    }
     int dev = 0;
     WL_CUDA(cudaGetDevice(&dev));
-    WL_CUDA(cudaPointerGetAttributes(&a, p));
-    if (a.type == cudaMemoryTypeManaged) return "";
-    if (a.type != cudaMemoryTypeDevice) return std::string(what) + " is not device memory";
-    if (a.device != dev)
-        return std::string(what) + " is on device " + std::to_string(a.device) + ", the current device is " + std::to_string(dev);
+    for (const DevBuffer& b : list) {
+        cudaPointerAttributes a{};
+        WL_CUDA(cudaPointerGetAttributes(&a, b.p));
+        if (a.type == cudaMemoryTypeManaged || (b.table && a.type == cudaMemoryTypeHost && a.devicePointer == b.p)) continue;
+        if (a.type != cudaMemoryTypeDevice) return std::string(b.what) + " is not device memory";
+        if (a.device != dev)
+            return std::string(b.what) + " is on device " + std::to_string(a.device) + ", the current device is " + std::to_string(dev);
+    }
     return "";
 }
 
@@ -740,13 +753,10 @@ int32_t kv4_shape(const char* name, int32_t heads, int32_t kv_heads, int32_t hea
     return WL_OK;
 }
 
-#define WL_CHECK_BUFFERS(name, ...)                                                                     \
-    do {                                                                                                \
-        const std::pair<const void*, const char*> list_[] = {__VA_ARGS__};                              \
-        for (const auto& b_ : list_) {                                                                  \
-            const std::string f_ = device_buffer_fault(b_.first, b_.second);                            \
-            if (!f_.empty()) return wl::fail(WL_EINVAL, std::string(name) + ": " + f_);                 \
-        }                                                                                               \
+#define WL_CHECK_BUFFERS(name, ...)                                                       \
+    do {                                                                                  \
+        const std::string f_ = device_buffers_fault({__VA_ARGS__});                       \
+        if (!f_.empty()) return wl::fail(WL_EINVAL, std::string(name) + ": " + f_);       \
     } while (0)
 }  // namespace
 
@@ -771,7 +781,10 @@ int32_t wl_kv4_append(const float* dev_q, float* dev_q_out, const float* dev_k, 
         if (!dev_q || !dev_q_out || !dev_k || !dev_v || !dev_caches || !dev_pos || (rope_dims > 0 && !dev_rope_table))
             return wl::fail(WL_EINVAL, "wl_kv4_append: null pointer");
         if (T == 0) return WL_OK;
-        WL_CHECK_BUFFERS("wl_kv4_append", {dev_q, "dev_q"}, {dev_q_out, "dev_q_out"}, {dev_k, "dev_k"}, {dev_v, "dev_v"});
+        // (without rotated dims the rope table is not read)
+        WL_CHECK_BUFFERS("wl_kv4_append", {dev_q, "dev_q"}, {dev_q_out, "dev_q_out"}, {dev_k, "dev_k"}, {dev_v, "dev_v"},
+                         {dev_caches, "dev_caches", 8, true}, {dev_pos, "dev_pos", 4, true},
+                         {rope_dims > 0 ? dev_rope_table : dev_q, "dev_rope_table", 4});
         wl::k::kv4_append(dev_q, dev_q_out, dev_k, dev_v, T, heads, kv_heads, head_dim, dev_rope_table, rope_dims, neox ? 1 : 0,
                           wl::k::Kv4Cache{dev_caches, 8, 0}, dev_pos, capacity, (cudaStream_t)stream);
         return WL_OK;
@@ -786,7 +799,7 @@ int32_t wl_kv4_read(void* const* dev_caches, const int32_t* dev_pos, int32_t T, 
         if (const int32_t st = kv4_shape("wl_kv4_read", kv_heads, kv_heads, head_dim, capacity)) return st;
         if (!dev_caches || !dev_pos || !dev_k || !dev_v) return wl::fail(WL_EINVAL, "wl_kv4_read: null pointer");
         if (T == 0) return WL_OK;
-        WL_CHECK_BUFFERS("wl_kv4_read", {dev_k, "dev_k"}, {dev_v, "dev_v"});
+        WL_CHECK_BUFFERS("wl_kv4_read", {dev_k, "dev_k"}, {dev_v, "dev_v"}, {dev_caches, "dev_caches", 8, true}, {dev_pos, "dev_pos", 4, true});
         wl::k::kv4_read(wl::k::Kv4Cache{dev_caches, 8, 0}, dev_pos, T, kv_heads, head_dim, capacity, dev_k, dev_v, (cudaStream_t)stream);
         return WL_OK;
     });
@@ -820,6 +833,7 @@ int32_t wl_kv4_workspace_init(void* dev_workspace, int64_t workspace_bytes, void
     return guarded([&]() -> int32_t {
         if (!dev_workspace) return wl::fail(WL_EINVAL, "wl_kv4_workspace_init: null pointer");
         if (workspace_bytes < (int64_t)wl::k::kv4_ticket_bytes()) return wl::fail(WL_EINVAL, "wl_kv4_workspace_init: the workspace is too small");
+        WL_CHECK_BUFFERS("wl_kv4_workspace_init", {dev_workspace, "dev_workspace"});
         WL_CUDA(cudaMemsetAsync(dev_workspace, 0, wl::k::kv4_ticket_bytes(), (cudaStream_t)stream));
         return WL_OK;
     });
@@ -836,7 +850,8 @@ int32_t wl_kv4_attention(const float* dev_q, int32_t T, int32_t rows_per_seq, in
         if (workspace_bytes < wl::k::kv4_workspace_bytes(T, rows_per_seq, heads, kv_heads, head_dim, capacity, window, sinks))
             return wl::fail(WL_EINVAL, "wl_kv4_attention: the workspace is too small (wl_kv4_workspace_bytes)");
         if (T == 0) return WL_OK;
-        WL_CHECK_BUFFERS("wl_kv4_attention", {dev_q, "dev_q"}, {dev_out, "dev_out"}, {dev_workspace, "dev_workspace"});
+        WL_CHECK_BUFFERS("wl_kv4_attention", {dev_q, "dev_q"}, {dev_out, "dev_out"}, {dev_workspace, "dev_workspace"},
+                         {dev_caches, "dev_caches", 8, true}, {dev_pos, "dev_pos", 4, true});
         wl::k::kv4_attention(dev_q, T, rows_per_seq, heads, kv_heads, head_dim, scale, wl::k::Kv4Cache{dev_caches, 8, 0}, dev_pos,
                              capacity, window, sinks, dev_out, dev_workspace, (int*)wl::k::static_scratch(), (cudaStream_t)stream);
         return WL_OK;
@@ -850,10 +865,7 @@ int32_t wl_sample_rows(const float* dev_logits, int64_t ld, int32_t V, int32_t r
         if (V <= 0 || rows < 0 || ld < V) return wl::fail(WL_EINVAL, "wl_sample_rows: V must be positive, rows not negative and ld at least V");
         if (!dev_logits || !dev_opts || !dev_ids) return wl::fail(WL_EINVAL, "wl_sample_rows: null pointer");
         if (rows == 0) return WL_OK;
-        const std::string f = device_buffer_fault(dev_logits, "dev_logits", 4);
-        if (!f.empty()) return wl::fail(WL_EINVAL, "wl_sample_rows: " + f);
-        const std::string g = device_buffer_fault(dev_opts, "dev_opts", 8);
-        if (!g.empty()) return wl::fail(WL_EINVAL, "wl_sample_rows: " + g);
+        WL_CHECK_BUFFERS("wl_sample_rows", {dev_logits, "dev_logits", 4}, {dev_opts, "dev_opts", 8}, {dev_ids, "dev_ids", 4, true});
         wl::k::sample_rows(dev_logits, ld, V, rows, dev_opts, dev_ids, (cudaStream_t)stream);
         return WL_OK;
     });
