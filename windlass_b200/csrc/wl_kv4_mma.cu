@@ -194,8 +194,8 @@ __device__ __forceinline__ uint32_t slots16(uint32_t x)
     return spread(x) | spread(x >> 8) << 2;
 }
 
-// What the values' scales of a step call for (slot j % PM_SLOTS): the largest scale of 2 or more, and where scales are NaN (a value
-// row that held an infinity or NaN): bit n of word n / 32 of block b is slot n.
+// What the scales of a step call for (slot j % PM_SLOTS): whether a key's is 2^13 or more; the largest of the values' of 2 or
+// more, and where those are NaN (a value row that held an infinity or NaN): bit n of word n / 32 of block b is slot n.
 template <int NB> struct StepCare {
     uint32_t vmax;              // its float's bits; 0: all below 2
     int any_nan;

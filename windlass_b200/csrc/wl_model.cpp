@@ -878,7 +878,6 @@ void Model::free_seq(Seq* s)
     delete s;
 }
 
-// Transformer.Reserve (src/Transformer.cs:62-73): grow to max(positions, min(context, max(256, 2*capacity))).
 int64_t Model::kv_layer_words(int capacity) const
 {
     return kv4_ ? k::kv4_bytes(c_.kv_heads, c_.head_dim, capacity) / 2 : (int64_t)capacity * c_.kvdim();
@@ -890,6 +889,7 @@ RowKV Model::row_kv(const Seq* s) const
     return RowKV{s->kv, kv4_ ? s->kv : s->kv + (int64_t)c_.layers * stride, stride};
 }
 
+// Transformer.Reserve (src/Transformer.cs:62-73): grow to max(positions, min(context, max(256, 2*capacity))).
 void Model::reserve(Seq* s, int positions)
 {
     if (positions <= s->capacity) return;
