@@ -87,6 +87,7 @@ void* export_scratch(size_t bytes)
         }
         WL_CUDA(cudaMalloc(&g_scratch[dev], bytes));
         WL_CUDA(cudaMemset(g_scratch[dev], 0, 256));
+        WL_CUDA(cudaStreamSynchronize(nullptr));       // (the call's stream need not wait for the default one)
         g_scratch_size[dev] = bytes;
     }
     return g_scratch[dev];
@@ -641,6 +642,7 @@ int32_t wl_kernel_status(int32_t device)
                 if (e) {
                     if (!code) code = e;
                     WL_CUDA(cudaMemset(g_scratch[device], 0, sizeof e));
+                    WL_CUDA(cudaStreamSynchronize(nullptr));
                 }
             }
         }
@@ -649,6 +651,7 @@ int32_t wl_kernel_status(int32_t device)
         if (e) {
             if (!code) code = e;
             WL_CUDA(cudaMemset(wl::k::static_scratch(), 0, sizeof e));
+            WL_CUDA(cudaStreamSynchronize(nullptr));
         }
         if (code) return wl::fail(WL_ETIMEDOUT, "a device-side wait of a kernel-level call gave up (code " + std::to_string(code) + ")");
         return WL_OK;

@@ -48,6 +48,7 @@ void init_tables()
     WL_CUDA(cudaMemcpyToSymbol(g_ksigns, WL_KSIGNS_IQ2XS, sizeof(WL_KSIGNS_IQ2XS)));
     WL_CUDA(cudaMemcpyToSymbol(g_kvalues, WL_KVALUES_IQ4NL, sizeof(WL_KVALUES_IQ4NL)));
     init_i8_tables();
+    WL_CUDA(cudaStreamSynchronize(nullptr));       // (the kernels' streams need not wait for the default one)
     if (dev < 64) done |= 1ull << dev;
 }
 

@@ -147,7 +147,7 @@ void Model::init_fused_ar(const wl_options& opt)
     if (opt.tp_nccl_only || G > k::AR_MAX_RANKS || 2 * c_.layers + 2 > k::AR_STEP || !k::norm_prep_supported(c_.embd)) return;
     const size_t bytes = k::ar_buffer_bytes(c_.embd);
     ar_buf_ = dalloc<uint8_t>((int64_t)bytes);
-    WL_CUDA(cudaMemset(ar_buf_, 0, bytes));
+    WL_CUDA(cudaMemsetAsync(ar_buf_, 0, bytes, stream_));      // (done when the ranks' records have been exchanged)
     struct PeerRec {
         cudaIpcMemHandle_t handle;
         uint64_t ptr;
@@ -164,7 +164,7 @@ void Model::init_fused_ar(const wl_options& opt)
     mine.device = device_;
     uint8_t* hd = dalloc<uint8_t>(128 * G);
     std::vector<PeerRec> all(G);
-    WL_CUDA(cudaMemcpy(hd + 128 * tp_rank_, &mine, 128, cudaMemcpyHostToDevice));
+    WL_CUDA(cudaMemcpyAsync(hd + 128 * tp_rank_, &mine, 128, cudaMemcpyHostToDevice, stream_));
     comm_->allgather(hd + 128 * tp_rank_, hd, 128, stream_);
     WL_CUDA(cudaStreamSynchronize(stream_));
     WL_CUDA(cudaMemcpy(all.data(), hd, 128 * (size_t)G, cudaMemcpyDeviceToHost));
@@ -482,6 +482,8 @@ void Model::load_from_gguf(const Gguf& g)
     arena_size_ = total;
     if (streamed_) plan_streaming(raw_upper, slot_upper);
 
+    // Every upload goes by the model's own stream, which does not wait for the default one: a copy from pageable memory returns
+    // when it has been staged, and what comes next (tiles, conversions) would read the place before the copy is there.
     // split: WHOLE on every rank; ROWS this rank's 1/G of the rows; COLS its 1/G of every row's blocks; HEAD rows
     // rank*vocab_part_ .. +vocab_part_ (the last rank's may be fewer); EXPERTS a stacked tensor's experts
     // e_lo_ .. e_lo_ + e_n_ - 1, whole.
@@ -492,7 +494,7 @@ void Model::load_from_gguf(const Gguf& g)
         const uint8_t* src = g.data(*t);
         if (G == 1 || sp == WHOLE) {
             w.d = weight_alloc(w.bytes);
-            WL_CUDA(cudaMemcpy(w.d, src, (size_t)w.bytes, cudaMemcpyHostToDevice));
+            WL_CUDA(cudaMemcpyAsync(w.d, src, (size_t)w.bytes, cudaMemcpyHostToDevice, stream_));
             if (stream_file_ && cur_stage_ >= 0) file_src_.push_back({(int64_t)(w.d - staging_), {t->offset, t->size}});
         } else if (sp == EXPERTS) {
             if (w.experts != c_.expert_count || w.experts % G)
@@ -501,7 +503,7 @@ void Model::load_from_gguf(const Gguf& g)
             w.experts = e_n_;
             w.bytes = per * e_n_;
             w.d = weight_alloc(w.bytes);
-            WL_CUDA(cudaMemcpy(w.d, src + (int64_t)e_lo_ * per, (size_t)w.bytes, cudaMemcpyHostToDevice));
+            WL_CUDA(cudaMemcpyAsync(w.d, src + (int64_t)e_lo_ * per, (size_t)w.bytes, cudaMemcpyHostToDevice, stream_));
         } else if (sp == ROWS || sp == HEAD) {
             if (w.experts != 1) WL_THROW(WL_EUNSUPPORTED, "Tensor parallelism does not split stacked tensors.");
             int r0, n;
@@ -513,7 +515,7 @@ void Model::load_from_gguf(const Gguf& g)
             w.rows = n;
             w.bytes = (int64_t)n * w.row_bytes;
             w.d = weight_alloc(w.bytes);
-            WL_CUDA(cudaMemcpy(w.d, src + (int64_t)r0 * w.row_bytes, (size_t)w.bytes, cudaMemcpyHostToDevice));
+            WL_CUDA(cudaMemcpyAsync(w.d, src + (int64_t)r0 * w.row_bytes, (size_t)w.bytes, cudaMemcpyHostToDevice, stream_));
         } else {
             int b = 0, bb = 0;
             layout(w.type, &b, &bb);
@@ -522,8 +524,8 @@ void Model::load_from_gguf(const Gguf& g)
                                           type_name(w.type) + " blocks over " + std::to_string(G) + " GPUs.");
             const int64_t lrb = w.row_bytes / G;
             w.d = weight_alloc(lrb * w.rows);
-            WL_CUDA(cudaMemcpy2D(w.d, (size_t)lrb, src + tp_rank_ * lrb, (size_t)w.row_bytes, (size_t)lrb, (size_t)w.rows,
-                                 cudaMemcpyHostToDevice));
+            WL_CUDA(cudaMemcpy2DAsync(w.d, (size_t)lrb, src + tp_rank_ * lrb, (size_t)w.row_bytes, (size_t)lrb, (size_t)w.rows,
+                                      cudaMemcpyHostToDevice, stream_));
             w.cols /= G;
             w.row_bytes = lrb;
             w.bytes = lrb * w.rows;
@@ -547,7 +549,7 @@ void Model::load_from_gguf(const Gguf& g)
             bytes = n * esz;
         }
         uint8_t* d = arena_alloc(bytes);
-        WL_CUDA(cudaMemcpy(d, src, (size_t)bytes, cudaMemcpyHostToDevice));
+        WL_CUDA(cudaMemcpyAsync(d, src, (size_t)bytes, cudaMemcpyHostToDevice, stream_));
         stats_.bytes_h2d += bytes;
         weight_bytes_ += bytes;
         v.n = (int)n;
@@ -622,7 +624,8 @@ void Model::build_rope_table(const float* rope_freqs, int n_rope_freqs)
         }
     }
     rope_table_ = dalloc<float>((int64_t)t.size());
-    WL_CUDA(cudaMemcpy(rope_table_, t.data(), t.size() * 4, cudaMemcpyHostToDevice));
+    WL_CUDA(cudaMemcpyAsync(rope_table_, t.data(), t.size() * 4, cudaMemcpyHostToDevice, stream_));
+    WL_CUDA(cudaStreamSynchronize(stream_));
 }
 
 Model* Model::open_file(const std::string& path, const wl_options& opt)
@@ -989,7 +992,7 @@ void Model::ensure_workspace(int T, int logit_rows)
         WL_CUDA(cudaMalloc(&xprep_buf_, k::xprep_bytes(max_cols, 8)));
         const size_t apf = k::attention_part_floats(c_.heads, c_.kv_heads, c_.head_dim);
         att_part_ = dalloc<float>((int64_t)apf);
-        WL_CUDA(cudaMemset(att_part_, 0, sizeof(float) * apf));     // the merge tickets start at zero
+        WL_CUDA(cudaMemsetAsync(att_part_, 0, sizeof(float) * apf, stream_));     // the merge tickets start at zero
     }
     if (logit_rows > ws_logit_rows_) {
         dfree(logits_); dfree(ids_d_); dfree(amax_key_); dfree(amax_count_); hfree(h_ids_);
@@ -997,8 +1000,8 @@ void Model::ensure_workspace(int T, int logit_rows)
         ids_d_ = dalloc<int32_t>(logit_rows);
         amax_key_ = dalloc<unsigned long long>(logit_rows);
         amax_count_ = dalloc<unsigned>(logit_rows);
-        WL_CUDA(cudaMemset(amax_key_, 0, sizeof(unsigned long long) * (size_t)logit_rows));
-        WL_CUDA(cudaMemset(amax_count_, 0, sizeof(unsigned) * (size_t)logit_rows));
+        WL_CUDA(cudaMemsetAsync(amax_key_, 0, sizeof(unsigned long long) * (size_t)logit_rows, stream_));
+        WL_CUDA(cudaMemsetAsync(amax_count_, 0, sizeof(unsigned) * (size_t)logit_rows, stream_));
         h_ids_ = halloc<int32_t>(logit_rows);
         if (tp_size_ > 1) {
             dfree(logits_part_); dfree(logits_all_);
@@ -1152,12 +1155,12 @@ void Model::build_maps()
     mk(output_);
     if (!err_d_) {
         err_d_ = dalloc<int>(1);
-        WL_CUDA(cudaMemset(err_d_, 0, sizeof(int)));
+        WL_CUDA(cudaMemsetAsync(err_d_, 0, sizeof(int), stream_));
     }
     if (c_.expert_count > 0 && !expert_count_d_) {
         // [0] the count, [1] where a graph capture keeps it while its warm-up run repeats a step
         expert_count_d_ = dalloc<unsigned long long>(2);
-        WL_CUDA(cudaMemset(expert_count_d_, 0, 2 * sizeof(unsigned long long)));
+        WL_CUDA(cudaMemsetAsync(expert_count_d_, 0, 2 * sizeof(unsigned long long), stream_));
     }
 }
 
@@ -1169,13 +1172,13 @@ void Model::check_device_error()
         WL_CUDA(cudaMemcpy(&n, expert_count_d_, sizeof n, cudaMemcpyDeviceToHost));
         if (n) {
             stats_.expert_runs += (int64_t)n;
-            WL_CUDA(cudaMemset(expert_count_d_, 0, sizeof n));
+            WL_CUDA(cudaMemsetAsync(expert_count_d_, 0, sizeof n, stream_));
         }
     }
     int e = 0;
     WL_CUDA(cudaMemcpy(&e, err_d_, sizeof(int), cudaMemcpyDeviceToHost));
     if (e != 0) {
-        WL_CUDA(cudaMemset(err_d_, 0, sizeof(int)));
+        WL_CUDA(cudaMemsetAsync(err_d_, 0, sizeof(int), stream_));
         WL_THROW(WL_ETIMEDOUT, "a device-side wait gave up (code " + std::to_string(e) + ")");
     }
 }
@@ -1708,7 +1711,7 @@ double Model::bench_decode(Seq* const* seqs, int N, int steps)
         for (int s = 0; s < steps; ++s) pos_all[(size_t)s * N + i] = len[i] + s;
     }
     int32_t* pos_all_d = dalloc<int32_t>((int64_t)steps * N);
-    WL_CUDA(cudaMemcpy(pos_all_d, pos_all.data(), pos_all.size() * 4, cudaMemcpyHostToDevice));
+    WL_CUDA(cudaMemcpyAsync(pos_all_d, pos_all.data(), pos_all.size() * 4, cudaMemcpyHostToDevice, stream_));
     upload_step(N, rows.data(), pos_all.data(), toks.data());
     // ForwardBatch steps (every row as if alone); a graph is captured (or found) before the timed loop so capture
     // costs are not timed
