@@ -237,8 +237,8 @@ int32_t wl_forward_batch_sample(wl_model* model, wl_seq* const* seqs, const int3
                                 volatile const int32_t* cancel, wl_progress_fn progress, void* user);
 
 /* A row's sampling options beyond Sampler.Sample's. The ids in order: logit descending, equal logits by ascending id;
- * p[i] = exp((logit[i] - max) / temperature) in double (none for a NaN or -inf logit). Kept: of the first top_k ids
- * (top_k <= 0: all) the shortest prefix whose sum of p reaches top_p times theirs (top_p >= 1: all), of it the ids with
+ * p[i] = exp((logit[i] - max) / temperature) in double, the difference in float as Sampler.Sample's (none for a NaN or
+ * -inf logit). Kept: of the first top_k ids (top_k <= 0: all) the shortest prefix whose sum of p reaches top_p times theirs (top_p >= 1: all), of it the ids with
  * p >= min_p (min_p <= 0: all), at least the first. The choice is the first kept id at which the running sum reaches draw *
  * (the kept ids' sum), in that order, or in id order when nothing is filtered (top_k <= 0 or >= V, top_p >= 1, min_p <= 0).
  * temperature <= 0: the greedy id, the rest is not read. A row without a logit above -inf gives 0. The sums are exact

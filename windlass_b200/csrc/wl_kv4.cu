@@ -471,9 +471,9 @@ constexpr int att_ctas(int HD) { return HD <= 128 ? 2 : 1; }
 // every eighth pair of the range, through its ring of bulk copies, and the warps' sums are joined in warp order. The last
 // CTA of a row joins the ranges, or, where there are rows enough to fill the SMs (ALONE: rows of up to a.alone ranges), one
 // CTA walks a row's ranges: a row's bits do not depend on that, nor on the other rows.
-// Measured: 64 heads on 8 of 128 dims over 131001 positions 56.7 us (151 MB, 2.7 TB/s, 0.41 of a copy's rate), 8 such rows of up
-// to 4100 15.8 us, 64 rows of 32 on 8 behind a window of 1024 41.0 us (78 MB, 1.9 TB/s), 8 heads of 64 dims over 300
-// positions 4.6 us. Bound by the warps' instructions: about 380 a tile of 16 positions and warp (the codes' masks, the scales'
+// Measured: 64 heads on 8 of 128 dims over 131001 positions 57.9 us (151 MB, 2.6 TB/s, 0.40 of a copy's rate), 8 such rows of up
+// to 4100 16.1 us, 64 rows of 32 on 8 behind a window of 1024 41.8 us (78 MB, 1.9 TB/s), 8 heads of 64 dims over 300
+// positions 4.7 us. Bound by the warps' instructions: about 390 a tile of 16 positions and warp (the codes' masks, the scales'
 // products, weights split in two), with the loads always two tiles ahead.
 __device__ __forceinline__ int att_range(int tiles, int s_max)
 {
@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, att_ctas(HD)) k_kv4_attn(const
 // Runs of R rows that read one cache (prompts): the (row, head) pairs of a run and KV head are queries 0 .. R G - 1; a CTA
 // takes QB of them, each warp MT tiles of 8, and all warps share each tile of the cache (one ring of bulk copies), so
 // a tile's codes are unpacked once for 8 MT queries. Only for head sizes that wl_kv4_mma.cu does not take (96 and 256).
-// Measured: 500 rows behind 4000 positions, 32 heads on 8 of 96 dims 373 us, 16 on 8 of 256 446 us: bound by mma.sync's rate
+// Measured: 500 rows behind 4000 positions, 32 heads on 8 of 96 dims 387 us, 16 on 8 of 256 456 us: bound by mma.sync's rate
 // and the unpacking (32 rows of 8 heads of 128 dims, 5000 positions: 54 us so, 30 by wl_kv4_mma.cu).
 template <int HD, int MT>
 __global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att a, int q_blocks)
@@ -783,9 +783,10 @@ __global__ void __launch_bounds__(32 * RUN_WARPS, 2) k_kv4_attn_run(const Kv4Att
 
 constexpr int64_t KV4_TICKETS = 1 << 18;    // tickets at the head of a workspace (zero between calls)
 
-// Rows of a run up to which each is attended to by itself. 9 rows, 32 heads on 4, 4000 positions: 15 us so, 37 by tensor
-// cores and 67 by k_kv4_attn_run; 12 rows of 500 positions: 9, 21 and 34; 16 rows of 3000: 27, 32 and 64; the other way
-// round where runs are few and long (10 rows, 64 heads on 8, 20000 positions: 96, 65 and 161), which the shape does not tell.
+// Rows of a run up to which each is attended to by itself. 9 rows, 32 heads on 4, 4000 positions: 16 us so, 37 by tensor
+// cores and 67 by k_kv4_attn_run; 12 rows of 500 positions: 10, 21 and 34; 16 rows of 3000: 28, 32 and 64. The rule looks at
+// the rows alone, so it is wrong for few rows of many heads over a long cache (10 rows, 64 heads on 8, 20000 positions: 100,
+// 65 and 161): there a rule on heads and room as well would gain a third.
 constexpr int RUN_MIN_ROWS = 17;
 constexpr int RUN_MAX_RANGES = 32;          // ranges a run may be cut into
 
@@ -835,7 +836,8 @@ Kv4Plan kv4_plan(int T, int R, int heads, int kv_heads, int head_dim, int64_t ca
         // enough rows for the SMs: short ones are walked by one CTA each (64 rows with a window of 1024: 49.7 us with a CTA a
         // range); a row of more than 8 ranges among them is still spread, so that the call does not wait for it. Beyond 64
         // rows every row is walked by one CTA a KV head, whatever its length, so that calls of any size need no partials: the
-        // same ranges joined in the same order, so the same bits, but the call does wait for its longest row.
+        // same ranges joined in the same order, so the same bits, but the call does wait for its longest row. (100 rows of 1000 to
+        // 4000 positions, 32 heads on 8: 127 us so, 109 us with one range a row, which gave long rows other bits than alone.)
         p.alone = T > 64 || ctas > KV4_TICKETS ? INT_MAX : ctas >= 2 * 148 ? 8 : 0;
         if (p.alone >= p.S) p.S = 1;
     }

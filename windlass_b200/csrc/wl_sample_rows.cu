@@ -2,7 +2,7 @@
 // uniform draw.
 //
 //   temperature <= 0: the greedy id (wl_argmax's rule).
-//   p[i] = exp((x[i] - max) / temperature) in double; NaN and -inf logits have none, and every id at the maximum has 1.
+//   p[i] = exp((x[i] - max) / temperature) in double, the difference in float (Sampler.Sample's arithmetic); NaN and -inf logits have none, and every id at the maximum has 1.
 //   The ids in order: logit descending, equal logits by ascending id. Kept is a prefix of that order: the top_k first ids
 //   (top_k > 0), of these the shortest prefix whose sum reaches top_p * (their sum) (top_p < 1), of these the ones with
 //   p >= min_p (min_p > 0), and at least the first. The choice is the first id at which the running sum reaches draw * (the
@@ -19,8 +19,9 @@
 // boundary between two ids by at most V * 2^-(F+1), 4e-9 of the sum at 151936 ids, and as a rule by the square root of V such
 // halves, 1e-11.
 //
-// Measured: 12.2 us for a row of 32000 logits with a top-k, 24.6 us for 8 rows of 151936 with mixed filters, 77.9 us for 64 rows
-// of 128256 (33 MB: 0.42 TB/s). A latency chain, not bandwidth: of a CTA's 45000 cycles with a nucleus 5000 are the load, 17000 the
+// Measured: 12.1 us for a row of 32000 logits with a top-k, 24.7 us for 8 rows of 151936 with mixed filters, 77.7 us for 64 rows
+// of 128256 (33 MB: 0.42 TB/s). The time follows the rows: other draws of the same 8 rows took 26 to 70 us (a row whose nucleus
+// ends in a bin of more than SR_CAP ids is cut again), of the 64 rows 57 to 82, each the same to 1 % when repeated. A latency chain, not bandwidth: of a CTA's 45000 cycles with a nucleus 5000 are the load, 17000 the
 // histogram of masses (an exponential in double and one or two shared atomics a logit; two CTAs share an SM), 6000 a
 // join of the cluster's histograms, 8000 the gather and 7000 the ranking. Two CTAs an SM, 512 threads each: the 512 CTAs of
 // 64 rows are 1.7 waves. Tried and slower: every CTA's gathered ids in a list of its own with the counts exchanged (no
