@@ -242,7 +242,8 @@ int32_t wl_forward_batch_sample(wl_model* model, wl_seq* const* seqs, const int3
  * p >= min_p (min_p <= 0: all), at least the first. The choice is the first kept id at which the running sum reaches draw *
  * (the kept ids' sum), in that order, or in id order when nothing is filtered (top_k <= 0 or >= V, top_p >= 1, min_p <= 0).
  * temperature <= 0: the greedy id, the rest is not read. A row without a logit above -inf gives 0. The sums are exact
- * sums of p rounded to multiples of 2^-F, F = min(51, 62 - ceil(log2 V)), so the choice is the same in every run. */
+ * sums of p rounded to multiples of 2^-F, F = min(51, 62 - ceil(log2 V)), so the choice is the same in every run; an id
+ * whose p rounds to 0 is not chosen, at a draw of 0 neither. */
 typedef struct wl_sample_opts {
     double temperature, top_p, min_p;
     double draw;             /* the caller's uniform double in [0, 1) */
